@@ -14,7 +14,9 @@ SOURCES = ["capi.hip", "forward.hip", "backward.hip", "scan_sort.hip", "aux.hip"
 # only explicit FMA() fuses.  (No float atomics anywhere in the library.)
 # -fno-slp-vectorize: the SLP pass pairs scalar fp32 ops into v_pk_* instructions (1.7x the issue cost of one op) and pays
 # for it with v_mov shuffles -- a net loss in the compositing kernels (measured -3 % on render_bwd_kernel).
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fno-slp-vectorize", "-fPIC"]
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 by any other route either (some of their forms have given wrong results).
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fno-slp-vectorize",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-fPIC"]
 
 
 def build(force=False, verbose=False):
