@@ -8,7 +8,7 @@ import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SRC = os.path.join(HERE, "csrc", "ext.cpp")
+SRCS = [os.path.join(HERE, "csrc", "ext.cpp"), os.path.join(HERE, "csrc", "features_ext.cpp")]
 NAME = "_C_native"
 OUT = os.path.join(HERE, NAME + sysconfig.get_config_var("EXT_SUFFIX"))
 
@@ -20,12 +20,12 @@ def build(force=False, verbose=False):
     if not os.path.exists(lib):
         from event_3dgs_amd import build as hip_build
         hip_build.build()
-    deps = [SRC, os.path.join(ROOT, "include", "e3dgs_hip.h")]
+    deps = SRCS + [os.path.join(ROOT, "include", "e3dgs_hip.h")]
     if not force and os.path.exists(OUT) and os.path.getmtime(OUT) >= max(os.path.getmtime(d) for d in deps):
         return OUT
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
     inc = ce.include_paths(device_type="cuda") + [sysconfig.get_paths()["include"], os.path.join(ROOT, "include")]
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", SRC, "-o", OUT,
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", *SRCS, "-o", OUT,
            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-DTORCH_EXTENSION_NAME={NAME}", "-DTORCH_API_INCLUDE_EXTENSION_H",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-Wno-deprecated-declarations"]
     cmd += [f"-I{p}" for p in inc]

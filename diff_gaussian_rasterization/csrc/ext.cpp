@@ -220,10 +220,13 @@ Tensor mark_visible(const Tensor& means3D, const Tensor& viewmatrix, const Tenso
 
 }  // namespace
 
+void bind_features(pybind11::module& m);      // features_ext.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("rasterize_gaussians", &rasterize_gaussians);
     m.def("rasterize_gaussians_backward", &rasterize_gaussians_backward);
     m.def("mark_visible", &mark_visible);
     m.def("rasterize_autograd", &rasterize_autograd);
     m.def("abi_version", []() { return e3dgs_abi_version(); });
+    bind_features(m);
 }

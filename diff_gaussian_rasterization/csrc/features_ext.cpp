@@ -1,0 +1,324 @@
+// features_ext.cpp -- the learned-feature operators as autograd nodes over the C ABI (include/e3dgs_hip.h): embedding, layer
+// norm, distillation.  Bound by event_3dgs_amd.features and event_3dgs_amd.losses, which hold the documentation; this file
+// checks the arguments, lays tensors out where the ABI needs it, allocates the results on the tensors' device and launches
+// on the current stream of that device.
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/extension.h>
+
+#include <cmath>
+#include <stdexcept>
+#include <string>
+#include <tuple>
+
+#include "e3dgs_hip.h"
+
+namespace {
+
+using torch::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using Guard = c10::hip::HIPGuardMasqueradingAsCUDA;      // (torch-ROCm tensors say "cuda")
+
+void check(int rc, const char* what) {
+    if (rc != 0) throw std::runtime_error(std::string(what) + " failed (code " + std::to_string(rc) + "): " + e3dgs_last_error());
+}
+void* stream() { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream(); }
+
+int dtype_of(const Tensor& t, const char* name) {
+    if (t.scalar_type() == torch::kFloat32) return E3DGS_F32;
+    if (t.scalar_type() == torch::kFloat16) return E3DGS_F16;
+    TORCH_CHECK(t.scalar_type() == torch::kBFloat16, name, " must be float32, float16 or bfloat16");
+    return E3DGS_BF16;
+}
+int index_bytes_of(const Tensor& t) {
+    TORCH_CHECK(t.scalar_type() == torch::kInt32 || t.scalar_type() == torch::kInt64, "index must be int32 or int64");
+    return t.scalar_type() == torch::kInt64 ? 8 : 4;
+}
+void on_gpu(const Tensor& t, const char* name) { TORCH_CHECK(t.is_cuda(), name, " must be a CUDA/HIP tensor (this op has no CPU path)"); }
+void same_device(const Tensor& t, const Tensor& with, const char* name) {
+    on_gpu(t, name);
+    TORCH_CHECK(t.device() == with.device(), name, " is on ", t.device(), ", the operator runs on ", with.device());
+}
+// a second derivative would silently be zero: refuse the graph of the gradient
+void once(const char* who) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), who, " is differentiable once only (create_graph is not supported)");
+}
+char* bytes(const Tensor& t) { return reinterpret_cast<char*>(t.data_ptr()); }
+Tensor scratch_of(size_t n, const Tensor& like) { return torch::empty({(int64_t)n}, like.options().dtype(torch::kByte)); }
+
+// (rows, dim) view of a tensor with unit stride along the last dimension; copied only when there is no such view
+Tensor as_rows(const Tensor& t) {
+    const int64_t dim = t.size(-1);
+    if (t.numel() == 0) return t.reshape({t.numel() / std::max<int64_t>(dim, 1), dim});
+    Tensor r = t.reshape({-1, dim});
+    return r.stride(1) == 1 || dim == 1 ? r : r.contiguous();
+}
+
+// ------------------------------------------------------------------------------------------------ embedding
+Tensor embedding_forward(const Tensor& index, const Tensor& table, double scale) {
+    const Guard guard(table.device());
+    std::vector<int64_t> shape = index.sizes().vec();
+    shape.push_back(table.size(1));
+    Tensor out = torch::empty(shape, table.options());
+    const Tensor idx = index.contiguous(), tab = as_rows(table);
+    check(e3dgs_embedding_forward((size_t)idx.numel(), (size_t)table.size(0), (size_t)table.size(1), idx.data_ptr(),
+                                  index_bytes_of(idx), tab.data_ptr(), (size_t)tab.stride(0), dtype_of(table, "table"),
+                                  (float)scale, out.data_ptr(), stream()),
+          "e3dgs_embedding_forward");
+    return out;
+}
+
+struct EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& index, const Tensor& table, double scale) {
+        ctx->save_for_backward({index});
+        ctx->saved_data["rows"] = table.size(0);
+        ctx->saved_data["scale"] = scale;
+        return embedding_forward(index, table, scale);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("embedding");
+        const auto saved = ctx->get_saved_variables();
+        if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
+        const Guard guard(grads[0].device());
+        const int64_t rows = ctx->saved_data["rows"].toInt();
+        const Tensor index = saved[0].contiguous(), g = as_rows(grads[0]);
+        const int64_t dim = g.size(1), n = index.numel();
+        Tensor d = torch::empty({rows, dim}, g.options());
+        Tensor scratch = scratch_of(e3dgs_embedding_backward_scratch_bytes((size_t)n, (size_t)rows, (size_t)dim), g);
+        check(e3dgs_embedding_backward((size_t)n, (size_t)rows, (size_t)dim, index.data_ptr(), index_bytes_of(index),
+                                       g.data_ptr(), (size_t)g.stride(0), dtype_of(g, "grad"),
+                                       (float)ctx->saved_data["scale"].toDouble(), d.data_ptr(), bytes(scratch), stream()),
+              "e3dgs_embedding_backward");
+        return {Tensor(), d, Tensor()};
+    }
+};
+
+Tensor embedding(const Tensor& index, const Tensor& table, double scale) {
+    on_gpu(table, "table");
+    same_device(index, table, "index");
+    TORCH_CHECK(table.dim() == 2 && table.size(1) >= 1, "table must have dimensions (rows, dim)");
+    TORCH_CHECK(table.size(1) <= E3DGS_FEATURE_MAX_DIM, "at most ", E3DGS_FEATURE_MAX_DIM, " values to a row");
+    TORCH_CHECK(index.numel() < 0x7FFFFFFF && table.size(0) < 0x7FFFFFFF, "embedding takes fewer than 2^31 - 1 indices and rows");
+    TORCH_CHECK(std::isfinite(scale), "scale must be finite");
+    dtype_of(table, "table");
+    index_bytes_of(index);
+    if (!(at::GradMode::is_enabled() && table.requires_grad())) return embedding_forward(index, table, scale);
+    return EmbeddingFunction::apply(index, table, scale);
+}
+
+// ------------------------------------------------------------------------------------------------ layer norm
+std::tuple<Tensor, Tensor> layer_norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, bool stats) {
+    const Guard guard(x.device());
+    const Tensor r = as_rows(x);
+    const int64_t rows = r.size(0), dim = r.size(1);
+    Tensor out = torch::empty(x.sizes(), x.options());
+    Tensor st = stats ? torch::empty({2, rows}, x.options().dtype(torch::kFloat32)) : Tensor();
+    const Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
+    const int affine = w.defined() ? dtype_of(w, "weight") : b.defined() ? dtype_of(b, "bias") : E3DGS_F32;
+    check(e3dgs_layer_norm_forward((size_t)rows, (size_t)dim, r.data_ptr(), (size_t)r.stride(0), dtype_of(x, "x"),
+                                   w.defined() ? w.data_ptr() : nullptr, b.defined() ? b.data_ptr() : nullptr, affine,
+                                   (float)eps, out.data_ptr(), stats ? st.data_ptr<float>() : nullptr,
+                                   stats ? st.data_ptr<float>() + rows : nullptr, stream()),
+          "e3dgs_layer_norm_forward");
+    return std::make_tuple(out, st);
+}
+
+struct LayerNormFunction : public torch::autograd::Function<LayerNormFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const c10::optional<Tensor>& weight_,
+                          const c10::optional<Tensor>& bias_, double eps) {
+        const Tensor weight = weight_ ? *weight_ : Tensor(), bias = bias_ ? *bias_ : Tensor();
+        auto r = layer_norm_forward(x, weight, bias, eps, true);
+        ctx->save_for_backward({x, weight, std::get<1>(r)});
+        ctx->saved_data["x_grad"] = x.requires_grad();
+        ctx->saved_data["weight_grad"] = weight.defined() && weight.requires_grad();
+        ctx->saved_data["bias_grad"] = bias.defined() && bias.requires_grad();
+        ctx->saved_data["affine"] = (int64_t)(weight.defined() ? weight.scalar_type() : bias.defined() ? bias.scalar_type() : x.scalar_type());
+        return std::get<0>(r);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("layer_norm");
+        const auto saved = ctx->get_saved_variables();
+        if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+        const Tensor &x = saved[0], &weight = saved[1], &st = saved[2];
+        const Guard guard(x.device());
+        const Tensor r = as_rows(x), g = as_rows(grads[0]);
+        const int64_t rows = r.size(0), dim = r.size(1);
+        const Tensor w = weight.defined() ? weight.contiguous() : weight;
+        const auto affine = x.options().dtype((c10::ScalarType)ctx->saved_data["affine"].toInt());
+        Tensor dx = ctx->saved_data["x_grad"].toBool() ? torch::empty(x.sizes(), x.options()) : Tensor();
+        Tensor dw = ctx->saved_data["weight_grad"].toBool() ? torch::empty({dim}, affine) : Tensor();
+        Tensor db = ctx->saved_data["bias_grad"].toBool() ? torch::empty({dim}, affine) : Tensor();
+        Tensor scratch;
+        if (dw.defined() || db.defined()) scratch = scratch_of(e3dgs_layer_norm_backward_scratch_bytes((size_t)rows, (size_t)dim), x);
+        const auto kind = affine.dtype().toScalarType();
+        check(e3dgs_layer_norm_backward((size_t)rows, (size_t)dim, g.data_ptr(), (size_t)g.stride(0), r.data_ptr(),
+                                        (size_t)r.stride(0), dtype_of(x, "x"), w.defined() ? w.data_ptr() : nullptr,
+                                        kind == torch::kFloat32 ? E3DGS_F32 : kind == torch::kFloat16 ? E3DGS_F16 : E3DGS_BF16,
+                                        st.data_ptr<float>(), st.data_ptr<float>() + rows, dx.defined() ? dx.data_ptr() : nullptr,
+                                        dw.defined() ? dw.data_ptr() : nullptr, db.defined() ? db.data_ptr() : nullptr,
+                                        scratch.defined() ? bytes(scratch) : nullptr, stream()),
+              "e3dgs_layer_norm_backward");
+        return {dx, dw, db, Tensor()};
+    }
+};
+
+Tensor layer_norm(const Tensor& x, const c10::optional<Tensor>& weight_, const c10::optional<Tensor>& bias_, double eps) {
+    const Tensor weight = weight_ ? *weight_ : Tensor(), bias = bias_ ? *bias_ : Tensor();
+    on_gpu(x, "x");
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "x must have at least one value to a row");
+    TORCH_CHECK(x.size(-1) <= E3DGS_FEATURE_MAX_DIM, "at most ", E3DGS_FEATURE_MAX_DIM, " values to a row");
+    TORCH_CHECK(std::isfinite(eps) && eps >= 0.0, "eps must be finite and not negative");
+    dtype_of(x, "x");
+    bool grad = x.requires_grad();
+    for (const auto& p : {std::make_pair(&weight, "weight"), std::make_pair(&bias, "bias")}) {
+        if (!p.first->defined()) continue;
+        same_device(*p.first, x, p.second);
+        dtype_of(*p.first, p.second);
+        TORCH_CHECK(p.first->dim() == 1 && p.first->size(0) == x.size(-1), p.second, " must have dimensions (", x.size(-1), ",)");
+        grad = grad || p.first->requires_grad();
+    }
+    TORCH_CHECK(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(), "weight and bias must have one type");
+    if (!(at::GradMode::is_enabled() && grad)) return std::get<0>(layer_norm_forward(x, weight, bias, eps, false));
+    return LayerNormFunction::apply(x, weight_, bias_, eps);
+}
+
+// ------------------------------------------------------------------------------------------------ distillation
+// The scores as (rows, classes) in one of the two layouts of the ABI, and the labels with whatever strides they have.
+struct Scores {
+    Tensor logits, teacher, index;                // 2-D views (or copies)
+    std::vector<int64_t> shape;                   // of the logits with the classes last
+    int64_t class_dim;
+    size_t rows, classes, k, row_stride, class_stride;
+    bool planes;
+};
+
+Tensor as_2d(const Tensor& t) { return t.reshape({t.numel() / std::max<int64_t>(t.size(-1), 1), t.size(-1)}); }
+
+Scores scores_of(const Tensor& logits, const Tensor& teacher, const Tensor& index, int64_t class_dim) {
+    Scores s;
+    s.class_dim = class_dim;
+    const Tensor z = logits.movedim(class_dim, -1);
+    s.shape = z.sizes().vec();
+    s.logits = as_2d(z);
+    s.teacher = as_2d(teacher.movedim(class_dim, -1));
+    s.index = as_2d(index.movedim(class_dim, -1));
+    s.rows = (size_t)s.logits.size(0);
+    s.classes = (size_t)s.logits.size(1);
+    s.k = (size_t)s.teacher.size(1);
+    s.planes = s.rows > 1 && s.classes > 1 && s.logits.stride(1) != 1 && s.logits.stride(0) == 1 && s.classes <= E3DGS_DISTILL_MAX_PLANES;
+    if (!s.planes && s.classes > 1 && s.logits.stride(1) != 1) s.logits = s.logits.contiguous();
+    s.row_stride = (size_t)s.logits.stride(0);
+    s.class_stride = s.planes ? (size_t)s.logits.stride(1) : 1;
+    return s;
+}
+
+// value (0-dim, or one per row), stats, loss pair
+std::tuple<Tensor, Tensor, Tensor> distill_forward(const Scores& s, double temperature, int64_t reduction) {
+    const auto opt = s.logits.options().dtype(torch::kFloat32);
+    Tensor stats = torch::empty({(int64_t)s.rows, 2}, opt), loss = torch::empty({2}, opt);
+    Tensor row_loss = reduction == 0 ? torch::empty({(int64_t)s.rows}, opt) : Tensor();
+    Tensor scratch = scratch_of(e3dgs_distill_scratch_bytes(s.rows), s.logits);
+    check(e3dgs_distill_forward(s.rows, s.classes, s.k, s.logits.data_ptr(), s.row_stride, s.class_stride,
+                                dtype_of(s.logits, "logits"), s.teacher.data_ptr(), (size_t)s.teacher.stride(0),
+                                (size_t)s.teacher.stride(1), dtype_of(s.teacher, "teacher_logits"), s.index.data_ptr(),
+                                (size_t)s.index.stride(0), (size_t)s.index.stride(1), index_bytes_of(s.index),
+                                (float)temperature, (int)reduction, stats.data_ptr<float>(),
+                                row_loss.defined() ? row_loss.data_ptr<float>() : nullptr, loss.data_ptr<float>(),
+                                bytes(scratch), stream()),
+          "e3dgs_distill_forward");
+    if (reduction == 0) return std::make_tuple(row_loss.view(std::vector<int64_t>(s.shape.begin(), s.shape.end() - 1)), stats, loss);
+    return std::make_tuple(loss.select(0, 0), stats, loss);
+}
+
+Tensor distill_backward(const Scores& s, double temperature, int64_t reduction, const Tensor& stats, const Tensor& loss,
+                        const Tensor& d_loss) {
+    const int64_t rows = (int64_t)s.rows, classes = (int64_t)s.classes;
+    Tensor grad = s.planes ? torch::empty({classes, rows}, s.logits.options()).t() : torch::empty({rows, classes}, s.logits.options());
+    check(e3dgs_distill_backward(s.rows, s.classes, s.k, s.logits.data_ptr(), s.row_stride, s.class_stride,
+                                 dtype_of(s.logits, "logits"), s.teacher.data_ptr(), (size_t)s.teacher.stride(0),
+                                 (size_t)s.teacher.stride(1), dtype_of(s.teacher, "teacher_logits"), s.index.data_ptr(),
+                                 (size_t)s.index.stride(0), (size_t)s.index.stride(1), index_bytes_of(s.index),
+                                 (float)temperature, (int)reduction, stats.data_ptr<float>(), loss.data_ptr<float>(),
+                                 d_loss.defined() ? d_loss.data_ptr<float>() : nullptr, grad.data_ptr(),
+                                 (size_t)(s.planes ? 1 : classes), (size_t)(s.planes ? rows : 1), stream()),
+          "e3dgs_distill_backward");
+    return grad.view(s.shape).movedim(-1, s.class_dim);
+}
+
+struct DistillFunction : public torch::autograd::Function<DistillFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher, const Tensor& index,
+                          double temperature, int64_t reduction, int64_t class_dim) {
+        const Guard guard(logits.device());
+        auto r = distill_forward(scores_of(logits, teacher, index, class_dim), temperature, reduction);
+        ctx->save_for_backward({logits, teacher, index, std::get<1>(r), std::get<2>(r)});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["reduction"] = reduction;
+        ctx->saved_data["class_dim"] = class_dim;
+        // (the pair of the gradient is a tensor of its own: the caller may change the value it was handed)
+        return reduction == 0 ? std::get<0>(r) : std::get<0>(r).clone();
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("distill_loss");
+        const auto saved = ctx->get_saved_variables();
+        if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        const Guard guard(saved[0].device());
+        const Scores s = scores_of(saved[0], saved[1], saved[2], ctx->saved_data["class_dim"].toInt());
+        const Tensor g = grads[0].to(torch::kFloat32).contiguous();
+        Tensor d = distill_backward(s, ctx->saved_data["temperature"].toDouble(), ctx->saved_data["reduction"].toInt(), saved[3],
+                                    saved[4], g);
+        return {d, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+int64_t distill_check(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature, int64_t class_dim) {
+    on_gpu(logits, "logits");
+    same_device(teacher, logits, "teacher_logits");
+    same_device(index, logits, "teacher_index");
+    dtype_of(logits, "logits");
+    dtype_of(teacher, "teacher_logits");
+    index_bytes_of(index);
+    TORCH_CHECK(logits.dim() >= 1 && class_dim >= -logits.dim() && class_dim < logits.dim(), "class_dim is not a dimension of logits");
+    if (class_dim < 0) class_dim += logits.dim();
+    TORCH_CHECK(teacher.sizes() == index.sizes(), "teacher_logits and teacher_index must have the same shape");
+    TORCH_CHECK(teacher.dim() == logits.dim(), "teacher_logits must have as many dimensions as logits");
+    for (int64_t d = 0; d < logits.dim(); ++d)
+        TORCH_CHECK(d == class_dim || teacher.size(d) == logits.size(d), "teacher_logits and logits differ in dimension ", d);
+    TORCH_CHECK(logits.size(class_dim) >= 1 && logits.size(class_dim) < 0x7FFFFFFF, "logits must have between 1 and 2^31 - 2 classes");
+    TORCH_CHECK(logits.numel() / logits.size(class_dim) < 0x7FFFFFFF, "distill_loss takes fewer than 2^31 - 1 rows");
+    TORCH_CHECK(teacher.size(class_dim) >= 1 && teacher.size(class_dim) <= E3DGS_DISTILL_MAX_K,
+                "teacher_logits must list between 1 and ", E3DGS_DISTILL_MAX_K, " classes");
+    TORCH_CHECK(std::isfinite(temperature) && temperature > 1e-6 && temperature < 1e6, "temperature must lie between 1e-6 and 1e6");
+    TORCH_CHECK(!teacher.requires_grad() || !at::GradMode::is_enabled(), "teacher_logits takes no gradient: detach it");
+    return class_dim;
+}
+
+Tensor distill(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature, int64_t reduction, int64_t class_dim) {
+    class_dim = distill_check(logits, teacher, index, temperature, class_dim);
+    if (at::GradMode::is_enabled() && logits.requires_grad())
+        return DistillFunction::apply(logits, teacher, index, temperature, reduction, class_dim);
+    const Guard guard(logits.device());
+    return std::get<0>(distill_forward(scores_of(logits, teacher, index, class_dim), temperature, reduction));
+}
+
+std::tuple<Tensor, Tensor> distill_raw(const Tensor& logits_, const Tensor& teacher, const Tensor& index, double temperature,
+                                       int64_t reduction, int64_t class_dim) {
+    const Tensor logits = logits_.detach();
+    class_dim = distill_check(logits, teacher.detach(), index, temperature, class_dim);
+    const Guard guard(logits.device());
+    at::NoGradGuard no_grad;
+    const Scores s = scores_of(logits, teacher, index, class_dim);
+    auto r = distill_forward(s, temperature, reduction);
+    return std::make_tuple(std::get<0>(r), distill_backward(s, temperature, reduction, std::get<1>(r), std::get<2>(r), Tensor()));
+}
+
+}  // namespace
+
+void bind_features(pybind11::module& m) {
+    const auto free = pybind11::call_guard<pybind11::gil_scoped_release>();
+    m.def("embedding", &embedding, free);
+    m.def("layer_norm", &layer_norm, free);
+    m.def("distill", &distill, free);
+    m.def("distill_raw", &distill_raw, free);
+}

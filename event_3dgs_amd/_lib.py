@@ -158,6 +158,27 @@ def lib():
     L.e3dgs_sort_pairs.restype = C.c_int
     L.e3dgs_sort_pairs.argtypes = [C.c_size_t, C.c_int, C.c_int, _vp, _vp, _vp, _vp, C.c_int, _cp, _vp, _vp, C.c_uint32,
                                    C.POINTER(C.c_int), _vp]
+    _sz = C.c_size_t
+    L.e3dgs_embedding_forward.restype = C.c_int
+    L.e3dgs_embedding_forward.argtypes = [_sz] * 3 + [_vp, C.c_int, _vp, _sz, C.c_int, C.c_float, _vp, _vp]
+    L.e3dgs_embedding_backward_scratch_bytes.restype = _sz
+    L.e3dgs_embedding_backward_scratch_bytes.argtypes = [_sz] * 3
+    L.e3dgs_embedding_backward.restype = C.c_int
+    L.e3dgs_embedding_backward.argtypes = [_sz] * 3 + [_vp, C.c_int, _vp, _sz, C.c_int, C.c_float, _vp, _cp, _vp]
+    L.e3dgs_layer_norm_forward.restype = C.c_int
+    L.e3dgs_layer_norm_forward.argtypes = [_sz] * 2 + [_vp, _sz, C.c_int, _vp, _vp, C.c_int, C.c_float, _vp, _fp, _fp, _vp]
+    L.e3dgs_layer_norm_backward_scratch_bytes.restype = _sz
+    L.e3dgs_layer_norm_backward_scratch_bytes.argtypes = [_sz] * 2
+    L.e3dgs_layer_norm_backward.restype = C.c_int
+    L.e3dgs_layer_norm_backward.argtypes = ([_sz] * 2 + [_vp, _sz, _vp, _sz, C.c_int, _vp, C.c_int, _fp, _fp]
+                                            + [_vp] * 3 + [_cp, _vp])
+    L.e3dgs_distill_scratch_bytes.restype = _sz
+    L.e3dgs_distill_scratch_bytes.argtypes = [_sz]
+    _scores = [_sz] * 3 + [_vp, _sz, _sz, C.c_int] * 2 + [_vp, _sz, _sz, C.c_int, C.c_float, C.c_int]
+    L.e3dgs_distill_forward.restype = C.c_int
+    L.e3dgs_distill_forward.argtypes = _scores + [_fp] * 3 + [_cp, _vp]
+    L.e3dgs_distill_backward.restype = C.c_int
+    L.e3dgs_distill_backward.argtypes = _scores + [_fp] * 3 + [_vp, _sz, _sz, _vp]
     L.e3dgs_profile_enable.restype = None
     L.e3dgs_profile_enable.argtypes = [C.c_int]
     L.e3dgs_profile_select.restype = None
@@ -239,4 +260,7 @@ EXPORTED_SYMBOLS = [
     "e3dgs_sort_scratch_bytes", "e3dgs_sort_pairs", "e3dgs_rasterize_forward_multi_capacity",
     "e3dgs_rasterize_backward_multi_rank1", "e3dgs_event_loss_rank1", "e3dgs_image_loss_rank1",
     "e3dgs_state_offsets_binning", "e3dgs_depth_sort_scratch_bytes", "e3dgs_sort_depth_keys",
+    "e3dgs_embedding_forward", "e3dgs_embedding_backward_scratch_bytes", "e3dgs_embedding_backward",
+    "e3dgs_layer_norm_forward", "e3dgs_layer_norm_backward_scratch_bytes", "e3dgs_layer_norm_backward",
+    "e3dgs_distill_scratch_bytes", "e3dgs_distill_forward", "e3dgs_distill_backward",
 ]

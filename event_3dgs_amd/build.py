@@ -9,7 +9,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "build")
 OUT = os.path.join(HERE, "libe3dgs_hip.so")
-SOURCES = ["capi.hip", "forward.hip", "backward.hip", "scan_sort.hip", "aux.hip", "densify.hip"]
+SOURCES = ["capi.hip", "forward.hip", "backward.hip", "scan_sort.hip", "aux.hip", "densify.hip", "features.hip",
+           "distill.hip"]
 # -ffp-contract=off is part of the arithmetic contract (bit-exact forward vs the oracle):
 # only explicit FMA() fuses.  (No float atomics anywhere in the library.)
 # -fno-slp-vectorize: the SLP pass pairs scalar fp32 ops into v_pk_* instructions (1.7x the issue cost of one op) and pays
@@ -22,7 +23,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fn
 def build(force=False, verbose=False):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     sources = [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
-    headers = [os.path.join(CSRC, "common.h"), os.path.join(HERE, "..", "include", "e3dgs_hip.h")]
+    headers = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "rows.h"), os.path.join(HERE, "..", "include", "e3dgs_hip.h")]
     hdr_time = max(os.path.getmtime(h) for h in headers)
     os.makedirs(OBJ, exist_ok=True)
     jobs, objs = [], []
@@ -37,7 +38,7 @@ def build(force=False, verbose=False):
             print(" ".join(cmd))
         subprocess.check_call(cmd)
     if jobs:
-        with ThreadPoolExecutor(max_workers=min(len(jobs), 6)) as ex:
+        with ThreadPoolExecutor(max_workers=min(len(jobs), 8)) as ex:
             list(ex.map(run, jobs))
     if jobs or not os.path.exists(OUT) or os.path.getmtime(OUT) < max(os.path.getmtime(o) for o in objs):
         run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", OUT] + objs)
@@ -49,7 +50,7 @@ def status():
     relinked, modification time of the library).  smoke() prints it on the GPU box, so that the driver's records say whether
     the box ran the binaries that travelled with the tree or rebuilt them."""
     sources = [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
-    headers = [os.path.join(CSRC, "common.h"), os.path.join(HERE, "..", "include", "e3dgs_hip.h")]
+    headers = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "rows.h"), os.path.join(HERE, "..", "include", "e3dgs_hip.h")]
     hdr_time = max(os.path.getmtime(h) for h in headers)
     stale = []
     for src in sources:

@@ -113,6 +113,22 @@ void prof_end(int slot, int k, hipStream_t s) {
 int e3_mark_visible_impl(int, const float*, const float*, uint8_t*, hipStream_t);
 size_t e3_knn_scratch_bytes(int);
 int e3_knn_impl(int, const float*, float*, char*, hipStream_t);
+int e3_embedding_forward_impl(size_t, size_t, size_t, const void*, int, const void*, size_t, int, float, void*, hipStream_t);
+size_t e3_embedding_scratch_bytes(size_t, size_t);
+int e3_embedding_backward_impl(size_t, size_t, size_t, const void*, int, const void*, size_t, int, float, void*, char*,
+                               hipStream_t);
+int e3_layer_norm_forward_impl(size_t, size_t, const void*, size_t, int, const void*, const void*, int, float, void*, float*,
+                               float*, hipStream_t);
+size_t e3_layer_norm_scratch_bytes(size_t, size_t);
+int e3_layer_norm_backward_impl(size_t, size_t, const void*, size_t, const void*, size_t, int, const void*, int, const float*,
+                                const float*, void*, void*, void*, char*, hipStream_t);
+bool e3_distill_layout_ok(size_t, size_t, size_t, size_t);
+size_t e3_distill_scratch_bytes(size_t);
+int e3_distill_forward_impl(size_t, size_t, size_t, const void*, size_t, size_t, int, const void*, size_t, size_t, int,
+                            const void*, size_t, size_t, int, float, int, float*, float*, float*, char*, hipStream_t);
+int e3_distill_backward_impl(size_t, size_t, size_t, const void*, size_t, size_t, int, const void*, size_t, size_t, int,
+                             const void*, size_t, size_t, int, float, int, const float*, const float*, const float*, void*,
+                             size_t, size_t, hipStream_t);
 size_t e3_event_scratch_bytes(int, int);
 int e3_event_loss_impl(int, int, const float*, const float*, const float*, const float*, const float*, const float*,
                        const float*, const float*, float, float*, float*, float*, float*, char*, hipStream_t, float*, double*,
@@ -827,6 +843,123 @@ int e3dgs_sort_depth_keys(size_t n, uint32_t* keys0, uint32_t* keys1, uint32_t* 
         return e == hipSuccess ? 0 : e3_fail(e, "hipMemsetAsync(kept_count_dev)");
     }
     return launch_depth_sort_wide(keys0, keys1, order, order_alt, n, (uint32_t*)scratch, (hipStream_t)stream, kept_count_dev);
+}
+
+/* ---- rows of learned features (features.hip, distill.hip) */
+static int feature_args_fail(const char* who, size_t rows, size_t dim, int dtype, const char* extra) {
+    char text[200];
+    snprintf(text, sizeof text, "%s: %s (rows %zu, dim %zu, dtype %d)", who, extra, rows, dim, dtype);
+    return e3_fail(hipErrorInvalidValue, text);
+}
+int e3dgs_embedding_forward(size_t n, size_t rows, size_t dim, const void* index, int index_bytes, const void* table,
+                            size_t table_stride, int dtype, float scale, void* out, void* stream) {
+    g_err[0] = 0;
+    const char* who = "e3dgs_embedding_forward";
+    if (dim < 1 || dim > E3DGS_FEATURE_MAX_DIM || rows >= 0x7FFFFFFFull || n >= 0x7FFFFFFFull)
+        return feature_args_fail(who, rows, dim, dtype, "bad sizes");
+    if (dtype < E3DGS_F32 || dtype > E3DGS_BF16 || (index_bytes != 4 && index_bytes != 8))
+        return feature_args_fail(who, rows, dim, dtype, "bad element type");
+    if (n > 0 && (!index || !out || (rows > 0 && !table))) return feature_args_fail(who, rows, dim, dtype, "null pointer");
+    return e3_embedding_forward_impl(n, rows, dim, index, index_bytes, table, table_stride, dtype, scale, out,
+                                     (hipStream_t)stream);
+}
+size_t e3dgs_embedding_backward_scratch_bytes(size_t n, size_t rows, size_t dim) {
+    (void)rows;
+    return e3_embedding_scratch_bytes(n, dim);
+}
+int e3dgs_embedding_backward(size_t n, size_t rows, size_t dim, const void* index, int index_bytes, const void* grad_out,
+                             size_t grad_stride, int dtype, float scale, void* grad_table, char* scratch, void* stream) {
+    g_err[0] = 0;
+    const char* who = "e3dgs_embedding_backward";
+    if (dim < 1 || dim > E3DGS_FEATURE_MAX_DIM || rows >= 0x7FFFFFFFull || n >= 0x7FFFFFFFull)
+        return feature_args_fail(who, rows, dim, dtype, "bad sizes");
+    if (dtype < E3DGS_F32 || dtype > E3DGS_BF16 || (index_bytes != 4 && index_bytes != 8))
+        return feature_args_fail(who, rows, dim, dtype, "bad element type");
+    if (rows == 0) return 0;
+    if (!grad_table || !scratch || (n > 0 && (!index || !grad_out))) return feature_args_fail(who, rows, dim, dtype, "null pointer");
+    if ((reinterpret_cast<uintptr_t>(scratch) & 255) != 0) return feature_args_fail(who, rows, dim, dtype, "scratch must be 256-byte aligned");
+    return e3_embedding_backward_impl(n, rows, dim, index, index_bytes, grad_out, grad_stride, dtype, scale, grad_table,
+                                      scratch, (hipStream_t)stream);
+}
+int e3dgs_layer_norm_forward(size_t rows, size_t dim, const void* x, size_t x_stride, int dtype, const void* weight,
+                             const void* bias, int affine_dtype, float eps, void* out, float* mean, float* rstd,
+                             void* stream) {
+    g_err[0] = 0;
+    const char* who = "e3dgs_layer_norm_forward";
+    if (dim < 1 || dim > E3DGS_FEATURE_MAX_DIM || !(eps >= 0.0f))
+        return feature_args_fail(who, rows, dim, dtype, "bad sizes or eps");
+    if (dtype < E3DGS_F32 || dtype > E3DGS_BF16 || affine_dtype < E3DGS_F32 || affine_dtype > E3DGS_BF16)
+        return feature_args_fail(who, rows, dim, dtype, "bad element type");
+    if (rows > 0 && (!x || !out)) return feature_args_fail(who, rows, dim, dtype, "null pointer");
+    return e3_layer_norm_forward_impl(rows, dim, x, x_stride, dtype, weight, bias, affine_dtype, eps, out, mean, rstd,
+                                      (hipStream_t)stream);
+}
+size_t e3dgs_layer_norm_backward_scratch_bytes(size_t rows, size_t dim) { return e3_layer_norm_scratch_bytes(rows, dim); }
+int e3dgs_layer_norm_backward(size_t rows, size_t dim, const void* grad_out, size_t grad_stride, const void* x,
+                              size_t x_stride, int dtype, const void* weight, int affine_dtype, const float* mean,
+                              const float* rstd, void* grad_x, void* grad_weight, void* grad_bias, char* scratch,
+                              void* stream) {
+    g_err[0] = 0;
+    const char* who = "e3dgs_layer_norm_backward";
+    if (dim < 1 || dim > E3DGS_FEATURE_MAX_DIM)
+        return feature_args_fail(who, rows, dim, dtype, "bad sizes");
+    if (dtype < E3DGS_F32 || dtype > E3DGS_BF16 || affine_dtype < E3DGS_F32 || affine_dtype > E3DGS_BF16)
+        return feature_args_fail(who, rows, dim, dtype, "bad element type");
+    if (rows > 0 && (!x || !grad_out || !mean || !rstd)) return feature_args_fail(who, rows, dim, dtype, "null pointer");
+    if ((grad_weight || grad_bias) && !scratch) return feature_args_fail(who, rows, dim, dtype, "null pointer");
+    if (!grad_x && !grad_weight && !grad_bias) return 0;
+    return e3_layer_norm_backward_impl(rows, dim, grad_out, grad_stride, x, x_stride, dtype, weight, affine_dtype, mean,
+                                       rstd, grad_x, grad_weight, grad_bias, scratch, (hipStream_t)stream);
+}
+size_t e3dgs_distill_scratch_bytes(size_t rows) { return e3_distill_scratch_bytes(rows); }
+static int distill_args(const char* who, size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride,
+                        size_t class_stride, int dtype, const void* teacher, int teacher_dtype, const void* index,
+                        int index_bytes, float temperature, int reduction) {
+    if (classes < 1 || classes >= 0x7FFFFFFFull || k < 1 || k > E3DGS_DISTILL_MAX_K || rows >= 0x7FFFFFFFull)
+        return feature_args_fail(who, rows, classes, dtype, "bad sizes");
+    if (!(temperature > 0.0f) || temperature > 1e30f || reduction < 0 || reduction > 2)
+        return feature_args_fail(who, rows, classes, dtype, "bad temperature or reduction");
+    if (dtype < E3DGS_F32 || dtype > E3DGS_BF16 || teacher_dtype < E3DGS_F32 || teacher_dtype > E3DGS_BF16 ||
+        (index_bytes != 4 && index_bytes != 8))
+        return feature_args_fail(who, rows, classes, dtype, "bad element type");
+    if (rows > 0 && (!logits || !teacher || !index)) return feature_args_fail(who, rows, classes, dtype, "null pointer");
+    if (!e3_distill_layout_ok(rows, classes, row_stride, class_stride))
+        return feature_args_fail(who, rows, classes, dtype, "neither rows of classes nor at most 256 planes");
+    return 0;
+}
+int e3dgs_distill_forward(size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride, size_t class_stride,
+                          int dtype, const void* teacher, size_t teacher_row_stride, size_t teacher_entry_stride,
+                          int teacher_dtype, const void* index, size_t index_row_stride, size_t index_entry_stride,
+                          int index_bytes, float temperature, int reduction, float* stats, float* row_loss, float* loss,
+                          char* scratch, void* stream) {
+    g_err[0] = 0;
+    const int rc = distill_args("e3dgs_distill_forward", rows, classes, k, logits, row_stride, class_stride, dtype, teacher,
+                                teacher_dtype, index, index_bytes, temperature, reduction);
+    if (rc) return rc;
+    if (!loss || (rows > 0 && (!stats || !scratch)))
+        return feature_args_fail("e3dgs_distill_forward", rows, classes, dtype, "null pointer");
+    return e3_distill_forward_impl(rows, classes, k, logits, row_stride, class_stride, dtype, teacher, teacher_row_stride,
+                                   teacher_entry_stride, teacher_dtype, index, index_row_stride, index_entry_stride,
+                                   index_bytes, temperature, reduction, stats, row_loss, loss, scratch, (hipStream_t)stream);
+}
+int e3dgs_distill_backward(size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride, size_t class_stride,
+                           int dtype, const void* teacher, size_t teacher_row_stride, size_t teacher_entry_stride,
+                           int teacher_dtype, const void* index, size_t index_row_stride, size_t index_entry_stride,
+                           int index_bytes, float temperature, int reduction, const float* stats, const float* loss,
+                           const float* d_loss, void* grad, size_t grad_row_stride, size_t grad_class_stride, void* stream) {
+    g_err[0] = 0;
+    const char* who = "e3dgs_distill_backward";
+    const int rc = distill_args(who, rows, classes, k, logits, row_stride, class_stride, dtype, teacher, teacher_dtype, index,
+                                index_bytes, temperature, reduction);
+    if (rc) return rc;
+    if (rows > 0 && (!stats || !loss || !grad)) return feature_args_fail(who, rows, classes, dtype, "null pointer");
+    if (!e3_distill_layout_ok(rows, classes, grad_row_stride, grad_class_stride) ||
+        (grad_class_stride == 1) != (class_stride == 1))
+        return feature_args_fail(who, rows, classes, dtype, "the gradient's layout differs from the scores'");
+    return e3_distill_backward_impl(rows, classes, k, logits, row_stride, class_stride, dtype, teacher, teacher_row_stride,
+                                    teacher_entry_stride, teacher_dtype, index, index_row_stride, index_entry_stride,
+                                    index_bytes, temperature, reduction, stats, loss, d_loss, grad, grad_row_stride,
+                                    grad_class_stride, (hipStream_t)stream);
 }
 
 extern unsigned long long* g_trace;

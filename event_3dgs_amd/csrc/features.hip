@@ -1,0 +1,798 @@
+// features.hip -- rows of learned features: lookup in a shared table with the gradient by sorted index, layer norm.
+//
+// Both are bound by memory: a value is touched by a handful of operations, so the kernels are laid out for 16-byte packs,
+// few passes over the data and enough bytes in flight.  All sums run in fp32 and in an order that depends on the sizes
+// alone (no floating-point atomics): results are the same bit for bit from call to call.
+#include "rows.h"
+
+int e3_fail(hipError_t e, const char* what);
+int launch_radix_sort_pairs(uint32_t* k0, uint32_t* k1, uint32_t* v0, uint32_t* v1, size_t n, int nbits,
+                            uint32_t* scratch, uint32_t** keys_out, uint32_t** vals_out, hipStream_t s,
+                            bool identity_payload, uint32_t* drop_count_dev, const uint32_t* n_dev, uint2* ranges_out,
+                            uint32_t nranges, uint32_t* lpt_cnt, uint32_t* lpt_list);
+#define LAUNCH_OK(name)                                       \
+    do {                                                      \
+        hipError_t _e = hipGetLastError();                    \
+        if (_e != hipSuccess) return e3_fail(_e, name);       \
+    } while (0)
+
+// ============================================================================================== embedding, forward
+// out[i, :] = round(scale * table[index[i], :]).  An index below 0 stands for "no row" (zeros); one past the table gives a
+// row of NaN -- an error that only the device sees, made visible without a wait.
+// One thread moves EMBED_PACKS packs of the flat output, a workgroup's packs are contiguous: every lane works whatever the
+// row length, the stores are whole lines, and the rows of a pack-block are found by one division each.
+constexpr int EMBED_PACKS = 4;
+template <typename T, int V>
+__global__ __launch_bounds__(256) void embed_fwd_kernel(size_t n, long long rows, uint32_t ppr /* packs per row */,
+                                                        const void* __restrict__ index, int index_bytes,
+                                                        const T* __restrict__ table, size_t stride, float scale,
+                                                        T* __restrict__ out) {
+    const size_t total = n * (size_t)ppr, base = (size_t)blockIdx.x * (256 * EMBED_PACKS);
+    const size_t row0 = base / ppr;                                  // (uniform)
+    const uint32_t rem0 = (uint32_t)(base - row0 * ppr);
+    long long id[EMBED_PACKS];
+    uint32_t col[EMBED_PACKS];
+    Pack<T, V> p[EMBED_PACKS];
+#pragma unroll
+    for (int u = 0; u < EMBED_PACKS; ++u) {
+        const uint32_t x = rem0 + (uint32_t)u * 256 + threadIdx.x, q = x / ppr;
+        col[u] = x - q * ppr;
+        const bool ok = base + (size_t)u * 256 + threadIdx.x < total;
+        id[u] = ok ? load_index(index, row0 + q, index_bytes) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < EMBED_PACKS; ++u) {
+        if (id[u] >= 0 && id[u] < rows)
+            p[u] = *reinterpret_cast<const Pack<T, V>*>(table + (size_t)id[u] * stride + (size_t)col[u] * V);
+    }
+#pragma unroll
+    for (int u = 0; u < EMBED_PACKS; ++u) {
+        const size_t at = base + (size_t)u * 256 + threadIdx.x;
+        if (at >= total) continue;
+        Pack<T, V> r;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            r.v[j] = id[u] < 0 ? (T)0.0f : (id[u] < rows ? (T)(scale * (float)p[u].v[j]) : (T)__builtin_nanf(""));
+        reinterpret_cast<Pack<T, V>*>(out)[at] = r;
+    }
+}
+
+template <typename T>
+static int embed_fwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_bytes, const void* table,
+                       size_t stride, int dtype, float scale, void* out, hipStream_t s) {
+    const bool wide = e3_rows_wide(table, stride, dim, dtype) && e3_rows_wide(out, dim, dim, dtype);
+    const size_t ppr = wide ? dim / Wide<T>::N : dim;
+    const size_t blocks = (n * ppr + 256 * EMBED_PACKS - 1) / (256 * EMBED_PACKS);
+    if (blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_forward: too many values");
+    if (wide)
+        embed_fwd_kernel<T, Wide<T>::N><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(
+            n, (long long)rows, (uint32_t)ppr, index, index_bytes, (const T*)table, stride, scale, (T*)out);
+    else
+        embed_fwd_kernel<T, 1><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(
+            n, (long long)rows, (uint32_t)ppr, index, index_bytes, (const T*)table, stride, scale, (T*)out);
+    LAUNCH_OK("embed_fwd_kernel");
+    return 0;
+}
+
+int e3_embedding_forward_impl(size_t n, size_t rows, size_t dim, const void* index, int index_bytes, const void* table,
+                              size_t stride, int dtype, float scale, void* out, hipStream_t s) {
+    if (n == 0) return 0;
+    if (dtype == E3_F32) return embed_fwd_t<float>(n, rows, dim, index, index_bytes, table, stride, dtype, scale, out, s);
+    if (dtype == E3_F16) return embed_fwd_t<f16_t>(n, rows, dim, index, index_bytes, table, stride, dtype, scale, out, s);
+    return embed_fwd_t<bf16_t>(n, rows, dim, index, index_bytes, table, stride, dtype, scale, out, s);
+}
+
+// ============================================================================================== embedding, gradient
+// d_table[v, :] = round(scale * sum of d_out[i, :] over the positions i with index[i] == v, in the order of i).
+// The positions are sorted by index (stable), so that a row's positions are one run of the sorted list; the list is cut
+// into chunks of equal length, a group of lanes sums the rows of one chunk (times a slice of the columns), and
+//   * a run inside a chunk is finished there,
+//   * a run that crosses chunks leaves one fp32 partial row per chunk, which embed_join_kernel adds up in order,
+//   * a table row without a position is cleared by embed_zero_kernel.
+// So a row that half of all positions share costs no more than rows with one position each.
+constexpr uint32_t EMBED_NONE = 0xFFFFFFFFu;
+
+__global__ __launch_bounds__(256) void embed_keys_kernel(size_t n, unsigned long long rows, const void* __restrict__ index,
+                                                         int index_bytes, uint32_t* __restrict__ keys) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const unsigned long long id = (unsigned long long)load_index(index, i, index_bytes);   // (negative: beyond any row)
+    keys[i] = id < rows ? (uint32_t)id : EMBED_NONE;
+}
+
+// first position of the sorted keys [lo, hi) that holds a key >= k
+__device__ __forceinline__ uint32_t lower_bound_u32(const uint32_t* __restrict__ keys, uint32_t lo, uint32_t hi, uint32_t k) {
+    while (lo < hi) {
+        const uint32_t mid = lo + ((hi - lo) >> 1);
+        if (keys[mid] < k) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void embed_store(T* __restrict__ d_table, size_t dim, uint32_t row, size_t col, float scale,
+                                            const float acc[V]) {
+    Pack<T, V> r;
+#pragma unroll
+    for (int j = 0; j < V; ++j) r.v[j] = (T)(scale * acc[j]);
+    *reinterpret_cast<Pack<T, V>*>(d_table + (size_t)row * dim + col) = r;
+}
+
+constexpr int EMBED_UNROLL = 8;
+template <typename T, int V, int G>
+__global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restrict__ kept, const uint32_t* __restrict__ keys,
+                                                        const uint32_t* __restrict__ pos, uint32_t chunk, uint32_t nchunks,
+                                                        uint32_t nslices, size_t dim, const T* __restrict__ d_out,
+                                                        size_t stride, float scale, T* __restrict__ d_table,
+                                                        float* __restrict__ part) {
+    const size_t unit = (size_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const uint32_t c = (uint32_t)(unit / nslices), slice = (uint32_t)(unit - (size_t)c * nslices);
+    const size_t col = ((size_t)slice * G + threadIdx.x % G) * V;
+    const uint32_t n = *kept;
+    if (c >= nchunks || (size_t)c * chunk >= n || col >= dim) return;
+    const uint32_t j0 = c * chunk, j1 = n - j0 < chunk ? n : j0 + chunk;
+    float acc[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = 0.0f;
+    uint32_t cur = keys[j0];
+    bool from_before = j0 > 0 && keys[j0 - 1] == cur;       // the run in hand began in an earlier chunk
+    for (uint32_t b = j0; b < j1; b += EMBED_UNROLL) {
+        uint32_t k[EMBED_UNROLL];
+        Pack<T, V> r[EMBED_UNROLL];
+#pragma unroll
+        for (int u = 0; u < EMBED_UNROLL; ++u) {            // (entries behind the chunk read its last one and are not added)
+            const uint32_t at = b + u < j1 ? b + u : j1 - 1;
+            k[u] = keys[at];
+            r[u] = *reinterpret_cast<const Pack<T, V>*>(d_out + (size_t)pos[at] * stride + col);
+        }
+#pragma unroll
+        for (int u = 0; u < EMBED_UNROLL; ++u) {
+            if (b + u >= j1) break;
+            if (k[u] != cur) {
+                if (from_before) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) part[(size_t)(2 * c) * dim + col + j] = acc[j];
+                } else {
+                    embed_store<T, V>(d_table, dim, cur, col, scale, acc);
+                }
+                from_before = false;
+                cur = k[u];
+#pragma unroll
+                for (int j = 0; j < V; ++j) acc[j] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] += (float)r[u].v[j];
+        }
+    }
+    const bool goes_on = j1 < n && keys[j1] == cur;
+    if (from_before || goes_on) {
+        const size_t slot = from_before ? 2 * (size_t)c : 2 * (size_t)c + 1;
+#pragma unroll
+        for (int j = 0; j < V; ++j) part[slot * dim + col + j] = acc[j];
+    } else {
+        embed_store<T, V>(d_table, dim, cur, col, scale, acc);
+    }
+}
+
+// One workgroup per chunk (times a slice of 64 columns): if a run starts in the chunk and goes on behind it, add its
+// partials: slot 1 of this chunk, slot 0 of the following ones up to the run's end.  Wave w takes the w-th sixteenth of
+// them, the sixteen sums are added in order.
+template <typename T>
+__global__ __launch_bounds__(1024) void embed_join_kernel(const uint32_t* __restrict__ kept,
+                                                          const uint32_t* __restrict__ keys, uint32_t chunk, size_t dim,
+                                                          const float* __restrict__ part, float scale,
+                                                          T* __restrict__ d_table) {
+    __shared__ float sums[16][64];
+    const uint32_t n = *kept, c = blockIdx.x;
+    if ((size_t)(c + 1) * chunk >= n) return;                            // nothing lies behind the chunk (uniform)
+    const uint32_t j0 = c * chunk, j1 = j0 + chunk, key = keys[j1 - 1];
+    if (keys[j1] != key) return;                                         // no run goes on (uniform)
+    if (keys[j0] == key && j0 > 0 && keys[j0 - 1] == key) return;        // it began earlier: an earlier chunk adds it up
+    const uint32_t end = lower_bound_u32(keys, j1, n, key + 1u);         // (key < rows <= 2^32 - 2)
+    const uint32_t last = (end - 1u) / chunk, m = last - c + 1u;         // m partials
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const size_t col = (size_t)blockIdx.y * 64 + lane;
+    const uint32_t lo = (uint32_t)((unsigned long long)m * wave / 16), hi = (uint32_t)((unsigned long long)m * (wave + 1) / 16);
+    float s = 0.0f;
+    if (col < dim) {
+#pragma unroll 8
+        for (uint32_t k = lo; k < hi; ++k) s += part[(k == 0 ? 2 * (size_t)c + 1 : 2 * (size_t)(c + k)) * dim + col];
+    }
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && col < dim) {
+        s = sums[0][lane];
+#pragma unroll
+        for (int w = 1; w < 16; ++w) s += sums[w][lane];
+        d_table[(size_t)key * dim + col] = (T)(scale * s);
+    }
+}
+
+// Clears the table rows without a position: a wave looks `per` rows up in the sorted keys (one lane each) and clears those
+// that are not there.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void embed_zero_kernel(const uint32_t* __restrict__ kept, const uint32_t* __restrict__ keys,
+                                                         uint32_t rows, uint32_t per, size_t dim, T* __restrict__ d_table) {
+    const int lane = threadIdx.x & 63;
+    const size_t first = ((size_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * per;
+    if (first >= rows) return;
+    const uint32_t n = *kept;
+    bool empty = false;
+    if ((uint32_t)lane < per && first + lane < rows) {
+        const uint32_t row = (uint32_t)(first + lane), at = lower_bound_u32(keys, 0, n, row);
+        empty = at >= n || keys[at] != row;
+    }
+    unsigned long long todo = __ballot(empty);
+    Pack<T, V> z;
+#pragma unroll
+    for (int j = 0; j < V; ++j) z.v[j] = (T)0.0f;
+    while (todo) {
+        const int r = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        T* row = d_table + (first + r) * dim;
+        for (size_t col = (size_t)lane * V; col < dim; col += 64 * V) *reinterpret_cast<Pack<T, V>*>(row + col) = z;
+    }
+}
+
+namespace {
+struct EmbedScratch {
+    uint32_t *key0, *key1, *pos0, *pos1, *kept, *sort;
+    float* part;
+    static uint32_t chunk(size_t n, size_t dim) {
+        // Rows of a chunk: 64 where there is plenty of work, fewer where the groups would otherwise not fill the chip (each
+        // group moves `chunk` row slices of at most 1 KB).
+        uint32_t c = 64;
+        while (c > 8 && (n / c) * ((dim + 511) / 512) < 4096) c >>= 1;
+        return c;
+    }
+    static uint32_t chunks(size_t n, size_t dim) { return (uint32_t)((n + chunk(n, dim) - 1) / chunk(n, dim)); }
+    static EmbedScratch from(char*& p, size_t n, size_t dim) {
+        EmbedScratch s;
+        const size_t m = n ? n : 1;
+        s.key0 = carve<uint32_t>(p, m);
+        s.key1 = carve<uint32_t>(p, m);
+        s.pos0 = carve<uint32_t>(p, m);
+        s.pos1 = carve<uint32_t>(p, m);
+        s.kept = carve<uint32_t>(p, 1);
+        s.sort = carve<uint32_t>(p, sort_scratch_words(m));
+        s.part = carve<float>(p, 2 * (size_t)chunks(m, dim) * dim);
+        return s;
+    }
+};
+
+template <typename T, int V, int G>
+int embed_sum_launch(const EmbedScratch& w, const uint32_t* keys, const uint32_t* pos, size_t n, size_t dim,
+                     const void* d_out, size_t stride, float scale, void* d_table, hipStream_t s) {
+    const uint32_t chunk = EmbedScratch::chunk(n, dim), nchunks = EmbedScratch::chunks(n, dim);
+    const size_t nslices = (dim + (size_t)G * V - 1) / ((size_t)G * V), units = nslices * nchunks;
+    const size_t blocks = (units + 256 / G - 1) / (256 / G);
+    if (blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
+    embed_sum_kernel<T, V, G><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(w.kept, keys, pos, chunk, nchunks,
+                                                                          (uint32_t)nslices, dim, (const T*)d_out, stride,
+                                                                          scale, (T*)d_table, w.part);
+    LAUNCH_OK("embed_sum_kernel");
+    return 0;
+}
+
+template <typename T>
+int embed_bwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_bytes, const void* d_out, size_t stride,
+                int dtype, float scale, void* d_table, char* scratch, hipStream_t s) {
+    EmbedScratch w = EmbedScratch::from(scratch, n, dim);
+    uint32_t *keys = w.key0, *pos = w.pos0;
+    embed_keys_kernel<<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s>>>(n, rows, index, index_bytes, w.key0);
+    LAUNCH_OK("embed_keys_kernel");
+    int nbits = 1;
+    while (nbits < 32 && (rows - 1) >> nbits) ++nbits;
+    int rc = launch_radix_sort_pairs(w.key0, w.key1, w.pos0, w.pos1, n, nbits, w.sort, &keys, &pos, s, true, w.kept, nullptr,
+                                     nullptr, 0, nullptr, nullptr);
+    if (rc) return rc;
+    const bool wide = e3_rows_wide(d_out, stride, dim, dtype) && e3_rows_wide(d_table, dim, dim, dtype);
+    const size_t packs = wide ? dim / Wide<T>::N : dim;
+    constexpr int N = Wide<T>::N;
+#define E3_SUM(V, G) rc = embed_sum_launch<T, V, G>(w, keys, pos, n, dim, d_out, stride, scale, d_table, s)
+    if (wide) {
+        if (packs <= 4) E3_SUM(N, 4);
+        else if (packs <= 8) E3_SUM(N, 8);
+        else if (packs <= 16) E3_SUM(N, 16);
+        else if (packs <= 32) E3_SUM(N, 32);
+        else E3_SUM(N, 64);
+    } else {
+        if (packs <= 4) E3_SUM(1, 4);
+        else if (packs <= 16) E3_SUM(1, 16);
+        else E3_SUM(1, 64);
+    }
+#undef E3_SUM
+    if (rc) return rc;
+    const uint32_t chunk = EmbedScratch::chunk(n, dim), nchunks = EmbedScratch::chunks(n, dim);
+    if (nchunks > 1) {
+        embed_join_kernel<T><<<dim3(nchunks - 1, (unsigned)((dim + 63) / 64)), dim3(1024), 0, s>>>(
+            w.kept, keys, chunk, dim, w.part, scale, (T*)d_table);
+        LAUNCH_OK("embed_join_kernel");
+    }
+    // about 16 KB of table rows to a wave
+    size_t per = 16384 / (dim * sizeof(T));
+    per = per < 1 ? 1 : (per > 64 ? 64 : per);
+    const size_t zb = (rows + 4 * per - 1) / (4 * per);
+    if (e3_rows_wide(d_table, dim, dim, dtype))
+        embed_zero_kernel<T, N><<<dim3((unsigned)zb), dim3(256), 0, s>>>(w.kept, keys, (uint32_t)rows, (uint32_t)per, dim, (T*)d_table);
+    else
+        embed_zero_kernel<T, 1><<<dim3((unsigned)zb), dim3(256), 0, s>>>(w.kept, keys, (uint32_t)rows, (uint32_t)per, dim, (T*)d_table);
+    LAUNCH_OK("embed_zero_kernel");
+    return 0;
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void fill_zero_kernel(size_t packs, Pack<T, V>* __restrict__ out) {
+    Pack<T, V> z;
+#pragma unroll
+    for (int j = 0; j < V; ++j) z.v[j] = (T)0.0f;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < packs; i += (size_t)gridDim.x * 256) out[i] = z;
+}
+}  // namespace
+
+size_t e3_embedding_scratch_bytes(size_t n, size_t dim) {
+    char* p = nullptr;
+    EmbedScratch::from(p, n, dim);
+    return (size_t)p + 256;
+}
+
+int e3_embedding_backward_impl(size_t n, size_t rows, size_t dim, const void* index, int index_bytes, const void* d_out,
+                               size_t stride, int dtype, float scale, void* d_table, char* scratch, hipStream_t s) {
+    if (n == 0) {
+        // no positions: clear the table's gradient with a kernel (a captured memset is not repeatable on every replay)
+        const size_t bytes = rows * dim * e3_elem_bytes(dtype);
+        const size_t blocks = (bytes / 2 + 255) / 256;
+        fill_zero_kernel<f16_t, 1><<<dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s>>>(
+            bytes / 2, (Pack<f16_t, 1>*)d_table);
+        LAUNCH_OK("fill_zero_kernel");
+        return 0;
+    }
+    if (dtype == E3_F32) return embed_bwd_t<float>(n, rows, dim, index, index_bytes, d_out, stride, dtype, scale, d_table, scratch, s);
+    if (dtype == E3_F16) return embed_bwd_t<f16_t>(n, rows, dim, index, index_bytes, d_out, stride, dtype, scale, d_table, scratch, s);
+    return embed_bwd_t<bf16_t>(n, rows, dim, index, index_bytes, d_out, stride, dtype, scale, d_table, scratch, s);
+}
+
+// ============================================================================================== layer norm
+// y = (x - mean) * rstd * weight + bias per row, mean and rstd = 1 / sqrt(var + eps) in fp32.  A row stays in the registers
+// of its lanes between the statistics and the output (one pass over memory); the variance is the mean square of
+// x - mean, not a difference of sums, so a row far from zero keeps its digits.
+// Lanes per row: a group of 8 .. 64 lanes of one wave, or a workgroup of 256 threads for long rows (NormRow).
+template <int G>
+struct NormRow {      // sums over the lanes of a row
+    static constexpr int THREADS = G > 256 ? G : 256;
+    static constexpr int PER_BLOCK = THREADS / G;
+    static __device__ __forceinline__ float sum(float v, float* lds) {
+        if (G <= 64) return group_sum<(G <= 64 ? G : 64)>(v);
+        v = group_sum<64>(v);
+        const int wave = threadIdx.x >> 6;
+        __syncthreads();                                    // (the previous use of `lds` has been read)
+        if ((threadIdx.x & 63) == 0) lds[wave] = v;
+        __syncthreads();
+        float t = lds[0];
+#pragma unroll
+        for (int w = 1; w < THREADS / 64; ++w) t += lds[w];
+        return t;
+    }
+};
+
+template <typename T, int V, int G, int ITEMS>
+__global__ __launch_bounds__(NormRow<G>::THREADS) void norm_fwd_kernel(size_t rows, int dim, const T* __restrict__ x,
+                                                                       size_t stride, const void* __restrict__ weight,
+                                                                       const void* __restrict__ bias, int affine_dtype,
+                                                                       float eps, T* __restrict__ out,
+                                                                       float* __restrict__ mean_out,
+                                                                       float* __restrict__ rstd_out) {
+    using R = NormRow<G>;
+    __shared__ float lds[16];
+    const int lane = threadIdx.x % G;
+    float w[ITEMS][V], b[ITEMS][V];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int col = (i * G + lane) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            w[i][j] = weight && col < dim ? load_elem(weight, col + j, affine_dtype) : 1.0f;
+            b[i][j] = bias && col < dim ? load_elem(bias, col + j, affine_dtype) : 0.0f;
+        }
+    }
+    const float inv = 1.0f / (float)dim;
+    const size_t step = (size_t)gridDim.x * R::PER_BLOCK;
+    // (every lane of a wave, and every wave of a workgroup that shares a row, runs the same number of rounds)
+    for (size_t base = (size_t)blockIdx.x * R::PER_BLOCK; base < rows; base += step) {
+        const size_t row = base + threadIdx.x / G;
+        const bool live = row < rows;
+        float v[ITEMS][V], s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int col = (i * G + lane) * V;
+            if (live && col < dim) {
+                const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(x + row * stride + col);
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[i][j] = (float)p.v[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j) s += v[i][j];
+        }
+        const float mean = R::sum(s, lds) * inv;
+        float q = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int col = (i * G + lane) * V;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                v[i][j] -= mean;
+                if (col < dim) q = FMA(v[i][j], v[i][j], q);
+            }
+        }
+        const float rstd = 1.0f / __builtin_sqrtf(FMA(R::sum(q, lds), inv, eps));
+        if (!live) continue;
+        if (lane == 0) {
+            if (mean_out) mean_out[row] = mean;
+            if (rstd_out) rstd_out[row] = rstd;
+        }
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int col = (i * G + lane) * V;
+            if (col >= dim) continue;
+            Pack<T, V> r;
+#pragma unroll
+            for (int j = 0; j < V; ++j) r.v[j] = (T)FMA(v[i][j] * rstd, w[i][j], b[i][j]);
+            *reinterpret_cast<Pack<T, V>*>(out + row * (size_t)dim + col) = r;
+        }
+    }
+}
+
+// Rows longer than the registers of a workgroup hold: the row is read three times (the second and third time from cache).
+template <typename T, int V>
+__global__ __launch_bounds__(1024) void norm_fwd_long_kernel(size_t rows, size_t dim, const T* __restrict__ x, size_t stride,
+                                                             const void* __restrict__ weight, const void* __restrict__ bias,
+                                                             int affine_dtype, float eps, T* __restrict__ out,
+                                                             float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+    using R = NormRow<1024>;
+    __shared__ float lds[16];
+    const float inv = 1.0f / (float)dim;
+    for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T* xr = x + row * stride;
+        float s = 0.0f;
+        for (size_t col = (size_t)threadIdx.x * V; col < dim; col += 1024 * V) {
+            const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(xr + col);
+#pragma unroll
+            for (int j = 0; j < V; ++j) s += (float)p.v[j];
+        }
+        const float mean = R::sum(s, lds) * inv;
+        float q = 0.0f;
+        for (size_t col = (size_t)threadIdx.x * V; col < dim; col += 1024 * V) {
+            const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(xr + col);
+#pragma unroll
+            for (int j = 0; j < V; ++j) { const float d = (float)p.v[j] - mean; q = FMA(d, d, q); }
+        }
+        const float rstd = 1.0f / __builtin_sqrtf(FMA(R::sum(q, lds), inv, eps));
+        if (threadIdx.x == 0) {
+            if (mean_out) mean_out[row] = mean;
+            if (rstd_out) rstd_out[row] = rstd;
+        }
+        for (size_t col = (size_t)threadIdx.x * V; col < dim; col += 1024 * V) {
+            const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(xr + col);
+            Pack<T, V> r;
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                r.v[j] = (T)FMA(((float)p.v[j] - mean) * rstd, weight ? load_elem(weight, col + j, affine_dtype) : 1.0f,
+                                bias ? load_elem(bias, col + j, affine_dtype) : 0.0f);
+            *reinterpret_cast<Pack<T, V>*>(out + row * dim + col) = r;
+        }
+    }
+}
+
+// Gradient.  With h = (x - mean) * rstd and g = dy * weight:  dx = rstd * (g - mean(g) - h * mean(g h)),
+// dweight = sum over the rows of dy h, dbias = sum of dy.  The column sums stay in registers while a workgroup walks over
+// its rows, are added up over the workgroup's groups in LDS, and leave one fp32 row pair per workgroup, which
+// norm_join_kernel adds up.
+template <typename T, int V, int G, int ITEMS>
+__global__ __launch_bounds__(NormRow<G>::THREADS) void norm_bwd_kernel(size_t rows, int dim, const T* __restrict__ dy,
+                                                                       size_t dy_stride, const T* __restrict__ x,
+                                                                       size_t stride, const void* __restrict__ weight,
+                                                                       int affine_dtype, const float* __restrict__ mean_in,
+                                                                       const float* __restrict__ rstd_in,
+                                                                       T* __restrict__ dx, float* __restrict__ part) {
+    using R = NormRow<G>;
+    __shared__ float lds[16];
+    __shared__ float cols[R::PER_BLOCK > 1 ? R::THREADS * ITEMS * V : 1];
+    const int lane = threadIdx.x % G;
+    float w[ITEMS][V], dw[ITEMS][V], db[ITEMS][V];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int col = (i * G + lane) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            w[i][j] = weight && col < dim ? load_elem(weight, col + j, affine_dtype) : 1.0f;
+            dw[i][j] = db[i][j] = 0.0f;
+        }
+    }
+    const float inv = 1.0f / (float)dim;
+    const size_t step = (size_t)gridDim.x * R::PER_BLOCK;
+    for (size_t base = (size_t)blockIdx.x * R::PER_BLOCK; base < rows; base += step) {
+        const size_t row = base + threadIdx.x / G;
+        const bool live = row < rows;
+        const float mean = live ? mean_in[row] : 0.0f, rstd = live ? rstd_in[row] : 0.0f;
+        float h[ITEMS][V], g[ITEMS][V], s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int col = (i * G + lane) * V;
+            if (live && col < dim) {
+                const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(x + row * stride + col);
+                const Pack<T, V> d = *reinterpret_cast<const Pack<T, V>*>(dy + row * dy_stride + col);
+#pragma unroll
+                for (int j = 0; j < V; ++j) { h[i][j] = (float)p.v[j]; g[i][j] = (float)d.v[j]; }
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) { h[i][j] = mean; g[i][j] = 0.0f; }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                h[i][j] = (h[i][j] - mean) * rstd;
+                dw[i][j] = FMA(g[i][j], h[i][j], dw[i][j]);
+                db[i][j] += g[i][j];
+                g[i][j] *= w[i][j];
+                s1 += g[i][j];
+                s2 = FMA(g[i][j], h[i][j], s2);
+            }
+        s1 = R::sum(s1, lds) * inv;
+        s2 = R::sum(s2, lds) * inv;
+        if (!live || !dx) continue;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int col = (i * G + lane) * V;
+            if (col >= dim) continue;
+            Pack<T, V> r;
+#pragma unroll
+            for (int j = 0; j < V; ++j) r.v[j] = (T)((g[i][j] - s1 - h[i][j] * s2) * rstd);
+            *reinterpret_cast<Pack<T, V>*>(dx + row * (size_t)dim + col) = r;
+        }
+    }
+    if (!part) return;
+    float* mine = part + (size_t)blockIdx.x * 2 * dim;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        float(&a)[ITEMS][V] = which ? db : dw;
+        if (R::PER_BLOCK > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) cols[(threadIdx.x / G) * (G * ITEMS * V) + (i * G + lane) * V + j] = a[i][j];
+            __syncthreads();
+            for (int col = threadIdx.x; col < dim; col += R::THREADS) {
+                float s = cols[col];
+                for (int k = 1; k < R::PER_BLOCK; ++k) s += cols[k * (G * ITEMS * V) + col];
+                mine[which * (size_t)dim + col] = s;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int col = (i * G + lane) * V;
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (col < dim) mine[which * (size_t)dim + col + j] = a[i][j];
+            }
+        }
+    }
+}
+
+// dx of rows longer than the registers hold
+template <typename T, int V>
+__global__ __launch_bounds__(1024) void norm_bwd_long_kernel(size_t rows, size_t dim, const T* __restrict__ dy,
+                                                             size_t dy_stride, const T* __restrict__ x, size_t stride,
+                                                             const void* __restrict__ weight, int affine_dtype,
+                                                             const float* __restrict__ mean_in,
+                                                             const float* __restrict__ rstd_in, T* __restrict__ dx) {
+    using R = NormRow<1024>;
+    __shared__ float lds[16];
+    const float inv = 1.0f / (float)dim;
+    for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T *xr = x + row * stride, *dr = dy + row * dy_stride;
+        const float mean = mean_in[row], rstd = rstd_in[row];
+        float s1 = 0.0f, s2 = 0.0f;
+        for (size_t col = (size_t)threadIdx.x * V; col < dim; col += 1024 * V) {
+            const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(xr + col), d = *reinterpret_cast<const Pack<T, V>*>(dr + col);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float g = (float)d.v[j] * (weight ? load_elem(weight, col + j, affine_dtype) : 1.0f);
+                s1 += g;
+                s2 = FMA(g, ((float)p.v[j] - mean) * rstd, s2);
+            }
+        }
+        s1 = R::sum(s1, lds) * inv;
+        s2 = R::sum(s2, lds) * inv;
+        for (size_t col = (size_t)threadIdx.x * V; col < dim; col += 1024 * V) {
+            const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(xr + col), d = *reinterpret_cast<const Pack<T, V>*>(dr + col);
+            Pack<T, V> r;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float g = (float)d.v[j] * (weight ? load_elem(weight, col + j, affine_dtype) : 1.0f);
+                r.v[j] = (T)((g - s1 - ((float)p.v[j] - mean) * rstd * s2) * rstd);
+            }
+            *reinterpret_cast<Pack<T, V>*>(dx + row * dim + col) = r;
+        }
+    }
+}
+// ... and their column sums: a thread per column, a workgroup per 256 columns and slice of the rows
+template <typename T>
+__global__ __launch_bounds__(256) void norm_cols_kernel(size_t rows, size_t dim, const T* __restrict__ dy, size_t dy_stride,
+                                                        const T* __restrict__ x, size_t stride,
+                                                        const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
+                                                        float* __restrict__ part) {
+    const size_t col = (size_t)blockIdx.y * 256 + threadIdx.x;
+    if (col >= dim) return;
+    float dw = 0.0f, db = 0.0f;
+#pragma unroll 4
+    for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const float g = (float)dy[row * dy_stride + col];
+        dw = FMA(g, ((float)x[row * stride + col] - mean_in[row]) * rstd_in[row], dw);
+        db += g;
+    }
+    part[(size_t)blockIdx.x * 2 * dim + col] = dw;
+    part[(size_t)blockIdx.x * 2 * dim + dim + col] = db;
+}
+
+// dweight and dbias = sums over the workgroups' partial rows: 64 columns to a workgroup, wave w takes the w-th sixteenth of
+// the rows, the sixteen sums are added in order.
+__global__ __launch_bounds__(1024) void norm_join_kernel(uint32_t nparts, size_t dim, const float* __restrict__ part,
+                                                         int affine_dtype, void* __restrict__ dweight,
+                                                         void* __restrict__ dbias) {
+    __shared__ float sums[16][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const size_t col = (size_t)blockIdx.x * 64 + lane;                  // 0 .. 2 dim
+    const uint32_t lo = (uint32_t)((unsigned long long)nparts * wave / 16);
+    const uint32_t hi = (uint32_t)((unsigned long long)nparts * (wave + 1) / 16);
+    float s = 0.0f;
+    if (col < 2 * dim) {
+#pragma unroll 8
+        for (uint32_t k = lo; k < hi; ++k) s += part[(size_t)k * 2 * dim + col];
+    }
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave != 0 || col >= 2 * dim) return;
+    s = sums[0][lane];
+#pragma unroll
+    for (int w = 1; w < 16; ++w) s += sums[w][lane];
+    void* out = col < dim ? dweight : dbias;
+    if (!out) return;
+    const size_t at = col < dim ? col : col - dim;
+    if (affine_dtype == E3_F32) reinterpret_cast<float*>(out)[at] = s;
+    else if (affine_dtype == E3_F16) reinterpret_cast<f16_t*>(out)[at] = (f16_t)s;
+    else reinterpret_cast<bf16_t*>(out)[at] = (bf16_t)s;
+}
+
+namespace {
+// workgroups of a launch over `rows` rows: enough to fill 256 CUs several times over, each with a few rows of its own
+unsigned norm_blocks(size_t rows, int per_block, size_t most) {
+    const size_t need = (rows + per_block - 1) / per_block;
+    return (unsigned)(need < most ? need : most);
+}
+constexpr size_t NORM_FWD_BLOCKS = 4096, NORM_BWD_BLOCKS = 1024, NORM_LONG_PARTS = 64;
+
+struct NormArgs {
+    size_t rows, dim, x_stride, dy_stride;
+    const void *x, *dy, *weight, *bias;
+    int affine_dtype;
+    float eps;
+    void *out, *dx, *dweight, *dbias;
+    float *mean, *rstd, *part;
+    hipStream_t s;
+};
+
+template <typename T, int V, int G, int ITEMS>
+int norm_fwd_launch(const NormArgs& a) {
+    norm_fwd_kernel<T, V, G, ITEMS><<<dim3(norm_blocks(a.rows, NormRow<G>::PER_BLOCK, NORM_FWD_BLOCKS)),
+                                      dim3(NormRow<G>::THREADS), 0, a.s>>>(a.rows, (int)a.dim, (const T*)a.x, a.x_stride,
+                                                                         a.weight, a.bias, a.affine_dtype, a.eps, (T*)a.out,
+                                                                         a.mean, a.rstd);
+    LAUNCH_OK("norm_fwd_kernel");
+    return 0;
+}
+template <typename T, int V, int G, int ITEMS>
+int norm_bwd_launch(const NormArgs& a, uint32_t& nparts) {
+    nparts = norm_blocks(a.rows, NormRow<G>::PER_BLOCK, NORM_BWD_BLOCKS);
+    norm_bwd_kernel<T, V, G, ITEMS><<<dim3(nparts), dim3(NormRow<G>::THREADS), 0, a.s>>>(
+        a.rows, (int)a.dim, (const T*)a.dy, a.dy_stride, (const T*)a.x, a.x_stride, a.weight, a.affine_dtype, a.mean, a.rstd,
+        (T*)a.dx, a.part);
+    LAUNCH_OK("norm_bwd_kernel");
+    return 0;
+}
+template <typename T, int V>
+int norm_fwd_v(const NormArgs& a) {
+    const size_t packs = a.dim / V;
+    if (packs <= 8) return norm_fwd_launch<T, V, 8, 1>(a);
+    if (packs <= 16) return norm_fwd_launch<T, V, 16, 1>(a);
+    if (packs <= 32) return norm_fwd_launch<T, V, 32, 1>(a);
+    if (packs <= 64) return norm_fwd_launch<T, V, 64, 1>(a);
+    if (packs <= 128) return norm_fwd_launch<T, V, 64, 2>(a);
+    if (packs <= 256) return norm_fwd_launch<T, V, 64, 4>(a);
+    if (packs <= 512) return norm_fwd_launch<T, V, 256, 2>(a);
+    if (packs <= 1024) return norm_fwd_launch<T, V, 256, 4>(a);
+    const unsigned blocks = (unsigned)(a.rows < 2048 ? a.rows : 2048);
+    norm_fwd_long_kernel<T, V><<<dim3(blocks), dim3(1024), 0, a.s>>>(a.rows, a.dim, (const T*)a.x, a.x_stride, a.weight,
+                                                                    a.bias, a.affine_dtype, a.eps, (T*)a.out, a.mean, a.rstd);
+    LAUNCH_OK("norm_fwd_long_kernel");
+    return 0;
+}
+template <typename T, int V>
+int norm_bwd_v(const NormArgs& a) {
+    const size_t packs = a.dim / V;
+    uint32_t nparts = 0;
+    int rc = 0;
+    if (packs <= 8) rc = norm_bwd_launch<T, V, 8, 1>(a, nparts);
+    else if (packs <= 16) rc = norm_bwd_launch<T, V, 16, 1>(a, nparts);
+    else if (packs <= 32) rc = norm_bwd_launch<T, V, 32, 1>(a, nparts);
+    else if (packs <= 64) rc = norm_bwd_launch<T, V, 64, 1>(a, nparts);
+    else if (packs <= 128) rc = norm_bwd_launch<T, V, 64, 2>(a, nparts);
+    else if (packs <= 256) rc = norm_bwd_launch<T, V, 256, 1>(a, nparts);
+    else if (packs <= 512) rc = norm_bwd_launch<T, V, 256, 2>(a, nparts);
+    else if (packs <= 1024) rc = norm_bwd_launch<T, V, 256, 4>(a, nparts);
+    else {
+        if (a.dx) {
+            const unsigned blocks = (unsigned)(a.rows < 2048 ? a.rows : 2048);
+            norm_bwd_long_kernel<T, V><<<dim3(blocks), dim3(1024), 0, a.s>>>(a.rows, a.dim, (const T*)a.dy, a.dy_stride,
+                                                                            (const T*)a.x, a.x_stride, a.weight,
+                                                                            a.affine_dtype, a.mean, a.rstd, (T*)a.dx);
+            LAUNCH_OK("norm_bwd_long_kernel");
+        }
+        if (a.part) {
+            nparts = (uint32_t)(a.rows < NORM_LONG_PARTS ? a.rows : NORM_LONG_PARTS);
+            norm_cols_kernel<T><<<dim3(nparts, (unsigned)((a.dim + 255) / 256)), dim3(256), 0, a.s>>>(
+                a.rows, a.dim, (const T*)a.dy, a.dy_stride, (const T*)a.x, a.x_stride, a.mean, a.rstd, a.part);
+            LAUNCH_OK("norm_cols_kernel");
+        }
+    }
+    if (rc || !a.part) return rc;
+    norm_join_kernel<<<dim3((unsigned)((2 * a.dim + 63) / 64)), dim3(1024), 0, a.s>>>(nparts, a.dim, a.part, a.affine_dtype,
+                                                                                    a.dweight, a.dbias);
+    LAUNCH_OK("norm_join_kernel");
+    return 0;
+}
+}  // namespace
+
+int e3_layer_norm_forward_impl(size_t rows, size_t dim, const void* x, size_t x_stride, int dtype, const void* weight,
+                               const void* bias, int affine_dtype, float eps, void* out, float* mean, float* rstd,
+                               hipStream_t s) {
+    if (rows == 0) return 0;
+    NormArgs a{};
+    a.rows = rows; a.dim = dim; a.x = x; a.x_stride = x_stride; a.weight = weight; a.bias = bias;
+    a.affine_dtype = affine_dtype; a.eps = eps; a.out = out; a.mean = mean; a.rstd = rstd; a.s = s;
+    const bool wide = e3_rows_wide(x, x_stride, dim, dtype) && e3_rows_wide(out, dim, dim, dtype);
+    if (dtype == E3_F32) return wide ? norm_fwd_v<float, 4>(a) : norm_fwd_v<float, 1>(a);
+    if (dtype == E3_F16) return wide ? norm_fwd_v<f16_t, 8>(a) : norm_fwd_v<f16_t, 1>(a);
+    return wide ? norm_fwd_v<bf16_t, 8>(a) : norm_fwd_v<bf16_t, 1>(a);
+}
+
+size_t e3_layer_norm_scratch_bytes(size_t rows, size_t dim) {
+    return (rows < NORM_BWD_BLOCKS ? (rows ? rows : 1) : NORM_BWD_BLOCKS) * 2 * dim * sizeof(float) + 256;
+}
+
+int e3_layer_norm_backward_impl(size_t rows, size_t dim, const void* dy, size_t dy_stride, const void* x, size_t x_stride,
+                                int dtype, const void* weight, int affine_dtype, const float* mean, const float* rstd,
+                                void* dx, void* dweight, void* dbias, char* scratch, hipStream_t s) {
+    NormArgs a{};
+    a.rows = rows; a.dim = dim; a.x = x; a.x_stride = x_stride; a.dy = dy; a.dy_stride = dy_stride; a.weight = weight;
+    a.affine_dtype = affine_dtype; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd); a.dx = dx;
+    a.dweight = dweight; a.dbias = dbias; a.s = s;
+    a.part = dweight || dbias ? reinterpret_cast<float*>(scratch) : nullptr;
+    if (rows == 0) {
+        if (!a.part) return 0;
+        norm_join_kernel<<<dim3((unsigned)((2 * dim + 63) / 64)), dim3(1024), 0, s>>>(0, dim, a.part, affine_dtype, dweight, dbias);
+        LAUNCH_OK("norm_join_kernel");
+        return 0;
+    }
+    const bool wide = e3_rows_wide(x, x_stride, dim, dtype) && e3_rows_wide(dy, dy_stride, dim, dtype) &&
+                      (!dx || e3_rows_wide(dx, dim, dim, dtype));
+    if (dtype == E3_F32) return wide ? norm_bwd_v<float, 4>(a) : norm_bwd_v<float, 1>(a);
+    if (dtype == E3_F16) return wide ? norm_bwd_v<f16_t, 8>(a) : norm_bwd_v<f16_t, 1>(a);
+    return wide ? norm_bwd_v<bf16_t, 8>(a) : norm_bwd_v<bf16_t, 1>(a);
+}

@@ -1,0 +1,56 @@
+// rows.h -- row-wise helpers of the learned-feature operators (features.hip, distill.hip): element types, packs of
+// consecutive elements, loads by a runtime type, reductions over a group of lanes.
+#pragma once
+#include "common.h"
+
+typedef _Float16 f16_t;
+typedef __bf16 bf16_t;
+
+enum { E3_F32 = 0, E3_F16 = 1, E3_BF16 = 2 };     // E3DGS_F32 / _F16 / _BF16 (include/e3dgs_hip.h)
+
+// V consecutive elements, loaded and stored as one memory instruction (V * sizeof(T) = 16 bytes, or a single element).
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack {
+    T v[V];
+};
+
+// elements of a 16-byte pack
+template <typename T>
+struct Wide {
+    static constexpr int N = 16 / (int)sizeof(T);
+};
+
+static inline size_t e3_elem_bytes(int dtype) { return dtype == E3_F32 ? 4 : 2; }
+static inline bool e3_dtype_ok(int dtype) { return dtype >= E3_F32 && dtype <= E3_BF16; }
+
+// Whether rows at `p`, `stride` elements apart and `dim` long, can be read as 16-byte packs.
+static inline bool e3_rows_wide(const void* p, size_t stride, size_t dim, int dtype) {
+    const size_t b = e3_elem_bytes(dtype), n = 16 / b;
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % n == 0 && dim % n == 0;
+}
+
+// One element of an array whose type is a launch argument (uniform branch): parameters and labels, which are read once per
+// workgroup or row, so that the kernels need no instance per combination of types.
+__device__ __forceinline__ float load_elem(const void* __restrict__ p, size_t i, int dtype) {
+    if (dtype == E3_F32) return reinterpret_cast<const float*>(p)[i];
+    if (dtype == E3_F16) return (float)reinterpret_cast<const f16_t*>(p)[i];
+    return (float)reinterpret_cast<const bf16_t*>(p)[i];
+}
+__device__ __forceinline__ long long load_index(const void* __restrict__ p, size_t i, int bytes) {
+    return bytes == 8 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
+}
+
+// Sum / maximum over aligned groups of G lanes (G a power of two, 1 .. 64): every lane of the group gets the result, and
+// every lane adds in the same tree, so the result does not depend on the lane.
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+    for (int o = 1; o < G; o <<= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+template <int G>
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+    for (int o = 1; o < G; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}

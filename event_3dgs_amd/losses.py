@@ -295,3 +295,37 @@ def psnr(img1, img2):
     """utils/image_utils.py:19-21"""
     mse = ((img1 - img2) ** 2).reshape(img1.shape[0], -1).mean(1, keepdim=True)
     return 20 * torch.log10(1.0 / torch.sqrt(mse))
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Distillation of class scores (a decoder behind learned features, features.py; an image of scores behind the rasteriser)
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _reduction(reduction):
+    if reduction not in _REDUCTIONS:
+        raise ValueError("reduction must be 'none', 'mean' or 'sum'")
+    return _REDUCTIONS[reduction]
+
+
+def distill_loss(logits, teacher_logits, teacher_index, temperature=1.0, reduction="mean", class_dim=-1):
+    """Distillation from a teacher's best scores:  T^2 * KL(q || p)  per row, with q the softmax of the teacher's k listed
+    scores / T and p the softmax of all of `logits` / T along `class_dim`.
+
+    teacher_logits / teacher_index have the shape of `logits` with k entries along `class_dim`: the scores the teacher gave
+    its best classes, and which classes those are.  `logits` may be rows of classes (class_dim=-1) or planes of an image
+    (class_dim=0 of (classes, H, W), read as they lie up to 256 classes).  An entry counts when its index is >= 0 and its
+    score above -inf; a row without one is unlabelled: it adds 0, its gradient is 0, the mean leaves it out (a mean over no
+    row is 0).  A class may be listed twice (its weights add up); an index past the classes makes the row NaN.  Logits of
+    -inf or the type's lowest value switch a class off.
+
+    Returns fp32: a scalar ('mean', 'sum') or one value per row ('none').  The gradient goes to `logits` only."""
+    from .features import _ext
+    return _ext().distill(logits, teacher_logits, teacher_index, float(temperature), _reduction(reduction), int(class_dim))
+
+
+def distill_loss_raw(logits, teacher_logits, teacher_index, temperature=1.0, reduction="mean", class_dim=-1):
+    """distill_loss and its gradient in one call, no autograd: (value, d value / d logits); with reduction 'none' the gradient
+    of the sum."""
+    from .features import _ext
+    return _ext().distill_raw(logits, teacher_logits, teacher_index, float(temperature), _reduction(reduction), int(class_dim))

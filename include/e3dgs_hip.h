@@ -720,6 +720,83 @@ void e3dgs_profile_select(int slot_mask);
 int e3dgs_profile_query(int slot, double* total_ms, int* launches);
 const char* e3dgs_profile_slot_name(int slot);
 
+/*
+ * Rows of learned features (operators that train a shared codebook for the Gaussians, and the decoder behind it).  They
+ * replace nothing of the reference; they stand beside its losses and its optimizer.
+ *
+ * Element types of the row operators; `dtype` arguments take one of them.  Sums and statistics are fp32 for all of them,
+ * every result is rounded once, to the nearest.
+ */
+#define E3DGS_F32 0
+#define E3DGS_F16 1
+#define E3DGS_BF16 2
+#define E3DGS_FEATURE_MAX_DIM 1048576   /* values of a row */
+
+/*
+ * out[i, :] = scale * table[index[i], :], out contiguous (n, dim); rows of the table are `table_stride` elements apart.
+ * index: int32 or int64 (index_bytes 4 / 8), contiguous.  An index below 0 stands for no row (zeros, no gradient); one at
+ * or past `rows` gives a row of NaN (and no gradient): the device's way to report it, as nothing here waits for the GPU.
+ */
+int e3dgs_embedding_forward(size_t n, size_t rows, size_t dim, const void* index, int index_bytes, const void* table,
+                            size_t table_stride, int dtype, float scale, void* out, void* stream);
+/*
+ * grad_table[v, :] = scale * sum of grad_out[i, :] over all i with index[i] == v, in the order of i; contiguous (rows, dim),
+ * every row is written (zeros where no i names it).  Deterministic (a stable sort of the positions, no atomics).
+ * n < 2^31, rows < 2^31.  scratch: e3dgs_embedding_backward_scratch_bytes(n, rows, dim) bytes, 256-B aligned.
+ */
+size_t e3dgs_embedding_backward_scratch_bytes(size_t n, size_t rows, size_t dim);
+int e3dgs_embedding_backward(size_t n, size_t rows, size_t dim, const void* index, int index_bytes, const void* grad_out,
+                             size_t grad_stride, int dtype, float scale, void* grad_table, char* scratch, void* stream);
+
+/*
+ * out = (x - mean) / sqrt(var + eps) * weight + bias over rows of `dim` values, `x_stride` elements apart; out contiguous.
+ * weight / bias (dim values of affine_dtype) may be NULL (1 / 0); mean / rstd (fp32, one per row) may be NULL when no
+ * gradient is wanted.
+ */
+int e3dgs_layer_norm_forward(size_t rows, size_t dim, const void* x, size_t x_stride, int dtype, const void* weight,
+                             const void* bias, int affine_dtype, float eps, void* out, float* mean, float* rstd,
+                             void* stream);
+/*
+ * Its gradient from the mean / rstd of the forward call.  grad_x (contiguous), grad_weight and grad_bias (affine_dtype) may
+ * each be NULL.  scratch: e3dgs_layer_norm_backward_scratch_bytes(rows, dim) bytes, 16-B aligned.  Deterministic.
+ */
+size_t e3dgs_layer_norm_backward_scratch_bytes(size_t rows, size_t dim);
+int e3dgs_layer_norm_backward(size_t rows, size_t dim, const void* grad_out, size_t grad_stride, const void* x,
+                              size_t x_stride, int dtype, const void* weight, int affine_dtype, const float* mean,
+                              const float* rstd, void* grad_x, void* grad_weight, void* grad_bias, char* scratch,
+                              void* stream);
+
+/*
+ * Distillation of class scores from a teacher's best scores:
+ *   q = softmax over the k listed classes of a row (teacher / temperature), p = softmax over all classes of logits / temperature,
+ *   row = temperature^2 * sum_k q_k (log q_k - log p[index_k]).
+ * An entry counts when its index is >= 0 and its teacher score is above -infinity; a row without one has no label: its value
+ * and gradient are 0 and the mean does not count it (its logits are not looked at).  The same class may be listed twice
+ * (the weights add up).  An index at or past `classes` makes the row and its gradient NaN.
+ * Strides in elements: logits (row_stride, class_stride) with class_stride 1, or row_stride 1 and at most
+ * E3DGS_DISTILL_MAX_PLANES classes (planes, as an image lies); teacher and index (row, entry) as they are.
+ * reduction: 0 none, 1 mean over the labelled rows, 2 sum.
+ *   stats     2 floats per row, for the backward call
+ *   row_loss  one float per row (may be NULL)
+ *   loss      2 floats: the value (sum or mean; for `none` the sum) and the weight of a row, for the backward call
+ * backward: d_loss = the gradient of the value (device; one float, or with reduction 0 one per row; NULL: 1); grad has the
+ * layout kind of logits with strides of its own, every element of it is written.
+ * scratch: e3dgs_distill_scratch_bytes(rows) bytes, 8-B aligned.
+ */
+#define E3DGS_DISTILL_MAX_PLANES 256
+#define E3DGS_DISTILL_MAX_K 1024
+size_t e3dgs_distill_scratch_bytes(size_t rows);
+int e3dgs_distill_forward(size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride, size_t class_stride,
+                          int dtype, const void* teacher, size_t teacher_row_stride, size_t teacher_entry_stride,
+                          int teacher_dtype, const void* index, size_t index_row_stride, size_t index_entry_stride,
+                          int index_bytes, float temperature, int reduction, float* stats, float* row_loss, float* loss,
+                          char* scratch, void* stream);
+int e3dgs_distill_backward(size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride, size_t class_stride,
+                           int dtype, const void* teacher, size_t teacher_row_stride, size_t teacher_entry_stride,
+                           int teacher_dtype, const void* index, size_t index_row_stride, size_t index_entry_stride,
+                           int index_bytes, float temperature, int reduction, const float* stats, const float* loss,
+                           const float* d_loss, void* grad, size_t grad_row_stride, size_t grad_class_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,82 @@
+"""Arguments the learned-feature operators refuse, and what they need, without a GPU: every refusal comes from the host checks."""
+import ctypes as C
+
+import pytest
+import torch
+
+from event_3dgs_amd import _lib, features, losses
+
+PTR = C.c_void_p(4096)          # never followed: the calls below are refused before anything is launched
+
+
+def text():
+    return _lib.lib().e3dgs_last_error().decode()
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(3, 4)
+    i = torch.zeros(3, 1, dtype=torch.int64)
+    for call in (lambda: features.embedding(i, x), lambda: features.layer_norm(x), lambda: losses.distill_loss(x, x[:, :1], i),
+                 lambda: losses.distill_loss_raw(x, x[:, :1], i)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+
+
+def test_unknown_reduction_is_refused():
+    x = torch.zeros(3, 4)
+    for call in (losses.distill_loss, losses.distill_loss_raw):
+        with pytest.raises(ValueError, match="reduction"):
+            call(x, x[:, :1], torch.zeros(3, 1, dtype=torch.int64), reduction="average")
+
+
+@pytest.mark.parametrize("n, rows, dim, index_bytes, dtype, ptr", [
+    (4, 8, 0, 4, 0, PTR), (4, 8, (1 << 20) + 1, 4, 0, PTR), (4, 1 << 31, 4, 4, 0, PTR), (1 << 31, 8, 4, 4, 0, PTR),
+    (4, 8, 4, 2, 0, PTR), (4, 8, 4, 4, 3, PTR), (4, 8, 4, 4, -1, PTR), (4, 8, 4, 4, 0, None)])
+def test_embedding_arguments(hip_lib, n, rows, dim, index_bytes, dtype, ptr):
+    assert hip_lib.e3dgs_embedding_forward(n, rows, dim, PTR, index_bytes, PTR, dim, dtype, 1.0, ptr, None) != 0
+    assert "e3dgs_embedding_forward" in text()
+    assert hip_lib.e3dgs_embedding_backward(n, rows, dim, PTR, index_bytes, PTR, dim, dtype, 1.0, ptr, PTR, None) != 0
+    assert "e3dgs_embedding_backward" in text()
+
+
+def test_embedding_scratch(hip_lib):
+    assert hip_lib.e3dgs_embedding_backward(4, 8, 4, PTR, 4, PTR, 4, 0, 1.0, PTR, C.c_void_p(4096 + 8), None) != 0
+    assert "aligned" in text()
+    small, large = (hip_lib.e3dgs_embedding_backward_scratch_bytes(n, 4096, 48) for n in (0, 1000000))
+    assert 0 < small < large
+
+
+@pytest.mark.parametrize("dim, eps, dtype, affine, ptr", [
+    (0, 1e-5, 0, 0, PTR), ((1 << 20) + 1, 1e-5, 0, 0, PTR), (4, -1.0, 0, 0, PTR), (4, float("nan"), 0, 0, PTR),
+    (4, 1e-5, 3, 0, PTR), (4, 1e-5, 0, 5, PTR), (4, 1e-5, 0, 0, None)])
+def test_layer_norm_arguments(hip_lib, dim, eps, dtype, affine, ptr):
+    assert hip_lib.e3dgs_layer_norm_forward(3, dim, ptr, dim, dtype, PTR, PTR, affine, eps, PTR, PTR, PTR, None) != 0
+    assert "e3dgs_layer_norm_forward" in text()
+    if eps == 1e-5:
+        assert hip_lib.e3dgs_layer_norm_backward(3, dim, PTR, dim, ptr, dim, dtype, PTR, affine, PTR, PTR, PTR, PTR, PTR, PTR, None) != 0
+        assert "e3dgs_layer_norm_backward" in text()
+
+
+@pytest.mark.parametrize("change", [
+    dict(classes=0), dict(classes=1 << 31), dict(k=0), dict(k=1025), dict(rows=1 << 31), dict(temperature=0.0),
+    dict(temperature=float("nan")), dict(temperature=float("inf")), dict(reduction=3), dict(dtype=3), dict(teacher_dtype=-1),
+    dict(index_bytes=2), dict(logits=None), dict(index=None),
+    dict(row_stride=1, class_stride=5, classes=257), dict(row_stride=7, class_stride=5)])
+def test_distill_arguments(hip_lib, change):
+    a = dict(rows=5, classes=9, k=2, logits=PTR, row_stride=9, class_stride=1, dtype=0, teacher_dtype=0, index=PTR,
+             index_bytes=4, temperature=1.0, reduction=1)
+    a.update(change)
+    head = (a["rows"], a["classes"], a["k"], a["logits"], a["row_stride"], a["class_stride"], a["dtype"], PTR, a["k"], 1,
+            a["teacher_dtype"], a["index"], a["k"], 1, a["index_bytes"], a["temperature"], a["reduction"])
+    assert hip_lib.e3dgs_distill_forward(*head, PTR, PTR, PTR, PTR, None) != 0
+    assert "e3dgs_distill_forward" in text()
+    assert hip_lib.e3dgs_distill_backward(*head, PTR, PTR, PTR, PTR, a["row_stride"], a["class_stride"], None) != 0
+    assert "e3dgs_distill_backward" in text()
+
+
+def test_distill_gradient_layout(hip_lib):
+    head = (5, 9, 2, PTR, 9, 1, 0, PTR, 2, 1, 0, PTR, 2, 1, 4, 1.0, 1)
+    assert hip_lib.e3dgs_distill_backward(*head, PTR, PTR, PTR, PTR, 1, 5, None) != 0
+    assert "layout" in text()
+    assert hip_lib.e3dgs_distill_forward(*head, PTR, PTR, None, PTR, None) != 0
+    assert "null pointer" in text()
