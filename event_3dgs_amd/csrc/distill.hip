@@ -277,13 +277,18 @@ __global__ __launch_bounds__(Lanes<G>::THREADS) void distill_bwd_rows_kernel(con
             const Pack<T, V>* zp = reinterpret_cast<const Pack<T, V>*>(z + cut.head);
             Pack<T, V>* gp = reinterpret_cast<Pack<T, V>*>(g + cut.head);
             if (any) {
-#pragma unroll 4
-                for (uint32_t i = lane; i < cut.packs; i += G) {
-                    const Pack<T, V> p = zp[i];
-                    Pack<T, V> r;
+                for (uint32_t i = lane; i < cut.packs; i += SOFT_UNROLL * G) {      // (a batch of loads, then the stores)
+                    Pack<T, V> p[SOFT_UNROLL];
 #pragma unroll
-                    for (int j = 0; j < V; ++j) r.v[j] = (T)(exp2_hw(((float)p.v[j] - st.x) * c) * fi);
-                    gp[i] = r;
+                    for (int u = 0; u < SOFT_UNROLL; ++u) p[u] = zp[i + u * G < cut.packs ? i + u * G : i];
+#pragma unroll
+                    for (int u = 0; u < SOFT_UNROLL; ++u) {
+                        if (i + u * G >= cut.packs) break;
+                        Pack<T, V> r;
+#pragma unroll
+                        for (int j = 0; j < V; ++j) r.v[j] = (T)(exp2_hw(((float)p[u].v[j] - st.x) * c) * fi);
+                        gp[i + u * G] = r;
+                    }
                 }
             } else {
                 Pack<T, V> r;
@@ -319,38 +324,72 @@ struct PlaneLabel {
     float top, inv, qlogq;
     bool any, broken;
 };
-// adds the label's weights to the column (`set`) or clears their places again
+// Adds the weights of a pixel's label to its column.
+constexpr int PLANE_ENTRIES = 8;      // a list up to this long is read once and stays in registers
 __device__ __forceinline__ PlaneLabel plane_label(const DistillArgs& a, size_t row, float c, float rt, float* col) {
     PlaneLabel l;
-    float top = -__builtin_inff(), sum = 0.0f;
+    float top = -__builtin_inff(), sum = 0.0f, qlogq = 0.0f;
     l.any = l.broken = false;
-    for (size_t k = 0; k < a.k; ++k) {
-        long long id;
-        const float t = entry_score(a, row, k, id);
-        if (t == -__builtin_inff()) continue;
-        l.any = true;
-        if (id >= (long long)a.classes) l.broken = true;
-        top = fmaxf(top, t);
+    float t[PLANE_ENTRIES];
+    long long id[PLANE_ENTRIES];
+    const bool shortlist = a.k <= PLANE_ENTRIES;
+    if (shortlist) {
+#pragma unroll
+        for (int k = 0; k < PLANE_ENTRIES; ++k) {
+            const size_t at = k < (int)a.k ? k : a.k - 1;           // (unconditional loads, all in flight)
+            id[k] = load_index(a.index, row * a.i_row + at * a.i_entry, a.index_bytes);
+            t[k] = load_elem(a.teacher, row * a.t_row + at * a.t_entry, a.teacher_dtype);
+        }
+#pragma unroll
+        for (int k = 0; k < PLANE_ENTRIES; ++k) {
+            if (k >= (int)a.k || id[k] < 0) t[k] = -__builtin_inff();
+            if (t[k] == -__builtin_inff()) continue;
+            l.any = true;
+            l.broken |= id[k] >= (long long)a.classes;
+            top = fmaxf(top, t[k]);
+        }
+    } else {
+        for (size_t k = 0; k < a.k; ++k) {
+            long long i;
+            const float v = entry_score(a, row, k, i);
+            if (v == -__builtin_inff()) continue;
+            l.any = true;
+            l.broken |= i >= (long long)a.classes;
+            top = fmaxf(top, v);
+        }
     }
-    l.qlogq = 0.0f;
     l.top = top;
-    l.inv = 0.0f;
+    l.inv = l.qlogq = 0.0f;
     if (!l.any) return l;
-    for (size_t k = 0; k < a.k; ++k) {
-        long long id;
-        const float t = entry_score(a, row, k, id);
-        if (t != -__builtin_inff()) sum += exp2_hw((t - top) * c);
+    if (shortlist) {
+#pragma unroll
+        for (int k = 0; k < PLANE_ENTRIES; ++k) sum += t[k] == -__builtin_inff() ? 0.0f : exp2_hw((t[k] - top) * c);
+    } else {
+        for (size_t k = 0; k < a.k; ++k) {
+            long long i;
+            const float v = entry_score(a, row, k, i);
+            if (v != -__builtin_inff()) sum += exp2_hw((v - top) * c);
+        }
     }
     l.inv = 1.0f / sum;
     const float rest = log2_hw(l.inv) * LN2;
-    for (size_t k = 0; k < a.k; ++k) {
-        long long id;
-        const float t = entry_score(a, row, k, id);
-        if (t == -__builtin_inff() || id >= (long long)a.classes) continue;
-        const float q = exp2_hw((t - top) * c) * l.inv;
-        if (q != 0.0f) l.qlogq += q * ((t - top) * rt + rest);
-        col[(size_t)id * 64] += q;
+    auto add = [&](float v, long long i) {
+        if (v == -__builtin_inff() || i >= (long long)a.classes) return;
+        const float q = exp2_hw((v - top) * c) * l.inv;
+        if (q != 0.0f) qlogq += q * ((v - top) * rt + rest);
+        col[(size_t)i * 64] += q;
+    };
+    if (shortlist) {
+#pragma unroll
+        for (int k = 0; k < PLANE_ENTRIES; ++k) add(t[k], id[k]);
+    } else {
+        for (size_t k = 0; k < a.k; ++k) {
+            long long i;
+            const float v = entry_score(a, row, k, i);
+            add(v, i);
+        }
     }
+    l.qlogq = qlogq;
     return l;
 }
 __device__ __forceinline__ void plane_clear(const DistillArgs& a, size_t row, float* col) {
@@ -360,7 +399,21 @@ __device__ __forceinline__ void plane_clear(const DistillArgs& a, size_t row, fl
     }
 }
 
-constexpr int PLANE_UNROLL = 8;
+// The planes go by in batches: the loads of the next batch are in flight while one is worked on (a lane's label takes
+// 4 bytes of LDS per class, so that few waves fit a CU and each has to keep many loads in flight).
+constexpr int PLANE_BATCH = 16;
+template <typename T>
+struct PlaneBatch {
+    T v[PLANE_BATCH];
+    __device__ __forceinline__ void load(const T* __restrict__ z, uint32_t first, uint32_t classes, size_t stride) {
+#pragma unroll
+        for (int u = 0; u < PLANE_BATCH; ++u) {          // (the last plane again behind the last one: never used)
+            const uint32_t j = first + u < classes ? first + u : classes - 1;
+            v[u] = z[(size_t)j * stride];
+        }
+    }
+};
+
 template <typename T>
 __global__ __launch_bounds__(64) void distill_fwd_planes_kernel(const DistillArgs a) {
     extern __shared__ float cols[];
@@ -371,22 +424,26 @@ __global__ __launch_bounds__(64) void distill_fwd_planes_kernel(const DistillArg
     float total = 0.0f;
     uint32_t count = 0;
     for (size_t row = (size_t)blockIdx.x * 64 + lane; row < a.rows; row += (size_t)gridDim.x * 64) {
+        const T* z = reinterpret_cast<const T*>(a.logits) + row;
+        PlaneBatch<T> next;
+        next.load(z, 0, a.classes, a.class_stride);
         const PlaneLabel l = plane_label(a, row, c, rt, col);
         if (!l.any) {
             a.stats[row] = make_float2(0.0f, 0.0f);
             if (a.row_loss) a.row_loss[row] = 0.0f;
             continue;
         }
-        const T* z = reinterpret_cast<const T*>(a.logits) + row;
         float m = -__builtin_inff(), s = 0.0f;
         float qz = 0.0f, qs = 0.0f;              // sum of q (z - m) and of q over the classes so far
-        for (uint32_t j = 0; j < a.classes; j += PLANE_UNROLL) {
-            float v[PLANE_UNROLL], M = m;
+        for (uint32_t j = 0; j < a.classes; j += PLANE_BATCH) {
+            const PlaneBatch<T> b = next;
+            if (j + PLANE_BATCH < a.classes) next.load(z, j + PLANE_BATCH, a.classes, a.class_stride);
+            float v[PLANE_BATCH], M = m;
 #pragma unroll
-            for (int u = 0; u < PLANE_UNROLL; ++u)
-                v[u] = j + u < a.classes ? (float)z[(size_t)(j + u) * a.class_stride] : -__builtin_inff();
-#pragma unroll
-            for (int u = 0; u < PLANE_UNROLL; ++u) M = fmaxf(M, v[u]);
+            for (int u = 0; u < PLANE_BATCH; ++u) {
+                v[u] = j + u < a.classes ? (float)b.v[u] : -__builtin_inff();
+                M = fmaxf(M, v[u]);
+            }
             if (M != m) {
                 s *= exp2_hw((m - M) * c);
                 if (qs != 0.0f) qz += qs * (m - M);
@@ -394,13 +451,11 @@ __global__ __launch_bounds__(64) void distill_fwd_planes_kernel(const DistillArg
             }
             const float off = M == -__builtin_inff() ? 0.0f : M;
 #pragma unroll
-            for (int u = 0; u < PLANE_UNROLL; ++u) {
-                s += exp2_hw((v[u] - off) * c);
-                const float q = j + u < a.classes ? col[(j + u) * 64] : 0.0f;
-                if (q != 0.0f) {
-                    qz += q * (v[u] - off);
-                    qs += q;
-                }
+            for (int u = 0; u < PLANE_BATCH; ++u) {
+                const float d = v[u] - off, q = j + u < a.classes ? col[(j + u) * 64] : 0.0f;
+                s += exp2_hw(d * c);
+                qz += q != 0.0f ? q * d : 0.0f;              // (a class that is switched off has d = -inf)
+                qs += q;
             }
         }
         // sum of q = 1:  sum q (log q - log p) = qlogq - sum q (z - m) / T + log s
@@ -435,12 +490,18 @@ __global__ __launch_bounds__(64) void distill_bwd_planes_kernel(const DistillArg
             continue;
         }
         const T* z = reinterpret_cast<const T*>(a.logits) + row;
+        PlaneBatch<T> next;
+        next.load(z, 0, a.classes, a.class_stride);
         const float f = f_all * (a.scale ? a.scale[a.reduction == 0 ? row : 0] : 1.0f);
         plane_label(a, row, c, rt, col);
-#pragma unroll 8
-        for (uint32_t j = 0; j < a.classes; ++j)
-            g[(size_t)j * a.g_class] =
-                (T)(f * (exp2_hw(((float)z[(size_t)j * a.class_stride] - st.x) * c) * st.y - col[j * 64]));
+        for (uint32_t j = 0; j < a.classes; j += PLANE_BATCH) {
+            const PlaneBatch<T> b = next;
+            if (j + PLANE_BATCH < a.classes) next.load(z, j + PLANE_BATCH, a.classes, a.class_stride);
+#pragma unroll
+            for (int u = 0; u < PLANE_BATCH; ++u)
+                if (j + u < a.classes)
+                    g[(size_t)(j + u) * a.g_class] = (T)(f * (exp2_hw(((float)b.v[u] - st.x) * c) * st.y - col[(j + u) * 64]));
+        }
         plane_clear(a, row, col);
     }
 }
