@@ -325,71 +325,36 @@ struct PlaneLabel {
     bool any, broken;
 };
 // Adds the weights of a pixel's label to its column.
-constexpr int PLANE_ENTRIES = 8;      // a list up to this long is read once and stays in registers
 __device__ __forceinline__ PlaneLabel plane_label(const DistillArgs& a, size_t row, float c, float rt, float* col) {
     PlaneLabel l;
-    float top = -__builtin_inff(), sum = 0.0f, qlogq = 0.0f;
+    float top = -__builtin_inff(), sum = 0.0f;
     l.any = l.broken = false;
-    float t[PLANE_ENTRIES];
-    long long id[PLANE_ENTRIES];
-    const bool shortlist = a.k <= PLANE_ENTRIES;
-    if (shortlist) {
-#pragma unroll
-        for (int k = 0; k < PLANE_ENTRIES; ++k) {
-            const size_t at = k < (int)a.k ? k : a.k - 1;           // (unconditional loads, all in flight)
-            id[k] = load_index(a.index, row * a.i_row + at * a.i_entry, a.index_bytes);
-            t[k] = load_elem(a.teacher, row * a.t_row + at * a.t_entry, a.teacher_dtype);
-        }
-#pragma unroll
-        for (int k = 0; k < PLANE_ENTRIES; ++k) {
-            if (k >= (int)a.k || id[k] < 0) t[k] = -__builtin_inff();
-            if (t[k] == -__builtin_inff()) continue;
-            l.any = true;
-            l.broken |= id[k] >= (long long)a.classes;
-            top = fmaxf(top, t[k]);
-        }
-    } else {
-        for (size_t k = 0; k < a.k; ++k) {
-            long long i;
-            const float v = entry_score(a, row, k, i);
-            if (v == -__builtin_inff()) continue;
-            l.any = true;
-            l.broken |= i >= (long long)a.classes;
-            top = fmaxf(top, v);
-        }
+    for (size_t k = 0; k < a.k; ++k) {
+        long long id;
+        const float t = entry_score(a, row, k, id);
+        if (t == -__builtin_inff()) continue;
+        l.any = true;
+        l.broken |= id >= (long long)a.classes;
+        top = fmaxf(top, t);
     }
     l.top = top;
     l.inv = l.qlogq = 0.0f;
     if (!l.any) return l;
-    if (shortlist) {
-#pragma unroll
-        for (int k = 0; k < PLANE_ENTRIES; ++k) sum += t[k] == -__builtin_inff() ? 0.0f : exp2_hw((t[k] - top) * c);
-    } else {
-        for (size_t k = 0; k < a.k; ++k) {
-            long long i;
-            const float v = entry_score(a, row, k, i);
-            if (v != -__builtin_inff()) sum += exp2_hw((v - top) * c);
-        }
+    for (size_t k = 0; k < a.k; ++k) {
+        long long id;
+        const float t = entry_score(a, row, k, id);
+        if (t != -__builtin_inff()) sum += exp2_hw((t - top) * c);
     }
     l.inv = 1.0f / sum;
     const float rest = log2_hw(l.inv) * LN2;
-    auto add = [&](float v, long long i) {
-        if (v == -__builtin_inff() || i >= (long long)a.classes) return;
-        const float q = exp2_hw((v - top) * c) * l.inv;
-        if (q != 0.0f) qlogq += q * ((v - top) * rt + rest);
-        col[(size_t)i * 64] += q;
-    };
-    if (shortlist) {
-#pragma unroll
-        for (int k = 0; k < PLANE_ENTRIES; ++k) add(t[k], id[k]);
-    } else {
-        for (size_t k = 0; k < a.k; ++k) {
-            long long i;
-            const float v = entry_score(a, row, k, i);
-            add(v, i);
-        }
+    for (size_t k = 0; k < a.k; ++k) {
+        long long id;
+        const float t = entry_score(a, row, k, id);
+        if (t == -__builtin_inff() || id >= (long long)a.classes) continue;
+        const float q = exp2_hw((t - top) * c) * l.inv;
+        if (q != 0.0f) l.qlogq += q * ((t - top) * rt + rest);
+        col[(size_t)id * 64] += q;
     }
-    l.qlogq = qlogq;
     return l;
 }
 __device__ __forceinline__ void plane_clear(const DistillArgs& a, size_t row, float* col) {
@@ -506,6 +471,192 @@ __global__ __launch_bounds__(64) void distill_bwd_planes_kernel(const DistillArg
     }
 }
 
+// ---- planes, short lists: P neighbouring pixels to a lane, their labels in registers (KR entries each: the class of an entry
+// is compared with every class that goes by, which is cheaper than LDS up to 8 entries and leaves the occupancy to the
+// loads: P * sizeof(T) bytes per lane and load).
+template <int KR>
+struct PixelLabel {
+    float q[KR];       // weight of the entry's class, at its first entry (0 elsewhere)
+    int id[KR];        // its class, or -1
+    float qlogq;
+    bool any, broken;
+};
+template <int KR>
+__device__ __forceinline__ void pixel_label(const DistillArgs& a, size_t row, float c, float rt, PixelLabel<KR>& l) {
+    float t[KR], top = -__builtin_inff(), sum = 0.0f;
+    l.any = l.broken = false;
+    l.qlogq = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KR; ++k) {
+        const size_t at = k < (int)a.k ? k : a.k - 1;               // (unconditional loads, all in flight)
+        const long long id = load_index(a.index, row * a.i_row + at * a.i_entry, a.index_bytes);
+        t[k] = load_elem(a.teacher, row * a.t_row + at * a.t_entry, a.teacher_dtype);
+        l.id[k] = id >= (long long)a.classes ? 0x7FFFFFFF : id < 0 || k >= (int)a.k ? -1 : (int)id;
+    }
+#pragma unroll
+    for (int k = 0; k < KR; ++k) {
+        if (t[k] == -__builtin_inff()) l.id[k] = -1;
+        if (l.id[k] < 0) continue;
+        l.any = true;
+        l.broken |= l.id[k] == 0x7FFFFFFF;
+        top = fmaxf(top, t[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < KR; ++k) {
+        l.q[k] = l.id[k] < 0 ? 0.0f : exp2_hw((t[k] - top) * c);
+        sum += l.q[k];
+    }
+    const float inv = l.any ? 1.0f / sum : 0.0f, rest = l.any ? log2_hw(inv) * LN2 : 0.0f;
+#pragma unroll
+    for (int k = 0; k < KR; ++k) {
+        l.q[k] *= inv;
+        if (l.q[k] != 0.0f) l.qlogq += l.q[k] * ((t[k] - top) * rt + rest);
+    }
+#pragma unroll
+    for (int k = 0; k < KR; ++k)        // the same class again: its weight goes to the first entry
+#pragma unroll
+        for (int j = k + 1; j < KR; ++j)
+            if (l.id[k] >= 0 && l.id[j] == l.id[k]) {
+                l.q[k] += l.q[j];
+                l.id[j] = -1;
+            }
+}
+
+constexpr int WIDE_BATCH = 8;
+template <typename T, int P>
+struct WideBatch {
+    Pack<T, P> v[WIDE_BATCH];
+    __device__ __forceinline__ void load(const T* __restrict__ z, uint32_t first, uint32_t classes, size_t stride) {
+#pragma unroll
+        for (int u = 0; u < WIDE_BATCH; ++u) {
+            const uint32_t j = first + u < classes ? first + u : classes - 1;
+            v[u] = *reinterpret_cast<const Pack<T, P>*>(z + (size_t)j * stride);
+        }
+    }
+};
+
+template <typename T, int P, int KR>
+__global__ __launch_bounds__(256) void distill_fwd_wide_kernel(const DistillArgs a) {
+    __shared__ float lds[16];
+    const float rt = 1.0f / a.temperature, c = LOG2E * rt;
+    float total = 0.0f;
+    uint32_t count = 0;
+    for (size_t row = ((size_t)blockIdx.x * 256 + threadIdx.x) * P; row < a.rows; row += (size_t)gridDim.x * 256 * P) {
+        const T* z = reinterpret_cast<const T*>(a.logits) + row;
+        WideBatch<T, P> next;
+        next.load(z, 0, a.classes, a.class_stride);
+        PixelLabel<KR> l[P];
+        bool some = false;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            pixel_label<KR>(a, row + p, c, rt, l[p]);
+            some |= l[p].any;
+        }
+        float m[P], s[P], zk[P][KR];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            m[p] = -__builtin_inff();
+            s[p] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KR; ++k) zk[p][k] = 0.0f;
+        }
+        for (uint32_t j = 0; some && j < a.classes; j += WIDE_BATCH) {
+            const WideBatch<T, P> b = next;
+            if (j + WIDE_BATCH < a.classes) next.load(z, j + WIDE_BATCH, a.classes, a.class_stride);
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                float v[WIDE_BATCH], M = m[p];
+#pragma unroll
+                for (int u = 0; u < WIDE_BATCH; ++u) {
+                    v[u] = j + u < a.classes ? (float)b.v[u].v[p] : -__builtin_inff();
+                    M = fmaxf(M, v[u]);
+#pragma unroll
+                    for (int k = 0; k < KR; ++k) zk[p][k] = l[p].id[k] == (int)(j + u) ? v[u] : zk[p][k];
+                }
+                const float off = M == -__builtin_inff() ? 0.0f : M;
+                s[p] *= exp2_hw((m[p] - off) * c);
+                m[p] = M;
+#pragma unroll
+                for (int u = 0; u < WIDE_BATCH; ++u) s[p] += exp2_hw((v[u] - off) * c);
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            float d = 0.0f;
+            float2 st = make_float2(0.0f, 0.0f);
+            if (l[p].any) {
+                // sum of q = 1:  sum q (log q - log p) = qlogq - sum q (z - m) / T + log s
+                float qz = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KR; ++k)
+                    if (l[p].id[k] >= 0 && l[p].q[k] != 0.0f) qz += l[p].q[k] * (zk[p][k] - m[p]);
+                d = (l[p].qlogq - qz * rt + log2_hw(s[p]) * LN2) * (a.temperature * a.temperature);
+                if (l[p].broken) d = __builtin_nanf("");
+                st = make_float2(m[p], l[p].broken ? __builtin_nanf("") : 1.0f / s[p]);
+                ++count;
+            }
+            a.stats[row + p] = st;
+            if (a.row_loss) a.row_loss[row + p] = d;
+            total += d;
+        }
+    }
+    total = group_sum<64>(total);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) count += __shfl_xor(count, o, 64);
+    store_part<4, 64>(total, count, a.part, lds);
+}
+
+template <typename T, int P, int KR>
+__global__ __launch_bounds__(256) void distill_bwd_wide_kernel(const DistillArgs a) {
+    const float rt = 1.0f / a.temperature, c = LOG2E * rt;
+    const float f_all = a.temperature * (a.weight ? *a.weight : 1.0f);
+    for (size_t row = ((size_t)blockIdx.x * 256 + threadIdx.x) * P; row < a.rows; row += (size_t)gridDim.x * 256 * P) {
+        T* g = reinterpret_cast<T*>(a.grad) + row;
+        const T* z = reinterpret_cast<const T*>(a.logits) + row;
+        float2 st[P];
+        bool some = false;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            st[p] = a.stats[row + p];
+            some |= st[p].y != 0.0f;
+        }
+        if (!some) {
+            Pack<T, P> r;
+#pragma unroll
+            for (int p = 0; p < P; ++p) r.v[p] = (T)0.0f;
+            for (uint32_t j = 0; j < a.classes; ++j) *reinterpret_cast<Pack<T, P>*>(g + (size_t)j * a.g_class) = r;
+            continue;
+        }
+        WideBatch<T, P> next;
+        next.load(z, 0, a.classes, a.class_stride);
+        PixelLabel<KR> l[P];
+        float f[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            pixel_label<KR>(a, row + p, c, rt, l[p]);
+            f[p] = f_all * (a.scale ? a.scale[a.reduction == 0 ? row + p : 0] : 1.0f);
+        }
+        for (uint32_t j = 0; j < a.classes; j += WIDE_BATCH) {
+            const WideBatch<T, P> b = next;
+            if (j + WIDE_BATCH < a.classes) next.load(z, j + WIDE_BATCH, a.classes, a.class_stride);
+#pragma unroll
+            for (int u = 0; u < WIDE_BATCH; ++u) {
+                if (j + u >= a.classes) break;
+                Pack<T, P> r;
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    float q = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < KR; ++k) q = l[p].id[k] == (int)(j + u) ? l[p].q[k] : q;
+                    const float d = f[p] * (exp2_hw(((float)b.v[u].v[p] - st[p].x) * c) * st[p].y - q);
+                    r.v[p] = st[p].y == 0.0f ? (T)0.0f : (T)d;
+                }
+                *reinterpret_cast<Pack<T, P>*>(g + (size_t)(j + u) * a.g_class) = r;
+            }
+        }
+    }
+}
+
 // loss[0] = sum of the partial sums (over the labelled rows for the mean), loss[1] = the weight of a row
 __global__ __launch_bounds__(1024) void distill_join_kernel(uint32_t nparts, const float2* __restrict__ part, int reduction,
                                                             float* __restrict__ loss) {
@@ -557,9 +708,41 @@ int distill_rows(const DistillArgs& a, bool backward, unsigned& blocks, hipStrea
     return 0;
 }
 
+// pixels per lane: 4 for the gradient; 2 for the value, whose registers (the scores of the label's entries) would leave two
+// waves to a SIMD with 4 (64 fp32 planes of 1920 x 1080: 173 us with 4, 157 us with 2); 1 where the planes do not lie on
+// such boundaries
+template <typename T, int P, int KR>
+int distill_wide_fwd(const DistillArgs& a, unsigned& blocks, hipStream_t s) {
+    blocks = distill_blocks(a.rows, 256 * P);
+    distill_fwd_wide_kernel<T, P, KR><<<dim3(blocks), dim3(256), 0, s>>>(a);
+    LAUNCH_OK("distill_fwd_wide_kernel");
+    return 0;
+}
+template <typename T, int P, int KR>
+int distill_wide_bwd(const DistillArgs& a, hipStream_t s) {
+    distill_bwd_wide_kernel<T, P, KR><<<dim3(distill_blocks(a.rows, 256 * P)), dim3(256), 0, s>>>(a);
+    LAUNCH_OK("distill_bwd_wide_kernel");
+    return 0;
+}
+// whether P neighbouring pixels of every plane can be moved at once
+template <typename T>
+bool planes_wide(const void* p, size_t stride, size_t rows, size_t n) {
+    return rows % n == 0 && stride % n == 0 && (reinterpret_cast<uintptr_t>(p) & (n * sizeof(T) - 1)) == 0;
+}
+
 template <typename T>
 int distill_t(const DistillArgs& a, bool backward, unsigned& blocks, hipStream_t s) {
     if (planes_layout(a.row_stride, a.class_stride)) {
+        if (a.k <= 8) {
+            if (!backward) {
+                if (planes_wide<T>(a.logits, a.class_stride, a.rows, 2))
+                    return a.k <= 4 ? distill_wide_fwd<T, 2, 4>(a, blocks, s) : distill_wide_fwd<T, 2, 8>(a, blocks, s);
+                return a.k <= 4 ? distill_wide_fwd<T, 1, 4>(a, blocks, s) : distill_wide_fwd<T, 1, 8>(a, blocks, s);
+            }
+            if (planes_wide<T>(a.logits, a.class_stride, a.rows, 4) && planes_wide<T>(a.grad, a.g_class, a.rows, 4))
+                return a.k <= 4 ? distill_wide_bwd<T, 4, 4>(a, s) : distill_wide_bwd<T, 4, 8>(a, s);
+            return a.k <= 4 ? distill_wide_bwd<T, 1, 4>(a, s) : distill_wide_bwd<T, 1, 8>(a, s);
+        }
         const size_t lds = (size_t)a.classes * 64 * sizeof(float);
         blocks = distill_blocks(a.rows, 64);
         if (backward) distill_bwd_planes_kernel<T><<<dim3(blocks), dim3(64), lds, s>>>(a);
