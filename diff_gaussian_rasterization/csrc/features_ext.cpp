@@ -214,8 +214,16 @@ Scores scores_of(const Tensor& logits, const Tensor& teacher, const Tensor& inde
     return s;
 }
 
-// value (0-dim, or one per row), stats, loss pair
-std::tuple<Tensor, Tensor, Tensor> distill_forward(const Scores& s, double temperature, int64_t reduction) {
+Tensor empty_grad(const Scores& s) {
+    const int64_t rows = (int64_t)s.rows, classes = (int64_t)s.classes;
+    return s.planes ? torch::empty({classes, rows}, s.logits.options()).t() : torch::empty({rows, classes}, s.logits.options());
+}
+size_t grad_row(const Scores& s) { return s.planes ? 1 : s.classes; }
+size_t grad_class(const Scores& s) { return s.planes ? s.rows : 1; }
+Tensor shaped(const Scores& s, const Tensor& grad) { return grad.view(s.shape).movedim(-1, s.class_dim); }
+
+// value (0-dim, or one per row), stats, loss pair; fills `grad` (of empty_grad) if it is defined
+std::tuple<Tensor, Tensor, Tensor> distill_forward(const Scores& s, double temperature, int64_t reduction, const Tensor& grad) {
     const auto opt = s.logits.options().dtype(torch::kFloat32);
     Tensor stats = torch::empty({(int64_t)s.rows, 2}, opt), loss = torch::empty({2}, opt);
     Tensor row_loss = reduction == 0 ? torch::empty({(int64_t)s.rows}, opt) : Tensor();
@@ -226,7 +234,7 @@ std::tuple<Tensor, Tensor, Tensor> distill_forward(const Scores& s, double tempe
                                 (size_t)s.index.stride(0), (size_t)s.index.stride(1), index_bytes_of(s.index),
                                 (float)temperature, (int)reduction, stats.data_ptr<float>(),
                                 row_loss.defined() ? row_loss.data_ptr<float>() : nullptr, loss.data_ptr<float>(),
-                                bytes(scratch), stream()),
+                                grad.defined() ? grad.data_ptr() : nullptr, grad_row(s), grad_class(s), bytes(scratch), stream()),
           "e3dgs_distill_forward");
     if (reduction == 0) return std::make_tuple(row_loss.view(std::vector<int64_t>(s.shape.begin(), s.shape.end() - 1)), stats, loss);
     return std::make_tuple(loss.select(0, 0), stats, loss);
@@ -234,24 +242,22 @@ std::tuple<Tensor, Tensor, Tensor> distill_forward(const Scores& s, double tempe
 
 Tensor distill_backward(const Scores& s, double temperature, int64_t reduction, const Tensor& stats, const Tensor& loss,
                         const Tensor& d_loss) {
-    const int64_t rows = (int64_t)s.rows, classes = (int64_t)s.classes;
-    Tensor grad = s.planes ? torch::empty({classes, rows}, s.logits.options()).t() : torch::empty({rows, classes}, s.logits.options());
+    Tensor grad = empty_grad(s);
     check(e3dgs_distill_backward(s.rows, s.classes, s.k, s.logits.data_ptr(), s.row_stride, s.class_stride,
                                  dtype_of(s.logits, "logits"), s.teacher.data_ptr(), (size_t)s.teacher.stride(0),
                                  (size_t)s.teacher.stride(1), dtype_of(s.teacher, "teacher_logits"), s.index.data_ptr(),
                                  (size_t)s.index.stride(0), (size_t)s.index.stride(1), index_bytes_of(s.index),
                                  (float)temperature, (int)reduction, stats.data_ptr<float>(), loss.data_ptr<float>(),
-                                 d_loss.defined() ? d_loss.data_ptr<float>() : nullptr, grad.data_ptr(),
-                                 (size_t)(s.planes ? 1 : classes), (size_t)(s.planes ? rows : 1), stream()),
+                                 d_loss.data_ptr<float>(), grad.data_ptr(), grad_row(s), grad_class(s), stream()),
           "e3dgs_distill_backward");
-    return grad.view(s.shape).movedim(-1, s.class_dim);
+    return shaped(s, grad);
 }
 
 struct DistillFunction : public torch::autograd::Function<DistillFunction> {
     static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher, const Tensor& index,
                           double temperature, int64_t reduction, int64_t class_dim) {
         const Guard guard(logits.device());
-        auto r = distill_forward(scores_of(logits, teacher, index, class_dim), temperature, reduction);
+        auto r = distill_forward(scores_of(logits, teacher, index, class_dim), temperature, reduction, Tensor());
         ctx->save_for_backward({logits, teacher, index, std::get<1>(r), std::get<2>(r)});
         ctx->saved_data["temperature"] = temperature;
         ctx->saved_data["reduction"] = reduction;
@@ -299,7 +305,7 @@ Tensor distill(const Tensor& logits, const Tensor& teacher, const Tensor& index,
     if (at::GradMode::is_enabled() && logits.requires_grad())
         return DistillFunction::apply(logits, teacher, index, temperature, reduction, class_dim);
     const Guard guard(logits.device());
-    return std::get<0>(distill_forward(scores_of(logits, teacher, index, class_dim), temperature, reduction));
+    return std::get<0>(distill_forward(scores_of(logits, teacher, index, class_dim), temperature, reduction, Tensor()));
 }
 
 std::tuple<Tensor, Tensor> distill_raw(const Tensor& logits_, const Tensor& teacher, const Tensor& index, double temperature,
@@ -309,8 +315,9 @@ std::tuple<Tensor, Tensor> distill_raw(const Tensor& logits_, const Tensor& teac
     const Guard guard(logits.device());
     at::NoGradGuard no_grad;
     const Scores s = scores_of(logits, teacher, index, class_dim);
-    auto r = distill_forward(s, temperature, reduction);
-    return std::make_tuple(std::get<0>(r), distill_backward(s, temperature, reduction, std::get<1>(r), std::get<2>(r), Tensor()));
+    const Tensor grad = empty_grad(s);
+    auto r = distill_forward(s, temperature, reduction, grad);
+    return std::make_tuple(std::get<0>(r), shaped(s, grad));
 }
 
 }  // namespace

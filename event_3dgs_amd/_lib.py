@@ -176,7 +176,7 @@ def lib():
     L.e3dgs_distill_scratch_bytes.argtypes = [_sz]
     _scores = [_sz] * 3 + [_vp, _sz, _sz, C.c_int] * 2 + [_vp, _sz, _sz, C.c_int, C.c_float, C.c_int]
     L.e3dgs_distill_forward.restype = C.c_int
-    L.e3dgs_distill_forward.argtypes = _scores + [_fp] * 3 + [_cp, _vp]
+    L.e3dgs_distill_forward.argtypes = _scores + [_fp] * 3 + [_vp, _sz, _sz, _cp, _vp]
     L.e3dgs_distill_backward.restype = C.c_int
     L.e3dgs_distill_backward.argtypes = _scores + [_fp] * 3 + [_vp, _sz, _sz, _vp]
     L.e3dgs_profile_enable.restype = None

@@ -125,7 +125,8 @@ int e3_layer_norm_backward_impl(size_t, size_t, const void*, size_t, const void*
 bool e3_distill_layout_ok(size_t, size_t, size_t, size_t);
 size_t e3_distill_scratch_bytes(size_t);
 int e3_distill_forward_impl(size_t, size_t, size_t, const void*, size_t, size_t, int, const void*, size_t, size_t, int,
-                            const void*, size_t, size_t, int, float, int, float*, float*, float*, char*, hipStream_t);
+                            const void*, size_t, size_t, int, float, int, float*, float*, float*, void*, size_t, size_t, char*,
+                            hipStream_t);
 int e3_distill_backward_impl(size_t, size_t, size_t, const void*, size_t, size_t, int, const void*, size_t, size_t, int,
                              const void*, size_t, size_t, int, float, int, const float*, const float*, const float*, void*,
                              size_t, size_t, hipStream_t);
@@ -927,20 +928,27 @@ static int distill_args(const char* who, size_t rows, size_t classes, size_t k, 
         return feature_args_fail(who, rows, classes, dtype, "neither rows of classes nor at most 256 planes");
     return 0;
 }
+static bool distill_grad_ok(size_t rows, size_t classes, size_t class_stride, size_t grad_row_stride, size_t grad_class_stride) {
+    return e3_distill_layout_ok(rows, classes, grad_row_stride, grad_class_stride) &&
+           (grad_class_stride == 1) == (class_stride == 1);
+}
 int e3dgs_distill_forward(size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride, size_t class_stride,
                           int dtype, const void* teacher, size_t teacher_row_stride, size_t teacher_entry_stride,
                           int teacher_dtype, const void* index, size_t index_row_stride, size_t index_entry_stride,
                           int index_bytes, float temperature, int reduction, float* stats, float* row_loss, float* loss,
-                          char* scratch, void* stream) {
+                          void* grad, size_t grad_row_stride, size_t grad_class_stride, char* scratch, void* stream) {
     g_err[0] = 0;
-    const int rc = distill_args("e3dgs_distill_forward", rows, classes, k, logits, row_stride, class_stride, dtype, teacher,
-                                teacher_dtype, index, index_bytes, temperature, reduction);
+    const char* who = "e3dgs_distill_forward";
+    const int rc = distill_args(who, rows, classes, k, logits, row_stride, class_stride, dtype, teacher, teacher_dtype, index,
+                                index_bytes, temperature, reduction);
     if (rc) return rc;
-    if (!loss || (rows > 0 && (!stats || !scratch)))
-        return feature_args_fail("e3dgs_distill_forward", rows, classes, dtype, "null pointer");
+    if (!loss || (rows > 0 && (!stats || !scratch))) return feature_args_fail(who, rows, classes, dtype, "null pointer");
+    if (grad && !distill_grad_ok(rows, classes, class_stride, grad_row_stride, grad_class_stride))
+        return feature_args_fail(who, rows, classes, dtype, "the gradient's layout differs from the scores'");
     return e3_distill_forward_impl(rows, classes, k, logits, row_stride, class_stride, dtype, teacher, teacher_row_stride,
                                    teacher_entry_stride, teacher_dtype, index, index_row_stride, index_entry_stride,
-                                   index_bytes, temperature, reduction, stats, row_loss, loss, scratch, (hipStream_t)stream);
+                                   index_bytes, temperature, reduction, stats, row_loss, loss, grad, grad_row_stride,
+                                   grad_class_stride, scratch, (hipStream_t)stream);
 }
 int e3dgs_distill_backward(size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride, size_t class_stride,
                            int dtype, const void* teacher, size_t teacher_row_stride, size_t teacher_entry_stride,
@@ -953,8 +961,7 @@ int e3dgs_distill_backward(size_t rows, size_t classes, size_t k, const void* lo
                                 index_bytes, temperature, reduction);
     if (rc) return rc;
     if (rows > 0 && (!stats || !loss || !grad)) return feature_args_fail(who, rows, classes, dtype, "null pointer");
-    if (!e3_distill_layout_ok(rows, classes, grad_row_stride, grad_class_stride) ||
-        (grad_class_stride == 1) != (class_stride == 1))
+    if (!distill_grad_ok(rows, classes, class_stride, grad_row_stride, grad_class_stride))
         return feature_args_fail(who, rows, classes, dtype, "the gradient's layout differs from the scores'");
     return e3_distill_backward_impl(rows, classes, k, logits, row_stride, class_stride, dtype, teacher, teacher_row_stride,
                                     teacher_entry_stride, teacher_dtype, index, index_row_stride, index_entry_stride,

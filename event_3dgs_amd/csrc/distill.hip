@@ -41,6 +41,9 @@ struct DistillArgs {
     const float* scale;
     void* grad;
     size_t g_row, g_class;
+    float* loss;            // (value, weight of a row), written by the only workgroup of a launch
+    const uint32_t* counts; // partial counts of the labelled rows (a value formed with its gradient)
+    uint32_t ncounts;
 };
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -65,258 +68,576 @@ __device__ __forceinline__ void soft_add(float& m, float& s, const float z[V], f
 }
 
 
-// ---- the label of a row, worked out by a group of lanes (lane, G): entries lane, lane + G, ...
+// ---- labels.  An entry is listed when its index is >= 0 and its score above -infinity.
 struct Label {
     float top, inv;          // largest listed score; 1 / sum of exp2((t - top) c)
-    bool any, broken;
+    bool any, broken;        // an entry is listed; a listed one names a class past the end
 };
+constexpr int ID_BROKEN = 0x7FFFFFFF;
 __device__ __forceinline__ float entry_score(const DistillArgs& a, size_t row, size_t k, long long& id) {
     id = load_index(a.index, row * a.i_row + k * a.i_entry, a.index_bytes);
     return id < 0 ? -__builtin_inff() : load_elem(a.teacher, row * a.t_row + k * a.t_entry, a.teacher_dtype);
 }
-// reductions over the lanes of a row: a group of one wave, or the whole workgroup (G > 64)
-template <int G>
-struct Lanes {
-    static constexpr int THREADS = G > 256 ? G : 256;
-    static constexpr int ROWS = THREADS / G;
-    static constexpr int WAVES = G > 64 ? G / 64 : 1;
-    static __device__ __forceinline__ float sum(float v, float* lds) {
-        v = group_sum<(G < 64 ? G : 64)>(v);
-        if (G <= 64) return v;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = lds[0];
-#pragma unroll
-        for (int w = 1; w < WAVES; ++w) v += lds[w];
-        return v;
-    }
-    static __device__ __forceinline__ float max(float v, float* lds) {
-        v = group_max<(G < 64 ? G : 64)>(v);
-        if (G <= 64) return v;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = lds[0];
-#pragma unroll
-        for (int w = 1; w < WAVES; ++w) v = fmaxf(v, lds[w]);
-        return v;
-    }
-    static __device__ __forceinline__ void soft(float& m, float& s, float c, float* lds) {
-#pragma unroll
-        for (int o = 1; o < (G < 64 ? G : 64); o <<= 1) {
-            const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
-            soft_merge(m, s, m2, s2, c);
-        }
-        if (G <= 64) return;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) { lds[2 * (threadIdx.x >> 6)] = m; lds[2 * (threadIdx.x >> 6) + 1] = s; }
-        __syncthreads();
-        m = lds[0];
-        s = lds[1];
-#pragma unroll
-        for (int w = 1; w < WAVES; ++w) soft_merge(m, s, lds[2 * w], lds[2 * w + 1], c);
-    }
-    // what a lane stored before is seen by the row's lanes behind this point, and stores behind it land later
-    static __device__ __forceinline__ void sync() {
-        if (G <= 64) wave_sync();
-        else __syncthreads();
-    }
-};
-
-template <int G>
-__device__ __forceinline__ Label row_label(const DistillArgs& a, size_t row, bool live, int lane, float c, float* lds) {
-    Label l;
-    float top = -__builtin_inff(), sum = 0.0f, flags = 0.0f;          // flags: 1 a listed entry, 2 a broken one
-    if (live)
-        for (size_t k = lane; k < a.k; k += G) {
-            long long id;
-            const float t = entry_score(a, row, k, id);
-            if (t == -__builtin_inff()) continue;
-            flags = fmaxf(flags, id >= (long long)a.classes ? 2.0f : 1.0f);
-            top = fmaxf(top, t);                                        // (a NaN score makes the sum NaN)
-        }
-    flags = Lanes<G>::max(flags, lds);
-    top = Lanes<G>::max(top, lds);
-    l.any = flags > 0.0f;
-    l.broken = flags > 1.5f;
-    if (live && l.any)
-        for (size_t k = lane; k < a.k; k += G) {
-            long long id;
-            const float t = entry_score(a, row, k, id);
-            if (t != -__builtin_inff()) sum += exp2_hw((t - top) * c);
-        }
-    sum = Lanes<G>::sum(sum, lds);
-    l.top = top;
-    l.inv = 1.0f / sum;
-    return l;
+// the class of an entry as it is kept in LDS: -1 not listed, ID_BROKEN past the end
+__device__ __forceinline__ int entry_class(const DistillArgs& a, float t, long long id) {
+    return t == -__builtin_inff() ? -1 : id >= (long long)a.classes ? ID_BROKEN : (int)id;
 }
 
+// The label of a row, worked out by one wave: classes and weights exp2((t - top) c) of all entries to LDS.
+__device__ __forceinline__ Label wave_label(const DistillArgs& a, size_t row, float c, int* ids, float* ws) {
+    const int lane = threadIdx.x & 63;
+    float top = -__builtin_inff(), sum = 0.0f, flags = 0.0f;
+    for (int k = lane; k < (int)a.k; k += 64) {
+        long long id;
+        const float t = entry_score(a, row, k, id);
+        const int cls = entry_class(a, t, id);
+        ids[k] = cls;
+        ws[k] = t;
+        if (cls < 0) continue;
+        flags = fmaxf(flags, cls == ID_BROKEN ? 2.0f : 1.0f);
+        top = fmaxf(top, t);                                        // (a NaN score makes the sum NaN)
+    }
+    Label l;
+    l.top = top = group_max<64>(top);
+    flags = group_max<64>(flags);
+    for (int k = lane; k < (int)a.k; k += 64) {
+        const float w = ids[k] < 0 ? 0.0f : exp2_hw((ws[k] - top) * c);
+        ws[k] = w;
+        sum += w;
+    }
+    sum = group_sum<64>(sum);
+    l.inv = 1.0f / sum;
+    l.any = flags > 0.0f;
+    l.broken = flags > 1.5f;
+    wave_sync();
+    return l;
+}
+// whether a row has a listed entry; every lane of a wave gets the answer
+__device__ __forceinline__ bool wave_any(const DistillArgs& a, size_t row) {
+    bool any = false;
+    for (int k = threadIdx.x & 63; k < (int)a.k; k += 64) {
+        long long id;
+        any |= entry_score(a, row, k, id) != -__builtin_inff();
+    }
+    return __ballot(any) != 0ull;
+}
+// Sum over the entries of q (log q - log p), with log p = (z - m) / T - log s; one lane's entries, `score(k)` gives z.
+template <typename F>
+__device__ __forceinline__ float label_value(const DistillArgs& a, size_t row, const Label& l, const int* ids, const float* ws,
+                                             int first, int step, float m, float s, float rt, F score) {
+    float d = 0.0f;
+    const float rest = (log2_hw(l.inv) + log2_hw(s)) * LN2;
+    for (int k = first; k < (int)a.k; k += step) {
+        if (ids[k] < 0) continue;
+        if (ids[k] == ID_BROKEN) { d = __builtin_nanf(""); continue; }
+        const float q = ws[k] * l.inv;
+        if (q == 0.0f) continue;
+        long long id;
+        const float t = entry_score(a, row, k, id);
+        d += q * (((t - l.top) - (score(ids[k]) - m)) * rt + rest);
+    }
+    return d;
+}
+// Weight of the class of entry k: all its entries added up in order; 0 entries before k name it (else false).
+__device__ __forceinline__ bool class_weight(const DistillArgs& a, const int* ids, const float* ws, int k, float& w) {
+    const int id = ids[k];
+    if (id < 0 || id == ID_BROKEN) return false;
+    w = 0.0f;
+    bool first = true;
+    for (int j = 0; j < (int)a.k; ++j) {
+        if (ids[j] != id) continue;
+        first &= j >= k;
+        w += ws[j];
+    }
+    return first;
+}
+
+// ---- sums over a launch
+// Number of labelled rows; one thread's share.  The entries of a row are read by as many neighbouring lanes as there are
+// entries (a power of two, at most a wave); the row counts for the first of them.
+__device__ __forceinline__ uint32_t count_rows(const DistillArgs& a, size_t thread, size_t threads) {
+    int lanes = 64;
+    while (lanes > 1 && lanes > (int)a.k) lanes >>= 1;
+    const int lane = threadIdx.x & (lanes - 1), group = (threadIdx.x & 63) & ~(lanes - 1);
+    const unsigned long long mine = (lanes == 64 ? ~0ull : (1ull << lanes) - 1ull) << group;
+    uint32_t n = 0;
+    const size_t step = threads / lanes, rounds = (a.rows + step - 1) / step;
+    for (size_t i = 0; i < rounds; ++i) {                 // (the same number of rounds for every lane of a wave)
+        const size_t row = i * step + thread / lanes;
+        bool any = false;
+        if (row < a.rows)
+            for (int k = lane; k < (int)a.k; k += lanes) {
+                long long id;
+                any |= entry_score(a, row, k, id) != -__builtin_inff();
+            }
+        const unsigned long long all = __ballot(any);
+        if (lane == 0 && (all & mine) != 0ull) ++n;
+    }
+    return n;
+}
+template <int THREADS>
+__device__ __forceinline__ uint32_t block_sum_u32(uint32_t n, uint32_t* lds) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = n;
+    __syncthreads();
+    n = lds[0];
+    for (int w = 1; w < THREADS / 64; ++w) n += lds[w];
+    __syncthreads();
+    return n;
+}
+constexpr int COUNT_BLOCKS = 256;
+__global__ __launch_bounds__(256) void distill_count_kernel(const DistillArgs a, uint32_t* __restrict__ counts) {
+    __shared__ uint32_t lds[4];
+    const uint32_t n = block_sum_u32<256>(count_rows(a, (size_t)blockIdx.x * 256 + threadIdx.x, (size_t)gridDim.x * 256), lds);
+    if (threadIdx.x == 0) counts[blockIdx.x] = n;
+}
+// Weight of a row for a kernel that forms the gradient with the value: 1 / labelled rows for the mean, from the partial
+// counts of distill_count_kernel, or counted by the only workgroup of the launch.
+template <int THREADS>
+__device__ __forceinline__ float row_weight(const DistillArgs& a, uint32_t* lds) {
+    if (a.reduction != 1 || a.rows == 1) return 1.0f;
+    uint32_t n = 0;
+    if (a.counts) {
+        for (uint32_t i = threadIdx.x; i < a.ncounts; i += THREADS) n += a.counts[i];
+    } else {
+        n = count_rows(a, threadIdx.x, THREADS);
+    }
+    n = block_sum_u32<THREADS>(n, lds);
+    return 1.0f / (float)(n ? n : 1u);
+}
+__device__ __forceinline__ void store_loss(const DistillArgs& a, double total, unsigned long long count) {
+    const double weight = a.reduction == 1 ? 1.0 / (double)(count ? count : 1) : 1.0;
+    a.loss[0] = (float)(total * weight);
+    a.loss[1] = (float)weight;
+}
+// Adds up what the workgroup's threads hold (in a fixed tree): one pair per workgroup, or the result itself when there is
+// only one.
+template <int THREADS>
+__device__ __forceinline__ void store_part(const DistillArgs& a, float total, uint32_t count, float* lds) {
+    total = group_sum<64>(total);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) count += __shfl_xor(count, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) { lds[2 * (threadIdx.x >> 6)] = total; lds[2 * (threadIdx.x >> 6) + 1] = __uint_as_float(count); }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < THREADS / 64; ++w) { total += lds[2 * w]; count += __float_as_uint(lds[2 * w + 1]); }
+    if (gridDim.x == 1) store_loss(a, total, count);
+    else a.part[blockIdx.x] = make_float2(total, __uint_as_float(count));
+}
+
+// ---- long rows: a wave (G = 64) or a workgroup of G threads to a row
 // A row of `n` elements at p as single elements up to the first 16-byte boundary, packs, and single elements behind the
 // last pack: [0, head) and [tail, n) are singles.
 struct Cut {
-    uint32_t head, packs, tail;
+    uint32_t head, packs, tail, singles;
+    __device__ __forceinline__ uint32_t single(uint32_t e) const { return e < head ? e : tail + (e - head); }
 };
 template <typename T, int V>
 __device__ __forceinline__ Cut cut_row(const T* p, uint32_t n) {
     Cut r;
-    if (V == 1) { r.head = 0; r.packs = n; r.tail = n; return r; }
+    if (V == 1) { r.head = 0; r.packs = n; r.tail = n; r.singles = 0; return r; }
     const uint32_t off = (uint32_t)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
     r.head = off ? V - off : 0;
     if (r.head > n) r.head = n;
     r.packs = (n - r.head) / V;
     r.tail = r.head + r.packs * V;
+    r.singles = n - r.packs * V;
     return r;
 }
 
-// Sum of a value over the workgroup's rows (lane 0 of each group holds one), one pair per workgroup.
-template <int ROWS, int G>
-__device__ __forceinline__ void store_part(float total, uint32_t count, float2* part, float* lds) {
-    __syncthreads();
-    if (threadIdx.x % G == 0) { lds[2 * (threadIdx.x / G)] = total; lds[2 * (threadIdx.x / G) + 1] = __uint_as_float(count); }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int r = 1; r < ROWS; ++r) { total += lds[2 * r]; count += __float_as_uint(lds[2 * r + 1]); }
-        part[blockIdx.x] = make_float2(total, __uint_as_float(count));
+// LDS of a workgroup of the row kernels: a label per row, the waves' (max, sum), the label's summary
+template <int G>
+struct RowsLds {
+    static constexpr int THREADS = G > 256 ? G : 256;
+    static constexpr int ROWS = THREADS / G;
+    int ids[ROWS][DISTILL_MAX_K];
+    float ws[ROWS][DISTILL_MAX_K];
+    float ms[2 * THREADS / 64];
+    Label label;
+};
+// (max, sum) over the lanes of a row.  Workgroup rows: ONE barrier (the caller keeps another between two uses).
+template <int G>
+__device__ __forceinline__ void row_soft(float& m, float& s, float c, RowsLds<G>& L) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
+        soft_merge(m, s, m2, s2, c);
     }
+    if (G == 64) return;
+    if ((threadIdx.x & 63) == 0) { L.ms[2 * (threadIdx.x >> 6)] = m; L.ms[2 * (threadIdx.x >> 6) + 1] = s; }
+    __syncthreads();
+    m = L.ms[0];
+    s = L.ms[1];
+#pragma unroll
+    for (int w = 1; w < G / 64; ++w) soft_merge(m, s, L.ms[2 * w], L.ms[2 * w + 1], c);
+}
+template <int G>
+__device__ __forceinline__ void row_sync() {      // orders the row's stores before and behind this point
+    if (G == 64) wave_sync();
+    else __syncthreads();
 }
 
 constexpr int SOFT_UNROLL = 4;
 template <typename T, int V, int G>
-__global__ __launch_bounds__(Lanes<G>::THREADS) void distill_fwd_rows_kernel(const DistillArgs a) {
-    using L = Lanes<G>;
-    __shared__ float lds[64];
-    const int lane = threadIdx.x % G;
+__global__ __launch_bounds__(RowsLds<G>::THREADS) void distill_fwd_rows_kernel(const DistillArgs a) {
+    __shared__ RowsLds<G> L;
+    const int lane = threadIdx.x % G, slot = threadIdx.x / G;
+    const bool labeller = G == 64 || threadIdx.x < 64;
     const float rt = 1.0f / a.temperature, c = LOG2E * rt;
     float total = 0.0f;
     uint32_t count = 0;
-    for (size_t base = (size_t)blockIdx.x * L::ROWS; base < a.rows; base += (size_t)gridDim.x * L::ROWS) {
-        const size_t row = base + threadIdx.x / G;
-        const bool live = row < a.rows;
-        const Label l = row_label<G>(a, row, live, lane, c, lds);
+    for (size_t row = (size_t)blockIdx.x * RowsLds<G>::ROWS + slot; row < a.rows; row += (size_t)gridDim.x * RowsLds<G>::ROWS) {
+        if (!wave_any(a, row)) {                          // (the same answer in every wave of the row: it is not read)
+            if (lane == 0) {
+                a.stats[row] = make_float2(0.0f, 0.0f);
+                if (a.row_loss) a.row_loss[row] = 0.0f;
+            }
+            continue;
+        }
         const T* z = reinterpret_cast<const T*>(a.logits) + row * a.row_stride;
         float m = -__builtin_inff(), s = 0.0f;
-        if (live && l.any) {                             // (a row without a label is not read)
-            const Cut cut = cut_row<T, V>(z, a.classes);
-            if (V > 1) {
-                const uint32_t singles = cut.head + (a.classes - cut.tail);
-                for (uint32_t e = lane; e < singles; e += G) {
-                    const float v = (float)z[e < cut.head ? e : cut.tail + (e - cut.head)];
-                    soft_add<1>(m, s, &v, c);
-                }
-            }
-            const Pack<T, V>* zp = reinterpret_cast<const Pack<T, V>*>(z + cut.head);
-            uint32_t i = lane;
-            for (; i + (SOFT_UNROLL - 1) * G < cut.packs; i += SOFT_UNROLL * G) {
-                Pack<T, V> p[SOFT_UNROLL];
+        const Cut cut = cut_row<T, V>(z, a.classes);
+        for (uint32_t e = lane; e < cut.singles; e += G) {
+            const float v = (float)z[cut.single(e)];
+            soft_add<1>(m, s, &v, c);
+        }
+        const Pack<T, V>* zp = reinterpret_cast<const Pack<T, V>*>(z + cut.head);
+        uint32_t i = lane;
+        for (; i + (SOFT_UNROLL - 1) * G < cut.packs; i += SOFT_UNROLL * G) {
+            Pack<T, V> p[SOFT_UNROLL];
 #pragma unroll
-                for (int u = 0; u < SOFT_UNROLL; ++u) p[u] = zp[i + u * G];
-                float v[SOFT_UNROLL * V];
+            for (int u = 0; u < SOFT_UNROLL; ++u) p[u] = zp[i + u * G];
+            float v[SOFT_UNROLL * V];
 #pragma unroll
-                for (int u = 0; u < SOFT_UNROLL; ++u)
+            for (int u = 0; u < SOFT_UNROLL; ++u)
 #pragma unroll
-                    for (int j = 0; j < V; ++j) v[u * V + j] = (float)p[u].v[j];
-                soft_add<SOFT_UNROLL * V>(m, s, v, c);
-            }
-            for (; i < cut.packs; i += G) {
-                const Pack<T, V> p = zp[i];
-                float v[V];
+                for (int j = 0; j < V; ++j) v[u * V + j] = (float)p[u].v[j];
+            soft_add<SOFT_UNROLL * V>(m, s, v, c);
+        }
+        for (; i < cut.packs; i += G) {
+            const Pack<T, V> p = zp[i];
+            float v[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[j] = (float)p.v[j];
-                soft_add<V>(m, s, v, c);
+            for (int j = 0; j < V; ++j) v[j] = (float)p.v[j];
+            soft_add<V>(m, s, v, c);
+        }
+        row_soft<G>(m, s, c, L);
+        if (labeller) {
+            const Label l = wave_label(a, row, c, L.ids[slot], L.ws[slot]);
+            float d = label_value(a, row, l, L.ids[slot], L.ws[slot], threadIdx.x & 63, 64, m, s, rt,
+                                  [&](int id) { return (float)z[id]; });
+            d = group_sum<64>(d) * (a.temperature * a.temperature);
+            if (lane == 0) {
+                a.stats[row] = make_float2(m, l.broken ? __builtin_nanf("") : 1.0f / s);
+                if (a.row_loss) a.row_loss[row] = d;
+                total += d;
+                ++count;
             }
         }
-        L::soft(m, s, c, lds);
-        // sum of q (log q - log p) over the entries: log q = (t - top) / T + log inv,  log p = (z - m) / T - log s
-        float d = 0.0f;
-        if (live && l.any) {
-            const float rest = (log2_hw(l.inv) + log2_hw(s)) * LN2;
-            for (size_t k = lane; k < a.k; k += G) {
-                long long id;
-                const float t = entry_score(a, row, k, id);
-                if (t == -__builtin_inff()) continue;
-                const float q = exp2_hw((t - l.top) * c) * l.inv;
-                if (id >= (long long)a.classes) d = __builtin_nanf("");
-                else if (q != 0.0f) d += q * (((t - l.top) - ((float)z[id] - m)) * rt + rest);
-            }
-        }
-        d = L::sum(d, lds) * (a.temperature * a.temperature);
-        if (!live || lane != 0) continue;
-        a.stats[row] = l.any ? make_float2(m, l.broken ? __builtin_nanf("") : 1.0f / s) : make_float2(0.0f, 0.0f);
-        if (a.row_loss) a.row_loss[row] = d;
-        total += d;
-        count += l.any ? 1u : 0u;
+        if (G > 64) __syncthreads();                      // (L.ms has been read)
     }
-    store_part<L::ROWS, G>(total, count, a.part, lds);
+    store_part<RowsLds<G>::THREADS>(a, total, count, L.ms);
+}
+
+// The listed classes of a row again, from the full-precision value: one lane per class (its first entry).
+template <typename T>
+__device__ __forceinline__ void patch_row(const DistillArgs& a, const Label& l, const int* ids, const float* ws, const T* z,
+                                          T* g, float m, float inv, float f, float c) {
+    for (int k = threadIdx.x & 63; k < (int)a.k; k += 64) {
+        float w;
+        if (class_weight(a, ids, ws, k, w)) g[ids[k]] = (T)(f * (exp2_hw(((float)z[ids[k]] - m) * c) * inv - w * l.inv));
+    }
 }
 
 template <typename T, int V, int G>
-__global__ __launch_bounds__(Lanes<G>::THREADS) void distill_bwd_rows_kernel(const DistillArgs a) {
-    using L = Lanes<G>;
-    __shared__ float lds[64];
-    const int lane = threadIdx.x % G;
+__global__ __launch_bounds__(RowsLds<G>::THREADS) void distill_bwd_rows_kernel(const DistillArgs a) {
+    __shared__ RowsLds<G> L;
+    const int lane = threadIdx.x % G, slot = threadIdx.x / G;
+    const bool labeller = G == 64 || threadIdx.x < 64;
     const float c = LOG2E / a.temperature;
     const float f_all = a.temperature * (a.weight ? *a.weight : 1.0f);
-    for (size_t base = (size_t)blockIdx.x * L::ROWS; base < a.rows; base += (size_t)gridDim.x * L::ROWS) {
-        const size_t row = base + threadIdx.x / G;
-        const bool live = row < a.rows;
-        const float2 st = live ? a.stats[row] : make_float2(0.0f, 0.0f);
+    for (size_t row = (size_t)blockIdx.x * RowsLds<G>::ROWS + slot; row < a.rows; row += (size_t)gridDim.x * RowsLds<G>::ROWS) {
+        const float2 st = a.stats[row];
         const bool any = st.y != 0.0f;
         const T* z = reinterpret_cast<const T*>(a.logits) + row * a.row_stride;
         T* g = reinterpret_cast<T*>(a.grad) + row * a.g_row;
-        const float f = f_all * (a.scale ? a.scale[a.reduction == 0 && live ? row : 0] : 1.0f), fi = f * st.y;
-        if (live) {
-            const Cut cut = cut_row<T, V>(g, a.classes);
-            if (V > 1) {
-                const uint32_t singles = cut.head + (a.classes - cut.tail);
-                for (uint32_t e = lane; e < singles; e += G) {
-                    const uint32_t col = e < cut.head ? e : cut.tail + (e - cut.head);
-                    g[col] = any ? (T)(exp2_hw(((float)z[col] - st.x) * c) * fi) : (T)0.0f;
-                }
-            }
-            const Pack<T, V>* zp = reinterpret_cast<const Pack<T, V>*>(z + cut.head);
-            Pack<T, V>* gp = reinterpret_cast<Pack<T, V>*>(g + cut.head);
-            if (any) {
-                for (uint32_t i = lane; i < cut.packs; i += SOFT_UNROLL * G) {      // (a batch of loads, then the stores)
-                    Pack<T, V> p[SOFT_UNROLL];
+        const float f = f_all * (a.scale ? a.scale[a.reduction == 0 ? row : 0] : 1.0f), fi = f * st.y;
+        const Cut cut = cut_row<T, V>(g, a.classes);
+        for (uint32_t e = lane; e < cut.singles; e += G) {
+            const uint32_t col = cut.single(e);
+            g[col] = any ? (T)(exp2_hw(((float)z[col] - st.x) * c) * fi) : (T)0.0f;
+        }
+        const Pack<T, V>* zp = reinterpret_cast<const Pack<T, V>*>(z + cut.head);
+        Pack<T, V>* gp = reinterpret_cast<Pack<T, V>*>(g + cut.head);
+        if (!any) {
+            Pack<T, V> r;
 #pragma unroll
-                    for (int u = 0; u < SOFT_UNROLL; ++u) p[u] = zp[i + u * G < cut.packs ? i + u * G : i];
+            for (int j = 0; j < V; ++j) r.v[j] = (T)0.0f;
+            for (uint32_t i = lane; i < cut.packs; i += G) gp[i] = r;
+            continue;                                     // (the same in every wave of the row)
+        }
+        for (uint32_t i = lane; i < cut.packs; i += SOFT_UNROLL * G) {      // (a batch of loads, then the stores)
+            Pack<T, V> p[SOFT_UNROLL];
 #pragma unroll
-                    for (int u = 0; u < SOFT_UNROLL; ++u) {
-                        if (i + u * G >= cut.packs) break;
-                        Pack<T, V> r;
+            for (int u = 0; u < SOFT_UNROLL; ++u) p[u] = zp[i + u * G < cut.packs ? i + u * G : i];
 #pragma unroll
-                        for (int j = 0; j < V; ++j) r.v[j] = (T)(exp2_hw(((float)p[u].v[j] - st.x) * c) * fi);
-                        gp[i + u * G] = r;
-                    }
-                }
-            } else {
+            for (int u = 0; u < SOFT_UNROLL; ++u) {
+                if (i + u * G >= cut.packs) break;
                 Pack<T, V> r;
 #pragma unroll
-                for (int j = 0; j < V; ++j) r.v[j] = (T)0.0f;
-                for (uint32_t i = lane; i < cut.packs; i += G) gp[i] = r;
+                for (int j = 0; j < V; ++j) r.v[j] = (T)(exp2_hw(((float)p[u].v[j] - st.x) * c) * fi);
+                gp[i + u * G] = r;
             }
         }
-        // the listed classes again, from the full-precision value: one lane per class (its first entry)
-        const Label l = row_label<G>(a, row, live && any, lane, c, lds);
-        L::sync();
-        if (live && any)
-            for (size_t k = lane; k < a.k; k += G) {
-                long long id, other;
-                float t = entry_score(a, row, k, id);
-                if (t == -__builtin_inff() || id >= (long long)a.classes) continue;
-                float q = 0.0f;
-                bool first = true;
-                for (size_t j = 0; j < a.k; ++j) {
-                    t = entry_score(a, row, j, other);
-                    if (other != id || t == -__builtin_inff()) continue;
-                    if (j < k) first = false;
-                    q += exp2_hw((t - l.top) * c) * l.inv;
-                }
-                if (first) g[id] = (T)(f * (exp2_hw(((float)z[id] - st.x) * c) * st.y - q));
-            }
-        L::sync();
+        row_sync<G>();
+        if (labeller) {
+            const Label l = wave_label(a, row, c, L.ids[slot], L.ws[slot]);
+            patch_row<T>(a, l, L.ids[slot], L.ws[slot], z, g, st.x, st.y, f, c);
+            wave_sync();
+        }
     }
+}
+
+// Value and gradient in one pass: the row stays in the registers of its workgroup (ITEMS packs to a thread) between the
+// statistics and the gradient, so the scores are read once and the gradient is written once.
+template <typename T, int V, int G, int ITEMS>
+__global__ __launch_bounds__(G) void distill_both_rows_kernel(const DistillArgs a) {
+    __shared__ RowsLds<G> L;
+    const int lane = threadIdx.x;
+    const float rt = 1.0f / a.temperature, c = LOG2E * rt;
+    const float f = a.temperature * row_weight<G>(a, reinterpret_cast<uint32_t*>(L.ms));
+    float total = 0.0f;
+    uint32_t count = 0;
+    for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* z = reinterpret_cast<const T*>(a.logits) + row * a.row_stride;
+        T* g = reinterpret_cast<T*>(a.grad) + row * a.g_row;
+        const Cut cut = cut_row<T, V>(z, a.classes);
+        const char* zp = reinterpret_cast<const char*>(z + cut.head);      // (a uniform base and 32-bit offsets: one register
+        char* gp = reinterpret_cast<char*>(g + cut.head);                  // per address instead of two)
+        if (!wave_any(a, row)) {                          // (the same in every wave: the row is not read)
+            Pack<T, V> r;
+#pragma unroll
+            for (int j = 0; j < V; ++j) r.v[j] = (T)0.0f;
+            for (uint32_t i = lane; i < cut.packs; i += G) *reinterpret_cast<Pack<T, V>*>(gp + i * 16u) = r;
+            if (lane < (int)cut.singles) g[cut.single(lane)] = (T)0.0f;
+            if (lane == 0 && a.row_loss) a.row_loss[row] = 0.0f;
+            continue;
+        }
+        // (the label first, by the first wave alone: the other waves' loads are on their way meanwhile)
+        Label l;
+        if (threadIdx.x < 64) l = wave_label(a, row, c, L.ids[0], L.ws[0]);
+        words_t p[ITEMS];
+        uint32_t at = lane;
+        forget(at);                                       // (offsets are formed where they are used rather than kept)
+#pragma unroll
+        for (int u = 0; u < ITEMS; ++u)                   // (behind the row's last pack: that pack again, not used)
+            p[u] = *reinterpret_cast<const words_t*>(zp + (at + u * G < cut.packs ? at + u * G : cut.packs - 1) * 16u);
+        const bool has_single = lane < (int)cut.singles;  // (at most 2 V - 2 of them, fewer than a wave)
+        const float single = has_single ? (float)z[cut.single(lane)] : 0.0f;
+        float m = has_single ? single : -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < ITEMS; ++u)
+            if ((uint32_t)(lane + u * G) < cut.packs) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) m = fmaxf(m, word_elem<T>(p[u], j));
+            }
+#pragma unroll
+        for (int u = 0; u < ITEMS; ++u) forget(p[u]);
+        const float off = m == -__builtin_inff() ? 0.0f : m;
+        float s = has_single ? exp2_hw((single - off) * c) : 0.0f;
+#pragma unroll
+        for (int u = 0; u < ITEMS; ++u)
+            if ((uint32_t)(lane + u * G) < cut.packs) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) s += exp2_hw((word_elem<T>(p[u], j) - off) * c);
+            }
+#pragma unroll
+        for (int u = 0; u < ITEMS; ++u) forget(p[u]);
+        row_soft<G>(m, s, c, L);
+        if (threadIdx.x < 64) {
+            float d = label_value(a, row, l, L.ids[0], L.ws[0], lane, 64, m, s, rt, [&](int id) { return (float)z[id]; });
+            d = group_sum<64>(d) * (a.temperature * a.temperature);
+            if (lane == 0) {
+                if (a.row_loss) a.row_loss[row] = d;
+                total += d;
+                ++count;
+                L.label = l;
+            }
+        }
+        const float inv = 1.0f / s, fi = f * inv;
+        forget(at);
+#pragma unroll
+        for (int u = 0; u < ITEMS; ++u)
+            if (at + u * G < cut.packs) {
+                Pack<T, V> r;
+#pragma unroll
+                for (int j = 0; j < V; ++j) r.v[j] = (T)(exp2_hw((word_elem<T>(p[u], j) - m) * c) * fi);
+                *reinterpret_cast<Pack<T, V>*>(gp + (at + u * G) * 16u) = r;
+            }
+        if (has_single) g[cut.single(lane)] = (T)(exp2_hw((single - m) * c) * fi);
+        __syncthreads();
+        if (L.label.broken) {                             // (uniform; rare: an index past the classes)
+            for (uint32_t i = lane; i < a.classes; i += G) g[i] = (T)__builtin_nanf("");
+        } else if (threadIdx.x < 64) {
+            patch_row<T>(a, l, L.ids[0], L.ws[0], z, g, m, inv, f, c);
+        }
+        if (threadIdx.x < 64) wave_sync();
+    }
+    store_part<G>(a, total, count, L.ms);
+}
+
+// ---- short rows, one behind the other: a workgroup takes `tile` rows at a time through LDS, so that memory is moved in
+// whole packs whatever the row length; 256 / tile lanes work on a row there.
+constexpr int TILE_BYTES = 32768, TILE_LABEL_BYTES = 24576, TILE_PACKS = TILE_BYTES / 16 / 256;
+constexpr int VALUE = 1, GRADIENT = 2;
+__host__ __device__ constexpr size_t tile_lds(size_t tile, size_t classes, size_t k, size_t bytes) {
+    return (tile * classes * bytes + 15) / 16 * 16 + tile * k * 12;
+}
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void distill_tile_kernel(const DistillArgs a, int tile) {
+    extern __shared__ words_t tile_mem[];
+    __shared__ float lds[16];
+    T* rows = reinterpret_cast<T*>(tile_mem);
+    float* ts = reinterpret_cast<float*>(tile_mem + ((size_t)tile * a.classes * sizeof(T) + 15) / 16);
+    int* ids = reinterpret_cast<int*>(ts + tile * (int)a.k);
+    float* ws = reinterpret_cast<float*>(ids + tile * (int)a.k);
+    const int K = (int)a.k, C = (int)a.classes, LANES = 256 / tile, r = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const float rt = 1.0f / a.temperature, c = LOG2E * rt;
+    float f_all = a.temperature;
+    if (MODE == GRADIENT) f_all *= a.weight ? *a.weight : 1.0f;
+    if (MODE == (VALUE | GRADIENT)) f_all *= row_weight<256>(a, reinterpret_cast<uint32_t*>(lds));
+    float total = 0.0f;
+    uint32_t count = 0;
+    T* z = rows + r * C;
+    int* id = ids + r * K;
+    float *t = ts + r * K, *w = ws + r * K;
+    for (size_t first = (size_t)blockIdx.x * tile; first < a.rows; first += (size_t)gridDim.x * tile) {
+        const int n = a.rows - first < (size_t)tile ? (int)(a.rows - first) : tile;
+        const int elems = n * C, packs = (int)(elems * sizeof(T) / 16), rest = packs * (16 / (int)sizeof(T));
+        const T* src = reinterpret_cast<const T*>(a.logits) + first * C;
+        {
+            words_t in[TILE_PACKS];
+#pragma unroll
+            for (int u = 0; u < TILE_PACKS; ++u) {
+                const int i = u * 256 + threadIdx.x;
+                if (i < packs) in[u] = reinterpret_cast<const words_t*>(src)[i];
+            }
+            for (int e = threadIdx.x; e < n * K; e += 256) {
+                const int er = e / K, k = e - er * K;
+                long long index;
+                ts[e] = entry_score(a, first + er, k, index);
+                ids[e] = entry_class(a, ts[e], index);
+            }
+#pragma unroll
+            for (int u = 0; u < TILE_PACKS; ++u) {
+                const int i = u * 256 + threadIdx.x;
+                if (i < packs) tile_mem[i] = in[u];
+            }
+            if (rest + (int)threadIdx.x < elems) rows[rest + threadIdx.x] = src[rest + threadIdx.x];
+        }
+        __syncthreads();
+        const size_t row = first + r;
+        const bool live = r < n;
+        // the label (the lanes of a row are neighbours in one wave: no barrier)
+        Label l;
+        float flags = 0.0f, sum = 0.0f;
+        l.top = -__builtin_inff();
+        if (live)
+            for (int k = lane; k < K; k += LANES) {
+                if (id[k] < 0) continue;
+                flags = fmaxf(flags, id[k] == ID_BROKEN ? 2.0f : 1.0f);
+                l.top = fmaxf(l.top, t[k]);
+            }
+        for (int o = 1; o < LANES; o <<= 1) {
+            flags = fmaxf(flags, __shfl_xor(flags, o, 64));
+            l.top = fmaxf(l.top, __shfl_xor(l.top, o, 64));
+        }
+        l.any = flags > 0.0f;
+        l.broken = flags > 1.5f;
+        if (live)
+            for (int k = lane; k < K; k += LANES) {
+                w[k] = id[k] < 0 ? 0.0f : exp2_hw((t[k] - l.top) * c);
+                sum += w[k];
+            }
+        for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor(sum, o, 64);
+        l.inv = 1.0f / sum;
+        wave_sync();
+        float m = -__builtin_inff(), s = 0.0f, inv = 0.0f;
+        if (MODE & VALUE) {
+            if (live && l.any) {
+                int col = lane;
+                for (; col + 7 * LANES < C; col += 8 * LANES) {
+                    float v[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) v[u] = (float)z[col + u * LANES];
+                    soft_add<8>(m, s, v, c);
+                }
+                for (; col < C; col += LANES) {
+                    const float v = (float)z[col];
+                    soft_add<1>(m, s, &v, c);
+                }
+            }
+            for (int o = 1; o < LANES; o <<= 1) {
+                const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
+                soft_merge(m, s, m2, s2, c);
+            }
+            inv = l.broken ? __builtin_nanf("") : 1.0f / s;
+            float d = 0.0f;
+            if (live && l.any) {
+                const float more = (log2_hw(l.inv) + log2_hw(s)) * LN2;
+                for (int k = lane; k < K; k += LANES) {
+                    if (id[k] < 0) continue;
+                    if (id[k] == ID_BROKEN) d = __builtin_nanf("");
+                    else if (w[k] * l.inv != 0.0f) d += w[k] * l.inv * (((t[k] - l.top) - ((float)z[id[k]] - m)) * rt + more);
+                }
+            }
+            for (int o = 1; o < LANES; o <<= 1) d += __shfl_xor(d, o, 64);
+            d *= a.temperature * a.temperature;
+            if (live && lane == 0) {
+                if (!(MODE & GRADIENT)) a.stats[row] = l.any ? make_float2(m, inv) : make_float2(0.0f, 0.0f);
+                if (a.row_loss) a.row_loss[row] = d;
+                total += d;
+                count += l.any ? 1u : 0u;
+            }
+        } else if (live) {
+            const float2 st = a.stats[row];
+            m = st.x;
+            inv = st.y;
+        }
+        if (MODE & GRADIENT) {
+            float f = f_all;
+            if (MODE == GRADIENT && a.scale && live) f *= a.scale[a.reduction == 0 ? row : 0];
+            const float fi = f * inv;
+            // (the listed classes' values first, while the scores are still there: they wait in t)
+            if (live && l.any)
+                for (int k = lane; k < K; k += LANES) {
+                    if (id[k] < 0 || id[k] == ID_BROKEN) continue;
+                    float q = 0.0f;
+                    for (int j = 0; j < K; ++j) q += id[j] == id[k] ? w[j] : 0.0f;
+                    t[k] = f * (exp2_hw(((float)z[id[k]] - m) * c) * inv - q * l.inv);
+                }
+            wave_sync();
+            if (live)
+                for (int col = lane; col < C; col += LANES) z[col] = l.any ? (T)(exp2_hw(((float)z[col] - m) * c) * fi) : (T)0.0f;
+            wave_sync();
+            if (live && l.any)      // (entries of the same class hold the same value)
+                for (int k = lane; k < K; k += LANES)
+                    if (id[k] >= 0 && id[k] != ID_BROKEN) z[id[k]] = (T)t[k];
+            __syncthreads();
+            T* dst = reinterpret_cast<T*>(a.grad) + first * C;
+#pragma unroll
+            for (int u = 0; u < TILE_PACKS; ++u) {
+                const int i = u * 256 + threadIdx.x;
+                if (i < packs) reinterpret_cast<words_t*>(dst)[i] = tile_mem[i];
+            }
+            if (rest + (int)threadIdx.x < elems) dst[rest + threadIdx.x] = rows[rest + threadIdx.x];
+        }
+        __syncthreads();
+    }
+    if (MODE & VALUE) store_part<256>(a, total, count, lds);
 }
 
 // ---- planes: a lane takes a pixel; its label is a column of `classes` weights in LDS (only its own lane touches it)
@@ -433,10 +754,8 @@ __global__ __launch_bounds__(64) void distill_fwd_planes_kernel(const DistillArg
         ++count;
         plane_clear(a, row, col);
     }
-    total = group_sum<64>(total);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) count += __shfl_xor(count, o, 64);
-    if (lane == 0) a.part[blockIdx.x] = make_float2(total, __uint_as_float(count));
+    __shared__ float lds[2];
+    store_part<64>(a, total, count, lds);
 }
 
 template <typename T>
@@ -600,10 +919,7 @@ __global__ __launch_bounds__(256) void distill_fwd_wide_kernel(const DistillArgs
             total += d;
         }
     }
-    total = group_sum<64>(total);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) count += __shfl_xor(count, o, 64);
-    store_part<4, 64>(total, count, a.part, lds);
+    store_part<256>(a, total, count, lds);
 }
 
 template <typename T, int P, int KR>
@@ -657,16 +973,15 @@ __global__ __launch_bounds__(256) void distill_bwd_wide_kernel(const DistillArgs
     }
 }
 
-// loss[0] = sum of the partial sums (over the labelled rows for the mean), loss[1] = the weight of a row
-__global__ __launch_bounds__(1024) void distill_join_kernel(uint32_t nparts, const float2* __restrict__ part, int reduction,
-                                                            float* __restrict__ loss) {
+// the value from the workgroups' partial sums
+__global__ __launch_bounds__(1024) void distill_join_kernel(const DistillArgs a, uint32_t nparts) {
     __shared__ double sums[16];
     __shared__ unsigned long long counts[16];
     double s = 0.0;
     unsigned long long n = 0;
     for (uint32_t i = threadIdx.x; i < nparts; i += 1024) {
-        s += (double)part[i].x;
-        n += __float_as_uint(part[i].y);
+        s += (double)a.part[i].x;
+        n += __float_as_uint(a.part[i].y);
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) { s += __shfl_xor(s, o, 64); n += __shfl_xor(n, o, 64); }
@@ -674,9 +989,7 @@ __global__ __launch_bounds__(1024) void distill_join_kernel(uint32_t nparts, con
     __syncthreads();
     if (threadIdx.x != 0) return;
     for (int w = 1; w < 16; ++w) { s += sums[w]; n += counts[w]; }
-    const double weight = reduction == 1 ? 1.0 / (double)(n ? n : 1) : 1.0;
-    loss[0] = (float)(s * weight);
-    loss[1] = (float)weight;
+    store_loss(a, s, n);
 }
 
 bool planes_layout(size_t row_stride, size_t class_stride) { return class_stride != 1 && row_stride == 1; }
@@ -686,26 +999,49 @@ unsigned distill_blocks(size_t rows, int per_block) {
     return (unsigned)(need < DISTILL_BLOCKS ? need : DISTILL_BLOCKS);
 }
 
-// Lanes of a row: 16 for a few classes, a wave up to some thousand, a workgroup beyond that.
-int row_lanes(size_t classes) { return classes <= 64 ? 16 : classes <= 2048 ? 64 : classes <= 16384 ? 256 : 1024; }
+// Rows of a tile: as many as fit (a power of two, so that a lane count of 256 / tile stays inside a wave), fewer when the
+// launch would not fill the chip otherwise.  0: the rows do not lie one behind the other from a 16-byte boundary on, or
+// fewer than 8 fit.
+int tile_rows(const DistillArgs& a, bool gradient) {
+    const size_t b = e3_elem_bytes(a.dtype);
+    if (a.row_stride != a.classes || (reinterpret_cast<uintptr_t>(a.logits) & 15) != 0) return 0;
+    if (gradient && (a.g_row != a.classes || (reinterpret_cast<uintptr_t>(a.grad) & 15) != 0)) return 0;
+    size_t t = 256;
+    while (t >= 8 && (t * a.classes * b > TILE_BYTES || t * a.k * 12 > TILE_LABEL_BYTES)) t >>= 1;
+    while (t > 8 && a.rows < t * 512) t >>= 1;
+    return t >= 8 ? (int)t : 0;
+}
+template <typename T, int MODE>
+int distill_tile(const DistillArgs& a, int tile, unsigned& blocks, hipStream_t s) {
+    blocks = distill_blocks(a.rows, tile);
+    distill_tile_kernel<T, MODE><<<dim3(blocks), dim3(256), tile_lds(tile, a.classes, a.k, sizeof(T)), s>>>(a, tile);
+    LAUNCH_OK("distill_tile_kernel");
+    return 0;
+}
 
+// Threads of a long row: a wave up to some thousand classes, a workgroup beyond that.
 template <typename T, int V>
 int distill_rows(const DistillArgs& a, bool backward, unsigned& blocks, hipStream_t s) {
-#define E3_ROWS(G)                                                                                            \
-    {                                                                                                         \
-        blocks = distill_blocks(a.rows, Lanes<G>::ROWS);                                                      \
-        if (backward) distill_bwd_rows_kernel<T, V, G><<<dim3(blocks), dim3(Lanes<G>::THREADS), 0, s>>>(a);   \
-        else distill_fwd_rows_kernel<T, V, G><<<dim3(blocks), dim3(Lanes<G>::THREADS), 0, s>>>(a);            \
+#define E3_ROWS(G)                                                                                              \
+    {                                                                                                           \
+        blocks = distill_blocks(a.rows, RowsLds<G>::ROWS);                                                      \
+        if (backward) distill_bwd_rows_kernel<T, V, G><<<dim3(blocks), dim3(RowsLds<G>::THREADS), 0, s>>>(a);   \
+        else distill_fwd_rows_kernel<T, V, G><<<dim3(blocks), dim3(RowsLds<G>::THREADS), 0, s>>>(a);            \
     }
-    switch (row_lanes(a.classes)) {
-        case 16: E3_ROWS(16) break;
-        case 64: E3_ROWS(64) break;
-        case 256: E3_ROWS(256) break;
-        default: E3_ROWS(1024)
-    }
+    if (a.classes <= 2048) E3_ROWS(64)
+    else if (a.classes <= 16384) E3_ROWS(256)
+    else E3_ROWS(1024)
 #undef E3_ROWS
     LAUNCH_OK("distill_rows_kernel");
     return 0;
+}
+
+// Packs need the scores and their gradient to lie the same way to a 16-byte boundary in every row.
+template <typename T>
+bool rows_wide(const DistillArgs& a, bool gradient) {
+    if (!gradient) return true;
+    return ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0 &&
+           (a.row_stride * sizeof(T)) % 16 == (a.g_row * sizeof(T)) % 16;
 }
 
 // pixels per lane: 4 for the gradient; 2 for the value, whose registers (the scores of the label's entries) would leave two
@@ -750,17 +1086,57 @@ int distill_t(const DistillArgs& a, bool backward, unsigned& blocks, hipStream_t
         LAUNCH_OK("distill_planes_kernel");
         return 0;
     }
-    // packs need the scores and their gradient to lie the same way to a 16-byte boundary in every row
-    const uintptr_t zp = reinterpret_cast<uintptr_t>(a.logits), gp = reinterpret_cast<uintptr_t>(backward ? a.grad : a.logits);
-    const size_t gr = backward ? a.g_row : a.row_stride;
-    const bool wide = zp % sizeof(T) == 0 && ((zp ^ gp) & 15) == 0 && (a.row_stride * sizeof(T)) % 16 == (gr * sizeof(T)) % 16;
-    return wide ? distill_rows<T, Wide<T>::N>(a, backward, blocks, s) : distill_rows<T, 1>(a, backward, blocks, s);
+    if (const int tile = tile_rows(a, backward))
+        return backward ? distill_tile<T, GRADIENT>(a, tile, blocks, s) : distill_tile<T, VALUE>(a, tile, blocks, s);
+    return rows_wide<T>(a, backward) ? distill_rows<T, Wide<T>::N>(a, backward, blocks, s) : distill_rows<T, 1>(a, backward, blocks, s);
 }
-
 int distill_any(const DistillArgs& a, bool backward, unsigned& blocks, hipStream_t s) {
     if (a.dtype == E3_F32) return distill_t<float>(a, backward, blocks, s);
     if (a.dtype == E3_F16) return distill_t<f16_t>(a, backward, blocks, s);
     return distill_t<bf16_t>(a, backward, blocks, s);
+}
+
+// Value and gradient in one pass over the scores.  blocks = 0: no such kernel for these (the caller runs both passes):
+// planes, rows too long for the registers of a workgroup, short rows that do not lie one behind the other.
+template <typename T>
+int distill_both_t(DistillArgs a, uint32_t* counts, unsigned& blocks, hipStream_t s) {
+    constexpr int V = Wide<T>::N;
+    blocks = 0;
+    if (planes_layout(a.row_stride, a.class_stride)) return 0;
+    const int tile = tile_rows(a, true);
+    const size_t packs = a.classes / V;
+    if (!tile && (a.classes * sizeof(T) <= 4096 || packs > 16384 || !rows_wide<T>(a, true))) return 0;
+    blocks = distill_blocks(a.rows, tile ? tile : 1);
+    if (a.reduction == 1 && blocks > 1) {
+        const size_t need = (a.rows * a.k + 255) / 256;
+        a.counts = counts;
+        a.ncounts = (uint32_t)(need < COUNT_BLOCKS ? need : COUNT_BLOCKS);
+        distill_count_kernel<<<dim3(a.ncounts), dim3(256), 0, s>>>(a, counts);
+        LAUNCH_OK("distill_count_kernel");
+    }
+    if (tile) return distill_tile<T, VALUE | GRADIENT>(a, tile, blocks, s);
+    if (packs <= 1024) distill_both_rows_kernel<T, V, 256, 4><<<dim3(blocks), dim3(256), 0, s>>>(a);
+    else if (packs <= 2048) distill_both_rows_kernel<T, V, 256, 8><<<dim3(blocks), dim3(256), 0, s>>>(a);
+    else if (packs <= 4096) distill_both_rows_kernel<T, V, 256, 16><<<dim3(blocks), dim3(256), 0, s>>>(a);
+    else if (packs <= 8192) distill_both_rows_kernel<T, V, 1024, 8><<<dim3(blocks), dim3(1024), 0, s>>>(a);
+    else distill_both_rows_kernel<T, V, 1024, 16><<<dim3(blocks), dim3(1024), 0, s>>>(a);
+    LAUNCH_OK("distill_both_rows_kernel");
+    return 0;
+}
+int distill_both(const DistillArgs& a, uint32_t* counts, unsigned& blocks, hipStream_t s) {
+    if (a.dtype == E3_F32) return distill_both_t<float>(a, counts, blocks, s);
+    if (a.dtype == E3_F16) return distill_both_t<f16_t>(a, counts, blocks, s);
+    return distill_both_t<bf16_t>(a, counts, blocks, s);
+}
+DistillArgs distill_args(size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride, size_t class_stride,
+                         int dtype, const void* teacher, size_t t_row, size_t t_entry, int teacher_dtype, const void* index,
+                         size_t i_row, size_t i_entry, int index_bytes, float temperature, int reduction) {
+    DistillArgs a{};
+    a.rows = rows; a.classes = (uint32_t)classes; a.k = k; a.logits = logits; a.row_stride = row_stride;
+    a.class_stride = class_stride; a.dtype = dtype; a.teacher = teacher; a.t_row = t_row; a.t_entry = t_entry;
+    a.teacher_dtype = teacher_dtype; a.index = index; a.i_row = i_row; a.i_entry = i_entry; a.index_bytes = index_bytes;
+    a.temperature = temperature; a.reduction = reduction;
+    return a;
 }
 }  // namespace
 
@@ -769,29 +1145,40 @@ bool e3_distill_layout_ok(size_t rows, size_t classes, size_t row_stride, size_t
 }
 size_t e3_distill_scratch_bytes(size_t rows) {
     (void)rows;
-    return DISTILL_BLOCKS * sizeof(float2) + 256;
+    return DISTILL_BLOCKS * sizeof(float2) + COUNT_BLOCKS * sizeof(uint32_t) + 256;
 }
 
 int e3_distill_forward_impl(size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride,
                             size_t class_stride, int dtype, const void* teacher, size_t t_row, size_t t_entry,
                             int teacher_dtype, const void* index, size_t i_row, size_t i_entry, int index_bytes,
-                            float temperature, int reduction, float* stats, float* row_loss, float* loss, char* scratch,
-                            hipStream_t s) {
-    DistillArgs a{};
-    a.rows = rows; a.classes = (uint32_t)classes; a.k = k; a.logits = logits; a.row_stride = row_stride;
-    a.class_stride = class_stride; a.dtype = dtype; a.teacher = teacher; a.t_row = t_row; a.t_entry = t_entry;
-    a.teacher_dtype = teacher_dtype; a.index = index; a.i_row = i_row; a.i_entry = i_entry; a.index_bytes = index_bytes;
-    a.temperature = temperature; a.reduction = reduction; a.stats = reinterpret_cast<float2*>(stats);
-    a.row_loss = row_loss; a.part = reinterpret_cast<float2*>(scratch);
+                            float temperature, int reduction, float* stats, float* row_loss, float* loss, void* grad,
+                            size_t g_row, size_t g_class, char* scratch, hipStream_t s) {
+    DistillArgs a = distill_args(rows, classes, k, logits, row_stride, class_stride, dtype, teacher, t_row, t_entry,
+                                 teacher_dtype, index, i_row, i_entry, index_bytes, temperature, reduction);
+    a.stats = reinterpret_cast<float2*>(stats);
+    a.row_loss = row_loss;
+    a.loss = loss;
+    a.part = reinterpret_cast<float2*>(scratch);
+    uint32_t* counts = reinterpret_cast<uint32_t*>(a.part + DISTILL_BLOCKS);
     unsigned blocks = 0;
-    if (rows > 0) {
-        const int rc = distill_any(a, false, blocks, s);
+    int rc = 0;
+    if (grad) {
+        a.grad = grad;
+        a.g_row = g_row;
+        a.g_class = g_class;
+        if (rows > 0) rc = distill_both(a, counts, blocks, s);
         if (rc) return rc;
     }
-    if (!loss) return 0;
-    distill_join_kernel<<<dim3(1), dim3(1024), 0, s>>>(blocks, a.part, reduction, loss);
-    LAUNCH_OK("distill_join_kernel");
-    return 0;
+    const bool both = blocks > 0;
+    if (!both && rows > 0) rc = distill_any(a, false, blocks, s);
+    if (rc) return rc;
+    if (blocks != 1) {
+        distill_join_kernel<<<dim3(1), dim3(1024), 0, s>>>(a, blocks);
+        LAUNCH_OK("distill_join_kernel");
+    }
+    if (!grad || both || rows == 0) return 0;
+    a.weight = loss + 1;
+    return distill_any(a, true, blocks, s);
 }
 
 int e3_distill_backward_impl(size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride,
@@ -800,12 +1187,14 @@ int e3_distill_backward_impl(size_t rows, size_t classes, size_t k, const void* 
                              float temperature, int reduction, const float* stats, const float* loss, const float* d_loss,
                              void* grad, size_t g_row, size_t g_class, hipStream_t s) {
     if (rows == 0) return 0;
-    DistillArgs a{};
-    a.rows = rows; a.classes = (uint32_t)classes; a.k = k; a.logits = logits; a.row_stride = row_stride;
-    a.class_stride = class_stride; a.dtype = dtype; a.teacher = teacher; a.t_row = t_row; a.t_entry = t_entry;
-    a.teacher_dtype = teacher_dtype; a.index = index; a.i_row = i_row; a.i_entry = i_entry; a.index_bytes = index_bytes;
-    a.temperature = temperature; a.reduction = reduction; a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
-    a.weight = loss ? loss + 1 : nullptr; a.scale = d_loss; a.grad = grad; a.g_row = g_row; a.g_class = g_class;
+    DistillArgs a = distill_args(rows, classes, k, logits, row_stride, class_stride, dtype, teacher, t_row, t_entry,
+                                 teacher_dtype, index, i_row, i_entry, index_bytes, temperature, reduction);
+    a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
+    a.weight = loss + 1;
+    a.scale = d_loss;
+    a.grad = grad;
+    a.g_row = g_row;
+    a.g_class = g_class;
     unsigned blocks = 0;
     return distill_any(a, true, blocks, s);
 }

@@ -20,6 +20,27 @@ struct Wide {
     static constexpr int N = 16 / (int)sizeof(T);
 };
 
+// A 16-byte pack that is kept in registers across phases of a kernel: four words that the compiler does not split into
+// elements (a 16-bit element would take a register of its own).
+typedef uint32_t words_t __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ float word_elem(words_t q, int j);
+template <>
+__device__ __forceinline__ float word_elem<float>(words_t q, int j) { return __uint_as_float(q[j]); }
+template <>
+__device__ __forceinline__ float word_elem<bf16_t>(words_t q, int j) {
+    return __uint_as_float(j & 1 ? q[j >> 1] & 0xFFFF0000u : q[j >> 1] << 16);
+}
+template <>
+__device__ __forceinline__ float word_elem<f16_t>(words_t q, int j) {
+    const uint16_t h = (uint16_t)(j & 1 ? q[j >> 1] >> 16 : q[j >> 1]);
+    return (float)__builtin_bit_cast(f16_t, h);
+}
+// Makes the compiler forget what it knows about a pack, so that it converts the elements again in the next phase instead of
+// holding their fp32 values.
+__device__ __forceinline__ void forget(words_t& q) { asm volatile("" : "+v"(q)); }
+__device__ __forceinline__ void forget(uint32_t& x) { asm volatile("" : "+v"(x)); }
+
 static inline size_t e3_elem_bytes(int dtype) { return dtype == E3_F32 ? 4 : 2; }
 static inline bool e3_dtype_ok(int dtype) { return dtype >= E3_F32 && dtype <= E3_BF16; }
 

@@ -779,6 +779,8 @@ int e3dgs_layer_norm_backward(size_t rows, size_t dim, const void* grad_out, siz
  *   stats     2 floats per row, for the backward call
  *   row_loss  one float per row (may be NULL)
  *   loss      2 floats: the value (sum or mean; for `none` the sum) and the weight of a row, for the backward call
+ *   grad      (may be NULL) the gradient of the value by logits, in the same pass where the layout allows; for `none` of the
+ *             sum.  Then stats is scratch
  * backward: d_loss = the gradient of the value (device; one float, or with reduction 0 one per row; NULL: 1); grad has the
  * layout kind of logits with strides of its own, every element of it is written.
  * scratch: e3dgs_distill_scratch_bytes(rows) bytes, 8-B aligned.
@@ -790,7 +792,7 @@ int e3dgs_distill_forward(size_t rows, size_t classes, size_t k, const void* log
                           int dtype, const void* teacher, size_t teacher_row_stride, size_t teacher_entry_stride,
                           int teacher_dtype, const void* index, size_t index_row_stride, size_t index_entry_stride,
                           int index_bytes, float temperature, int reduction, float* stats, float* row_loss, float* loss,
-                          char* scratch, void* stream);
+                          void* grad, size_t grad_row_stride, size_t grad_class_stride, char* scratch, void* stream);
 int e3dgs_distill_backward(size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride, size_t class_stride,
                            int dtype, const void* teacher, size_t teacher_row_stride, size_t teacher_entry_stride,
                            int teacher_dtype, const void* index, size_t index_row_stride, size_t index_entry_stride,
