@@ -22,23 +22,22 @@ int launch_radix_sort_pairs(uint32_t* k0, uint32_t* k1, uint32_t* v0, uint32_t* 
 // One thread moves EMBED_PACKS packs of the flat output, a workgroup's packs are contiguous: every lane works whatever the
 // row length, the stores are whole lines, and the rows of a pack-block are found by one division each.
 constexpr int EMBED_PACKS = 4;
-template <typename T, int V>
+template <typename T, int V, typename I>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(size_t n, long long rows, uint32_t ppr /* packs per row */,
-                                                        const void* __restrict__ index, int index_bytes,
-                                                        const T* __restrict__ table, size_t stride, float scale,
+                                                        const I* __restrict__ index, const T* __restrict__ table, size_t stride, float scale,
                                                         T* __restrict__ out) {
     const size_t total = n * (size_t)ppr, base = (size_t)blockIdx.x * (256 * EMBED_PACKS);
     const size_t row0 = base / ppr;                                  // (uniform)
     const uint32_t rem0 = (uint32_t)(base - row0 * ppr);
-    long long id[EMBED_PACKS];
+    I id[EMBED_PACKS];
     uint32_t col[EMBED_PACKS];
     Pack<T, V> p[EMBED_PACKS];
 #pragma unroll
     for (int u = 0; u < EMBED_PACKS; ++u) {
         const uint32_t x = rem0 + (uint32_t)u * 256 + threadIdx.x, q = x / ppr;
         col[u] = x - q * ppr;
-        const bool ok = base + (size_t)u * 256 + threadIdx.x < total;
-        id[u] = ok ? load_index(index, row0 + q, index_bytes) : -1;
+        const size_t row = row0 + q;
+        id[u] = index[row < n ? row : n - 1];                        // (unconditional loads, all in flight)
     }
 #pragma unroll
     for (int u = 0; u < EMBED_PACKS; ++u) {
@@ -57,19 +56,19 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(size_t n, long long rows
     }
 }
 
-template <typename T>
-static int embed_fwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_bytes, const void* table,
-                       size_t stride, int dtype, float scale, void* out, hipStream_t s) {
+template <typename T, typename I>
+static int embed_fwd_t(size_t n, size_t rows, size_t dim, const void* index, const void* table, size_t stride, int dtype,
+                       float scale, void* out, hipStream_t s) {
     const bool wide = e3_rows_wide(table, stride, dim, dtype) && e3_rows_wide(out, dim, dim, dtype);
     const size_t ppr = wide ? dim / Wide<T>::N : dim;
     const size_t blocks = (n * ppr + 256 * EMBED_PACKS - 1) / (256 * EMBED_PACKS);
     if (blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_forward: too many values");
     if (wide)
-        embed_fwd_kernel<T, Wide<T>::N><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(
-            n, (long long)rows, (uint32_t)ppr, index, index_bytes, (const T*)table, stride, scale, (T*)out);
+        embed_fwd_kernel<T, Wide<T>::N, I><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(
+            n, (long long)rows, (uint32_t)ppr, (const I*)index, (const T*)table, stride, scale, (T*)out);
     else
-        embed_fwd_kernel<T, 1><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(
-            n, (long long)rows, (uint32_t)ppr, index, index_bytes, (const T*)table, stride, scale, (T*)out);
+        embed_fwd_kernel<T, 1, I><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(
+            n, (long long)rows, (uint32_t)ppr, (const I*)index, (const T*)table, stride, scale, (T*)out);
     LAUNCH_OK("embed_fwd_kernel");
     return 0;
 }
@@ -77,9 +76,10 @@ static int embed_fwd_t(size_t n, size_t rows, size_t dim, const void* index, int
 int e3_embedding_forward_impl(size_t n, size_t rows, size_t dim, const void* index, int index_bytes, const void* table,
                               size_t stride, int dtype, float scale, void* out, hipStream_t s) {
     if (n == 0) return 0;
-    if (dtype == E3_F32) return embed_fwd_t<float>(n, rows, dim, index, index_bytes, table, stride, dtype, scale, out, s);
-    if (dtype == E3_F16) return embed_fwd_t<f16_t>(n, rows, dim, index, index_bytes, table, stride, dtype, scale, out, s);
-    return embed_fwd_t<bf16_t>(n, rows, dim, index, index_bytes, table, stride, dtype, scale, out, s);
+#define E3_FWD(T) (index_bytes == 8 ? embed_fwd_t<T, long long>(n, rows, dim, index, table, stride, dtype, scale, out, s) \
+                                    : embed_fwd_t<T, int>(n, rows, dim, index, table, stride, dtype, scale, out, s))
+    return dtype == E3_F32 ? E3_FWD(float) : dtype == E3_F16 ? E3_FWD(f16_t) : E3_FWD(bf16_t);
+#undef E3_FWD
 }
 
 // ============================================================================================== embedding, gradient
@@ -119,17 +119,47 @@ __device__ __forceinline__ void embed_store(T* __restrict__ d_table, size_t dim,
     *reinterpret_cast<Pack<T, V>*>(d_table + (size_t)row * dim + col) = r;
 }
 
+// Clears the table rows without a position: a wave looks `per` rows up in the sorted keys (one lane each) and clears those
+// that are not there.
+template <typename T, int V>
+__device__ __forceinline__ void embed_zero(uint32_t n, const uint32_t* __restrict__ keys, uint32_t rows, uint32_t per,
+                                           size_t dim, T* __restrict__ d_table, size_t wave) {
+    const int lane = threadIdx.x & 63;
+    const size_t first = wave * per;
+    if (first >= rows) return;
+    bool empty = false;
+    if ((uint32_t)lane < per && first + lane < rows) {
+        const uint32_t row = (uint32_t)(first + lane), at = lower_bound_u32(keys, 0, n, row);
+        empty = at >= n || keys[at] != row;
+    }
+    unsigned long long todo = __ballot(empty);
+    Pack<T, V> z;
+#pragma unroll
+    for (int j = 0; j < V; ++j) z.v[j] = (T)0.0f;
+    while (todo) {
+        const int r = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        T* row = d_table + (first + r) * dim;
+        for (size_t col = (size_t)lane * V; col < dim; col += 64 * V) *reinterpret_cast<Pack<T, V>*>(row + col) = z;
+    }
+}
+
 constexpr int EMBED_UNROLL = 8;
 template <typename T, int V, int G>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restrict__ kept, const uint32_t* __restrict__ keys,
                                                         const uint32_t* __restrict__ pos, uint32_t chunk, uint32_t nchunks,
                                                         uint32_t nslices, size_t dim, const T* __restrict__ d_out,
                                                         size_t stride, float scale, T* __restrict__ d_table,
-                                                        float* __restrict__ part) {
+                                                        float* __restrict__ part, uint32_t sum_blocks, uint32_t rows,
+                                                        uint32_t zero_rows) {
+    const uint32_t n = *kept;
+    if (blockIdx.x >= sum_blocks) {      // (in the same launch: the sums wait for their gathers, the stores do not)
+        embed_zero<T, V>(n, keys, rows, zero_rows, dim, d_table, (size_t)(blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6));
+        return;
+    }
     const size_t unit = (size_t)blockIdx.x * (256 / G) + threadIdx.x / G;
     const uint32_t c = (uint32_t)(unit / nslices), slice = (uint32_t)(unit - (size_t)c * nslices);
     const size_t col = ((size_t)slice * G + threadIdx.x % G) * V;
-    const uint32_t n = *kept;
     if (c >= nchunks || (size_t)c * chunk >= n || col >= dim) return;
     const uint32_t j0 = c * chunk, j1 = n - j0 < chunk ? n : j0 + chunk;
     float acc[V];
@@ -175,64 +205,189 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restri
     }
 }
 
-// One workgroup per chunk (times a slice of 64 columns): if a run starts in the chunk and goes on behind it, add its
-// partials: slot 1 of this chunk, slot 0 of the following ones up to the run's end.  Wave w takes the w-th sixteenth of
-// them, the sixteen sums are added in order.
-template <typename T>
+// Adds up the partials of the runs that cross chunks: slot 1 of the chunk a run starts in, slot 0 of the following ones.
+// Workgroups of two kinds in one launch:
+//   short runs   a group of 16 lanes takes a chunk (times a slice of 16 V columns) and adds up to JOIN_SHORT partials in order
+//   long runs    a workgroup looks at JOIN_SHORT neighbouring chunks (times a slice of 16 columns): only the last run that
+//                starts among them can be longer than JOIN_SHORT partials; 64 groups of 16 lanes take a 64th of them each,
+//                the 64 sums are added in order
+constexpr uint32_t JOIN_SHORT = 32;
+struct Crossing {
+    uint32_t key, partials;      // partials 0: no run starts in the chunk and goes on behind it
+};
+__device__ __forceinline__ Crossing embed_crossing(const uint32_t* __restrict__ keys, uint32_t n, uint32_t chunk, uint32_t c) {
+    Crossing r{0u, 0u};
+    if ((size_t)(c + 1) * chunk >= n) return r;                          // nothing lies behind the chunk
+    const uint32_t j0 = c * chunk, j1 = j0 + chunk, key = keys[j1 - 1];
+    if (keys[j1] != key) return r;                                       // its last run ends with it
+    if (keys[j0] == key && j0 > 0 && keys[j0 - 1] == key) return r;      // ... or began earlier
+    const uint32_t end = lower_bound_u32(keys, j1, n, key + 1u);         // (key < rows < 2^31)
+    r.key = key;
+    r.partials = (end - 1u) / chunk - c + 1u;
+    return r;
+}
+template <typename T, int V>
 __global__ __launch_bounds__(1024) void embed_join_kernel(const uint32_t* __restrict__ kept,
-                                                          const uint32_t* __restrict__ keys, uint32_t chunk, size_t dim,
+                                                          const uint32_t* __restrict__ keys, uint32_t chunk,
+                                                          uint32_t nchunks, uint32_t short_blocks, size_t dim,
                                                           const float* __restrict__ part, float scale,
                                                           T* __restrict__ d_table) {
-    __shared__ float sums[16][64];
-    const uint32_t n = *kept, c = blockIdx.x;
-    if ((size_t)(c + 1) * chunk >= n) return;                            // nothing lies behind the chunk (uniform)
-    const uint32_t j0 = c * chunk, j1 = j0 + chunk, key = keys[j1 - 1];
-    if (keys[j1] != key) return;                                         // no run goes on (uniform)
-    if (keys[j0] == key && j0 > 0 && keys[j0 - 1] == key) return;        // it began earlier: an earlier chunk adds it up
-    const uint32_t end = lower_bound_u32(keys, j1, n, key + 1u);         // (key < rows <= 2^32 - 2)
-    const uint32_t last = (end - 1u) / chunk, m = last - c + 1u;         // m partials
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const size_t col = (size_t)blockIdx.y * 64 + lane;
-    const uint32_t lo = (uint32_t)((unsigned long long)m * wave / 16), hi = (uint32_t)((unsigned long long)m * (wave + 1) / 16);
+    __shared__ float sums[64][17];
+    __shared__ Crossing longest;
+    __shared__ uint32_t longest_chunk;
+    const uint32_t n = *kept;
+    const int g = threadIdx.x >> 4, lane = threadIdx.x & 15;
+    if (blockIdx.x < short_blocks) {
+        const uint32_t nslices = (uint32_t)((dim + 16 * V - 1) / (16 * V));
+        const size_t unit = (size_t)blockIdx.x * 64 + g;
+        const uint32_t c = (uint32_t)(unit / nslices);
+        const size_t col = ((unit - (size_t)c * nslices) * 16 + lane) * V;
+        if (c >= nchunks || col >= dim) return;
+        const Crossing r = embed_crossing(keys, n, chunk, c);
+        if (r.partials == 0 || r.partials > JOIN_SHORT) return;
+        const Pack<float, V> p = *reinterpret_cast<const Pack<float, V>*>(part + (2 * (size_t)c + 1) * dim + col);
+        float acc[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] = p.v[j];
+#pragma unroll 4
+        for (uint32_t k = 1; k < r.partials; ++k) {
+            const Pack<float, V> q = *reinterpret_cast<const Pack<float, V>*>(part + 2 * (size_t)(c + k) * dim + col);
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] += q.v[j];
+        }
+        embed_store<T, V>(d_table, dim, r.key, col, scale, acc);
+        return;
+    }
+    const uint32_t nslices = (uint32_t)((dim + 15) / 16), unit = blockIdx.x - short_blocks;
+    const uint32_t first = unit / nslices * JOIN_SHORT;
+    const size_t col = (size_t)(unit % nslices) * 16 + lane;
+    if (threadIdx.x < 64) {
+        const uint32_t c = first + threadIdx.x;
+        Crossing r{0u, 0u};
+        if (threadIdx.x < JOIN_SHORT && c < nchunks) r = embed_crossing(keys, n, chunk, c);
+        const unsigned long long hit = __ballot(r.partials > JOIN_SHORT);      // (one lane at most)
+        if (hit == 0ull) {
+            if (threadIdx.x == 0) longest.partials = 0;
+        } else if ((int)threadIdx.x == __builtin_ctzll(hit)) {
+            longest = r;
+            longest_chunk = c;
+        }
+    }
+    __syncthreads();
+    const uint32_t m = longest.partials, c = longest_chunk;
+    if (m == 0) return;                                                        // (uniform)
+    const uint32_t lo = (uint32_t)((unsigned long long)m * g / 64), hi = (uint32_t)((unsigned long long)m * (g + 1) / 64);
     float s = 0.0f;
     if (col < dim) {
 #pragma unroll 8
         for (uint32_t k = lo; k < hi; ++k) s += part[(k == 0 ? 2 * (size_t)c + 1 : 2 * (size_t)(c + k)) * dim + col];
     }
-    sums[wave][lane] = s;
+    sums[g][lane] = s;
     __syncthreads();
-    if (wave == 0 && col < dim) {
+    if (g == 0 && col < dim) {
         s = sums[0][lane];
-#pragma unroll
-        for (int w = 1; w < 16; ++w) s += sums[w][lane];
-        d_table[(size_t)key * dim + col] = (T)(scale * s);
+        for (int w = 1; w < 64; ++w) s += sums[w][lane];
+        d_table[(size_t)longest.key * dim + col] = (T)(scale * s);
     }
 }
 
-// Clears the table rows without a position: a wave looks `per` rows up in the sorted keys (one lane each) and clears those
-// that are not there.
-template <typename T, int V>
-__global__ __launch_bounds__(256) void embed_zero_kernel(const uint32_t* __restrict__ kept, const uint32_t* __restrict__ keys,
-                                                         uint32_t rows, uint32_t per, size_t dim, T* __restrict__ d_table) {
-    const int lane = threadIdx.x & 63;
-    const size_t first = ((size_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * per;
-    if (first >= rows) return;
-    const uint32_t n = *kept;
-    bool empty = false;
-    if ((uint32_t)lane < per && first + lane < rows) {
-        const uint32_t row = (uint32_t)(first + lane), at = lower_bound_u32(keys, 0, n, row);
-        empty = at >= n || keys[at] != row;
-    }
-    unsigned long long todo = __ballot(empty);
-    Pack<T, V> z;
+// Sorts up to 1024 * ITEMS positions by index in one workgroup (stable, 8 bits a pass): for few positions the launches of the
+// general sort would cost more than everything else.  A wave owns 64 * ITEMS consecutive keys and ranks 64 at a time with
+// ballots; the digits' counters of the 16 waves are joined by a prefix over waves and digits.  Indices outside the table get
+// the key `rows`, so that they end up behind the others.
+template <int ITEMS>
+struct SmallSort {
+    static constexpr int N = 1024 * ITEMS;
+    uint32_t key[N];
+    uint16_t pos[N], rank[N];
+    uint32_t cnt[16][256];
+    uint32_t wtot[4], valid;
+};
+template <int ITEMS, typename I>
+__global__ __launch_bounds__(1024) void embed_sort_small_kernel(uint32_t n, uint32_t rows, int nbits,
+                                                                const I* __restrict__ index, uint32_t* __restrict__ keys,
+                                                                uint32_t* __restrict__ pos, uint32_t* __restrict__ kept) {
+    __shared__ SmallSort<ITEMS> L;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t base = (uint32_t)wave * (64 * ITEMS) + lane;
+    const unsigned long long before = (1ull << lane) - 1ull;
+    if (threadIdx.x == 0) L.valid = 0;
+    __syncthreads();
+    I id[ITEMS];
 #pragma unroll
-    for (int j = 0; j < V; ++j) z.v[j] = (T)0.0f;
-    while (todo) {
-        const int r = __builtin_ctzll(todo);
-        todo &= todo - 1;
-        T* row = d_table + (first + r) * dim;
-        for (size_t col = (size_t)lane * V; col < dim; col += 64 * V) *reinterpret_cast<Pack<T, V>*>(row + col) = z;
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t at = base + i * 64;
+        id[i] = index[at < n ? at : n - 1];
     }
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t at = base + i * 64;
+        const bool ok = at < n && id[i] >= 0 && (long long)id[i] < (long long)rows;
+        L.key[at] = ok ? (uint32_t)id[i] : rows;
+        L.pos[at] = (uint16_t)at;
+        mine += (uint32_t)__popcll(__ballot(ok));
+    }
+    if (lane == 0) atomicAdd(&L.valid, mine);
+    for (int shift = 0; shift < nbits; shift += 8) {
+        for (int d = threadIdx.x; d < 16 * 256; d += 1024) L.cnt[d >> 8][d & 255] = 0;
+        __syncthreads();
+#pragma unroll 1
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t d = (L.key[base + i * 64] >> shift) & 255u;
+            unsigned long long peers = ~0ull;
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                const unsigned long long bal = __ballot((d >> b) & 1u);
+                peers &= ((d >> b) & 1u) ? bal : ~bal;
+            }
+            const uint32_t first = L.cnt[wave][d];
+            wave_sync();
+            if ((peers & before) == 0ull) L.cnt[wave][d] = first + (uint32_t)__popcll(peers);
+            wave_sync();
+            L.rank[base + i * 64] = (uint16_t)(first + (uint32_t)__popcll(peers & before));
+        }
+        __syncthreads();
+        if (threadIdx.x < 256) {
+            uint32_t c[16], total = 0;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) { c[w] = L.cnt[w][threadIdx.x]; total += c[w]; }
+            uint32_t inc = total;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) { const uint32_t t = __shfl_up(inc, o, 64); if (lane >= o) inc += t; }
+            if (lane == 63) L.wtot[wave] = inc;
+            uint32_t run = inc - total;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) { L.cnt[w][threadIdx.x] = run; run += c[w]; }
+        }
+        __syncthreads();
+        uint32_t k[ITEMS], to[ITEMS];
+        uint16_t p[ITEMS];
+        const uint32_t t1 = L.wtot[0], t2 = t1 + L.wtot[1], t3 = t2 + L.wtot[2];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            k[i] = L.key[base + i * 64];
+            p[i] = L.pos[base + i * 64];
+            const uint32_t d = (k[i] >> shift) & 255u, q = d >> 6;
+            to[i] = L.cnt[wave][d] + L.rank[base + i * 64] + (q == 0 ? 0u : q == 1 ? t1 : q == 2 ? t2 : t3);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            L.key[to[i]] = k[i];
+            L.pos[to[i]] = p[i];
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t at = base + i * 64;
+        if (at < n) {
+            keys[at] = L.key[at];
+            pos[at] = L.pos[at];
+        }
+    }
+    if (threadIdx.x == 0) *kept = L.valid;
 }
 
 namespace {
@@ -262,17 +417,41 @@ struct EmbedScratch {
 };
 
 template <typename T, int V, int G>
-int embed_sum_launch(const EmbedScratch& w, const uint32_t* keys, const uint32_t* pos, size_t n, size_t dim,
+int embed_sum_launch(const EmbedScratch& w, const uint32_t* keys, const uint32_t* pos, size_t n, size_t rows, size_t dim,
                      const void* d_out, size_t stride, float scale, void* d_table, hipStream_t s) {
     const uint32_t chunk = EmbedScratch::chunk(n, dim), nchunks = EmbedScratch::chunks(n, dim);
     const size_t nslices = (dim + (size_t)G * V - 1) / ((size_t)G * V), units = nslices * nchunks;
     const size_t blocks = (units + 256 / G - 1) / (256 / G);
-    if (blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
-    embed_sum_kernel<T, V, G><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(w.kept, keys, pos, chunk, nchunks,
-                                                                          (uint32_t)nslices, dim, (const T*)d_out, stride,
-                                                                          scale, (T*)d_table, w.part);
+    size_t per = 16384 / (dim * sizeof(T));                    // about 16 KB of table rows to a wave that clears them
+    per = per < 1 ? 1 : (per > 64 ? 64 : per);
+    const size_t zero_blocks = (rows + 4 * per - 1) / (4 * per);
+    if (blocks + zero_blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
+    embed_sum_kernel<T, V, G><<<dim3((unsigned)(blocks + zero_blocks)), dim3(256), 0, s>>>(
+        w.kept, keys, pos, chunk, nchunks, (uint32_t)nslices, dim, (const T*)d_out, stride, scale, (T*)d_table, w.part,
+        (uint32_t)blocks, (uint32_t)rows, (uint32_t)per);
     LAUNCH_OK("embed_sum_kernel");
     return 0;
+}
+template <typename T, int V>
+int embed_join_launch(const EmbedScratch& w, const uint32_t* keys, size_t n, size_t dim, float scale, void* d_table,
+                      hipStream_t s) {
+    const uint32_t chunk = EmbedScratch::chunk(n, dim), nchunks = EmbedScratch::chunks(n, dim);
+    if (nchunks <= 1) return 0;
+    const size_t shorts = ((size_t)nchunks * ((dim + 16 * V - 1) / (16 * V)) + 63) / 64;
+    const size_t longs = nchunks > JOIN_SHORT ? (size_t)((nchunks + JOIN_SHORT - 1) / JOIN_SHORT) * ((dim + 15) / 16) : 0;
+    if (shorts + longs > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
+    embed_join_kernel<T, V><<<dim3((unsigned)(shorts + longs)), dim3(1024), 0, s>>>(w.kept, keys, chunk, nchunks, (uint32_t)shorts,
+                                                                                  dim, w.part, scale, (T*)d_table);
+    LAUNCH_OK("embed_join_kernel");
+    return 0;
+}
+
+template <typename I>
+void embed_sort_small(uint32_t n, uint32_t rows, int nbits, const I* index, uint32_t* keys, uint32_t* pos, uint32_t* kept,
+                      hipStream_t s) {
+    if (n <= 1024) embed_sort_small_kernel<1, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, nbits, index, keys, pos, kept);
+    else if (n <= 4096) embed_sort_small_kernel<4, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, nbits, index, keys, pos, kept);
+    else embed_sort_small_kernel<16, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, nbits, index, keys, pos, kept);
 }
 
 template <typename T>
@@ -280,17 +459,26 @@ int embed_bwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_
                 int dtype, float scale, void* d_table, char* scratch, hipStream_t s) {
     EmbedScratch w = EmbedScratch::from(scratch, n, dim);
     uint32_t *keys = w.key0, *pos = w.pos0;
-    embed_keys_kernel<<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s>>>(n, rows, index, index_bytes, w.key0);
-    LAUNCH_OK("embed_keys_kernel");
-    int nbits = 1;
-    while (nbits < 32 && (rows - 1) >> nbits) ++nbits;
-    int rc = launch_radix_sort_pairs(w.key0, w.key1, w.pos0, w.pos1, n, nbits, w.sort, &keys, &pos, s, true, w.kept, nullptr,
+    int rc = 0;
+    if (n <= 16384) {
+        int nbits = 1;
+        while (rows >> nbits) ++nbits;                         // (the key `rows` itself occurs)
+        if (index_bytes == 8) embed_sort_small((uint32_t)n, (uint32_t)rows, nbits, (const long long*)index, keys, pos, w.kept, s);
+        else embed_sort_small((uint32_t)n, (uint32_t)rows, nbits, (const int*)index, keys, pos, w.kept, s);
+        LAUNCH_OK("embed_sort_small_kernel");
+    } else {
+        embed_keys_kernel<<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s>>>(n, rows, index, index_bytes, w.key0);
+        LAUNCH_OK("embed_keys_kernel");
+        int nbits = 1;
+        while (nbits < 32 && (rows - 1) >> nbits) ++nbits;
+        rc = launch_radix_sort_pairs(w.key0, w.key1, w.pos0, w.pos1, n, nbits, w.sort, &keys, &pos, s, true, w.kept, nullptr,
                                      nullptr, 0, nullptr, nullptr);
-    if (rc) return rc;
+        if (rc) return rc;
+    }
     const bool wide = e3_rows_wide(d_out, stride, dim, dtype) && e3_rows_wide(d_table, dim, dim, dtype);
     const size_t packs = wide ? dim / Wide<T>::N : dim;
     constexpr int N = Wide<T>::N;
-#define E3_SUM(V, G) rc = embed_sum_launch<T, V, G>(w, keys, pos, n, dim, d_out, stride, scale, d_table, s)
+#define E3_SUM(V, G) rc = embed_sum_launch<T, V, G>(w, keys, pos, n, rows, dim, d_out, stride, scale, d_table, s)
     if (wide) {
         if (packs <= 4) E3_SUM(N, 4);
         else if (packs <= 8) E3_SUM(N, 8);
@@ -304,22 +492,9 @@ int embed_bwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_
     }
 #undef E3_SUM
     if (rc) return rc;
-    const uint32_t chunk = EmbedScratch::chunk(n, dim), nchunks = EmbedScratch::chunks(n, dim);
-    if (nchunks > 1) {
-        embed_join_kernel<T><<<dim3(nchunks - 1, (unsigned)((dim + 63) / 64)), dim3(1024), 0, s>>>(
-            w.kept, keys, chunk, dim, w.part, scale, (T*)d_table);
-        LAUNCH_OK("embed_join_kernel");
-    }
-    // about 16 KB of table rows to a wave
-    size_t per = 16384 / (dim * sizeof(T));
-    per = per < 1 ? 1 : (per > 64 ? 64 : per);
-    const size_t zb = (rows + 4 * per - 1) / (4 * per);
-    if (e3_rows_wide(d_table, dim, dim, dtype))
-        embed_zero_kernel<T, N><<<dim3((unsigned)zb), dim3(256), 0, s>>>(w.kept, keys, (uint32_t)rows, (uint32_t)per, dim, (T*)d_table);
-    else
-        embed_zero_kernel<T, 1><<<dim3((unsigned)zb), dim3(256), 0, s>>>(w.kept, keys, (uint32_t)rows, (uint32_t)per, dim, (T*)d_table);
-    LAUNCH_OK("embed_zero_kernel");
-    return 0;
+    // (partial rows start on 16-byte boundaries where dim is a multiple of 4)
+    return dim % 4 == 0 && e3_rows_wide(d_table, dim, dim, dtype) ? embed_join_launch<T, 4>(w, keys, n, dim, scale, d_table, s)
+                                                                 : embed_join_launch<T, 1>(w, keys, n, dim, scale, d_table, s);
 }
 
 template <typename T, int V>
