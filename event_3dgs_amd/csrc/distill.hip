@@ -352,7 +352,7 @@ __device__ __forceinline__ void patch_row(const DistillArgs& a, const Label& l, 
     }
 }
 
-template <typename T, int V, int G>
+template <bool STREAM, typename T, int V, int G>
 __global__ __launch_bounds__(RowsLds<G>::THREADS) void distill_bwd_rows_kernel(const DistillArgs a) {
     __shared__ RowsLds<G> L;
     const int lane = threadIdx.x % G, slot = threadIdx.x / G;
@@ -389,7 +389,7 @@ __global__ __launch_bounds__(RowsLds<G>::THREADS) void distill_bwd_rows_kernel(c
                 Pack<T, V> r;
 #pragma unroll
                 for (int j = 0; j < V; ++j) r.v[j] = (T)(exp2_hw(((float)p[u].v[j] - st.x) * c) * fi);
-                gp[i + u * G] = r;
+                put<STREAM, T, V>(reinterpret_cast<T*>(gp + i + u * G), r);
             }
         }
         row_sync<G>();
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(RowsLds<G>::THREADS) void distill_bwd_rows_kernel(c
 
 // Value and gradient in one pass: the row stays in the registers of its workgroup (ITEMS packs to a thread) between the
 // statistics and the gradient, so the scores are read once and the gradient is written once.
-template <typename T, int V, int G, int ITEMS>
+template <bool STREAM, typename T, int V, int G, int ITEMS>
 __global__ __launch_bounds__(G) void distill_both_rows_kernel(const DistillArgs a) {
     __shared__ RowsLds<G> L;
     const int lane = threadIdx.x;
@@ -475,7 +475,7 @@ __global__ __launch_bounds__(G) void distill_both_rows_kernel(const DistillArgs 
                 Pack<T, V> r;
 #pragma unroll
                 for (int j = 0; j < V; ++j) r.v[j] = (T)(exp2_hw((word_elem<T>(p[u], j) - m) * c) * fi);
-                *reinterpret_cast<Pack<T, V>*>(gp + (at + u * G) * 16u) = r;
+                put<STREAM, T, V>(reinterpret_cast<T*>(gp + (at + u * G) * 16u), r);
             }
         if (has_single) g[cut.single(lane)] = (T)(exp2_hw((single - m) * c) * fi);
         __syncthreads();
@@ -922,7 +922,7 @@ __global__ __launch_bounds__(256) void distill_fwd_wide_kernel(const DistillArgs
     store_part<256>(a, total, count, lds);
 }
 
-template <typename T, int P, int KR>
+template <bool STREAM, typename T, int P, int KR>
 __global__ __launch_bounds__(256) void distill_bwd_wide_kernel(const DistillArgs a) {
     const float rt = 1.0f / a.temperature, c = LOG2E * rt;
     const float f_all = a.temperature * (a.weight ? *a.weight : 1.0f);
@@ -967,7 +967,7 @@ __global__ __launch_bounds__(256) void distill_bwd_wide_kernel(const DistillArgs
                     const float d = f[p] * (exp2_hw(((float)b.v[u].v[p] - st[p].x) * c) * st[p].y - q);
                     r.v[p] = st[p].y == 0.0f ? (T)0.0f : (T)d;
                 }
-                *reinterpret_cast<Pack<T, P>*>(g + (size_t)(j + u) * a.g_class) = r;
+                put<STREAM, T, P>(g + (size_t)(j + u) * a.g_class, r);
             }
         }
     }
@@ -1020,20 +1020,21 @@ int distill_tile(const DistillArgs& a, int tile, unsigned& blocks, hipStream_t s
 }
 
 // Threads of a long row: a wave up to some thousand classes, a workgroup beyond that.
-template <typename T, int V>
-int distill_rows(const DistillArgs& a, bool backward, unsigned& blocks, hipStream_t s) {
-#define E3_ROWS(G)                                                                                              \
-    {                                                                                                           \
-        blocks = distill_blocks(a.rows, RowsLds<G>::ROWS);                                                      \
-        if (backward) distill_bwd_rows_kernel<T, V, G><<<dim3(blocks), dim3(RowsLds<G>::THREADS), 0, s>>>(a);   \
-        else distill_fwd_rows_kernel<T, V, G><<<dim3(blocks), dim3(RowsLds<G>::THREADS), 0, s>>>(a);            \
-    }
-    if (a.classes <= 2048) E3_ROWS(64)
-    else if (a.classes <= 16384) E3_ROWS(256)
-    else E3_ROWS(1024)
-#undef E3_ROWS
+template <typename T, int V, int G>
+int distill_rows_launch(const DistillArgs& a, bool backward, unsigned& blocks, hipStream_t s) {
+    blocks = distill_blocks(a.rows, RowsLds<G>::ROWS);
+    const dim3 threads(RowsLds<G>::THREADS);
+    if (!backward) distill_fwd_rows_kernel<T, V, G><<<dim3(blocks), threads, 0, s>>>(a);
+    else if (V > 1 && a.rows * a.classes * sizeof(T) > E3_STREAM_BYTES) distill_bwd_rows_kernel<(V > 1), T, V, G><<<dim3(blocks), threads, 0, s>>>(a);
+    else distill_bwd_rows_kernel<false, T, V, G><<<dim3(blocks), threads, 0, s>>>(a);
     LAUNCH_OK("distill_rows_kernel");
     return 0;
+}
+template <typename T, int V>
+int distill_rows(const DistillArgs& a, bool backward, unsigned& blocks, hipStream_t s) {
+    if (a.classes <= 2048) return distill_rows_launch<T, V, 64>(a, backward, blocks, s);
+    if (a.classes <= 16384) return distill_rows_launch<T, V, 256>(a, backward, blocks, s);
+    return distill_rows_launch<T, V, 1024>(a, backward, blocks, s);
 }
 
 // Packs need the scores and their gradient to lie the same way to a 16-byte boundary in every row.
@@ -1043,6 +1044,9 @@ bool rows_wide(const DistillArgs& a, bool gradient) {
     return ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0 &&
            (a.row_stride * sizeof(T)) % 16 == (a.g_row * sizeof(T)) % 16;
 }
+
+template <typename T>
+bool grad_streams(const DistillArgs& a) { return a.rows * a.classes * sizeof(T) > E3_STREAM_BYTES; }
 
 // pixels per lane: 4 for the gradient; 2 for the value, whose registers (the scores of the label's entries) would leave two
 // waves to a SIMD with 4 (64 fp32 planes of 1920 x 1080: 173 us with 4, 157 us with 2); 1 where the planes do not lie on
@@ -1056,7 +1060,8 @@ int distill_wide_fwd(const DistillArgs& a, unsigned& blocks, hipStream_t s) {
 }
 template <typename T, int P, int KR>
 int distill_wide_bwd(const DistillArgs& a, hipStream_t s) {
-    distill_bwd_wide_kernel<T, P, KR><<<dim3(distill_blocks(a.rows, 256 * P)), dim3(256), 0, s>>>(a);
+    if (P > 1 && grad_streams<T>(a)) distill_bwd_wide_kernel<(P > 1), T, P, KR><<<dim3(distill_blocks(a.rows, 256 * P)), dim3(256), 0, s>>>(a);
+    else distill_bwd_wide_kernel<false, T, P, KR><<<dim3(distill_blocks(a.rows, 256 * P)), dim3(256), 0, s>>>(a);
     LAUNCH_OK("distill_bwd_wide_kernel");
     return 0;
 }
@@ -1115,11 +1120,15 @@ int distill_both_t(DistillArgs a, uint32_t* counts, unsigned& blocks, hipStream_
         LAUNCH_OK("distill_count_kernel");
     }
     if (tile) return distill_tile<T, VALUE | GRADIENT>(a, tile, blocks, s);
-    if (packs <= 1024) distill_both_rows_kernel<T, V, 256, 4><<<dim3(blocks), dim3(256), 0, s>>>(a);
-    else if (packs <= 2048) distill_both_rows_kernel<T, V, 256, 8><<<dim3(blocks), dim3(256), 0, s>>>(a);
-    else if (packs <= 4096) distill_both_rows_kernel<T, V, 256, 16><<<dim3(blocks), dim3(256), 0, s>>>(a);
-    else if (packs <= 8192) distill_both_rows_kernel<T, V, 1024, 8><<<dim3(blocks), dim3(1024), 0, s>>>(a);
-    else distill_both_rows_kernel<T, V, 1024, 16><<<dim3(blocks), dim3(1024), 0, s>>>(a);
+#define E3_BOTH(G, ITEMS)                                                                                          \
+    if (grad_streams<T>(a)) distill_both_rows_kernel<true, T, V, G, ITEMS><<<dim3(blocks), dim3(G), 0, s>>>(a);    \
+    else distill_both_rows_kernel<false, T, V, G, ITEMS><<<dim3(blocks), dim3(G), 0, s>>>(a)
+    if (packs <= 1024) { E3_BOTH(256, 4); }
+    else if (packs <= 2048) { E3_BOTH(256, 8); }
+    else if (packs <= 4096) { E3_BOTH(256, 16); }
+    else if (packs <= 8192) { E3_BOTH(1024, 8); }
+    else { E3_BOTH(1024, 16); }
+#undef E3_BOTH
     LAUNCH_OK("distill_both_rows_kernel");
     return 0;
 }

@@ -22,7 +22,7 @@ int launch_radix_sort_pairs(uint32_t* k0, uint32_t* k1, uint32_t* v0, uint32_t* 
 // One thread moves EMBED_PACKS packs of the flat output, a workgroup's packs are contiguous: every lane works whatever the
 // row length, the stores are whole lines, and the rows of a pack-block are found by one division each.
 constexpr int EMBED_PACKS = 4;
-template <typename T, int V, typename I>
+template <bool STREAM, typename T, int V, typename I>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(size_t n, long long rows, uint32_t ppr /* packs per row */,
                                                         const I* __restrict__ index, const T* __restrict__ table, size_t stride, float scale,
                                                         T* __restrict__ out) {
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(size_t n, long long rows
 #pragma unroll
         for (int j = 0; j < V; ++j)
             r.v[j] = id[u] < 0 ? (T)0.0f : (id[u] < rows ? (T)(scale * (float)p[u].v[j]) : (T)__builtin_nanf(""));
-        reinterpret_cast<Pack<T, V>*>(out)[at] = r;
+        put<STREAM, T, V>(out + at * V, r);
     }
 }
 
@@ -63,12 +63,14 @@ static int embed_fwd_t(size_t n, size_t rows, size_t dim, const void* index, con
     const size_t ppr = wide ? dim / Wide<T>::N : dim;
     const size_t blocks = (n * ppr + 256 * EMBED_PACKS - 1) / (256 * EMBED_PACKS);
     if (blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_forward: too many values");
-    if (wide)
-        embed_fwd_kernel<T, Wide<T>::N, I><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(
-            n, (long long)rows, (uint32_t)ppr, (const I*)index, (const T*)table, stride, scale, (T*)out);
-    else
-        embed_fwd_kernel<T, 1, I><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(
-            n, (long long)rows, (uint32_t)ppr, (const I*)index, (const T*)table, stride, scale, (T*)out);
+#define E3_FWD(S, V)                                                                                                          \
+    embed_fwd_kernel<S, T, V, I><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(n, (long long)rows, (uint32_t)ppr,            \
+                                                                            (const I*)index, (const T*)table, stride, scale, \
+                                                                            (T*)out)
+    if (!wide) E3_FWD(false, 1);
+    else if (n * dim * sizeof(T) > E3_STREAM_BYTES) E3_FWD(true, Wide<T>::N);
+    else E3_FWD(false, Wide<T>::N);
+#undef E3_FWD
     LAUNCH_OK("embed_fwd_kernel");
     return 0;
 }
@@ -121,7 +123,7 @@ __device__ __forceinline__ void embed_store(T* __restrict__ d_table, size_t dim,
 
 // Clears the table rows without a position: a wave looks `per` rows up in the sorted keys (one lane each) and clears those
 // that are not there.
-template <typename T, int V>
+template <bool STREAM, typename T, int V>
 __device__ __forceinline__ void embed_zero(uint32_t n, const uint32_t* __restrict__ keys, uint32_t rows, uint32_t per,
                                            size_t dim, T* __restrict__ d_table, size_t wave) {
     const int lane = threadIdx.x & 63;
@@ -140,7 +142,7 @@ __device__ __forceinline__ void embed_zero(uint32_t n, const uint32_t* __restric
         const int r = __builtin_ctzll(todo);
         todo &= todo - 1;
         T* row = d_table + (first + r) * dim;
-        for (size_t col = (size_t)lane * V; col < dim; col += 64 * V) *reinterpret_cast<Pack<T, V>*>(row + col) = z;
+        for (size_t col = (size_t)lane * V; col < dim; col += 64 * V) put<STREAM, T, V>(row + col, z);
     }
 }
 
@@ -154,7 +156,9 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restri
                                                         uint32_t zero_rows) {
     const uint32_t n = *kept;
     if (blockIdx.x >= sum_blocks) {      // (in the same launch: the sums wait for their gathers, the stores do not)
-        embed_zero<T, V>(n, keys, rows, zero_rows, dim, d_table, (size_t)(blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6));
+        const size_t wave = (size_t)(blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6);
+        if (V > 1 && (size_t)rows * dim * sizeof(T) > E3_STREAM_BYTES) embed_zero<true, T, V>(n, keys, rows, zero_rows, dim, d_table, wave);
+        else embed_zero<false, T, V>(n, keys, rows, zero_rows, dim, d_table, wave);
         return;
     }
     const size_t unit = (size_t)blockIdx.x * (256 / G) + threadIdx.x / G;
@@ -208,23 +212,21 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restri
 // Adds up the partials of the runs that cross chunks: slot 1 of the chunk a run starts in, slot 0 of the following ones.
 // Workgroups of two kinds in one launch:
 //   short runs   a group of 16 lanes takes a chunk (times a slice of 16 V columns) and adds up to JOIN_SHORT partials in order
-//   long runs    a workgroup looks at JOIN_SHORT neighbouring chunks (times a slice of 16 columns): only the last run that
-//                starts among them can be longer than JOIN_SHORT partials; 64 groups of 16 lanes take a 64th of them each,
-//                the 64 sums are added in order
-constexpr uint32_t JOIN_SHORT = 32;
-struct Crossing {
-    uint32_t key, partials;      // partials 0: no run starts in the chunk and goes on behind it
-};
-__device__ __forceinline__ Crossing embed_crossing(const uint32_t* __restrict__ keys, uint32_t n, uint32_t chunk, uint32_t c) {
-    Crossing r{0u, 0u};
-    if ((size_t)(c + 1) * chunk >= n) return r;                          // nothing lies behind the chunk
-    const uint32_t j0 = c * chunk, j1 = j0 + chunk, key = keys[j1 - 1];
-    if (keys[j1] != key) return r;                                       // its last run ends with it
-    if (keys[j0] == key && j0 > 0 && keys[j0 - 1] == key) return r;      // ... or began earlier
-    const uint32_t end = lower_bound_u32(keys, j1, n, key + 1u);         // (key < rows < 2^31)
-    r.key = key;
-    r.partials = (end - 1u) / chunk - c + 1u;
-    return r;
+//   long runs    a workgroup looks at JOIN_SHORT neighbouring chunks (times a slice of JOIN_COLS columns): only the last run
+//                that starts among them can be longer than JOIN_SHORT partials; 64 groups of 16 lanes take a 64th of them
+//                each, the 64 sums are added in order
+constexpr uint32_t JOIN_SHORT = 32, JOIN_COLS = 64;
+// Whether a run starts in chunk c and goes on behind it; its key.
+__device__ __forceinline__ bool embed_crossing(const uint32_t* __restrict__ keys, uint32_t n, uint32_t chunk, uint32_t c,
+                                               uint32_t& key) {
+    if ((size_t)(c + 1) * chunk >= n) return false;                      // nothing lies behind the chunk
+    const uint32_t j0 = c * chunk, j1 = j0 + chunk, head = keys[j0], next = keys[j1], before = keys[j0 > 0 ? j0 - 1 : 0];
+    key = keys[j1 - 1];
+    return next == key && !(head == key && j0 > 0 && before == key);     // (it goes on, and did not begin earlier)
+}
+// Whether chunk c exists and begins with `key`: then it holds a partial of the run.
+__device__ __forceinline__ bool embed_in_run(const uint32_t* __restrict__ keys, uint32_t n, uint32_t chunk, uint32_t c, uint32_t key) {
+    return (size_t)c * chunk < n && keys[(size_t)c * chunk] == key;
 }
 template <typename T, int V>
 __global__ __launch_bounds__(1024) void embed_join_kernel(const uint32_t* __restrict__ kept,
@@ -233,8 +235,7 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(const uint32_t* __rest
                                                           const float* __restrict__ part, float scale,
                                                           T* __restrict__ d_table) {
     __shared__ float sums[64][17];
-    __shared__ Crossing longest;
-    __shared__ uint32_t longest_chunk;
+    __shared__ uint32_t long_chunk, long_key;
     const uint32_t n = *kept;
     const int g = threadIdx.x >> 4, lane = threadIdx.x & 15;
     if (blockIdx.x < short_blocks) {
@@ -242,52 +243,64 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(const uint32_t* __rest
         const size_t unit = (size_t)blockIdx.x * 64 + g;
         const uint32_t c = (uint32_t)(unit / nslices);
         const size_t col = ((unit - (size_t)c * nslices) * 16 + lane) * V;
-        if (c >= nchunks || col >= dim) return;
-        const Crossing r = embed_crossing(keys, n, chunk, c);
-        if (r.partials == 0 || r.partials > JOIN_SHORT) return;
+        uint32_t key = 0;
+        if (c >= nchunks || !embed_crossing(keys, n, chunk, c, key)) return;        // (the same for the whole group)
+        // partials behind the first: chunks c + 1, c + 2, ... that begin with the key, 16 looked at together
+        uint32_t m = 1;
+        for (uint32_t k = 1; k <= JOIN_SHORT; k += 16) {
+            const unsigned long long in = __ballot(embed_in_run(keys, n, chunk, c + k + lane, key));
+            const uint32_t mine = (uint32_t)(in >> (threadIdx.x & 48)) & 0xFFFFu;
+            m += (uint32_t)__popc(mine);
+            if (mine != 0xFFFFu) break;
+        }
+        if (m > JOIN_SHORT || col >= dim) return;
         const Pack<float, V> p = *reinterpret_cast<const Pack<float, V>*>(part + (2 * (size_t)c + 1) * dim + col);
         float acc[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) acc[j] = p.v[j];
 #pragma unroll 4
-        for (uint32_t k = 1; k < r.partials; ++k) {
+        for (uint32_t k = 1; k < m; ++k) {
             const Pack<float, V> q = *reinterpret_cast<const Pack<float, V>*>(part + 2 * (size_t)(c + k) * dim + col);
 #pragma unroll
             for (int j = 0; j < V; ++j) acc[j] += q.v[j];
         }
-        embed_store<T, V>(d_table, dim, r.key, col, scale, acc);
+        embed_store<T, V>(d_table, dim, key, col, scale, acc);
         return;
     }
-    const uint32_t nslices = (uint32_t)((dim + 15) / 16), unit = blockIdx.x - short_blocks;
-    const uint32_t first = unit / nslices * JOIN_SHORT;
-    const size_t col = (size_t)(unit % nslices) * 16 + lane;
+    const uint32_t nparts = (uint32_t)((dim + JOIN_COLS - 1) / JOIN_COLS), unit = blockIdx.x - short_blocks;
+    const uint32_t first = unit / nparts * JOIN_SHORT;
     if (threadIdx.x < 64) {
         const uint32_t c = first + threadIdx.x;
-        Crossing r{0u, 0u};
-        if (threadIdx.x < JOIN_SHORT && c < nchunks) r = embed_crossing(keys, n, chunk, c);
-        const unsigned long long hit = __ballot(r.partials > JOIN_SHORT);      // (one lane at most)
-        if (hit == 0ull) {
-            if (threadIdx.x == 0) longest.partials = 0;
-        } else if ((int)threadIdx.x == __builtin_ctzll(hit)) {
-            longest = r;
-            longest_chunk = c;
+        uint32_t key = 0;
+        const bool is_long = threadIdx.x < JOIN_SHORT && c < nchunks && embed_crossing(keys, n, chunk, c, key) &&
+                             embed_in_run(keys, n, chunk, c + JOIN_SHORT, key);
+        const unsigned long long hit = __ballot(is_long);                      // (one lane at most)
+        if (threadIdx.x == 0 && hit == 0ull) long_chunk = 0xFFFFFFFFu;
+        if (is_long) {
+            long_chunk = c;
+            long_key = key;
         }
     }
     __syncthreads();
-    const uint32_t m = longest.partials, c = longest_chunk;
-    if (m == 0) return;                                                        // (uniform)
+    const uint32_t c = long_chunk;
+    if (c == 0xFFFFFFFFu) return;                                              // (uniform)
+    const uint32_t m = (lower_bound_u32(keys, c * chunk + chunk, n, long_key + 1u) - 1u) / chunk - c + 1u;
     const uint32_t lo = (uint32_t)((unsigned long long)m * g / 64), hi = (uint32_t)((unsigned long long)m * (g + 1) / 64);
-    float s = 0.0f;
-    if (col < dim) {
+    const size_t col0 = (size_t)(unit % nparts) * JOIN_COLS, col1 = col0 + JOIN_COLS < dim ? col0 + JOIN_COLS : dim;
+    for (size_t col = col0 + lane; col < col1 + lane; col += 16) {             // (every lane takes part in the barriers)
+        float s = 0.0f;
+        if (col < col1) {
 #pragma unroll 8
-        for (uint32_t k = lo; k < hi; ++k) s += part[(k == 0 ? 2 * (size_t)c + 1 : 2 * (size_t)(c + k)) * dim + col];
-    }
-    sums[g][lane] = s;
-    __syncthreads();
-    if (g == 0 && col < dim) {
-        s = sums[0][lane];
-        for (int w = 1; w < 64; ++w) s += sums[w][lane];
-        d_table[(size_t)longest.key * dim + col] = (T)(scale * s);
+            for (uint32_t k = lo; k < hi; ++k) s += part[(k == 0 ? 2 * (size_t)c + 1 : 2 * (size_t)(c + k)) * dim + col];
+        }
+        sums[g][lane] = s;
+        __syncthreads();
+        if (g == 0 && col < col1) {
+            s = sums[0][lane];
+            for (int w = 1; w < 64; ++w) s += sums[w][lane];
+            d_table[(size_t)long_key * dim + col] = (T)(scale * s);
+        }
+        __syncthreads();
     }
 }
 
@@ -335,12 +348,15 @@ __global__ __launch_bounds__(1024) void embed_sort_small_kernel(uint32_t n, uint
 #pragma unroll 1
         for (int i = 0; i < ITEMS; ++i) {
             const uint32_t d = (L.key[base + i * 64] >> shift) & 255u;
-            unsigned long long peers = ~0ull;
+            uint32_t plo = ~0u, phi = ~0u;                   // lanes with the same digit
 #pragma unroll
             for (int b = 0; b < 8; ++b) {
-                const unsigned long long bal = __ballot((d >> b) & 1u);
-                peers &= ((d >> b) & 1u) ? bal : ~bal;
+                const int bit = (int)(d << (31 - b)) >> 31;  // 0 or -1
+                const unsigned long long bal = __ballot(bit < 0);
+                plo &= ~((uint32_t)bal ^ (uint32_t)bit);
+                phi &= ~((uint32_t)(bal >> 32) ^ (uint32_t)bit);
             }
+            const unsigned long long peers = (unsigned long long)phi << 32 | plo;
             const uint32_t first = L.cnt[wave][d];
             wave_sync();
             if ((peers & before) == 0ull) L.cnt[wave][d] = first + (uint32_t)__popcll(peers);
@@ -395,9 +411,9 @@ struct EmbedScratch {
     uint32_t *key0, *key1, *pos0, *pos1, *kept, *sort;
     float* part;
     static uint32_t chunk(size_t n, size_t dim) {
-        // Rows of a chunk: 64 where there is plenty of work, fewer where the groups would otherwise not fill the chip (each
+        // Rows of a chunk: 128 where there is plenty of work, fewer where the groups would otherwise not fill the chip (each
         // group moves `chunk` row slices of at most 1 KB).
-        uint32_t c = 64;
+        uint32_t c = 128;
         while (c > 8 && (n / c) * ((dim + 511) / 512) < 4096) c >>= 1;
         return c;
     }
@@ -438,7 +454,7 @@ int embed_join_launch(const EmbedScratch& w, const uint32_t* keys, size_t n, siz
     const uint32_t chunk = EmbedScratch::chunk(n, dim), nchunks = EmbedScratch::chunks(n, dim);
     if (nchunks <= 1) return 0;
     const size_t shorts = ((size_t)nchunks * ((dim + 16 * V - 1) / (16 * V)) + 63) / 64;
-    const size_t longs = nchunks > JOIN_SHORT ? (size_t)((nchunks + JOIN_SHORT - 1) / JOIN_SHORT) * ((dim + 15) / 16) : 0;
+    const size_t longs = nchunks > JOIN_SHORT ? (size_t)((nchunks + JOIN_SHORT - 1) / JOIN_SHORT) * ((dim + JOIN_COLS - 1) / JOIN_COLS) : 0;
     if (shorts + longs > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
     embed_join_kernel<T, V><<<dim3((unsigned)(shorts + longs)), dim3(1024), 0, s>>>(w.kept, keys, chunk, nchunks, (uint32_t)shorts,
                                                                                   dim, w.part, scale, (T*)d_table);
@@ -451,6 +467,7 @@ void embed_sort_small(uint32_t n, uint32_t rows, int nbits, const I* index, uint
                       hipStream_t s) {
     if (n <= 1024) embed_sort_small_kernel<1, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, nbits, index, keys, pos, kept);
     else if (n <= 4096) embed_sort_small_kernel<4, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, nbits, index, keys, pos, kept);
+    else if (n <= 8192) embed_sort_small_kernel<8, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, nbits, index, keys, pos, kept);
     else embed_sort_small_kernel<16, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, nbits, index, keys, pos, kept);
 }
 
@@ -551,7 +568,7 @@ struct NormRow {      // sums over the lanes of a row
     }
 };
 
-template <typename T, int V, int G, int ITEMS>
+template <bool STREAM, typename T, int V, int G, int ITEMS>
 __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_fwd_kernel(size_t rows, int dim, const T* __restrict__ x,
                                                                        size_t stride, const void* __restrict__ weight,
                                                                        const void* __restrict__ bias, int affine_dtype,
@@ -616,7 +633,7 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_fwd_kernel(size_t ro
             Pack<T, V> r;
 #pragma unroll
             for (int j = 0; j < V; ++j) r.v[j] = (T)FMA(v[i][j] * rstd, w[i][j], b[i][j]);
-            *reinterpret_cast<Pack<T, V>*>(out + row * (size_t)dim + col) = r;
+            put<STREAM, T, V>(out + row * (size_t)dim + col, r);
         }
     }
 }
@@ -666,7 +683,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(size_t rows, size_t
 // dweight = sum over the rows of dy h, dbias = sum of dy.  The column sums stay in registers while a workgroup walks over
 // its rows, are added up over the workgroup's groups in LDS, and leave one fp32 row pair per workgroup, which
 // norm_join_kernel adds up.
-template <typename T, int V, int G, int ITEMS>
+template <bool STREAM, typename T, int V, int G, int ITEMS>
 __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_bwd_kernel(size_t rows, int dim, const T* __restrict__ dy,
                                                                        size_t dy_stride, const T* __restrict__ x,
                                                                        size_t stride, const void* __restrict__ weight,
@@ -728,7 +745,7 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_bwd_kernel(size_t ro
             Pack<T, V> r;
 #pragma unroll
             for (int j = 0; j < V; ++j) r.v[j] = (T)((g[i][j] - s1 - h[i][j] * s2) * rstd);
-            *reinterpret_cast<Pack<T, V>*>(dx + row * (size_t)dim + col) = r;
+            put<STREAM, T, V>(dx + row * (size_t)dim + col, r);
         }
     }
     if (!part) return;
@@ -865,19 +882,27 @@ struct NormArgs {
 
 template <typename T, int V, int G, int ITEMS>
 int norm_fwd_launch(const NormArgs& a) {
-    norm_fwd_kernel<T, V, G, ITEMS><<<dim3(norm_blocks(a.rows, NormRow<G>::PER_BLOCK, NORM_FWD_BLOCKS)),
-                                      dim3(NormRow<G>::THREADS), 0, a.s>>>(a.rows, (int)a.dim, (const T*)a.x, a.x_stride,
-                                                                         a.weight, a.bias, a.affine_dtype, a.eps, (T*)a.out,
-                                                                         a.mean, a.rstd);
+    const dim3 blocks(norm_blocks(a.rows, NormRow<G>::PER_BLOCK, NORM_FWD_BLOCKS)), threads(NormRow<G>::THREADS);
+#define E3_NORM(S)                                                                                                            \
+    norm_fwd_kernel<(S), T, V, G, ITEMS><<<blocks, threads, 0, a.s>>>(a.rows, (int)a.dim, (const T*)a.x, a.x_stride, a.weight, \
+                                                                  a.bias, a.affine_dtype, a.eps, (T*)a.out, a.mean, a.rstd)
+    if (V > 1 && a.rows * a.dim * sizeof(T) > E3_STREAM_BYTES) E3_NORM(V > 1);
+    else E3_NORM(false);
+#undef E3_NORM
     LAUNCH_OK("norm_fwd_kernel");
     return 0;
 }
 template <typename T, int V, int G, int ITEMS>
 int norm_bwd_launch(const NormArgs& a, uint32_t& nparts) {
     nparts = norm_blocks(a.rows, NormRow<G>::PER_BLOCK, NORM_BWD_BLOCKS);
-    norm_bwd_kernel<T, V, G, ITEMS><<<dim3(nparts), dim3(NormRow<G>::THREADS), 0, a.s>>>(
-        a.rows, (int)a.dim, (const T*)a.dy, a.dy_stride, (const T*)a.x, a.x_stride, a.weight, a.affine_dtype, a.mean, a.rstd,
-        (T*)a.dx, a.part);
+    const dim3 blocks(nparts), threads(NormRow<G>::THREADS);
+#define E3_NORM(S)                                                                                                            \
+    norm_bwd_kernel<(S), T, V, G, ITEMS><<<blocks, threads, 0, a.s>>>(a.rows, (int)a.dim, (const T*)a.dy, a.dy_stride,          \
+                                                                  (const T*)a.x, a.x_stride, a.weight, a.affine_dtype,       \
+                                                                  a.mean, a.rstd, (T*)a.dx, a.part)
+    if (V > 1 && a.rows * a.dim * sizeof(T) > E3_STREAM_BYTES) E3_NORM(V > 1);
+    else E3_NORM(false);
+#undef E3_NORM
     LAUNCH_OK("norm_bwd_kernel");
     return 0;
 }

@@ -41,6 +41,22 @@ __device__ __forceinline__ float word_elem<f16_t>(words_t q, int j) {
 __device__ __forceinline__ void forget(words_t& q) { asm volatile("" : "+v"(q)); }
 __device__ __forceinline__ void forget(uint32_t& x) { asm volatile("" : "+v"(x)); }
 
+// Stores of a large result.  Past E3_STREAM_BYTES (half of the 256 MB Infinity Cache) the reader of a result finds little of
+// it there, while ordinary stores push the running kernel's inputs out and hold its reads up: such a result is streamed past
+// the cache.  A lookup of 192 MB of rows takes 55 us with ordinary and 30 us with streamed stores, and with a layer norm
+// behind it 122 us and 104 us; at 134 MB and below the reader loses more than the writer gains (lookup + layer norm of
+// 8192 x 4096 fp32: 86 us ordinary, 88 us streamed).  A template argument: the compiler joins the two stores of a runtime
+// choice into an ordinary one.
+constexpr size_t E3_STREAM_BYTES = 128u << 20;
+template <bool STREAM, typename T, int V>
+__device__ __forceinline__ void put(T* p, const Pack<T, V>& r) {
+    if constexpr (!STREAM) *reinterpret_cast<Pack<T, V>*>(p) = r;
+    else if constexpr (sizeof(r) == 16) __builtin_nontemporal_store(__builtin_bit_cast(words_t, r), reinterpret_cast<words_t*>(p));
+    else if constexpr (sizeof(r) == 8) __builtin_nontemporal_store(__builtin_bit_cast(unsigned long long, r), reinterpret_cast<unsigned long long*>(p));
+    else if constexpr (sizeof(r) == 4) __builtin_nontemporal_store(__builtin_bit_cast(uint32_t, r), reinterpret_cast<uint32_t*>(p));
+    else __builtin_nontemporal_store(__builtin_bit_cast(uint16_t, r), reinterpret_cast<uint16_t*>(p));
+}
+
 static inline size_t e3_elem_bytes(int dtype) { return dtype == E3_F32 ? 4 : 2; }
 static inline bool e3_dtype_ok(int dtype) { return dtype >= E3_F32 && dtype <= E3_BF16; }
 
