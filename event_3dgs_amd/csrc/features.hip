@@ -568,6 +568,26 @@ struct NormRow {      // sums over the lanes of a row
     }
 };
 
+// V parameters from `col` on (col a multiple of V), in 16-byte loads where the array allows it; `none` without an array.
+template <int V>
+__device__ __forceinline__ void load_affine(const void* __restrict__ p, int dtype, size_t col, float none, float v[V]) {
+    if (!p) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = none;
+    } else if (V == 1 || (reinterpret_cast<uintptr_t>(p) & 15) != 0 || (V == 4 && dtype != E3_F32)) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = load_elem(p, col + j, dtype);
+    } else if (dtype == E3_F32) {
+        const words_t* q = reinterpret_cast<const words_t*>(reinterpret_cast<const float*>(p) + col);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = word_elem<float>(q[j / 4], j % 4);
+    } else {
+        const words_t q = *reinterpret_cast<const words_t*>(reinterpret_cast<const uint16_t*>(p) + col);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = dtype == E3_F16 ? word_elem<f16_t>(q, j) : word_elem<bf16_t>(q, j);
+    }
+}
+
 template <bool STREAM, typename T, int V, int G, int ITEMS>
 __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_fwd_kernel(size_t rows, int dim, const T* __restrict__ x,
                                                                        size_t stride, const void* __restrict__ weight,
@@ -582,11 +602,8 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_fwd_kernel(size_t ro
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const int col = (i * G + lane) * V;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            w[i][j] = weight && col < dim ? load_elem(weight, col + j, affine_dtype) : 1.0f;
-            b[i][j] = bias && col < dim ? load_elem(bias, col + j, affine_dtype) : 0.0f;
-        }
+        load_affine<V>(col < dim ? weight : nullptr, affine_dtype, col, 1.0f, w[i]);
+        load_affine<V>(col < dim ? bias : nullptr, affine_dtype, col, 0.0f, b[i]);
     }
     const float inv = 1.0f / (float)dim;
     const size_t step = (size_t)gridDim.x * R::PER_BLOCK;
@@ -634,6 +651,175 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_fwd_kernel(size_t ro
 #pragma unroll
             for (int j = 0; j < V; ++j) r.v[j] = (T)FMA(v[i][j] * rstd, w[i][j], b[i][j]);
             put<STREAM, T, V>(out + row * (size_t)dim + col, r);
+        }
+    }
+}
+
+// Short rows whose length is no multiple of 16 bytes (or a few packs only), one behind the other: a workgroup moves `tile` rows
+// at a time through LDS, in whole packs whatever the row length; 256 / tile lanes work on a row there.  (200000 rows of 59
+// fp16 values, a lane per value straight from memory: 38 us forward, 51 us backward; through LDS NORM_TILE_TIMES.)
+constexpr int NORM_TILE = 16384, NORM_TILE_PACKS = NORM_TILE / 16 / 256, NORM_TILE_COLS = 4;
+template <typename T>
+__device__ __forceinline__ void tile_load(const T* __restrict__ src, words_t* dst, int elems) {
+    const int packs = (int)(elems * sizeof(T) / 16), rest = packs * (16 / (int)sizeof(T));
+    words_t in[NORM_TILE_PACKS];
+#pragma unroll
+    for (int u = 0; u < NORM_TILE_PACKS; ++u) {
+        const int i = u * 256 + threadIdx.x;
+        if (i < packs) in[u] = reinterpret_cast<const words_t*>(src)[i];
+    }
+#pragma unroll
+    for (int u = 0; u < NORM_TILE_PACKS; ++u) {
+        const int i = u * 256 + threadIdx.x;
+        if (i < packs) dst[i] = in[u];
+    }
+    if (rest + (int)threadIdx.x < elems) reinterpret_cast<T*>(dst)[rest + threadIdx.x] = src[rest + threadIdx.x];
+}
+template <typename T>
+__device__ __forceinline__ void tile_store(T* __restrict__ dst, const words_t* src, int elems) {
+    const int packs = (int)(elems * sizeof(T) / 16), rest = packs * (16 / (int)sizeof(T));
+#pragma unroll
+    for (int u = 0; u < NORM_TILE_PACKS; ++u) {
+        const int i = u * 256 + threadIdx.x;
+        if (i < packs) reinterpret_cast<words_t*>(dst)[i] = src[i];
+    }
+    if (rest + (int)threadIdx.x < elems) dst[rest + threadIdx.x] = reinterpret_cast<const T*>(src)[rest + threadIdx.x];
+}
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+    for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void norm_fwd_tile_kernel(size_t rows, int dim, int tile, const T* __restrict__ x,
+                                                            const void* __restrict__ weight, const void* __restrict__ bias,
+                                                            int affine_dtype, float eps, T* __restrict__ out,
+                                                            float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+    extern __shared__ words_t tile_mem[];
+    const int LANES = 256 / tile, r = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    T* z = reinterpret_cast<T*>(tile_mem) + r * dim;
+    float* w = reinterpret_cast<float*>(tile_mem + ((size_t)tile * dim * sizeof(T) + 15) / 16);
+    float* b = w + dim;
+    for (int c = threadIdx.x; c < dim; c += 256) {
+        w[c] = weight ? load_elem(weight, c, affine_dtype) : 1.0f;
+        b[c] = bias ? load_elem(bias, c, affine_dtype) : 0.0f;
+    }
+    const float inv = 1.0f / (float)dim;
+    for (size_t first = (size_t)blockIdx.x * tile; first < rows; first += (size_t)gridDim.x * tile) {
+        const int n = rows - first < (size_t)tile ? (int)(rows - first) : tile;
+        tile_load(x + first * dim, tile_mem, n * dim);
+        __syncthreads();
+        const bool live = r < n;
+        float s = 0.0f, q = 0.0f;
+        if (live)
+            for (int c = lane; c < dim; c += LANES) s += (float)z[c];
+        const float mean = lanes_sum(s, LANES) * inv;
+        if (live)
+            for (int c = lane; c < dim; c += LANES) { const float d = (float)z[c] - mean; q = FMA(d, d, q); }
+        const float rstd = 1.0f / __builtin_sqrtf(FMA(lanes_sum(q, LANES), inv, eps));
+        if (live) {
+            for (int c = lane; c < dim; c += LANES) z[c] = (T)FMA(((float)z[c] - mean) * rstd, w[c], b[c]);
+            if (lane == 0) {
+                if (mean_out) mean_out[first + r] = mean;
+                if (rstd_out) rstd_out[first + r] = rstd;
+            }
+        }
+        __syncthreads();
+        tile_store(out + first * dim, tile_mem, n * dim);
+        __syncthreads();
+    }
+}
+
+// Its gradient: dy and x of the tile in LDS; the column sums by one thread per column (and share of the rows), which keeps
+// them in registers over all tiles of the workgroup.
+template <typename T>
+__global__ __launch_bounds__(256) void norm_bwd_tile_kernel(size_t rows, int dim, int tile, const T* __restrict__ dy,
+                                                            const T* __restrict__ x, const void* __restrict__ weight,
+                                                            int affine_dtype, const float* __restrict__ mean_in,
+                                                            const float* __restrict__ rstd_in, T* __restrict__ dx,
+                                                            float* __restrict__ part) {
+    extern __shared__ words_t tile_mem[];
+    __shared__ float2 st[256];
+    __shared__ float cols[2 * 256];
+    const int LANES = 256 / tile, r = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const int tile_packs = (int)((tile * dim * (int)sizeof(T) + 15) / 16);
+    const T *xs = reinterpret_cast<const T*>(tile_mem), *gs = reinterpret_cast<const T*>(tile_mem + tile_packs);
+    T* z = reinterpret_cast<T*>(tile_mem) + r * dim;
+    const T* g = gs + r * dim;
+    float* w = reinterpret_cast<float*>(tile_mem + 2 * tile_packs);
+    for (int c = threadIdx.x; c < dim; c += 256) w[c] = weight ? load_elem(weight, c, affine_dtype) : 1.0f;
+    const float inv = 1.0f / (float)dim;
+    const int shares = dim < 256 ? 256 / dim : 1, share = threadIdx.x / dim;      // (of the rows, to threads of one column)
+    float dw[NORM_TILE_COLS], db[NORM_TILE_COLS];
+#pragma unroll
+    for (int i = 0; i < NORM_TILE_COLS; ++i) dw[i] = db[i] = 0.0f;
+    for (size_t first = (size_t)blockIdx.x * tile; first < rows; first += (size_t)gridDim.x * tile) {
+        const int n = rows - first < (size_t)tile ? (int)(rows - first) : tile;
+        tile_load(x + first * dim, tile_mem, n * dim);
+        tile_load(dy + first * dim, tile_mem + tile_packs, n * dim);
+        if ((int)threadIdx.x < n) st[threadIdx.x] = make_float2(mean_in[first + threadIdx.x], rstd_in[first + threadIdx.x]);
+        __syncthreads();
+        const bool live = r < n;
+        const float mean = live ? st[r].x : 0.0f, rstd = live ? st[r].y : 0.0f;
+        float s1 = 0.0f, s2 = 0.0f;
+        if (live && dx)
+            for (int c = lane; c < dim; c += LANES) {
+                const float d = (float)g[c] * w[c];
+                s1 += d;
+                s2 = FMA(d, ((float)z[c] - mean) * rstd, s2);
+            }
+        s1 = lanes_sum(s1, LANES) * inv;
+        s2 = lanes_sum(s2, LANES) * inv;
+        if (part) {
+            if (dim <= 256) {
+                if (share < shares) {
+                    const int c = threadIdx.x - share * dim;
+                    for (int k = share; k < n; k += shares) {
+                        const float d = (float)gs[k * dim + c];
+                        dw[0] = FMA(d, ((float)xs[k * dim + c] - st[k].x) * st[k].y, dw[0]);
+                        db[0] += d;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NORM_TILE_COLS; ++i) {
+                    const int c = i * 256 + threadIdx.x;
+                    if (c < dim)
+                        for (int k = 0; k < n; ++k) {
+                            const float d = (float)gs[k * dim + c];
+                            dw[i] = FMA(d, ((float)xs[k * dim + c] - st[k].x) * st[k].y, dw[i]);
+                            db[i] += d;
+                        }
+                }
+            }
+            __syncthreads();
+        }
+        if (dx) {
+            if (live)
+                for (int c = lane; c < dim; c += LANES)
+                    z[c] = (T)(((float)g[c] * w[c] - s1 - ((float)z[c] - mean) * rstd * s2) * rstd);
+            __syncthreads();
+            tile_store(dx + first * dim, tile_mem, n * dim);
+        }
+        __syncthreads();
+    }
+    if (!part) return;
+    float* mine = part + (size_t)blockIdx.x * 2 * dim;
+    if (dim <= 256) {
+        cols[2 * threadIdx.x] = dw[0];
+        cols[2 * threadIdx.x + 1] = db[0];
+        __syncthreads();
+        if ((int)threadIdx.x < dim) {
+            float a = dw[0], c = db[0];
+            for (int k = 1; k < shares; ++k) { a += cols[2 * (k * dim + threadIdx.x)]; c += cols[2 * (k * dim + threadIdx.x) + 1]; }
+            mine[threadIdx.x] = a;
+            mine[dim + threadIdx.x] = c;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NORM_TILE_COLS; ++i) {
+            const int c = i * 256 + threadIdx.x;
+            if (c < dim) { mine[c] = dw[i]; mine[dim + c] = db[i]; }
         }
     }
 }
@@ -698,11 +884,9 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_bwd_kernel(size_t ro
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const int col = (i * G + lane) * V;
+        load_affine<V>(col < dim ? weight : nullptr, affine_dtype, col, 1.0f, w[i]);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            w[i][j] = weight && col < dim ? load_elem(weight, col + j, affine_dtype) : 1.0f;
-            dw[i][j] = db[i][j] = 0.0f;
-        }
+        for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.0f;
     }
     const float inv = 1.0f / (float)dim;
     const size_t step = (size_t)gridDim.x * R::PER_BLOCK;
@@ -906,9 +1090,44 @@ int norm_bwd_launch(const NormArgs& a, uint32_t& nparts) {
     LAUNCH_OK("norm_bwd_kernel");
     return 0;
 }
+// Rows of a tile (a power of two, at least 8), or 0 where the tile kernels do not apply: rows that do not lie one behind the
+// other from a 16-byte boundary on, long ones, and those a group of lanes reads in packs as well (5 packs or more).
+int norm_tile_rows(const NormArgs& a, size_t bytes, bool backward) {
+    const bool whole = a.dim * bytes % 16 == 0;
+    if (a.x_stride != a.dim || a.dim * bytes * 8 > (size_t)NORM_TILE || a.dim > 256 * NORM_TILE_COLS) return 0;
+    if (whole && a.dim * bytes / 16 >= 5) return 0;
+    uintptr_t any = reinterpret_cast<uintptr_t>(a.x);
+    if (!backward) any |= reinterpret_cast<uintptr_t>(a.out);
+    else {
+        if (a.dy_stride != a.dim) return 0;
+        any |= reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.dx);
+    }
+    if (any & 15) return 0;
+    size_t t = 256;
+    while (t > 8 && (t * a.dim * bytes > (size_t)NORM_TILE || a.rows < t * 512)) t >>= 1;
+    return (int)t;
+}
+template <typename T>
+int norm_fwd_tile(const NormArgs& a, int tile) {
+    const size_t lds = (tile * a.dim * sizeof(T) + 15) / 16 * 16 + 2 * a.dim * sizeof(float);
+    norm_fwd_tile_kernel<T><<<dim3(norm_blocks(a.rows, tile, NORM_FWD_BLOCKS)), dim3(256), lds, a.s>>>(
+        a.rows, (int)a.dim, tile, (const T*)a.x, a.weight, a.bias, a.affine_dtype, a.eps, (T*)a.out, a.mean, a.rstd);
+    LAUNCH_OK("norm_fwd_tile_kernel");
+    return 0;
+}
+template <typename T>
+int norm_bwd_tile(const NormArgs& a, int tile, uint32_t& nparts) {
+    const size_t lds = 2 * ((tile * a.dim * sizeof(T) + 15) / 16 * 16) + a.dim * sizeof(float);
+    nparts = norm_blocks(a.rows, tile, NORM_BWD_BLOCKS);
+    norm_bwd_tile_kernel<T><<<dim3(nparts), dim3(256), lds, a.s>>>(a.rows, (int)a.dim, tile, (const T*)a.dy, (const T*)a.x, a.weight,
+                                                                  a.affine_dtype, a.mean, a.rstd, (T*)a.dx, a.part);
+    LAUNCH_OK("norm_bwd_tile_kernel");
+    return 0;
+}
 template <typename T, int V>
 int norm_fwd_v(const NormArgs& a) {
     const size_t packs = a.dim / V;
+    if (const int tile = norm_tile_rows(a, sizeof(T), false)) return norm_fwd_tile<T>(a, tile);
     if (packs <= 8) return norm_fwd_launch<T, V, 8, 1>(a);
     if (packs <= 16) return norm_fwd_launch<T, V, 16, 1>(a);
     if (packs <= 32) return norm_fwd_launch<T, V, 32, 1>(a);
@@ -928,7 +1147,8 @@ int norm_bwd_v(const NormArgs& a) {
     const size_t packs = a.dim / V;
     uint32_t nparts = 0;
     int rc = 0;
-    if (packs <= 8) rc = norm_bwd_launch<T, V, 8, 1>(a, nparts);
+    if (const int tile = norm_tile_rows(a, sizeof(T), true)) rc = norm_bwd_tile<T>(a, tile, nparts);
+    else if (packs <= 8) rc = norm_bwd_launch<T, V, 8, 1>(a, nparts);
     else if (packs <= 16) rc = norm_bwd_launch<T, V, 16, 1>(a, nparts);
     else if (packs <= 32) rc = norm_bwd_launch<T, V, 32, 1>(a, nparts);
     else if (packs <= 64) rc = norm_bwd_launch<T, V, 64, 1>(a, nparts);
