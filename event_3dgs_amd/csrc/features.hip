@@ -568,17 +568,42 @@ struct NormRow {      // sums over the lanes of a row
     }
 };
 
-// V parameters from `col` on (col a multiple of V), in 16-byte loads where the array allows it; `none` without an array.
-template <int V>
-__device__ __forceinline__ void load_affine(const void* __restrict__ p, int dtype, size_t col, float none, float v[V]) {
+// Parameters col, col + step, ... (N of them, `none` from dim on or without an array).  The branch on their type stands
+// outside the loop, so that all loads are in flight together.
+template <typename A, int N>
+__device__ __forceinline__ void load_params(const A* __restrict__ p, int col, int step, int dim, float none, float v[N]) {
+    A raw[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) raw[j] = p[col + j * step < dim ? col + j * step : dim - 1];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = col + j * step < dim ? (float)raw[j] : none;
+}
+template <int N>
+__device__ __forceinline__ void load_affine(const void* __restrict__ p, int dtype, int col, int step, int dim, float none, float v[N]) {
     if (!p) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = none;
-    } else if (V == 1 || (reinterpret_cast<uintptr_t>(p) & 15) != 0 || (V == 4 && dtype != E3_F32)) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = load_elem(p, col + j, dtype);
+        for (int j = 0; j < N; ++j) v[j] = none;
     } else if (dtype == E3_F32) {
-        const words_t* q = reinterpret_cast<const words_t*>(reinterpret_cast<const float*>(p) + col);
+        load_params<float, N>(reinterpret_cast<const float*>(p), col, step, dim, none, v);
+    } else if (dtype == E3_F16) {
+        load_params<f16_t, N>(reinterpret_cast<const f16_t*>(p), col, step, dim, none, v);
+    } else {
+        load_params<bf16_t, N>(reinterpret_cast<const bf16_t*>(p), col, step, dim, none, v);
+    }
+}
+
+// ... V neighbouring ones (col a multiple of V), in 16-byte loads where the array allows it
+template <int V>
+__device__ __forceinline__ void load_affine_pack(const void* __restrict__ p, int dtype, int col, int dim, float none, float v[V]) {
+    if (V == 1 || !p || (reinterpret_cast<uintptr_t>(p) & 15) != 0 || (V == 4 && dtype != E3_F32)) {
+        load_affine<V>(p, dtype, col, 1, dim, none, v);
+        return;
+    }
+    if (col >= dim) col = 0;                              // (lanes behind the row: any value)
+    if (dtype == E3_F32) {
+        words_t q[V / 4 ? V / 4 : 1];
+#pragma unroll
+        for (int j = 0; j < V / 4; ++j) q[j] = reinterpret_cast<const words_t*>(reinterpret_cast<const float*>(p) + col)[j];
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = word_elem<float>(q[j / 4], j % 4);
     } else {
@@ -602,8 +627,8 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_fwd_kernel(size_t ro
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const int col = (i * G + lane) * V;
-        load_affine<V>(col < dim ? weight : nullptr, affine_dtype, col, 1.0f, w[i]);
-        load_affine<V>(col < dim ? bias : nullptr, affine_dtype, col, 0.0f, b[i]);
+        load_affine_pack<V>(weight, affine_dtype, col, dim, 1.0f, w[i]);
+        load_affine_pack<V>(bias, affine_dtype, col, dim, 0.0f, b[i]);
     }
     const float inv = 1.0f / (float)dim;
     const size_t step = (size_t)gridDim.x * R::PER_BLOCK;
@@ -656,24 +681,36 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_fwd_kernel(size_t ro
 }
 
 // Short rows whose length is no multiple of 16 bytes (or a few packs only), one behind the other: a workgroup moves `tile` rows
-// at a time through LDS, in whole packs whatever the row length; 256 / tile lanes work on a row there.  (200000 rows of 59
-// fp16 values, a lane per value straight from memory: 38 us forward, 51 us backward; through LDS NORM_TILE_TIMES.)
-constexpr int NORM_TILE = 16384, NORM_TILE_PACKS = NORM_TILE / 16 / 256, NORM_TILE_COLS = 4;
+// at a time through LDS, in whole packs whatever the row length.  256 / tile lanes share a row there; each takes
+// NORM_TILE_ITEMS of its values into registers, in one batch of LDS reads.  (200000 rows of 59 fp16 values: a lane per
+// value straight from memory 38 us forward and 51 us backward, through LDS 15 us and 25 us.)
+constexpr int NORM_TILE = 16384, NORM_TILE_PACKS = NORM_TILE / 16 / 256, NORM_TILE_ITEMS = 16;
+// A tile on its way: loaded into registers while the tile before it is worked on, then put down in LDS.
 template <typename T>
-__device__ __forceinline__ void tile_load(const T* __restrict__ src, words_t* dst, int elems) {
-    const int packs = (int)(elems * sizeof(T) / 16), rest = packs * (16 / (int)sizeof(T));
+struct Tile {
     words_t in[NORM_TILE_PACKS];
+    T single;
+    __device__ __forceinline__ void load(const T* __restrict__ src, int elems) {
+        const int packs = (int)(elems * sizeof(T) / 16), rest = packs * (16 / (int)sizeof(T));
 #pragma unroll
-    for (int u = 0; u < NORM_TILE_PACKS; ++u) {
-        const int i = u * 256 + threadIdx.x;
-        if (i < packs) in[u] = reinterpret_cast<const words_t*>(src)[i];
+        for (int u = 0; u < NORM_TILE_PACKS; ++u) {
+            const int i = u * 256 + threadIdx.x;
+            if (i < packs) in[u] = reinterpret_cast<const words_t*>(src)[i];
+        }
+        if (rest + (int)threadIdx.x < elems) single = src[rest + threadIdx.x];
     }
+    __device__ __forceinline__ void put_down(words_t* dst, int elems) const {
+        const int packs = (int)(elems * sizeof(T) / 16), rest = packs * (16 / (int)sizeof(T));
 #pragma unroll
-    for (int u = 0; u < NORM_TILE_PACKS; ++u) {
-        const int i = u * 256 + threadIdx.x;
-        if (i < packs) dst[i] = in[u];
+        for (int u = 0; u < NORM_TILE_PACKS; ++u) {
+            const int i = u * 256 + threadIdx.x;
+            if (i < packs) dst[i] = in[u];
+        }
+        if (rest + (int)threadIdx.x < elems) reinterpret_cast<T*>(dst)[rest + threadIdx.x] = single;
     }
-    if (rest + (int)threadIdx.x < elems) reinterpret_cast<T*>(dst)[rest + threadIdx.x] = src[rest + threadIdx.x];
+};
+__device__ __forceinline__ int tile_count(size_t rows, size_t first, int tile) {
+    return first >= rows ? 0 : rows - first < (size_t)tile ? (int)(rows - first) : tile;
 }
 template <typename T>
 __device__ __forceinline__ void tile_store(T* __restrict__ dst, const words_t* src, int elems) {
@@ -698,27 +735,40 @@ __global__ __launch_bounds__(256) void norm_fwd_tile_kernel(size_t rows, int dim
     extern __shared__ words_t tile_mem[];
     const int LANES = 256 / tile, r = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     T* z = reinterpret_cast<T*>(tile_mem) + r * dim;
-    float* w = reinterpret_cast<float*>(tile_mem + ((size_t)tile * dim * sizeof(T) + 15) / 16);
-    float* b = w + dim;
-    for (int c = threadIdx.x; c < dim; c += 256) {
-        w[c] = weight ? load_elem(weight, c, affine_dtype) : 1.0f;
-        b[c] = bias ? load_elem(bias, c, affine_dtype) : 0.0f;
-    }
+    float w[NORM_TILE_ITEMS], b[NORM_TILE_ITEMS];
+    load_affine<NORM_TILE_ITEMS>(weight, affine_dtype, lane, LANES, dim, 1.0f, w);
+    load_affine<NORM_TILE_ITEMS>(bias, affine_dtype, lane, LANES, dim, 0.0f, b);
     const float inv = 1.0f / (float)dim;
-    for (size_t first = (size_t)blockIdx.x * tile; first < rows; first += (size_t)gridDim.x * tile) {
-        const int n = rows - first < (size_t)tile ? (int)(rows - first) : tile;
-        tile_load(x + first * dim, tile_mem, n * dim);
+    const size_t step = (size_t)gridDim.x * tile;
+    size_t first = (size_t)blockIdx.x * tile;
+    int n = tile_count(rows, first, tile);
+    Tile<T> next;
+    next.load(x + first * dim, n * dim);
+    for (; first < rows; first += step, n = tile_count(rows, first, tile)) {
+        next.put_down(tile_mem, n * dim);
         __syncthreads();
+        if (first + step < rows) next.load(x + (first + step) * dim, tile_count(rows, first + step, tile) * dim);
         const bool live = r < n;
-        float s = 0.0f, q = 0.0f;
-        if (live)
-            for (int c = lane; c < dim; c += LANES) s += (float)z[c];
+        float v[NORM_TILE_ITEMS], s = 0.0f, q = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NORM_TILE_ITEMS; ++i) {
+            const int c = i * LANES + lane;
+            v[i] = live && c < dim ? (float)z[c] : 0.0f;
+            s += v[i];
+        }
         const float mean = lanes_sum(s, LANES) * inv;
-        if (live)
-            for (int c = lane; c < dim; c += LANES) { const float d = (float)z[c] - mean; q = FMA(d, d, q); }
+#pragma unroll
+        for (int i = 0; i < NORM_TILE_ITEMS; ++i) {
+            v[i] -= mean;
+            if (i * LANES + lane < dim) q = FMA(v[i], v[i], q);
+        }
         const float rstd = 1.0f / __builtin_sqrtf(FMA(lanes_sum(q, LANES), inv, eps));
         if (live) {
-            for (int c = lane; c < dim; c += LANES) z[c] = (T)FMA(((float)z[c] - mean) * rstd, w[c], b[c]);
+#pragma unroll
+            for (int i = 0; i < NORM_TILE_ITEMS; ++i) {
+                const int c = i * LANES + lane;
+                if (c < dim) z[c] = (T)FMA(v[i] * rstd, w[i], b[i]);
+            }
             if (lane == 0) {
                 if (mean_out) mean_out[first + r] = mean;
                 if (rstd_out) rstd_out[first + r] = rstd;
@@ -730,97 +780,97 @@ __global__ __launch_bounds__(256) void norm_fwd_tile_kernel(size_t rows, int dim
     }
 }
 
-// Its gradient: dy and x of the tile in LDS; the column sums by one thread per column (and share of the rows), which keeps
-// them in registers over all tiles of the workgroup.
-template <typename T>
+// Its gradient; a lane keeps the column sums of its values over all tiles of the workgroup.
+template <typename T, int ITEMS>
 __global__ __launch_bounds__(256) void norm_bwd_tile_kernel(size_t rows, int dim, int tile, const T* __restrict__ dy,
                                                             const T* __restrict__ x, const void* __restrict__ weight,
                                                             int affine_dtype, const float* __restrict__ mean_in,
                                                             const float* __restrict__ rstd_in, T* __restrict__ dx,
                                                             float* __restrict__ part) {
     extern __shared__ words_t tile_mem[];
-    __shared__ float2 st[256];
-    __shared__ float cols[2 * 256];
     const int LANES = 256 / tile, r = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     const int tile_packs = (int)((tile * dim * (int)sizeof(T) + 15) / 16);
-    const T *xs = reinterpret_cast<const T*>(tile_mem), *gs = reinterpret_cast<const T*>(tile_mem + tile_packs);
     T* z = reinterpret_cast<T*>(tile_mem) + r * dim;
-    const T* g = gs + r * dim;
-    float* w = reinterpret_cast<float*>(tile_mem + 2 * tile_packs);
-    for (int c = threadIdx.x; c < dim; c += 256) w[c] = weight ? load_elem(weight, c, affine_dtype) : 1.0f;
-    const float inv = 1.0f / (float)dim;
-    const int shares = dim < 256 ? 256 / dim : 1, share = threadIdx.x / dim;      // (of the rows, to threads of one column)
-    float dw[NORM_TILE_COLS], db[NORM_TILE_COLS];
+    const T* gr = reinterpret_cast<const T*>(tile_mem + tile_packs) + r * dim;
+    float w[ITEMS], dw[ITEMS], db[ITEMS];
+    load_affine<ITEMS>(weight, affine_dtype, lane, LANES, dim, 1.0f, w);
 #pragma unroll
-    for (int i = 0; i < NORM_TILE_COLS; ++i) dw[i] = db[i] = 0.0f;
-    for (size_t first = (size_t)blockIdx.x * tile; first < rows; first += (size_t)gridDim.x * tile) {
-        const int n = rows - first < (size_t)tile ? (int)(rows - first) : tile;
-        tile_load(x + first * dim, tile_mem, n * dim);
-        tile_load(dy + first * dim, tile_mem + tile_packs, n * dim);
-        if ((int)threadIdx.x < n) st[threadIdx.x] = make_float2(mean_in[first + threadIdx.x], rstd_in[first + threadIdx.x]);
-        __syncthreads();
+    for (int i = 0; i < ITEMS; ++i) dw[i] = db[i] = 0.0f;
+    const float inv = 1.0f / (float)dim;
+    const size_t step = (size_t)gridDim.x * tile;
+    size_t first = (size_t)blockIdx.x * tile;
+    int n = tile_count(rows, first, tile);
+    Tile<T> next_x, next_dy;
+    float next_mean = 0.0f, next_rstd = 0.0f;
+    auto load = [&](size_t at, int count) {
+        next_x.load(x + at * dim, count * dim);
+        next_dy.load(dy + at * dim, count * dim);
+        if (r < count) {
+            next_mean = mean_in[at + r];
+            next_rstd = rstd_in[at + r];
+        }
+    };
+    load(first, n);
+    for (; first < rows; first += step, n = tile_count(rows, first, tile)) {
         const bool live = r < n;
-        const float mean = live ? st[r].x : 0.0f, rstd = live ? st[r].y : 0.0f;
-        float s1 = 0.0f, s2 = 0.0f;
-        if (live && dx)
-            for (int c = lane; c < dim; c += LANES) {
-                const float d = (float)g[c] * w[c];
-                s1 += d;
-                s2 = FMA(d, ((float)z[c] - mean) * rstd, s2);
-            }
+        const float mean = live ? next_mean : 0.0f, rstd = live ? next_rstd : 0.0f;
+        next_x.put_down(tile_mem, n * dim);
+        next_dy.put_down(tile_mem + tile_packs, n * dim);
+        __syncthreads();
+        if (first + step < rows) load(first + step, tile_count(rows, first + step, tile));
+        float h[ITEMS], g[ITEMS], s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int c = i * LANES + lane;
+            const bool in = live && c < dim;
+            h[i] = in ? (float)z[c] : mean;
+            g[i] = in ? (float)gr[c] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            h[i] = (h[i] - mean) * rstd;
+            dw[i] = FMA(g[i], h[i], dw[i]);
+            db[i] += g[i];
+            g[i] *= w[i];
+            s1 += g[i];
+            s2 = FMA(g[i], h[i], s2);
+        }
         s1 = lanes_sum(s1, LANES) * inv;
         s2 = lanes_sum(s2, LANES) * inv;
-        if (part) {
-            if (dim <= 256) {
-                if (share < shares) {
-                    const int c = threadIdx.x - share * dim;
-                    for (int k = share; k < n; k += shares) {
-                        const float d = (float)gs[k * dim + c];
-                        dw[0] = FMA(d, ((float)xs[k * dim + c] - st[k].x) * st[k].y, dw[0]);
-                        db[0] += d;
-                    }
-                }
-            } else {
+        if (dx) {
+            if (live) {
 #pragma unroll
-                for (int i = 0; i < NORM_TILE_COLS; ++i) {
-                    const int c = i * 256 + threadIdx.x;
-                    if (c < dim)
-                        for (int k = 0; k < n; ++k) {
-                            const float d = (float)gs[k * dim + c];
-                            dw[i] = FMA(d, ((float)xs[k * dim + c] - st[k].x) * st[k].y, dw[i]);
-                            db[i] += d;
-                        }
+                for (int i = 0; i < ITEMS; ++i) {
+                    const int c = i * LANES + lane;
+                    if (c < dim) z[c] = (T)((g[i] - s1 - h[i] * s2) * rstd);
                 }
             }
-            __syncthreads();
-        }
-        if (dx) {
-            if (live)
-                for (int c = lane; c < dim; c += LANES)
-                    z[c] = (T)(((float)g[c] * w[c] - s1 - ((float)z[c] - mean) * rstd * s2) * rstd);
             __syncthreads();
             tile_store(dx + first * dim, tile_mem, n * dim);
         }
         __syncthreads();
     }
     if (!part) return;
+    // the sums of the lanes that hold the same columns, in order: first within a wave, then over the waves through LDS
+    __shared__ float sums[2][4][32 * ITEMS];
     float* mine = part + (size_t)blockIdx.x * 2 * dim;
-    if (dim <= 256) {
-        cols[2 * threadIdx.x] = dw[0];
-        cols[2 * threadIdx.x + 1] = db[0];
-        __syncthreads();
-        if ((int)threadIdx.x < dim) {
-            float a = dw[0], c = db[0];
-            for (int k = 1; k < shares; ++k) { a += cols[2 * (k * dim + threadIdx.x)]; c += cols[2 * (k * dim + threadIdx.x) + 1]; }
-            mine[threadIdx.x] = a;
-            mine[dim + threadIdx.x] = c;
-        }
-    } else {
+    const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63;
 #pragma unroll
-        for (int i = 0; i < NORM_TILE_COLS; ++i) {
-            const int c = i * 256 + threadIdx.x;
-            if (c < dim) { mine[c] = dw[i]; mine[dim + c] = db[i]; }
+    for (int i = 0; i < ITEMS; ++i) {
+        float a = dw[i], c = db[i];
+        for (int o = LANES; o < 64; o <<= 1) {
+            a += __shfl_xor(a, o, 64);
+            c += __shfl_xor(c, o, 64);
         }
+        if (wl < LANES) {
+            sums[0][wave][i * LANES + wl] = a;
+            sums[1][wave][i * LANES + wl] = c;
+        }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < dim; c += 256) {
+        mine[c] = ((sums[0][0][c] + sums[0][1][c]) + sums[0][2][c]) + sums[0][3][c];
+        mine[dim + c] = ((sums[1][0][c] + sums[1][1][c]) + sums[1][2][c]) + sums[1][3][c];
     }
 }
 
@@ -884,7 +934,7 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_bwd_kernel(size_t ro
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const int col = (i * G + lane) * V;
-        load_affine<V>(col < dim ? weight : nullptr, affine_dtype, col, 1.0f, w[i]);
+        load_affine_pack<V>(weight, affine_dtype, col, dim, 1.0f, w[i]);
 #pragma unroll
         for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.0f;
     }
@@ -1052,7 +1102,7 @@ unsigned norm_blocks(size_t rows, int per_block, size_t most) {
     const size_t need = (rows + per_block - 1) / per_block;
     return (unsigned)(need < most ? need : most);
 }
-constexpr size_t NORM_FWD_BLOCKS = 4096, NORM_BWD_BLOCKS = 1024, NORM_LONG_PARTS = 64;
+constexpr size_t NORM_FWD_BLOCKS = 4096, NORM_BWD_BLOCKS = 1024, NORM_TILE_BLOCKS = 1024, NORM_LONG_PARTS = 64;
 
 struct NormArgs {
     size_t rows, dim, x_stride, dy_stride;
@@ -1090,12 +1140,17 @@ int norm_bwd_launch(const NormArgs& a, uint32_t& nparts) {
     LAUNCH_OK("norm_bwd_kernel");
     return 0;
 }
-// Rows of a tile (a power of two, at least 8), or 0 where the tile kernels do not apply: rows that do not lie one behind the
-// other from a 16-byte boundary on, long ones, and those a group of lanes reads in packs as well (5 packs or more).
+// Values of a row to a lane.  The gradient keeps five arrays of them in registers: 8 while 32 lanes are enough for the row.
+int norm_tile_items(size_t dim, bool backward) { return backward && dim <= 256 ? 8 : NORM_TILE_ITEMS; }
+
+// Rows of a tile, or 0 where the tile kernels do not apply: rows that do not lie one behind the other from a 16-byte boundary
+// on, rows past 64 lanes of NORM_TILE_ITEMS values, and those that a group of lanes reads in packs as well (5 packs or
+// more).  256 / the lanes of a row, with more lanes to it when the launch would not fill the chip otherwise; at least 8 rows,
+// so that every tile begins on a 16-byte boundary.
 int norm_tile_rows(const NormArgs& a, size_t bytes, bool backward) {
-    const bool whole = a.dim * bytes % 16 == 0;
-    if (a.x_stride != a.dim || a.dim * bytes * 8 > (size_t)NORM_TILE || a.dim > 256 * NORM_TILE_COLS) return 0;
-    if (whole && a.dim * bytes / 16 >= 5) return 0;
+    size_t lanes = 1;
+    while (lanes * norm_tile_items(a.dim, backward) < a.dim) lanes <<= 1;
+    if (lanes > 32 || a.x_stride != a.dim || (a.dim * bytes % 16 == 0 && a.dim * bytes / 16 >= 5)) return 0;
     uintptr_t any = reinterpret_cast<uintptr_t>(a.x);
     if (!backward) any |= reinterpret_cast<uintptr_t>(a.out);
     else {
@@ -1103,24 +1158,28 @@ int norm_tile_rows(const NormArgs& a, size_t bytes, bool backward) {
         any |= reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.dx);
     }
     if (any & 15) return 0;
-    size_t t = 256;
-    while (t > 8 && (t * a.dim * bytes > (size_t)NORM_TILE || a.rows < t * 512)) t >>= 1;
-    return (int)t;
+    while (lanes < 32 && lanes < a.dim && a.rows < 256 / lanes * 512) lanes <<= 1;
+    return (int)(256 / lanes);
 }
 template <typename T>
 int norm_fwd_tile(const NormArgs& a, int tile) {
-    const size_t lds = (tile * a.dim * sizeof(T) + 15) / 16 * 16 + 2 * a.dim * sizeof(float);
-    norm_fwd_tile_kernel<T><<<dim3(norm_blocks(a.rows, tile, NORM_FWD_BLOCKS)), dim3(256), lds, a.s>>>(
+    const size_t lds = (tile * a.dim * sizeof(T) + 15) / 16 * 16;
+    norm_fwd_tile_kernel<T><<<dim3(norm_blocks(a.rows, tile, NORM_TILE_BLOCKS)), dim3(256), lds, a.s>>>(
         a.rows, (int)a.dim, tile, (const T*)a.x, a.weight, a.bias, a.affine_dtype, a.eps, (T*)a.out, a.mean, a.rstd);
     LAUNCH_OK("norm_fwd_tile_kernel");
     return 0;
 }
 template <typename T>
 int norm_bwd_tile(const NormArgs& a, int tile, uint32_t& nparts) {
-    const size_t lds = 2 * ((tile * a.dim * sizeof(T) + 15) / 16 * 16) + a.dim * sizeof(float);
-    nparts = norm_blocks(a.rows, tile, NORM_BWD_BLOCKS);
-    norm_bwd_tile_kernel<T><<<dim3(nparts), dim3(256), lds, a.s>>>(a.rows, (int)a.dim, tile, (const T*)a.dy, (const T*)a.x, a.weight,
-                                                                  a.affine_dtype, a.mean, a.rstd, (T*)a.dx, a.part);
+    const size_t lds = 2 * ((tile * a.dim * sizeof(T) + 15) / 16 * 16);
+    nparts = norm_blocks(a.rows, tile, NORM_TILE_BLOCKS);
+#define E3_TILE_BWD(ITEMS)                                                                                                    \
+    norm_bwd_tile_kernel<T, ITEMS><<<dim3(nparts), dim3(256), lds, a.s>>>(a.rows, (int)a.dim, tile, (const T*)a.dy,           \
+                                                                        (const T*)a.x, a.weight, a.affine_dtype, a.mean,     \
+                                                                        a.rstd, (T*)a.dx, a.part)
+    if (norm_tile_items(a.dim, true) == 8) E3_TILE_BWD(8);
+    else E3_TILE_BWD(NORM_TILE_ITEMS);
+#undef E3_TILE_BWD
     LAUNCH_OK("norm_bwd_tile_kernel");
     return 0;
 }
