@@ -222,33 +222,33 @@ size_t grad_row(const Scores& s) { return s.planes ? 1 : s.classes; }
 size_t grad_class(const Scores& s) { return s.planes ? s.rows : 1; }
 Tensor shaped(const Scores& s, const Tensor& grad) { return grad.view(s.shape).movedim(-1, s.class_dim); }
 
-// value (0-dim, or one per row), stats, loss pair; fills `grad` (of empty_grad) if it is defined
-std::tuple<Tensor, Tensor, Tensor> distill_forward(const Scores& s, double temperature, int64_t reduction, const Tensor& grad) {
+// value (0-dim, or one per row) and what the backward call needs; fills `grad` (of empty_grad) if it is defined
+std::tuple<Tensor, Tensor> distill_forward(const Scores& s, double temperature, int64_t reduction, const Tensor& grad) {
     const auto opt = s.logits.options().dtype(torch::kFloat32);
-    Tensor stats = torch::empty({(int64_t)s.rows, 2}, opt), loss = torch::empty({2}, opt);
+    const size_t n_stats = (2 * s.rows + 1 + 1) / 2 * 2;                      // (the scratch behind it is 8-byte aligned)
+    Tensor stats = torch::empty({(int64_t)(n_stats + (e3dgs_distill_scratch_bytes(s.rows) + 3) / 4)}, opt);
+    Tensor loss = torch::empty({}, opt);
     Tensor row_loss = reduction == 0 ? torch::empty({(int64_t)s.rows}, opt) : Tensor();
-    Tensor scratch = scratch_of(e3dgs_distill_scratch_bytes(s.rows), s.logits);
     check(e3dgs_distill_forward(s.rows, s.classes, s.k, s.logits.data_ptr(), s.row_stride, s.class_stride,
                                 dtype_of(s.logits, "logits"), s.teacher.data_ptr(), (size_t)s.teacher.stride(0),
                                 (size_t)s.teacher.stride(1), dtype_of(s.teacher, "teacher_logits"), s.index.data_ptr(),
                                 (size_t)s.index.stride(0), (size_t)s.index.stride(1), index_bytes_of(s.index),
                                 (float)temperature, (int)reduction, stats.data_ptr<float>(),
                                 row_loss.defined() ? row_loss.data_ptr<float>() : nullptr, loss.data_ptr<float>(),
-                                grad.defined() ? grad.data_ptr() : nullptr, grad_row(s), grad_class(s), bytes(scratch), stream()),
+                                grad.defined() ? grad.data_ptr() : nullptr, grad_row(s), grad_class(s),
+                                reinterpret_cast<char*>(stats.data_ptr<float>() + n_stats), stream()),
           "e3dgs_distill_forward");
-    if (reduction == 0) return std::make_tuple(row_loss.view(std::vector<int64_t>(s.shape.begin(), s.shape.end() - 1)), stats, loss);
-    return std::make_tuple(loss.select(0, 0), stats, loss);
+    if (reduction == 0) return std::make_tuple(row_loss.view(std::vector<int64_t>(s.shape.begin(), s.shape.end() - 1)), stats);
+    return std::make_tuple(loss, stats);
 }
 
-Tensor distill_backward(const Scores& s, double temperature, int64_t reduction, const Tensor& stats, const Tensor& loss,
-                        const Tensor& d_loss) {
+Tensor distill_backward(const Scores& s, double temperature, int64_t reduction, const Tensor& stats, const Tensor& d_loss) {
     Tensor grad = empty_grad(s);
     check(e3dgs_distill_backward(s.rows, s.classes, s.k, s.logits.data_ptr(), s.row_stride, s.class_stride,
                                  dtype_of(s.logits, "logits"), s.teacher.data_ptr(), (size_t)s.teacher.stride(0),
                                  (size_t)s.teacher.stride(1), dtype_of(s.teacher, "teacher_logits"), s.index.data_ptr(),
                                  (size_t)s.index.stride(0), (size_t)s.index.stride(1), index_bytes_of(s.index),
-                                 (float)temperature, (int)reduction, stats.data_ptr<float>(), loss.data_ptr<float>(),
-                                 d_loss.data_ptr<float>(), grad.data_ptr(), grad_row(s), grad_class(s), stream()),
+                                 (float)temperature, (int)reduction, stats.data_ptr<float>(), d_loss.data_ptr<float>(), grad.data_ptr(), grad_row(s), grad_class(s), stream()),
           "e3dgs_distill_backward");
     return shaped(s, grad);
 }
@@ -258,12 +258,11 @@ struct DistillFunction : public torch::autograd::Function<DistillFunction> {
                           double temperature, int64_t reduction, int64_t class_dim) {
         const Guard guard(logits.device());
         auto r = distill_forward(scores_of(logits, teacher, index, class_dim), temperature, reduction, Tensor());
-        ctx->save_for_backward({logits, teacher, index, std::get<1>(r), std::get<2>(r)});
+        ctx->save_for_backward({logits, teacher, index, std::get<1>(r)});
         ctx->saved_data["temperature"] = temperature;
         ctx->saved_data["reduction"] = reduction;
         ctx->saved_data["class_dim"] = class_dim;
-        // (the pair of the gradient is a tensor of its own: the caller may change the value it was handed)
-        return reduction == 0 ? std::get<0>(r) : std::get<0>(r).clone();
+        return std::get<0>(r);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         once("distill_loss");
@@ -272,8 +271,7 @@ struct DistillFunction : public torch::autograd::Function<DistillFunction> {
         const Guard guard(saved[0].device());
         const Scores s = scores_of(saved[0], saved[1], saved[2], ctx->saved_data["class_dim"].toInt());
         const Tensor g = grads[0].to(torch::kFloat32).contiguous();
-        Tensor d = distill_backward(s, ctx->saved_data["temperature"].toDouble(), ctx->saved_data["reduction"].toInt(), saved[3],
-                                    saved[4], g);
+        Tensor d = distill_backward(s, ctx->saved_data["temperature"].toDouble(), ctx->saved_data["reduction"].toInt(), saved[3], g);
         return {d, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };

@@ -178,7 +178,7 @@ def lib():
     L.e3dgs_distill_forward.restype = C.c_int
     L.e3dgs_distill_forward.argtypes = _scores + [_fp] * 3 + [_vp, _sz, _sz, _cp, _vp]
     L.e3dgs_distill_backward.restype = C.c_int
-    L.e3dgs_distill_backward.argtypes = _scores + [_fp] * 3 + [_vp, _sz, _sz, _vp]
+    L.e3dgs_distill_backward.argtypes = _scores + [_fp] * 2 + [_vp, _sz, _sz, _vp]
     L.e3dgs_profile_enable.restype = None
     L.e3dgs_profile_enable.argtypes = [C.c_int]
     L.e3dgs_profile_select.restype = None

@@ -128,8 +128,8 @@ int e3_distill_forward_impl(size_t, size_t, size_t, const void*, size_t, size_t,
                             const void*, size_t, size_t, int, float, int, float*, float*, float*, void*, size_t, size_t, char*,
                             hipStream_t);
 int e3_distill_backward_impl(size_t, size_t, size_t, const void*, size_t, size_t, int, const void*, size_t, size_t, int,
-                             const void*, size_t, size_t, int, float, int, const float*, const float*, const float*, void*,
-                             size_t, size_t, hipStream_t);
+                             const void*, size_t, size_t, int, float, int, const float*, const float*, void*, size_t, size_t,
+                             hipStream_t);
 size_t e3_event_scratch_bytes(int, int);
 int e3_event_loss_impl(int, int, const float*, const float*, const float*, const float*, const float*, const float*,
                        const float*, const float*, float, float*, float*, float*, float*, char*, hipStream_t, float*, double*,
@@ -953,19 +953,19 @@ int e3dgs_distill_forward(size_t rows, size_t classes, size_t k, const void* log
 int e3dgs_distill_backward(size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride, size_t class_stride,
                            int dtype, const void* teacher, size_t teacher_row_stride, size_t teacher_entry_stride,
                            int teacher_dtype, const void* index, size_t index_row_stride, size_t index_entry_stride,
-                           int index_bytes, float temperature, int reduction, const float* stats, const float* loss,
+                           int index_bytes, float temperature, int reduction, const float* stats,
                            const float* d_loss, void* grad, size_t grad_row_stride, size_t grad_class_stride, void* stream) {
     g_err[0] = 0;
     const char* who = "e3dgs_distill_backward";
     const int rc = distill_args(who, rows, classes, k, logits, row_stride, class_stride, dtype, teacher, teacher_dtype, index,
                                 index_bytes, temperature, reduction);
     if (rc) return rc;
-    if (rows > 0 && (!stats || !loss || !grad)) return feature_args_fail(who, rows, classes, dtype, "null pointer");
+    if (rows > 0 && (!stats || !grad)) return feature_args_fail(who, rows, classes, dtype, "null pointer");
     if (!distill_grad_ok(rows, classes, class_stride, grad_row_stride, grad_class_stride))
         return feature_args_fail(who, rows, classes, dtype, "the gradient's layout differs from the scores'");
     return e3_distill_backward_impl(rows, classes, k, logits, row_stride, class_stride, dtype, teacher, teacher_row_stride,
                                     teacher_entry_stride, teacher_dtype, index, index_row_stride, index_entry_stride,
-                                    index_bytes, temperature, reduction, stats, loss, d_loss, grad, grad_row_stride,
+                                    index_bytes, temperature, reduction, stats, d_loss, grad, grad_row_stride,
                                     grad_class_stride, (hipStream_t)stream);
 }
 

@@ -41,7 +41,7 @@ struct DistillArgs {
     const float* scale;
     void* grad;
     size_t g_row, g_class;
-    float* loss;            // (value, weight of a row), written by the only workgroup of a launch
+    float *loss, *weight_out;   // the value and the weight of a row, written by the only workgroup of a launch
     const uint32_t* counts; // partial counts of the labelled rows (a value formed with its gradient)
     uint32_t ncounts;
 };
@@ -75,8 +75,9 @@ struct Label {
 };
 constexpr int ID_BROKEN = 0x7FFFFFFF;
 __device__ __forceinline__ float entry_score(const DistillArgs& a, size_t row, size_t k, long long& id) {
-    id = load_index(a.index, row * a.i_row + k * a.i_entry, a.index_bytes);
-    return id < 0 ? -__builtin_inff() : load_elem(a.teacher, row * a.t_row + k * a.t_entry, a.teacher_dtype);
+    id = load_index_flat(a.index, row * a.i_row + k * a.i_entry, a.index_bytes);
+    const float t = load_elem_flat(a.teacher, row * a.t_row + k * a.t_entry, a.teacher_dtype);
+    return id < 0 ? -__builtin_inff() : t;
 }
 // the class of an entry as it is kept in LDS: -1 not listed, ID_BROKEN past the end
 __device__ __forceinline__ int entry_class(const DistillArgs& a, float t, long long id) {
@@ -210,7 +211,7 @@ __device__ __forceinline__ float row_weight(const DistillArgs& a, uint32_t* lds)
 __device__ __forceinline__ void store_loss(const DistillArgs& a, double total, unsigned long long count) {
     const double weight = a.reduction == 1 ? 1.0 / (double)(count ? count : 1) : 1.0;
     a.loss[0] = (float)(total * weight);
-    a.loss[1] = (float)weight;
+    if (a.weight_out) *a.weight_out = (float)weight;
 }
 // Adds up what the workgroup's threads hold (in a fixed tree): one pair per workgroup, or the result itself when there is
 // only one.
@@ -646,35 +647,44 @@ struct PlaneLabel {
     bool any, broken;
 };
 // Adds the weights of a pixel's label to its column.
+constexpr int PLANE_ENTRIES = 8;       // of a label, read together
 __device__ __forceinline__ PlaneLabel plane_label(const DistillArgs& a, size_t row, float c, float rt, float* col) {
     PlaneLabel l;
     float top = -__builtin_inff(), sum = 0.0f;
     l.any = l.broken = false;
-    for (size_t k = 0; k < a.k; ++k) {
-        long long id;
-        const float t = entry_score(a, row, k, id);
-        if (t == -__builtin_inff()) continue;
-        l.any = true;
-        l.broken |= id >= (long long)a.classes;
-        top = fmaxf(top, t);
+    for (size_t k0 = 0; k0 < a.k; k0 += PLANE_ENTRIES) {
+        float t[PLANE_ENTRIES];
+#pragma unroll
+        for (int k = 0; k < PLANE_ENTRIES; ++k) {
+            long long id;
+            t[k] = entry_score(a, row, k0 + k < a.k ? k0 + k : a.k - 1, id);
+            if (k0 + k >= a.k) t[k] = -__builtin_inff();
+            l.any |= t[k] != -__builtin_inff();
+            l.broken |= t[k] != -__builtin_inff() && id >= (long long)a.classes;
+        }
+        soft_add<PLANE_ENTRIES>(top, sum, t, c);
     }
     l.top = top;
     l.inv = l.qlogq = 0.0f;
     if (!l.any) return l;
-    for (size_t k = 0; k < a.k; ++k) {
-        long long id;
-        const float t = entry_score(a, row, k, id);
-        if (t != -__builtin_inff()) sum += exp2_hw((t - top) * c);
-    }
     l.inv = 1.0f / sum;
     const float rest = log2_hw(l.inv) * LN2;
-    for (size_t k = 0; k < a.k; ++k) {
-        long long id;
-        const float t = entry_score(a, row, k, id);
-        if (t == -__builtin_inff() || id >= (long long)a.classes) continue;
-        const float q = exp2_hw((t - top) * c) * l.inv;
-        if (q != 0.0f) l.qlogq += q * ((t - top) * rt + rest);
-        col[(size_t)id * 64] += q;
+    for (size_t k0 = 0; k0 < a.k; k0 += PLANE_ENTRIES) {
+        float t[PLANE_ENTRIES];
+        int cls[PLANE_ENTRIES];
+#pragma unroll
+        for (int k = 0; k < PLANE_ENTRIES; ++k) {
+            long long id;
+            t[k] = entry_score(a, row, k0 + k < a.k ? k0 + k : a.k - 1, id);
+            cls[k] = k0 + k < a.k ? entry_class(a, t[k], id) : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < PLANE_ENTRIES; ++k) {
+            if (cls[k] < 0 || cls[k] == ID_BROKEN) continue;
+            const float q = exp2_hw((t[k] - top) * c) * l.inv;
+            if (q != 0.0f) l.qlogq += q * ((t[k] - top) * rt + rest);
+            col[(size_t)cls[k] * 64] += q;
+        }
     }
     return l;
 }
@@ -808,8 +818,8 @@ __device__ __forceinline__ void pixel_label(const DistillArgs& a, size_t row, fl
 #pragma unroll
     for (int k = 0; k < KR; ++k) {
         const size_t at = k < (int)a.k ? k : a.k - 1;               // (unconditional loads, all in flight)
-        const long long id = load_index(a.index, row * a.i_row + at * a.i_entry, a.index_bytes);
-        t[k] = load_elem(a.teacher, row * a.t_row + at * a.t_entry, a.teacher_dtype);
+        const long long id = load_index_flat(a.index, row * a.i_row + at * a.i_entry, a.index_bytes);
+        t[k] = load_elem_flat(a.teacher, row * a.t_row + at * a.t_entry, a.teacher_dtype);
         l.id[k] = id >= (long long)a.classes ? 0x7FFFFFFF : id < 0 || k >= (int)a.k ? -1 : (int)id;
     }
 #pragma unroll
@@ -1167,6 +1177,7 @@ int e3_distill_forward_impl(size_t rows, size_t classes, size_t k, const void* l
     a.stats = reinterpret_cast<float2*>(stats);
     a.row_loss = row_loss;
     a.loss = loss;
+    a.weight_out = rows > 0 ? stats + 2 * rows : nullptr;
     a.part = reinterpret_cast<float2*>(scratch);
     uint32_t* counts = reinterpret_cast<uint32_t*>(a.part + DISTILL_BLOCKS);
     unsigned blocks = 0;
@@ -1186,20 +1197,19 @@ int e3_distill_forward_impl(size_t rows, size_t classes, size_t k, const void* l
         LAUNCH_OK("distill_join_kernel");
     }
     if (!grad || both || rows == 0) return 0;
-    a.weight = loss + 1;
+    a.weight = a.weight_out;
     return distill_any(a, true, blocks, s);
 }
 
 int e3_distill_backward_impl(size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride,
                              size_t class_stride, int dtype, const void* teacher, size_t t_row, size_t t_entry,
                              int teacher_dtype, const void* index, size_t i_row, size_t i_entry, int index_bytes,
-                             float temperature, int reduction, const float* stats, const float* loss, const float* d_loss,
-                             void* grad, size_t g_row, size_t g_class, hipStream_t s) {
+                             float temperature, int reduction, const float* stats, const float* d_loss, void* grad, size_t g_row, size_t g_class, hipStream_t s) {
     if (rows == 0) return 0;
     DistillArgs a = distill_args(rows, classes, k, logits, row_stride, class_stride, dtype, teacher, t_row, t_entry,
                                  teacher_dtype, index, i_row, i_entry, index_bytes, temperature, reduction);
     a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
-    a.weight = loss + 1;
+    a.weight = stats + 2 * rows;
     a.scale = d_loss;
     a.grad = grad;
     a.g_row = g_row;

@@ -77,6 +77,20 @@ __device__ __forceinline__ long long load_index(const void* __restrict__ p, size
     return bytes == 8 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
 }
 
+// The same for labels, whose loads should be in flight together: without a branch on the type (a branch waits for its own
+// load), as the halves of a value, the second one only counting where the type has it.
+__device__ __forceinline__ float load_elem_flat(const void* __restrict__ p, size_t i, int dtype) {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + (dtype == E3_F32 ? 2 * i : i);
+    const uint32_t lo = h[0], hi = h[dtype == E3_F32 ? 1 : 0];
+    const float f16 = (float)__builtin_bit_cast(f16_t, (uint16_t)lo);
+    return dtype == E3_F32 ? __uint_as_float(hi << 16 | lo) : dtype == E3_F16 ? f16 : __uint_as_float(lo << 16);
+}
+__device__ __forceinline__ long long load_index_flat(const void* __restrict__ p, size_t i, int bytes) {
+    const int* w = reinterpret_cast<const int*>(p) + (bytes == 8 ? 2 * i : i);
+    const int lo = w[0], hi = w[bytes == 8 ? 1 : 0];
+    return (long long)(bytes == 8 ? hi : lo >> 31) << 32 | (uint32_t)lo;
+}
+
 // Sum / maximum over aligned groups of G lanes (G a power of two, 1 .. 64): every lane of the group gets the result, and
 // every lane adds in the same tree, so the result does not depend on the lane.
 template <int G>

@@ -776,9 +776,9 @@ int e3dgs_layer_norm_backward(size_t rows, size_t dim, const void* grad_out, siz
  * Strides in elements: logits (row_stride, class_stride) with class_stride 1, or row_stride 1 and at most
  * E3DGS_DISTILL_MAX_PLANES classes (planes, as an image lies); teacher and index (row, entry) as they are.
  * reduction: 0 none, 1 mean over the labelled rows, 2 sum.
- *   stats     2 floats per row, for the backward call
+ *   stats     2 floats per row and one more, for the backward call
  *   row_loss  one float per row (may be NULL)
- *   loss      2 floats: the value (sum or mean; for `none` the sum) and the weight of a row, for the backward call
+ *   loss      one float: the value (sum or mean; for `none` the sum)
  *   grad      (may be NULL) the gradient of the value by logits, in the same pass where the layout allows; for `none` of the
  *             sum.  Then stats is scratch
  * backward: d_loss = the gradient of the value (device; one float, or with reduction 0 one per row; NULL: 1); grad has the
@@ -796,7 +796,7 @@ int e3dgs_distill_forward(size_t rows, size_t classes, size_t k, const void* log
 int e3dgs_distill_backward(size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride, size_t class_stride,
                            int dtype, const void* teacher, size_t teacher_row_stride, size_t teacher_entry_stride,
                            int teacher_dtype, const void* index, size_t index_row_stride, size_t index_entry_stride,
-                           int index_bytes, float temperature, int reduction, const float* stats, const float* loss,
+                           int index_bytes, float temperature, int reduction, const float* stats,
                            const float* d_loss, void* grad, size_t grad_row_stride, size_t grad_class_stride, void* stream);
 
 #ifdef __cplusplus

@@ -70,13 +70,13 @@ def test_distill_arguments(hip_lib, change):
             a["teacher_dtype"], a["index"], a["k"], 1, a["index_bytes"], a["temperature"], a["reduction"])
     assert hip_lib.e3dgs_distill_forward(*head, PTR, PTR, PTR, None, 0, 0, PTR, None) != 0
     assert "e3dgs_distill_forward" in text()
-    assert hip_lib.e3dgs_distill_backward(*head, PTR, PTR, PTR, PTR, a["row_stride"], a["class_stride"], None) != 0
+    assert hip_lib.e3dgs_distill_backward(*head, PTR, PTR, PTR, a["row_stride"], a["class_stride"], None) != 0
     assert "e3dgs_distill_backward" in text()
 
 
 def test_distill_gradient_layout(hip_lib):
     head = (5, 9, 2, PTR, 9, 1, 0, PTR, 2, 1, 0, PTR, 2, 1, 4, 1.0, 1)
-    assert hip_lib.e3dgs_distill_backward(*head, PTR, PTR, PTR, PTR, 1, 5, None) != 0
+    assert hip_lib.e3dgs_distill_backward(*head, PTR, PTR, PTR, 1, 5, None) != 0
     assert "layout" in text()
     assert hip_lib.e3dgs_distill_forward(*head, PTR, PTR, PTR, PTR, 1, 5, PTR, None) != 0
     assert "layout" in text()
