@@ -497,15 +497,16 @@ constexpr int VALUE = 1, GRADIENT = 2;
 __host__ __device__ constexpr size_t tile_lds(size_t tile, size_t classes, size_t k, size_t bytes) {
     return (tile * classes * bytes + 15) / 16 * 16 + tile * k * 12;
 }
-template <typename T, int MODE>
-__global__ __launch_bounds__(256) void distill_tile_kernel(const DistillArgs a, int tile) {
+template <typename T, int MODE, int LANES>
+__global__ __launch_bounds__(256) void distill_tile_kernel(const DistillArgs a) {
+    constexpr int tile = 256 / LANES;
     extern __shared__ words_t tile_mem[];
     __shared__ float lds[16];
     T* rows = reinterpret_cast<T*>(tile_mem);
     float* ts = reinterpret_cast<float*>(tile_mem + ((size_t)tile * a.classes * sizeof(T) + 15) / 16);
     int* ids = reinterpret_cast<int*>(ts + tile * (int)a.k);
     float* ws = reinterpret_cast<float*>(ids + tile * (int)a.k);
-    const int K = (int)a.k, C = (int)a.classes, LANES = 256 / tile, r = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const int K = (int)a.k, C = (int)a.classes, r = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     const float rt = 1.0f / a.temperature, c = LOG2E * rt;
     float f_all = a.temperature;
     if (MODE == GRADIENT) f_all *= a.weight ? *a.weight : 1.0f;
@@ -552,10 +553,8 @@ __global__ __launch_bounds__(256) void distill_tile_kernel(const DistillArgs a, 
                 flags = fmaxf(flags, id[k] == ID_BROKEN ? 2.0f : 1.0f);
                 l.top = fmaxf(l.top, t[k]);
             }
-        for (int o = 1; o < LANES; o <<= 1) {
-            flags = fmaxf(flags, __shfl_xor(flags, o, 64));
-            l.top = fmaxf(l.top, __shfl_xor(l.top, o, 64));
-        }
+        flags = group_max<LANES>(flags);
+        l.top = group_max<LANES>(l.top);
         l.any = flags > 0.0f;
         l.broken = flags > 1.5f;
         if (live)
@@ -563,7 +562,7 @@ __global__ __launch_bounds__(256) void distill_tile_kernel(const DistillArgs a, 
                 w[k] = id[k] < 0 ? 0.0f : exp2_hw((t[k] - l.top) * c);
                 sum += w[k];
             }
-        for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor(sum, o, 64);
+        sum = group_sum<LANES>(sum);
         l.inv = 1.0f / sum;
         wave_sync();
         float m = -__builtin_inff(), s = 0.0f, inv = 0.0f;
@@ -581,6 +580,7 @@ __global__ __launch_bounds__(256) void distill_tile_kernel(const DistillArgs a, 
                     soft_add<1>(m, s, &v, c);
                 }
             }
+#pragma unroll
             for (int o = 1; o < LANES; o <<= 1) {
                 const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
                 soft_merge(m, s, m2, s2, c);
@@ -595,7 +595,7 @@ __global__ __launch_bounds__(256) void distill_tile_kernel(const DistillArgs a, 
                     else if (w[k] * l.inv != 0.0f) d += w[k] * l.inv * (((t[k] - l.top) - ((float)z[id[k]] - m)) * rt + more);
                 }
             }
-            for (int o = 1; o < LANES; o <<= 1) d += __shfl_xor(d, o, 64);
+            d = group_sum<LANES>(d);
             d *= a.temperature * a.temperature;
             if (live && lane == 0) {
                 if (!(MODE & GRADIENT)) a.stats[row] = l.any ? make_float2(m, inv) : make_float2(0.0f, 0.0f);
@@ -622,6 +622,7 @@ __global__ __launch_bounds__(256) void distill_tile_kernel(const DistillArgs a, 
                 }
             wave_sync();
             if (live)
+#pragma unroll 8
                 for (int col = lane; col < C; col += LANES) z[col] = l.any ? (T)(exp2_hw(((float)z[col] - m) * c) * fi) : (T)0.0f;
             wave_sync();
             if (live && l.any)      // (entries of the same class hold the same value)
@@ -1024,7 +1025,13 @@ int tile_rows(const DistillArgs& a, bool gradient) {
 template <typename T, int MODE>
 int distill_tile(const DistillArgs& a, int tile, unsigned& blocks, hipStream_t s) {
     blocks = distill_blocks(a.rows, tile);
-    distill_tile_kernel<T, MODE><<<dim3(blocks), dim3(256), tile_lds(tile, a.classes, a.k, sizeof(T)), s>>>(a, tile);
+    const size_t lds = tile_lds(tile, a.classes, a.k, sizeof(T));
+    if (tile == 256) distill_tile_kernel<T, MODE, 1><<<dim3(blocks), dim3(256), lds, s>>>(a);
+    else if (tile == 128) distill_tile_kernel<T, MODE, 2><<<dim3(blocks), dim3(256), lds, s>>>(a);
+    else if (tile == 64) distill_tile_kernel<T, MODE, 4><<<dim3(blocks), dim3(256), lds, s>>>(a);
+    else if (tile == 32) distill_tile_kernel<T, MODE, 8><<<dim3(blocks), dim3(256), lds, s>>>(a);
+    else if (tile == 16) distill_tile_kernel<T, MODE, 16><<<dim3(blocks), dim3(256), lds, s>>>(a);
+    else distill_tile_kernel<T, MODE, 32><<<dim3(blocks), dim3(256), lds, s>>>(a);
     LAUNCH_OK("distill_tile_kernel");
     return 0;
 }
