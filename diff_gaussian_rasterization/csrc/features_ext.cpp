@@ -186,71 +186,96 @@ Tensor layer_norm(const Tensor& x, const c10::optional<Tensor>& weight_, const c
 
 // ------------------------------------------------------------------------------------------------ distillation
 // The scores as (rows, classes) in one of the two layouts of the ABI, and the labels with whatever strides they have.
+struct Rows {                                     // a tensor as rows of `n` entries, the entry dimension anywhere
+    Tensor t;                                     // keeps the memory
+    size_t row_stride, entry_stride;
+};
 struct Scores {
-    Tensor logits, teacher, index;                // 2-D views (or copies)
-    std::vector<int64_t> shape;                   // of the logits with the classes last
+    Rows logits, teacher, index;
+    std::vector<int64_t> shape;                   // of the logits
     int64_t class_dim;
-    size_t rows, classes, k, row_stride, class_stride;
+    size_t rows, classes, k;
     bool planes;
 };
 
-Tensor as_2d(const Tensor& t) { return t.reshape({t.numel() / std::max<int64_t>(t.size(-1), 1), t.size(-1)}); }
+// Without a copy when the other dimensions run through memory in one stride; by a copy with the entries last otherwise.
+Rows rows_of(const Tensor& t, int64_t dim) {
+    const auto sizes = t.sizes(), strides = t.strides();
+    int64_t stride = 1, next = -1;                // of the rows; what the next outer dimension's stride has to be
+    bool one = true;
+    for (int64_t d = t.dim() - 1; d >= 0; --d) {
+        if (d == dim || sizes[d] == 1) continue;
+        if (next < 0) stride = strides[d];
+        else one = one && strides[d] == next;
+        next = strides[d] * sizes[d];
+    }
+    if (one) return {t, (size_t)stride, (size_t)(sizes[dim] == 1 ? 1 : strides[dim])};
+    const int64_t n = sizes[dim];
+    return {t.movedim(dim, -1).contiguous(), (size_t)n, 1};
+}
 
 Scores scores_of(const Tensor& logits, const Tensor& teacher, const Tensor& index, int64_t class_dim) {
     Scores s;
     s.class_dim = class_dim;
-    const Tensor z = logits.movedim(class_dim, -1);
-    s.shape = z.sizes().vec();
-    s.logits = as_2d(z);
-    s.teacher = as_2d(teacher.movedim(class_dim, -1));
-    s.index = as_2d(index.movedim(class_dim, -1));
-    s.rows = (size_t)s.logits.size(0);
-    s.classes = (size_t)s.logits.size(1);
-    s.k = (size_t)s.teacher.size(1);
-    s.planes = s.rows > 1 && s.classes > 1 && s.logits.stride(1) != 1 && s.logits.stride(0) == 1 && s.classes <= E3DGS_DISTILL_MAX_PLANES;
-    if (!s.planes && s.classes > 1 && s.logits.stride(1) != 1) s.logits = s.logits.contiguous();
-    s.row_stride = (size_t)s.logits.stride(0);
-    s.class_stride = s.planes ? (size_t)s.logits.stride(1) : 1;
+    s.shape = logits.sizes().vec();
+    s.classes = (size_t)logits.size(class_dim);
+    s.rows = (size_t)logits.numel() / s.classes;
+    s.k = (size_t)teacher.size(class_dim);
+    s.logits = rows_of(logits, class_dim);
+    s.teacher = rows_of(teacher, class_dim);
+    s.index = rows_of(index, class_dim);
+    s.planes = s.rows > 1 && s.logits.entry_stride != 1 && s.logits.row_stride == 1 && s.classes <= E3DGS_DISTILL_MAX_PLANES;
+    if (!s.planes && s.logits.entry_stride != 1) s.logits = {logits.movedim(class_dim, -1).contiguous(), s.classes, 1};
     return s;
 }
 
+// The gradient in the layout of the scores, and in their shape.
 Tensor empty_grad(const Scores& s) {
-    const int64_t rows = (int64_t)s.rows, classes = (int64_t)s.classes;
-    return s.planes ? torch::empty({classes, rows}, s.logits.options()).t() : torch::empty({rows, classes}, s.logits.options());
+    const auto opt = s.logits.t.options();
+    const int64_t last = (int64_t)s.shape.size() - 1;
+    if (s.class_dim == (s.planes ? 0 : last)) return torch::empty(s.shape, opt);
+    std::vector<int64_t> shape = s.shape;         // classes first (planes) or last in memory, back to their place in the shape
+    const int64_t to = s.planes ? 0 : last;
+    shape.erase(shape.begin() + s.class_dim);
+    shape.insert(shape.begin() + to, (int64_t)s.classes);
+    return torch::empty(shape, opt).movedim(to, s.class_dim);
 }
 size_t grad_row(const Scores& s) { return s.planes ? 1 : s.classes; }
 size_t grad_class(const Scores& s) { return s.planes ? s.rows : 1; }
-Tensor shaped(const Scores& s, const Tensor& grad) { return grad.view(s.shape).movedim(-1, s.class_dim); }
 
 // value (0-dim, or one per row) and what the backward call needs; fills `grad` (of empty_grad) if it is defined
 std::tuple<Tensor, Tensor> distill_forward(const Scores& s, double temperature, int64_t reduction, const Tensor& grad) {
-    const auto opt = s.logits.options().dtype(torch::kFloat32);
+    const auto opt = s.logits.t.options().dtype(torch::kFloat32);
     const size_t n_stats = (2 * s.rows + 1 + 1) / 2 * 2;                      // (the scratch behind it is 8-byte aligned)
     Tensor stats = torch::empty({(int64_t)(n_stats + (e3dgs_distill_scratch_bytes(s.rows) + 3) / 4)}, opt);
     Tensor loss = torch::empty({}, opt);
-    Tensor row_loss = reduction == 0 ? torch::empty({(int64_t)s.rows}, opt) : Tensor();
-    check(e3dgs_distill_forward(s.rows, s.classes, s.k, s.logits.data_ptr(), s.row_stride, s.class_stride,
-                                dtype_of(s.logits, "logits"), s.teacher.data_ptr(), (size_t)s.teacher.stride(0),
-                                (size_t)s.teacher.stride(1), dtype_of(s.teacher, "teacher_logits"), s.index.data_ptr(),
-                                (size_t)s.index.stride(0), (size_t)s.index.stride(1), index_bytes_of(s.index),
+    Tensor row_loss;
+    if (reduction == 0) {
+        std::vector<int64_t> shape = s.shape;
+        shape.erase(shape.begin() + s.class_dim);
+        row_loss = torch::empty(shape, opt);
+    }
+    check(e3dgs_distill_forward(s.rows, s.classes, s.k, s.logits.t.data_ptr(), s.logits.row_stride, s.logits.entry_stride,
+                                dtype_of(s.logits.t, "logits"), s.teacher.t.data_ptr(), s.teacher.row_stride,
+                                s.teacher.entry_stride, dtype_of(s.teacher.t, "teacher_logits"), s.index.t.data_ptr(),
+                                s.index.row_stride, s.index.entry_stride, index_bytes_of(s.index.t),
                                 (float)temperature, (int)reduction, stats.data_ptr<float>(),
                                 row_loss.defined() ? row_loss.data_ptr<float>() : nullptr, loss.data_ptr<float>(),
                                 grad.defined() ? grad.data_ptr() : nullptr, grad_row(s), grad_class(s),
                                 reinterpret_cast<char*>(stats.data_ptr<float>() + n_stats), stream()),
           "e3dgs_distill_forward");
-    if (reduction == 0) return std::make_tuple(row_loss.view(std::vector<int64_t>(s.shape.begin(), s.shape.end() - 1)), stats);
-    return std::make_tuple(loss, stats);
+    return std::make_tuple(reduction == 0 ? row_loss : loss, stats);
 }
 
 Tensor distill_backward(const Scores& s, double temperature, int64_t reduction, const Tensor& stats, const Tensor& d_loss) {
     Tensor grad = empty_grad(s);
-    check(e3dgs_distill_backward(s.rows, s.classes, s.k, s.logits.data_ptr(), s.row_stride, s.class_stride,
-                                 dtype_of(s.logits, "logits"), s.teacher.data_ptr(), (size_t)s.teacher.stride(0),
-                                 (size_t)s.teacher.stride(1), dtype_of(s.teacher, "teacher_logits"), s.index.data_ptr(),
-                                 (size_t)s.index.stride(0), (size_t)s.index.stride(1), index_bytes_of(s.index),
+    check(e3dgs_distill_backward(s.rows, s.classes, s.k, s.logits.t.data_ptr(), s.logits.row_stride, s.logits.entry_stride,
+                                 dtype_of(s.logits.t, "logits"), s.teacher.t.data_ptr(), s.teacher.row_stride,
+                                 s.teacher.entry_stride, dtype_of(s.teacher.t, "teacher_logits"), s.index.t.data_ptr(),
+                                 s.index.row_stride, s.index.entry_stride, index_bytes_of(s.index.t),
                                  (float)temperature, (int)reduction, stats.data_ptr<float>(), d_loss.data_ptr<float>(), grad.data_ptr(), grad_row(s), grad_class(s), stream()),
           "e3dgs_distill_backward");
-    return shaped(s, grad);
+    return grad;
 }
 
 struct DistillFunction : public torch::autograd::Function<DistillFunction> {
@@ -315,7 +340,7 @@ std::tuple<Tensor, Tensor> distill_raw(const Tensor& logits_, const Tensor& teac
     const Scores s = scores_of(logits, teacher, index, class_dim);
     const Tensor grad = empty_grad(s);
     auto r = distill_forward(s, temperature, reduction, grad);
-    return std::make_tuple(std::get<0>(r), shaped(s, grad));
+    return std::make_tuple(std::get<0>(r), grad);
 }
 
 }  // namespace
