@@ -48,12 +48,32 @@ void once(const char* who) {
 char* bytes(const Tensor& t) { return reinterpret_cast<char*>(t.data_ptr()); }
 Tensor scratch_of(size_t n, const Tensor& like) { return torch::empty({(int64_t)n}, like.options().dtype(torch::kByte)); }
 
-// (rows, dim) view of a tensor with unit stride along the last dimension; copied only when there is no such view
-Tensor as_rows(const Tensor& t) {
-    const int64_t dim = t.size(-1);
-    if (t.numel() == 0) return t.reshape({t.numel() / std::max<int64_t>(dim, 1), dim});
-    Tensor r = t.reshape({-1, dim});
-    return r.stride(1) == 1 || dim == 1 ? r : r.contiguous();
+struct Rows {                                     // a tensor as rows of `n` entries, the entry dimension anywhere
+    Tensor t;                                     // keeps the memory
+    size_t row_stride, entry_stride;
+};
+// Without a copy when the other dimensions run through memory in one stride; by a copy with the entries last otherwise.
+// (No tensor views: each would cost a small call a microsecond.)
+Rows rows_of(const Tensor& t, int64_t dim) {
+    const auto sizes = t.sizes(), strides = t.strides();
+    int64_t stride = 1, next = -1;                // of the rows; what the next outer dimension's stride has to be
+    bool one = true;
+    for (int64_t d = t.dim() - 1; d >= 0; --d) {
+        if (d == dim || sizes[d] == 1) continue;
+        if (next < 0) stride = strides[d];
+        else one = one && strides[d] == next;
+        next = strides[d] * sizes[d];
+    }
+    if (one) return {t, (size_t)stride, (size_t)(sizes[dim] == 1 ? 1 : strides[dim])};
+    const int64_t n = sizes[dim];
+    return {t.movedim(dim, -1).contiguous(), (size_t)n, 1};
+}
+
+// ... with the values of a row next to each other
+Rows rows_of(const Tensor& t) {
+    Rows r = rows_of(t, t.dim() - 1);
+    if (r.entry_stride != 1) r = {t.contiguous(), (size_t)t.size(-1), 1};
+    return r;
 }
 
 // ------------------------------------------------------------------------------------------------ embedding
@@ -62,9 +82,10 @@ Tensor embedding_forward(const Tensor& index, const Tensor& table, double scale)
     std::vector<int64_t> shape = index.sizes().vec();
     shape.push_back(table.size(1));
     Tensor out = torch::empty(shape, table.options());
-    const Tensor idx = index.contiguous(), tab = as_rows(table);
+    const Tensor idx = index.contiguous();
+    const Rows tab = rows_of(table);
     check(e3dgs_embedding_forward((size_t)idx.numel(), (size_t)table.size(0), (size_t)table.size(1), idx.data_ptr(),
-                                  index_bytes_of(idx), tab.data_ptr(), (size_t)tab.stride(0), dtype_of(table, "table"),
+                                  index_bytes_of(idx), tab.t.data_ptr(), tab.row_stride, dtype_of(table, "table"),
                                   (float)scale, out.data_ptr(), stream()),
           "e3dgs_embedding_forward");
     return out;
@@ -83,12 +104,13 @@ struct EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
         const Guard guard(grads[0].device());
         const int64_t rows = ctx->saved_data["rows"].toInt();
-        const Tensor index = saved[0].contiguous(), g = as_rows(grads[0]);
-        const int64_t dim = g.size(1), n = index.numel();
-        Tensor d = torch::empty({rows, dim}, g.options());
-        Tensor scratch = scratch_of(e3dgs_embedding_backward_scratch_bytes((size_t)n, (size_t)rows, (size_t)dim), g);
+        const Tensor index = saved[0].contiguous();
+        const Rows g = rows_of(grads[0]);
+        const int64_t dim = g.t.size(-1), n = index.numel();
+        Tensor d = torch::empty({rows, dim}, g.t.options());
+        Tensor scratch = scratch_of(e3dgs_embedding_backward_scratch_bytes((size_t)n, (size_t)rows, (size_t)dim), g.t);
         check(e3dgs_embedding_backward((size_t)n, (size_t)rows, (size_t)dim, index.data_ptr(), index_bytes_of(index),
-                                       g.data_ptr(), (size_t)g.stride(0), dtype_of(g, "grad"),
+                                       g.t.data_ptr(), g.row_stride, dtype_of(g.t, "grad"),
                                        (float)ctx->saved_data["scale"].toDouble(), d.data_ptr(), bytes(scratch), stream()),
               "e3dgs_embedding_backward");
         return {Tensor(), d, Tensor()};
@@ -111,13 +133,13 @@ Tensor embedding(const Tensor& index, const Tensor& table, double scale) {
 // ------------------------------------------------------------------------------------------------ layer norm
 std::tuple<Tensor, Tensor> layer_norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, bool stats) {
     const Guard guard(x.device());
-    const Tensor r = as_rows(x);
-    const int64_t rows = r.size(0), dim = r.size(1);
+    const Rows r = rows_of(x);
+    const int64_t dim = x.size(-1), rows = x.numel() / dim;
     Tensor out = torch::empty(x.sizes(), x.options());
     Tensor st = stats ? torch::empty({2, rows}, x.options().dtype(torch::kFloat32)) : Tensor();
     const Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
     const int affine = w.defined() ? dtype_of(w, "weight") : b.defined() ? dtype_of(b, "bias") : E3DGS_F32;
-    check(e3dgs_layer_norm_forward((size_t)rows, (size_t)dim, r.data_ptr(), (size_t)r.stride(0), dtype_of(x, "x"),
+    check(e3dgs_layer_norm_forward((size_t)rows, (size_t)dim, r.t.data_ptr(), r.row_stride, dtype_of(x, "x"),
                                    w.defined() ? w.data_ptr() : nullptr, b.defined() ? b.data_ptr() : nullptr, affine,
                                    (float)eps, out.data_ptr(), stats ? st.data_ptr<float>() : nullptr,
                                    stats ? st.data_ptr<float>() + rows : nullptr, stream()),
@@ -143,8 +165,8 @@ struct LayerNormFunction : public torch::autograd::Function<LayerNormFunction> {
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
         const Tensor &x = saved[0], &weight = saved[1], &st = saved[2];
         const Guard guard(x.device());
-        const Tensor r = as_rows(x), g = as_rows(grads[0]);
-        const int64_t rows = r.size(0), dim = r.size(1);
+        const Rows r = rows_of(x), g = rows_of(grads[0]);
+        const int64_t dim = x.size(-1), rows = x.numel() / dim;
         const Tensor w = weight.defined() ? weight.contiguous() : weight;
         const auto affine = x.options().dtype((c10::ScalarType)ctx->saved_data["affine"].toInt());
         Tensor dx = ctx->saved_data["x_grad"].toBool() ? torch::empty(x.sizes(), x.options()) : Tensor();
@@ -153,8 +175,8 @@ struct LayerNormFunction : public torch::autograd::Function<LayerNormFunction> {
         Tensor scratch;
         if (dw.defined() || db.defined()) scratch = scratch_of(e3dgs_layer_norm_backward_scratch_bytes((size_t)rows, (size_t)dim), x);
         const auto kind = affine.dtype().toScalarType();
-        check(e3dgs_layer_norm_backward((size_t)rows, (size_t)dim, g.data_ptr(), (size_t)g.stride(0), r.data_ptr(),
-                                        (size_t)r.stride(0), dtype_of(x, "x"), w.defined() ? w.data_ptr() : nullptr,
+        check(e3dgs_layer_norm_backward((size_t)rows, (size_t)dim, g.t.data_ptr(), g.row_stride, r.t.data_ptr(), r.row_stride,
+                                        dtype_of(x, "x"), w.defined() ? w.data_ptr() : nullptr,
                                         kind == torch::kFloat32 ? E3DGS_F32 : kind == torch::kFloat16 ? E3DGS_F16 : E3DGS_BF16,
                                         st.data_ptr<float>(), st.data_ptr<float>() + rows, dx.defined() ? dx.data_ptr() : nullptr,
                                         dw.defined() ? dw.data_ptr() : nullptr, db.defined() ? db.data_ptr() : nullptr,
@@ -186,10 +208,6 @@ Tensor layer_norm(const Tensor& x, const c10::optional<Tensor>& weight_, const c
 
 // ------------------------------------------------------------------------------------------------ distillation
 // The scores as (rows, classes) in one of the two layouts of the ABI, and the labels with whatever strides they have.
-struct Rows {                                     // a tensor as rows of `n` entries, the entry dimension anywhere
-    Tensor t;                                     // keeps the memory
-    size_t row_stride, entry_stride;
-};
 struct Scores {
     Rows logits, teacher, index;
     std::vector<int64_t> shape;                   // of the logits
@@ -197,22 +215,6 @@ struct Scores {
     size_t rows, classes, k;
     bool planes;
 };
-
-// Without a copy when the other dimensions run through memory in one stride; by a copy with the entries last otherwise.
-Rows rows_of(const Tensor& t, int64_t dim) {
-    const auto sizes = t.sizes(), strides = t.strides();
-    int64_t stride = 1, next = -1;                // of the rows; what the next outer dimension's stride has to be
-    bool one = true;
-    for (int64_t d = t.dim() - 1; d >= 0; --d) {
-        if (d == dim || sizes[d] == 1) continue;
-        if (next < 0) stride = strides[d];
-        else one = one && strides[d] == next;
-        next = strides[d] * sizes[d];
-    }
-    if (one) return {t, (size_t)stride, (size_t)(sizes[dim] == 1 ? 1 : strides[dim])};
-    const int64_t n = sizes[dim];
-    return {t.movedim(dim, -1).contiguous(), (size_t)n, 1};
-}
 
 Scores scores_of(const Tensor& logits, const Tensor& teacher, const Tensor& index, int64_t class_dim) {
     Scores s;

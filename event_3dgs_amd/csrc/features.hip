@@ -146,15 +146,56 @@ __device__ __forceinline__ void embed_zero(uint32_t n, const uint32_t* __restric
     }
 }
 
+// Up to EMBED_TINY positions: every workgroup of the sums sorts them for itself (the rank of a position is the number of smaller
+// indices, and of equal ones before it, counted in LDS), which is quicker than a launch that does it for all.  Indices outside
+// the table are left out.  Returns their number; keys and positions are in LDS.
+constexpr uint32_t EMBED_TINY = 256;
+struct TinySort {
+    uint32_t raw[EMBED_TINY], key[EMBED_TINY], pos[EMBED_TINY], kept;
+};
+__device__ __forceinline__ uint32_t embed_sort_tiny(TinySort& L, uint32_t n, uint32_t rows, const void* __restrict__ index,
+                                                    int index_bytes) {
+    const uint32_t i = threadIdx.x;
+    const unsigned long long id = i < n ? (unsigned long long)load_index_flat(index, i, index_bytes) : ~0ull;
+    const uint32_t k = id < rows ? (uint32_t)id : EMBED_NONE;
+    L.raw[i] = k;
+    if (i == 0) L.kept = 0;
+    __syncthreads();
+    const unsigned long long ok = __ballot(k != EMBED_NONE);
+    if ((i & 63) == 0) atomicAdd(&L.kept, (uint32_t)__popcll(ok));
+    uint32_t rank = 0;
+    for (uint32_t j = 0; j < n; j += 4) {
+        const uint4 q = *reinterpret_cast<const uint4*>(L.raw + j);      // (behind the last one: EMBED_NONE, not smaller)
+        rank += (q.x < k || (q.x == k && j < i)) + (q.y < k || (q.y == k && j + 1 < i)) + (q.z < k || (q.z == k && j + 2 < i)) +
+                (q.w < k || (q.w == k && j + 3 < i));
+    }
+    if (k != EMBED_NONE) {
+        L.key[rank] = k;
+        L.pos[rank] = i;
+    }
+    __syncthreads();
+    return L.kept;
+}
+
 constexpr int EMBED_UNROLL = 8;
-template <typename T, int V, int G>
-__global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restrict__ kept, const uint32_t* __restrict__ keys,
-                                                        const uint32_t* __restrict__ pos, uint32_t chunk, uint32_t nchunks,
+template <bool TINY, typename T, int V, int G>
+__global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restrict__ kept, const uint32_t* keys,
+                                                        const uint32_t* pos, uint32_t chunk, uint32_t nchunks,
                                                         uint32_t nslices, size_t dim, const T* __restrict__ d_out,
                                                         size_t stride, float scale, T* __restrict__ d_table,
                                                         float* __restrict__ part, uint32_t sum_blocks, uint32_t rows,
-                                                        uint32_t zero_rows) {
-    const uint32_t n = *kept;
+                                                        uint32_t zero_rows, uint32_t tiny_n, const void* __restrict__ index,
+                                                        int index_bytes) {
+    __shared__ __attribute__((aligned(16))) char tiny_mem[TINY ? sizeof(TinySort) : 4];
+    uint32_t n;
+    if (TINY) {
+        TinySort& L = *reinterpret_cast<TinySort*>(tiny_mem);
+        n = embed_sort_tiny(L, tiny_n, rows, index, index_bytes);
+        keys = L.key;
+        pos = L.pos;
+    } else {
+        n = *kept;
+    }
     if (blockIdx.x >= sum_blocks) {      // (in the same launch: the sums wait for their gathers, the stores do not)
         const size_t wave = (size_t)(blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6);
         if (V > 1 && (size_t)rows * dim * sizeof(T) > E3_STREAM_BYTES) embed_zero<true, T, V>(n, keys, rows, zero_rows, dim, d_table, wave);
@@ -413,6 +454,7 @@ struct EmbedScratch {
     static uint32_t chunk(size_t n, size_t dim) {
         // Rows of a chunk: 128 where there is plenty of work, fewer where the groups would otherwise not fill the chip (each
         // group moves `chunk` row slices of at most 1 KB).
+        if (n <= EMBED_TINY) return EMBED_TINY;                // (one chunk: nothing to join)
         uint32_t c = 128;
         while (c > 8 && (n / c) * ((dim + 511) / 512) < 4096) c >>= 1;
         return c;
@@ -434,7 +476,8 @@ struct EmbedScratch {
 
 template <typename T, int V, int G>
 int embed_sum_launch(const EmbedScratch& w, const uint32_t* keys, const uint32_t* pos, size_t n, size_t rows, size_t dim,
-                     const void* d_out, size_t stride, float scale, void* d_table, hipStream_t s) {
+                     const void* d_out, size_t stride, float scale, void* d_table, const void* index, int index_bytes,
+                     hipStream_t s) {
     const uint32_t chunk = EmbedScratch::chunk(n, dim), nchunks = EmbedScratch::chunks(n, dim);
     const size_t nslices = (dim + (size_t)G * V - 1) / ((size_t)G * V), units = nslices * nchunks;
     const size_t blocks = (units + 256 / G - 1) / (256 / G);
@@ -442,9 +485,13 @@ int embed_sum_launch(const EmbedScratch& w, const uint32_t* keys, const uint32_t
     per = per < 1 ? 1 : (per > 64 ? 64 : per);
     const size_t zero_blocks = (rows + 4 * per - 1) / (4 * per);
     if (blocks + zero_blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
-    embed_sum_kernel<T, V, G><<<dim3((unsigned)(blocks + zero_blocks)), dim3(256), 0, s>>>(
-        w.kept, keys, pos, chunk, nchunks, (uint32_t)nslices, dim, (const T*)d_out, stride, scale, (T*)d_table, w.part,
-        (uint32_t)blocks, (uint32_t)rows, (uint32_t)per);
+#define E3_SUM_LAUNCH(TINY)                                                                                                   \
+    embed_sum_kernel<TINY, T, V, G><<<dim3((unsigned)(blocks + zero_blocks)), dim3(256), 0, s>>>(                             \
+        w.kept, keys, pos, chunk, nchunks, (uint32_t)nslices, dim, (const T*)d_out, stride, scale, (T*)d_table, w.part,       \
+        (uint32_t)blocks, (uint32_t)rows, (uint32_t)per, (uint32_t)n, index, index_bytes)
+    if (n <= EMBED_TINY) E3_SUM_LAUNCH(true);
+    else E3_SUM_LAUNCH(false);
+#undef E3_SUM_LAUNCH
     LAUNCH_OK("embed_sum_kernel");
     return 0;
 }
@@ -477,7 +524,8 @@ int embed_bwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_
     EmbedScratch w = EmbedScratch::from(scratch, n, dim);
     uint32_t *keys = w.key0, *pos = w.pos0;
     int rc = 0;
-    if (n <= 16384) {
+    if (n <= EMBED_TINY) {                                      // (sorted by the workgroups of the sums)
+    } else if (n <= 16384) {
         int nbits = 1;
         while (rows >> nbits) ++nbits;                         // (the key `rows` itself occurs)
         if (index_bytes == 8) embed_sort_small((uint32_t)n, (uint32_t)rows, nbits, (const long long*)index, keys, pos, w.kept, s);
@@ -495,7 +543,7 @@ int embed_bwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_
     const bool wide = e3_rows_wide(d_out, stride, dim, dtype) && e3_rows_wide(d_table, dim, dim, dtype);
     const size_t packs = wide ? dim / Wide<T>::N : dim;
     constexpr int N = Wide<T>::N;
-#define E3_SUM(V, G) rc = embed_sum_launch<T, V, G>(w, keys, pos, n, rows, dim, d_out, stride, scale, d_table, s)
+#define E3_SUM(V, G) rc = embed_sum_launch<T, V, G>(w, keys, pos, n, rows, dim, d_out, stride, scale, d_table, index, index_bytes, s)
     if (wide) {
         if (packs <= 4) E3_SUM(N, 4);
         else if (packs <= 8) E3_SUM(N, 8);
@@ -680,6 +728,25 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_fwd_kernel(size_t ro
     }
 }
 
+// Where the column sums go: one fp32 row pair per workgroup (norm_join_kernel adds them up), or straight to the results when
+// there is only one workgroup.
+struct NormSums {
+    float* part;             // NULL: no column sums are wanted
+    void *dweight, *dbias;
+    int dtype;
+    __device__ __forceinline__ void put(int dim, int which, int col, float v) const {
+        if (gridDim.x > 1) {
+            part[((size_t)blockIdx.x * 2 + which) * dim + col] = v;
+            return;
+        }
+        void* out = which ? dbias : dweight;
+        if (!out) return;
+        if (dtype == E3_F32) reinterpret_cast<float*>(out)[col] = v;
+        else if (dtype == E3_F16) reinterpret_cast<f16_t*>(out)[col] = (f16_t)v;
+        else reinterpret_cast<bf16_t*>(out)[col] = (bf16_t)v;
+    }
+};
+
 // Short rows whose length is no multiple of 16 bytes (or a few packs only), one behind the other: a workgroup moves `tile` rows
 // at a time through LDS, in whole packs whatever the row length.  256 / tile lanes share a row there; each takes
 // NORM_TILE_ITEMS of its values into registers, in one batch of LDS reads.  (200000 rows of 59 fp16 values: a lane per
@@ -786,7 +853,7 @@ __global__ __launch_bounds__(256) void norm_bwd_tile_kernel(size_t rows, int dim
                                                             const T* __restrict__ x, const void* __restrict__ weight,
                                                             int affine_dtype, const float* __restrict__ mean_in,
                                                             const float* __restrict__ rstd_in, T* __restrict__ dx,
-                                                            float* __restrict__ part) {
+                                                            const NormSums out_sums) {
     extern __shared__ words_t tile_mem[];
     const int LANES = 256 / tile, r = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     const int tile_packs = (int)((tile * dim * (int)sizeof(T) + 15) / 16);
@@ -850,10 +917,9 @@ __global__ __launch_bounds__(256) void norm_bwd_tile_kernel(size_t rows, int dim
         }
         __syncthreads();
     }
-    if (!part) return;
+    if (!out_sums.part) return;
     // the sums of the lanes that hold the same columns, in order: first within a wave, then over the waves through LDS
     __shared__ float sums[2][4][32 * ITEMS];
-    float* mine = part + (size_t)blockIdx.x * 2 * dim;
     const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
@@ -869,8 +935,8 @@ __global__ __launch_bounds__(256) void norm_bwd_tile_kernel(size_t rows, int dim
     }
     __syncthreads();
     for (int c = threadIdx.x; c < dim; c += 256) {
-        mine[c] = ((sums[0][0][c] + sums[0][1][c]) + sums[0][2][c]) + sums[0][3][c];
-        mine[dim + c] = ((sums[1][0][c] + sums[1][1][c]) + sums[1][2][c]) + sums[1][3][c];
+        out_sums.put(dim, 0, c, ((sums[0][0][c] + sums[0][1][c]) + sums[0][2][c]) + sums[0][3][c]);
+        out_sums.put(dim, 1, c, ((sums[1][0][c] + sums[1][1][c]) + sums[1][2][c]) + sums[1][3][c]);
     }
 }
 
@@ -925,7 +991,7 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_bwd_kernel(size_t ro
                                                                        size_t stride, const void* __restrict__ weight,
                                                                        int affine_dtype, const float* __restrict__ mean_in,
                                                                        const float* __restrict__ rstd_in,
-                                                                       T* __restrict__ dx, float* __restrict__ part) {
+                                                                       T* __restrict__ dx, const NormSums sums) {
     using R = NormRow<G>;
     __shared__ float lds[16];
     __shared__ float cols[R::PER_BLOCK > 1 ? R::THREADS * ITEMS * V : 1];
@@ -982,8 +1048,7 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_bwd_kernel(size_t ro
             put<STREAM, T, V>(dx + row * (size_t)dim + col, r);
         }
     }
-    if (!part) return;
-    float* mine = part + (size_t)blockIdx.x * 2 * dim;
+    if (!sums.part) return;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         float(&a)[ITEMS][V] = which ? db : dw;
@@ -997,7 +1062,7 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_bwd_kernel(size_t ro
             for (int col = threadIdx.x; col < dim; col += R::THREADS) {
                 float s = cols[col];
                 for (int k = 1; k < R::PER_BLOCK; ++k) s += cols[k * (G * ITEMS * V) + col];
-                mine[which * (size_t)dim + col] = s;
+                sums.put(dim, which, col, s);
             }
         } else {
 #pragma unroll
@@ -1005,7 +1070,7 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_bwd_kernel(size_t ro
                 const int col = (i * G + lane) * V;
 #pragma unroll
                 for (int j = 0; j < V; ++j)
-                    if (col < dim) mine[which * (size_t)dim + col + j] = a[i][j];
+                    if (col < dim) sums.put(dim, which, col + j, a[i][j]);
             }
         }
     }
@@ -1102,6 +1167,12 @@ unsigned norm_blocks(size_t rows, int per_block, size_t most) {
     const size_t need = (rows + per_block - 1) / per_block;
     return (unsigned)(need < most ? need : most);
 }
+// ... of the gradient: what one workgroup does in four rounds goes to one, which saves the launch that would join the sums (10
+// rows of 64 values with autograd around it: 66 us of host time with the second launch, 61 us without; a round takes about
+// 1.5 us, the launch 2.5 us on the GPU and 4 us on the host)
+unsigned norm_bwd_blocks(size_t rows, int per_block, size_t most) {
+    return rows <= 4 * (size_t)per_block ? 1u : norm_blocks(rows, per_block, most);
+}
 constexpr size_t NORM_FWD_BLOCKS = 4096, NORM_BWD_BLOCKS = 1024, NORM_TILE_BLOCKS = 1024, NORM_LONG_PARTS = 64;
 
 struct NormArgs {
@@ -1113,6 +1184,8 @@ struct NormArgs {
     float *mean, *rstd, *part;
     hipStream_t s;
 };
+
+NormSums norm_sums(const NormArgs& a) { return {a.part, a.dweight, a.dbias, a.affine_dtype}; }
 
 template <typename T, int V, int G, int ITEMS>
 int norm_fwd_launch(const NormArgs& a) {
@@ -1128,12 +1201,12 @@ int norm_fwd_launch(const NormArgs& a) {
 }
 template <typename T, int V, int G, int ITEMS>
 int norm_bwd_launch(const NormArgs& a, uint32_t& nparts) {
-    nparts = norm_blocks(a.rows, NormRow<G>::PER_BLOCK, NORM_BWD_BLOCKS);
+    nparts = norm_bwd_blocks(a.rows, NormRow<G>::PER_BLOCK, NORM_BWD_BLOCKS);
     const dim3 blocks(nparts), threads(NormRow<G>::THREADS);
 #define E3_NORM(S)                                                                                                            \
     norm_bwd_kernel<(S), T, V, G, ITEMS><<<blocks, threads, 0, a.s>>>(a.rows, (int)a.dim, (const T*)a.dy, a.dy_stride,          \
                                                                   (const T*)a.x, a.x_stride, a.weight, a.affine_dtype,       \
-                                                                  a.mean, a.rstd, (T*)a.dx, a.part)
+                                                                  a.mean, a.rstd, (T*)a.dx, norm_sums(a))
     if (V > 1 && a.rows * a.dim * sizeof(T) > E3_STREAM_BYTES) E3_NORM(V > 1);
     else E3_NORM(false);
 #undef E3_NORM
@@ -1172,11 +1245,11 @@ int norm_fwd_tile(const NormArgs& a, int tile) {
 template <typename T>
 int norm_bwd_tile(const NormArgs& a, int tile, uint32_t& nparts) {
     const size_t lds = 2 * ((tile * a.dim * sizeof(T) + 15) / 16 * 16);
-    nparts = norm_blocks(a.rows, tile, NORM_TILE_BLOCKS);
+    nparts = norm_bwd_blocks(a.rows, tile, NORM_TILE_BLOCKS);
 #define E3_TILE_BWD(ITEMS)                                                                                                    \
     norm_bwd_tile_kernel<T, ITEMS><<<dim3(nparts), dim3(256), lds, a.s>>>(a.rows, (int)a.dim, tile, (const T*)a.dy,           \
                                                                         (const T*)a.x, a.weight, a.affine_dtype, a.mean,     \
-                                                                        a.rstd, (T*)a.dx, a.part)
+                                                                        a.rstd, (T*)a.dx, norm_sums(a))
     if (norm_tile_items(a.dim, true) == 8) E3_TILE_BWD(8);
     else E3_TILE_BWD(NORM_TILE_ITEMS);
 #undef E3_TILE_BWD
@@ -1206,6 +1279,7 @@ int norm_bwd_v(const NormArgs& a) {
     const size_t packs = a.dim / V;
     uint32_t nparts = 0;
     int rc = 0;
+    bool long_rows = false;
     if (const int tile = norm_tile_rows(a, sizeof(T), true)) rc = norm_bwd_tile<T>(a, tile, nparts);
     else if (packs <= 8) rc = norm_bwd_launch<T, V, 8, 1>(a, nparts);
     else if (packs <= 16) rc = norm_bwd_launch<T, V, 16, 1>(a, nparts);
@@ -1216,6 +1290,7 @@ int norm_bwd_v(const NormArgs& a) {
     else if (packs <= 512) rc = norm_bwd_launch<T, V, 256, 2>(a, nparts);
     else if (packs <= 1024) rc = norm_bwd_launch<T, V, 256, 4>(a, nparts);
     else {
+        long_rows = true;
         if (a.dx) {
             const unsigned blocks = (unsigned)(a.rows < 2048 ? a.rows : 2048);
             norm_bwd_long_kernel<T, V><<<dim3(blocks), dim3(1024), 0, a.s>>>(a.rows, a.dim, (const T*)a.dy, a.dy_stride,
@@ -1230,7 +1305,7 @@ int norm_bwd_v(const NormArgs& a) {
             LAUNCH_OK("norm_cols_kernel");
         }
     }
-    if (rc || !a.part) return rc;
+    if (rc || !a.part || (nparts == 1 && !long_rows)) return rc;
     norm_join_kernel<<<dim3((unsigned)((2 * a.dim + 63) / 64)), dim3(1024), 0, a.s>>>(nparts, a.dim, a.part, a.affine_dtype,
                                                                                     a.dweight, a.dbias);
     LAUNCH_OK("norm_join_kernel");

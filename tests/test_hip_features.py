@@ -617,3 +617,49 @@ def test_inputs_changed_in_between_are_noticed():
     t += 1
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         value.backward()
+
+
+@pytest.mark.parametrize("n, rows, dim", [(255, 40, 48), (256, 40, 48), (257, 40, 48), (256, 3, 1000), (1024, 9, 20), (1025, 9, 20),
+                                          (4096, 300, 16), (4097, 300, 16), (8192, 20, 12), (8193, 20, 12), (16384, 4000, 8),
+                                          (16385, 4000, 8), (300000, 70000, 4)])
+def test_embedding_sort_sizes(n, rows, dim):
+    """Position counts around which another sort takes over, int32 and int64 indices, masked ends."""
+    index = tokens(n, rows, skew=2.0, empty=0.2)
+    index[-1] = -1
+    a = check_embedding(index, rand(rows, dim), 1.0, rand(n, dim, seed=1))
+    assert torch.equal(a, check_embedding(index.int(), rand(rows, dim), 1.0, rand(n, dim, seed=1)))
+    first = torch.full((n,), rows, device=DEV)                   # all outside the table but one
+    first[n // 2] = rows - 1
+    check_embedding(first, rand(rows, dim), 1.0, rand(n, dim, seed=2))
+
+
+@pytest.mark.parametrize("n", [1, 3, 4, 5, 16, 17, 64, 65, 128, 129, 1024, 1025, 1300])
+@pytest.mark.parametrize("dim", [1, 7, 16, 64, 100, 300])
+def test_layer_norm_few_rows(n, dim):
+    """Row counts around which the column sums go from one workgroup to several."""
+    check_layer_norm(rand(n, dim) + 0.3, rand(dim), rand(dim, seed=1), rand(n, dim, seed=2))
+
+
+def test_large_results_are_streamed():
+    """Results past 128 MiB are stored past the cache: the same values."""
+    n, dim = 900000, 48
+    index, table = tokens(n, 500), rand(500, dim)
+    leaf = table.clone().requires_grad_(True)
+    out = features.embedding(index, leaf, 3.0)
+    assert torch.equal(out, table[index] * 3.0)
+    out = out.detach().requires_grad_(True)
+    y = features.layer_norm(out)
+    part = features.layer_norm(out.detach()[-5000:])
+    assert torch.equal(y[-5000:], part)
+    d = rand(n, dim)
+    (dx,) = torch.autograd.grad(y, out, d)
+    small = out.detach()[-5000:].requires_grad_(True)
+    (want,) = torch.autograd.grad(features.layer_norm(small), small, d[-5000:])
+    assert torch.equal(dx[-5000:], want)
+    big = rand(700000, 64).requires_grad_(True)                  # a gradient table of 179 MB, most of it empty
+    (g,) = torch.autograd.grad(features.embedding(index[:5000], big), big, rand(5000, 64))
+    keep = torch.zeros(500, 64, dtype=torch.float64, device=DEV).index_add_(0, index[:5000], rand(5000, 64).double())
+    count = torch.bincount(index[:5000], minlength=500).double().unsqueeze(1)
+    mag = torch.zeros(500, 64, dtype=torch.float64, device=DEV).index_add_(0, index[:5000], rand(5000, 64).double().abs())
+    close(g[:500], keep, half_step(keep, torch.float32) * 1.01 + (count + 2) * U * mag)
+    assert g[500:].count_nonzero() == 0
