@@ -56,7 +56,7 @@ struct Rows {                                     // a tensor as rows of `n` ent
 // (No tensor views: each would cost a small call a microsecond.)
 Rows rows_of(const Tensor& t, int64_t dim) {
     const auto sizes = t.sizes(), strides = t.strides();
-    int64_t stride = 1, next = -1;                // of the rows; what the next outer dimension's stride has to be
+    int64_t stride = sizes[dim], next = -1;       // of the rows (any for a single one); what the next outer dimension's has to be
     bool one = true;
     for (int64_t d = t.dim() - 1; d >= 0; --d) {
         if (d == dim || sizes[d] == 1) continue;
@@ -123,7 +123,7 @@ Tensor embedding(const Tensor& index, const Tensor& table, double scale) {
     TORCH_CHECK(table.dim() == 2 && table.size(1) >= 1, "table must have dimensions (rows, dim)");
     TORCH_CHECK(table.size(1) <= E3DGS_FEATURE_MAX_DIM, "at most ", E3DGS_FEATURE_MAX_DIM, " values to a row");
     TORCH_CHECK(index.numel() < 0x7FFFFFFF && table.size(0) < 0x7FFFFFFF, "embedding takes fewer than 2^31 - 1 indices and rows");
-    TORCH_CHECK(std::isfinite(scale), "scale must be finite");
+    TORCH_CHECK(std::isfinite((float)scale), "scale must be finite (in float32)");
     dtype_of(table, "table");
     index_bytes_of(index);
     if (!(at::GradMode::is_enabled() && table.requires_grad())) return embedding_forward(index, table, scale);
@@ -191,7 +191,7 @@ Tensor layer_norm(const Tensor& x, const c10::optional<Tensor>& weight_, const c
     on_gpu(x, "x");
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "x must have at least one value to a row");
     TORCH_CHECK(x.size(-1) <= E3DGS_FEATURE_MAX_DIM, "at most ", E3DGS_FEATURE_MAX_DIM, " values to a row");
-    TORCH_CHECK(std::isfinite(eps) && eps >= 0.0, "eps must be finite and not negative");
+    TORCH_CHECK(std::isfinite((float)eps) && eps >= 0.0, "eps must be finite (in float32) and not negative");
     dtype_of(x, "x");
     bool grad = x.requires_grad();
     for (const auto& p : {std::make_pair(&weight, "weight"), std::make_pair(&bias, "bias")}) {

@@ -225,6 +225,23 @@ def test_layer_norm_hard_rows():
     assert torch.isnan(out[1]).all() and torch.isnan(out[2]).all() and torch.isfinite(out[[0, 3]]).all()
 
 
+def test_layer_norm_past_32_bits():
+    n, dim = 1_100_000, 2048                                     # 2.25 G values
+    x = torch.zeros(n, dim, dtype=torch.bfloat16, device=DEV)
+    x[-3:] = rand(3, dim).bfloat16()
+    x[n // 2] = rand(dim, seed=1).bfloat16()
+    leaf = x.requires_grad_(True)
+    out = features.layer_norm(leaf)
+    for row in (n // 2, n - 2, n - 1):
+        assert torch.equal(out[row], features.layer_norm(x.detach()[row]))
+    d = torch.zeros_like(x)
+    d[-1] = rand(dim, seed=2).bfloat16()
+    (dx,) = torch.autograd.grad(out, leaf, d)
+    one = x.detach()[-1:].requires_grad_(True)
+    (want,) = torch.autograd.grad(features.layer_norm(one), one, d[-1:])
+    assert torch.equal(dx[-1], want[0]) and dx[:10].count_nonzero() == 0
+
+
 # ------------------------------------------------------------------------------------------------ distillation
 def label(n, classes, k, seed=0, empty=0.2):
     g = torch.Generator().manual_seed(seed + n + 31 * classes + k)
@@ -421,6 +438,22 @@ def test_distill_past_32_bits():
     close(d[-2:], grad, half_step(grad, torch.float16) * 1.01 + tol, "last gradients")
 
 
+def test_distill_planes_past_32_bits():
+    classes, n = 250, 8_650_000                                  # 2.16 G scores
+    z = torch.zeros(classes, n, dtype=torch.float16, device=DEV)
+    z[:, -4:] = (rand(classes, 4) * 2).half()
+    for k in (2, 12):                                            # the label in registers, and in LDS
+        t = torch.ones(k, n, device=DEV)
+        index = torch.full((k, n), -1, dtype=torch.int32, device=DEV)
+        index[:, -4:] = torch.arange(classes - 4 * k, classes, device=DEV, dtype=torch.int32).view(k, 4)
+        value, d = losses.distill_loss_raw(z, t, index, reduction="none", class_dim=0)
+        row, grad, _, row_tol, tol = distill_formula(z[:, -4:].t(), t[:, -4:].t(), index[:, -4:].t(), 1.0)
+        close(value[-4:], row, row_tol + U * row.abs(), "last pixels")
+        close(d[:, -4:].t(), grad, half_step(grad, torch.float16) * 1.01 + tol, "last gradients")
+        assert (value[:-4] == 0).all() and d[:, :1000].count_nonzero() == 0
+        del t, index, value, d
+
+
 # ------------------------------------------------------------------------------------------------ differences
 def test_gradients_against_differences():
     """A step of the inputs along the gradient changes the value by the squared norm of the gradient, to second order.  fp32
@@ -587,6 +620,7 @@ def test_refusals():
     bad = [
         lambda: features.embedding(i.float(), x), lambda: features.embedding(i, x.double()), lambda: features.embedding(i, x[0]),
         lambda: features.embedding(i.cpu(), x), lambda: features.embedding(i, x, float("inf")),
+        lambda: features.embedding(i, x, 1e300), lambda: features.layer_norm(x, eps=1e300),
         lambda: features.layer_norm(x.double()), lambda: features.layer_norm(x, rand(5)), lambda: features.layer_norm(x, rand(6, 1)),
         lambda: features.layer_norm(x, rand(6).cpu()), lambda: features.layer_norm(x, eps=-1.0),
         lambda: features.layer_norm(x, rand(6), rand(6).half()), lambda: features.layer_norm(x[:, :0]),
