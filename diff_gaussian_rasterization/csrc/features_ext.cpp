@@ -226,7 +226,8 @@ Scores scores_of(const Tensor& logits, const Tensor& teacher, const Tensor& inde
     s.logits = rows_of(logits, class_dim);
     s.teacher = rows_of(teacher, class_dim);
     s.index = rows_of(index, class_dim);
-    s.planes = s.rows > 1 && s.logits.entry_stride != 1 && s.logits.row_stride == 1 && s.classes <= E3DGS_DISTILL_MAX_PLANES;
+    s.planes = s.rows > 1 && s.logits.entry_stride != 1 && s.logits.row_stride == 1 && s.classes <= E3DGS_DISTILL_MAX_PLANES &&
+               s.k <= E3DGS_DISTILL_MAX_PLANES;
     if (!s.planes && s.logits.entry_stride != 1) s.logits = {logits.movedim(class_dim, -1).contiguous(), s.classes, 1};
     return s;
 }

@@ -122,7 +122,7 @@ int e3_layer_norm_forward_impl(size_t, size_t, const void*, size_t, int, const v
 size_t e3_layer_norm_scratch_bytes(size_t, size_t);
 int e3_layer_norm_backward_impl(size_t, size_t, const void*, size_t, const void*, size_t, int, const void*, int, const float*,
                                 const float*, void*, void*, void*, char*, hipStream_t);
-bool e3_distill_layout_ok(size_t, size_t, size_t, size_t);
+bool e3_distill_layout_ok(size_t, size_t, size_t, size_t, size_t);
 size_t e3_distill_scratch_bytes(size_t);
 int e3_distill_forward_impl(size_t, size_t, size_t, const void*, size_t, size_t, int, const void*, size_t, size_t, int,
                             const void*, size_t, size_t, int, float, int, float*, float*, float*, void*, size_t, size_t, char*,
@@ -924,12 +924,12 @@ static int distill_args(const char* who, size_t rows, size_t classes, size_t k, 
         (index_bytes != 4 && index_bytes != 8))
         return feature_args_fail(who, rows, classes, dtype, "bad element type");
     if (rows > 0 && (!logits || !teacher || !index)) return feature_args_fail(who, rows, classes, dtype, "null pointer");
-    if (!e3_distill_layout_ok(rows, classes, row_stride, class_stride))
-        return feature_args_fail(who, rows, classes, dtype, "neither rows of classes nor at most 256 planes");
+    if (!e3_distill_layout_ok(rows, classes, k, row_stride, class_stride))
+        return feature_args_fail(who, rows, classes, dtype, "neither rows of classes nor at most 256 planes with at most 256 entries");
     return 0;
 }
-static bool distill_grad_ok(size_t rows, size_t classes, size_t class_stride, size_t grad_row_stride, size_t grad_class_stride) {
-    return e3_distill_layout_ok(rows, classes, grad_row_stride, grad_class_stride) &&
+static bool distill_grad_ok(size_t rows, size_t classes, size_t k, size_t class_stride, size_t grad_row_stride, size_t grad_class_stride) {
+    return e3_distill_layout_ok(rows, classes, k, grad_row_stride, grad_class_stride) &&
            (grad_class_stride == 1) == (class_stride == 1);
 }
 int e3dgs_distill_forward(size_t rows, size_t classes, size_t k, const void* logits, size_t row_stride, size_t class_stride,
@@ -943,7 +943,7 @@ int e3dgs_distill_forward(size_t rows, size_t classes, size_t k, const void* log
                                 index_bytes, temperature, reduction);
     if (rc) return rc;
     if (!loss || (rows > 0 && (!stats || !scratch))) return feature_args_fail(who, rows, classes, dtype, "null pointer");
-    if (grad && !distill_grad_ok(rows, classes, class_stride, grad_row_stride, grad_class_stride))
+    if (grad && !distill_grad_ok(rows, classes, k, class_stride, grad_row_stride, grad_class_stride))
         return feature_args_fail(who, rows, classes, dtype, "the gradient's layout differs from the scores'");
     return e3_distill_forward_impl(rows, classes, k, logits, row_stride, class_stride, dtype, teacher, teacher_row_stride,
                                    teacher_entry_stride, teacher_dtype, index, index_row_stride, index_entry_stride,
@@ -961,7 +961,7 @@ int e3dgs_distill_backward(size_t rows, size_t classes, size_t k, const void* lo
                                 index_bytes, temperature, reduction);
     if (rc) return rc;
     if (rows > 0 && (!stats || !grad)) return feature_args_fail(who, rows, classes, dtype, "null pointer");
-    if (!distill_grad_ok(rows, classes, class_stride, grad_row_stride, grad_class_stride))
+    if (!distill_grad_ok(rows, classes, k, class_stride, grad_row_stride, grad_class_stride))
         return feature_args_fail(who, rows, classes, dtype, "the gradient's layout differs from the scores'");
     return e3_distill_backward_impl(rows, classes, k, logits, row_stride, class_stride, dtype, teacher, teacher_row_stride,
                                     teacher_entry_stride, teacher_dtype, index, index_row_stride, index_entry_stride,

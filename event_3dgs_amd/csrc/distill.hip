@@ -23,7 +23,7 @@ int e3_fail(hipError_t e, const char* what);
 namespace {
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int DISTILL_MAX_K = 1024;              // entries of a row's label (E3DGS_DISTILL_MAX_K)
-constexpr int DISTILL_PLANES = 256;              // classes of the plane layout: one label column per pixel in LDS
+constexpr int DISTILL_PLANES = 256;              // classes of the plane layout, and entries of its labels
 constexpr unsigned DISTILL_BLOCKS = 4096;        // workgroups = partial sums of a launch
 
 struct DistillArgs {
@@ -42,6 +42,7 @@ struct DistillArgs {
     void* grad;
     size_t g_row, g_class;
     float *loss, *weight_out;   // the value and the weight of a row, written by the only workgroup of a launch
+    bool planes_wide;       // the planes of the scores (and of the gradient) can be moved in 16-byte packs
     const uint32_t* counts; // partial counts of the labelled rows (a value formed with its gradient)
     uint32_t ncounts;
 };
@@ -143,6 +144,11 @@ __device__ __forceinline__ float label_value(const DistillArgs& a, size_t row, c
 __device__ __forceinline__ bool class_weight(const DistillArgs& a, const int* ids, const float* ws, int k, float& w) {
     const int id = ids[k];
     if (id < 0 || id == ID_BROKEN) return false;
+    w = ws[k];
+    int same = 0;
+#pragma unroll 4
+    for (int j = 0; j < (int)a.k; ++j) same += ids[j] == id ? 1 : 0;
+    if (same == 1) return true;
     w = 0.0f;
     bool first = true;
     for (int j = 0; j < (int)a.k; ++j) {
@@ -154,10 +160,11 @@ __device__ __forceinline__ bool class_weight(const DistillArgs& a, const int* id
 }
 
 // ---- sums over a launch
-// Number of labelled rows; one thread's share.  The entries of a row are read by as many neighbouring lanes as there are
-// entries (a power of two, at most a wave); the row counts for the first of them.
+// Number of labelled rows; one thread's share.  Where the entries of a row lie next to each other they are read by as many
+// neighbouring lanes as there are entries (a power of two, at most a wave), and the row counts for the first of them; where
+// neighbouring rows do (planes), a lane takes a row.
 __device__ __forceinline__ uint32_t count_rows(const DistillArgs& a, size_t thread, size_t threads) {
-    int lanes = 64;
+    int lanes = a.i_entry == 1 ? 64 : 1;
     while (lanes > 1 && lanes > (int)a.k) lanes >>= 1;
     const int lane = threadIdx.x & (lanes - 1), group = (threadIdx.x & 63) & ~(lanes - 1);
     const unsigned long long mine = (lanes == 64 ? ~0ull : (1ull << lanes) - 1ull) << group;
@@ -165,14 +172,14 @@ __device__ __forceinline__ uint32_t count_rows(const DistillArgs& a, size_t thre
     const size_t step = threads / lanes, rounds = (a.rows + step - 1) / step;
     for (size_t i = 0; i < rounds; ++i) {                 // (the same number of rounds for every lane of a wave)
         const size_t row = i * step + thread / lanes;
-        bool any = false;
-        if (row < a.rows)
-            for (int k = lane; k < (int)a.k; k += lanes) {
-                long long id;
-                any |= entry_score(a, row, k, id) != -__builtin_inff();
-            }
-        const unsigned long long all = __ballot(any);
-        if (lane == 0 && (all & mine) != 0ull) ++n;
+        unsigned long long any = 0ull;
+        for (int k0 = 0; k0 < (int)a.k; k0 += lanes) {    // (most rows are decided by their first entries)
+            long long id;
+            const bool in = row < a.rows && k0 + lane < (int)a.k;
+            any |= __ballot(in && entry_score(a, row, k0 + lane, id) != -__builtin_inff());
+            if (lanes == 1 && any == ~0ull) break;
+        }
+        if (lane == 0 && (any & mine) != 0ull) ++n;
     }
     return n;
 }
@@ -188,7 +195,7 @@ __device__ __forceinline__ uint32_t block_sum_u32(uint32_t n, uint32_t* lds) {
     __syncthreads();
     return n;
 }
-constexpr int COUNT_BLOCKS = 256;
+constexpr int COUNT_BLOCKS = 1024;
 __global__ __launch_bounds__(256) void distill_count_kernel(const DistillArgs a, uint32_t* __restrict__ counts) {
     __shared__ uint32_t lds[4];
     const uint32_t n = block_sum_u32<256>(count_rows(a, (size_t)blockIdx.x * 256 + threadIdx.x, (size_t)gridDim.x * 256), lds);
@@ -490,55 +497,122 @@ __global__ __launch_bounds__(G) void distill_both_rows_kernel(const DistillArgs 
     store_part<G>(a, total, count, L.ms);
 }
 
-// ---- short rows, one behind the other: a workgroup takes `tile` rows at a time through LDS, so that memory is moved in
-// whole packs whatever the row length; 256 / tile lanes work on a row there.
+// ---- short rows, one behind the other, and planes: a workgroup takes `tile` rows at a time through LDS, so that memory is moved
+// in whole packs whatever the row length, and planes are turned into rows; 256 / tile lanes work on a row there.
 constexpr int TILE_BYTES = 32768, TILE_LABEL_BYTES = 24576, TILE_PACKS = TILE_BYTES / 16 / 256;
 constexpr int VALUE = 1, GRADIENT = 2;
-__host__ __device__ constexpr size_t tile_lds(size_t tile, size_t classes, size_t k, size_t bytes) {
-    return (tile * classes * bytes + 15) / 16 * 16 + tile * k * 12;
+__host__ __device__ constexpr size_t tile_lds(size_t tile, size_t pitch, size_t k, size_t bytes) {
+    return (tile * pitch * bytes + 15) / 16 * 16 + tile * k * 12;
 }
-template <typename T, int MODE, int LANES>
+// A tile between memory and LDS, as it lies ...
+template <typename T>
+__device__ __forceinline__ void tile_in(const T* __restrict__ src, words_t* mem, int elems) {
+    const int packs = (int)(elems * sizeof(T) / 16), rest = packs * (16 / (int)sizeof(T));
+    if (packs > 0) {                     // (uniform; the loads are unconditional and in flight together)
+        words_t in[TILE_PACKS];
+#pragma unroll
+        for (int u = 0; u < TILE_PACKS; ++u) {
+            const int i = u * 256 + threadIdx.x;
+            in[u] = reinterpret_cast<const words_t*>(src)[i < packs ? i : packs - 1];
+        }
+#pragma unroll
+        for (int u = 0; u < TILE_PACKS; ++u) {
+            const int i = u * 256 + threadIdx.x;
+            if (i < packs) mem[i] = in[u];
+        }
+    }
+    if (rest + (int)threadIdx.x < elems) reinterpret_cast<T*>(mem)[rest + threadIdx.x] = src[rest + threadIdx.x];
+}
+template <typename T>
+__device__ __forceinline__ void tile_out(T* __restrict__ dst, const words_t* mem, int elems) {
+    const int packs = (int)(elems * sizeof(T) / 16), rest = packs * (16 / (int)sizeof(T));
+#pragma unroll
+    for (int u = 0; u < TILE_PACKS; ++u) {
+        const int i = u * 256 + threadIdx.x;
+        if (i < packs) reinterpret_cast<words_t*>(dst)[i] = mem[i];
+    }
+    if (rest + (int)threadIdx.x < elems) dst[rest + threadIdx.x] = reinterpret_cast<const T*>(mem)[rest + threadIdx.x];
+}
+// ... and from and to planes: V neighbouring pixels of a class to a thread, spread over the V rows of the tile (`pitch`
+// elements apart, an odd number: neighbouring pixels lie in different banks).
+template <typename T, int V, int TILE>
+__device__ __forceinline__ void planes_in(const T* __restrict__ src, size_t stride, T* rows, int pitch, int n, int classes) {
+    constexpr int PARTS = TILE / V, UN = 4;
+    for (int i0 = threadIdx.x; i0 < classes * PARTS; i0 += 256 * UN) {
+        Pack<T, V> in[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int i = i0 + u * 256, j = i / PARTS, r = i % PARTS * V;      // (unconditional loads: others again)
+            in[u] = *reinterpret_cast<const Pack<T, V>*>(src + (size_t)(j < classes ? j : classes - 1) * stride + (r < n ? r : 0));
+        }
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int i = i0 + u * 256, j = i / PARTS, r = i % PARTS * V;
+            if (j < classes && r < n) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) rows[(r + v) * pitch + j] = in[u].v[v];
+            }
+        }
+    }
+}
+template <typename T, int V, int TILE>
+__device__ __forceinline__ void planes_out(T* __restrict__ dst, size_t stride, const T* rows, int pitch, int n, int classes) {
+    constexpr int PARTS = TILE / V;
+    for (int i = threadIdx.x; i < classes * PARTS; i += 256) {
+        const int j = i / PARTS, r = i % PARTS * V;
+        if (r >= n) continue;
+        Pack<T, V> out;
+#pragma unroll
+        for (int v = 0; v < V; ++v) out.v[v] = rows[(r + v) * pitch + j];
+        *reinterpret_cast<Pack<T, V>*>(dst + (size_t)j * stride + r) = out;
+    }
+}
+
+template <bool PLANES, typename T, int MODE, int LANES>
 __global__ __launch_bounds__(256) void distill_tile_kernel(const DistillArgs a) {
     constexpr int tile = 256 / LANES;
     extern __shared__ words_t tile_mem[];
     __shared__ float lds[16];
     T* rows = reinterpret_cast<T*>(tile_mem);
-    float* ts = reinterpret_cast<float*>(tile_mem + ((size_t)tile * a.classes * sizeof(T) + 15) / 16);
+    const int C = (int)a.classes, pitch = PLANES ? C | 1 : C;
+    float* ts = reinterpret_cast<float*>(tile_mem + ((size_t)tile * pitch * sizeof(T) + 15) / 16);
     int* ids = reinterpret_cast<int*>(ts + tile * (int)a.k);
     float* ws = reinterpret_cast<float*>(ids + tile * (int)a.k);
-    const int K = (int)a.k, C = (int)a.classes, r = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const int K = (int)a.k, r = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     const float rt = 1.0f / a.temperature, c = LOG2E * rt;
     float f_all = a.temperature;
     if (MODE == GRADIENT) f_all *= a.weight ? *a.weight : 1.0f;
     if (MODE == (VALUE | GRADIENT)) f_all *= row_weight<256>(a, reinterpret_cast<uint32_t*>(lds));
     float total = 0.0f;
     uint32_t count = 0;
-    T* z = rows + r * C;
+    T* z = rows + r * pitch;
     int* id = ids + r * K;
     float *t = ts + r * K, *w = ws + r * K;
     for (size_t first = (size_t)blockIdx.x * tile; first < a.rows; first += (size_t)gridDim.x * tile) {
         const int n = a.rows - first < (size_t)tile ? (int)(a.rows - first) : tile;
-        const int elems = n * C, packs = (int)(elems * sizeof(T) / 16), rest = packs * (16 / (int)sizeof(T));
-        const T* src = reinterpret_cast<const T*>(a.logits) + first * C;
-        {
-            words_t in[TILE_PACKS];
-#pragma unroll
-            for (int u = 0; u < TILE_PACKS; ++u) {
-                const int i = u * 256 + threadIdx.x;
-                if (i < packs) in[u] = reinterpret_cast<const words_t*>(src)[i];
-            }
-            for (int e = threadIdx.x; e < n * K; e += 256) {
-                const int er = e / K, k = e - er * K;
+        constexpr int V = Wide<T>::N <= tile ? Wide<T>::N : 1;
+        const bool wide = a.planes_wide && n % V == 0;
+        if (!PLANES) tile_in(reinterpret_cast<const T*>(a.logits) + first * C, tile_mem, n * C);
+        else if (wide) planes_in<T, V, tile>(reinterpret_cast<const T*>(a.logits) + first, a.class_stride, rows, pitch, n, C);
+        else planes_in<T, 1, tile>(reinterpret_cast<const T*>(a.logits) + first, a.class_stride, rows, pitch, n, C);
+        // (planes: the labels lie as planes too, neighbouring lanes read neighbouring pixels; rows: the lanes of a row read it)
+        if (PLANES) {
+#pragma unroll 2
+            for (int e = threadIdx.x; e < K * tile; e += 256) {
+                const int k = e / tile, er = e % tile;
+                if (er >= n) continue;
                 long long index;
-                ts[e] = entry_score(a, first + er, k, index);
-                ids[e] = entry_class(a, ts[e], index);
+                const float score = entry_score(a, first + er, k, index);
+                ts[er * K + k] = score;
+                ids[er * K + k] = entry_class(a, score, index);
             }
-#pragma unroll
-            for (int u = 0; u < TILE_PACKS; ++u) {
-                const int i = u * 256 + threadIdx.x;
-                if (i < packs) tile_mem[i] = in[u];
+        } else if (r < n) {
+#pragma unroll 1
+            for (int k = lane; k < K; k += LANES) {
+                long long index;
+                t[k] = entry_score(a, first + r, k, index);
+                id[k] = entry_class(a, t[k], index);
             }
-            if (rest + (int)threadIdx.x < elems) rows[rest + threadIdx.x] = src[rest + threadIdx.x];
         }
         __syncthreads();
         const size_t row = first + r;
@@ -616,8 +690,15 @@ __global__ __launch_bounds__(256) void distill_tile_kernel(const DistillArgs a) 
             if (live && l.any)
                 for (int k = lane; k < K; k += LANES) {
                     if (id[k] < 0 || id[k] == ID_BROKEN) continue;
-                    float q = 0.0f;
-                    for (int j = 0; j < K; ++j) q += id[j] == id[k] ? w[j] : 0.0f;
+                    const int cls = id[k];
+                    float q = w[k];
+                    int same = 0;
+#pragma unroll 4
+                    for (int j = 0; j < K; ++j) same += id[j] == cls ? 1 : 0;
+                    if (same > 1) {                     // the class is listed more than once: its weights in order
+                        q = 0.0f;
+                        for (int j = 0; j < K; ++j) q += id[j] == cls ? w[j] : 0.0f;
+                    }
                     t[k] = f * (exp2_hw(((float)z[id[k]] - m) * c) * inv - q * l.inv);
                 }
             wave_sync();
@@ -629,176 +710,13 @@ __global__ __launch_bounds__(256) void distill_tile_kernel(const DistillArgs a) 
                 for (int k = lane; k < K; k += LANES)
                     if (id[k] >= 0 && id[k] != ID_BROKEN) z[id[k]] = (T)t[k];
             __syncthreads();
-            T* dst = reinterpret_cast<T*>(a.grad) + first * C;
-#pragma unroll
-            for (int u = 0; u < TILE_PACKS; ++u) {
-                const int i = u * 256 + threadIdx.x;
-                if (i < packs) reinterpret_cast<words_t*>(dst)[i] = tile_mem[i];
-            }
-            if (rest + (int)threadIdx.x < elems) dst[rest + threadIdx.x] = rows[rest + threadIdx.x];
+            if (!PLANES) tile_out(reinterpret_cast<T*>(a.grad) + first * C, tile_mem, n * C);
+            else if (wide) planes_out<T, V, tile>(reinterpret_cast<T*>(a.grad) + first, a.g_class, rows, pitch, n, C);
+            else planes_out<T, 1, tile>(reinterpret_cast<T*>(a.grad) + first, a.g_class, rows, pitch, n, C);
         }
         __syncthreads();
     }
     if (MODE & VALUE) store_part<256>(a, total, count, lds);
-}
-
-// ---- planes: a lane takes a pixel; its label is a column of `classes` weights in LDS (only its own lane touches it)
-struct PlaneLabel {
-    float top, inv, qlogq;
-    bool any, broken;
-};
-// Adds the weights of a pixel's label to its column.
-constexpr int PLANE_ENTRIES = 8;       // of a label, read together
-__device__ __forceinline__ PlaneLabel plane_label(const DistillArgs& a, size_t row, float c, float rt, float* col) {
-    PlaneLabel l;
-    float top = -__builtin_inff(), sum = 0.0f;
-    l.any = l.broken = false;
-    for (size_t k0 = 0; k0 < a.k; k0 += PLANE_ENTRIES) {
-        float t[PLANE_ENTRIES];
-#pragma unroll
-        for (int k = 0; k < PLANE_ENTRIES; ++k) {
-            long long id;
-            t[k] = entry_score(a, row, k0 + k < a.k ? k0 + k : a.k - 1, id);
-            if (k0 + k >= a.k) t[k] = -__builtin_inff();
-            l.any |= t[k] != -__builtin_inff();
-            l.broken |= t[k] != -__builtin_inff() && id >= (long long)a.classes;
-        }
-        soft_add<PLANE_ENTRIES>(top, sum, t, c);
-    }
-    l.top = top;
-    l.inv = l.qlogq = 0.0f;
-    if (!l.any) return l;
-    l.inv = 1.0f / sum;
-    const float rest = log2_hw(l.inv) * LN2;
-    for (size_t k0 = 0; k0 < a.k; k0 += PLANE_ENTRIES) {
-        float t[PLANE_ENTRIES];
-        int cls[PLANE_ENTRIES];
-#pragma unroll
-        for (int k = 0; k < PLANE_ENTRIES; ++k) {
-            long long id;
-            t[k] = entry_score(a, row, k0 + k < a.k ? k0 + k : a.k - 1, id);
-            cls[k] = k0 + k < a.k ? entry_class(a, t[k], id) : -1;
-        }
-#pragma unroll
-        for (int k = 0; k < PLANE_ENTRIES; ++k) {
-            if (cls[k] < 0 || cls[k] == ID_BROKEN) continue;
-            const float q = exp2_hw((t[k] - top) * c) * l.inv;
-            if (q != 0.0f) l.qlogq += q * ((t[k] - top) * rt + rest);
-            col[(size_t)cls[k] * 64] += q;
-        }
-    }
-    return l;
-}
-__device__ __forceinline__ void plane_clear(const DistillArgs& a, size_t row, float* col) {
-    for (size_t k = 0; k < a.k; ++k) {
-        const long long id = load_index(a.index, row * a.i_row + k * a.i_entry, a.index_bytes);
-        if (id >= 0 && id < (long long)a.classes) col[(size_t)id * 64] = 0.0f;
-    }
-}
-
-// The planes go by in batches: the loads of the next batch are in flight while one is worked on (a lane's label takes
-// 4 bytes of LDS per class, so that few waves fit a CU and each has to keep many loads in flight).
-constexpr int PLANE_BATCH = 16;
-template <typename T>
-struct PlaneBatch {
-    T v[PLANE_BATCH];
-    __device__ __forceinline__ void load(const T* __restrict__ z, uint32_t first, uint32_t classes, size_t stride) {
-#pragma unroll
-        for (int u = 0; u < PLANE_BATCH; ++u) {          // (the last plane again behind the last one: never used)
-            const uint32_t j = first + u < classes ? first + u : classes - 1;
-            v[u] = z[(size_t)j * stride];
-        }
-    }
-};
-
-template <typename T>
-__global__ __launch_bounds__(64) void distill_fwd_planes_kernel(const DistillArgs a) {
-    extern __shared__ float cols[];
-    const int lane = threadIdx.x;
-    float* col = cols + lane;
-    const float rt = 1.0f / a.temperature, c = LOG2E * rt;
-    for (uint32_t j = 0; j < a.classes; ++j) col[j * 64] = 0.0f;
-    float total = 0.0f;
-    uint32_t count = 0;
-    for (size_t row = (size_t)blockIdx.x * 64 + lane; row < a.rows; row += (size_t)gridDim.x * 64) {
-        const T* z = reinterpret_cast<const T*>(a.logits) + row;
-        PlaneBatch<T> next;
-        next.load(z, 0, a.classes, a.class_stride);
-        const PlaneLabel l = plane_label(a, row, c, rt, col);
-        if (!l.any) {
-            a.stats[row] = make_float2(0.0f, 0.0f);
-            if (a.row_loss) a.row_loss[row] = 0.0f;
-            continue;
-        }
-        float m = -__builtin_inff(), s = 0.0f;
-        float qz = 0.0f, qs = 0.0f;              // sum of q (z - m) and of q over the classes so far
-        for (uint32_t j = 0; j < a.classes; j += PLANE_BATCH) {
-            const PlaneBatch<T> b = next;
-            if (j + PLANE_BATCH < a.classes) next.load(z, j + PLANE_BATCH, a.classes, a.class_stride);
-            float v[PLANE_BATCH], M = m;
-#pragma unroll
-            for (int u = 0; u < PLANE_BATCH; ++u) {
-                v[u] = j + u < a.classes ? (float)b.v[u] : -__builtin_inff();
-                M = fmaxf(M, v[u]);
-            }
-            if (M != m) {
-                s *= exp2_hw((m - M) * c);
-                if (qs != 0.0f) qz += qs * (m - M);
-                m = M;
-            }
-            const float off = M == -__builtin_inff() ? 0.0f : M;
-#pragma unroll
-            for (int u = 0; u < PLANE_BATCH; ++u) {
-                const float d = v[u] - off, q = j + u < a.classes ? col[(j + u) * 64] : 0.0f;
-                s += exp2_hw(d * c);
-                qz += q != 0.0f ? q * d : 0.0f;              // (a class that is switched off has d = -inf)
-                qs += q;
-            }
-        }
-        // sum of q = 1:  sum q (log q - log p) = qlogq - sum q (z - m) / T + log s
-        float d = l.qlogq - qz * rt + log2_hw(s) * LN2;
-        if (l.broken) d = __builtin_nanf("");
-        d *= a.temperature * a.temperature;
-        a.stats[row] = make_float2(m, l.broken ? __builtin_nanf("") : 1.0f / s);
-        if (a.row_loss) a.row_loss[row] = d;
-        total += d;
-        ++count;
-        plane_clear(a, row, col);
-    }
-    __shared__ float lds[2];
-    store_part<64>(a, total, count, lds);
-}
-
-template <typename T>
-__global__ __launch_bounds__(64) void distill_bwd_planes_kernel(const DistillArgs a) {
-    extern __shared__ float cols[];
-    const int lane = threadIdx.x;
-    float* col = cols + lane;
-    const float rt = 1.0f / a.temperature, c = LOG2E * rt;
-    const float f_all = a.temperature * (a.weight ? *a.weight : 1.0f);
-    for (uint32_t j = 0; j < a.classes; ++j) col[j * 64] = 0.0f;
-    for (size_t row = (size_t)blockIdx.x * 64 + lane; row < a.rows; row += (size_t)gridDim.x * 64) {
-        const float2 st = a.stats[row];
-        T* g = reinterpret_cast<T*>(a.grad) + row;
-        if (st.y == 0.0f) {
-            for (uint32_t j = 0; j < a.classes; ++j) g[(size_t)j * a.g_class] = (T)0.0f;
-            continue;
-        }
-        const T* z = reinterpret_cast<const T*>(a.logits) + row;
-        PlaneBatch<T> next;
-        next.load(z, 0, a.classes, a.class_stride);
-        const float f = f_all * (a.scale ? a.scale[a.reduction == 0 ? row : 0] : 1.0f);
-        plane_label(a, row, c, rt, col);
-        for (uint32_t j = 0; j < a.classes; j += PLANE_BATCH) {
-            const PlaneBatch<T> b = next;
-            if (j + PLANE_BATCH < a.classes) next.load(z, j + PLANE_BATCH, a.classes, a.class_stride);
-#pragma unroll
-            for (int u = 0; u < PLANE_BATCH; ++u)
-                if (j + u < a.classes)
-                    g[(size_t)(j + u) * a.g_class] = (T)(f * (exp2_hw(((float)b.v[u] - st.x) * c) * st.y - col[(j + u) * 64]));
-        }
-        plane_clear(a, row, col);
-    }
 }
 
 // ---- planes, short lists: P neighbouring pixels to a lane, their labels in registers (KR entries each: the class of an entry
@@ -1014,26 +932,41 @@ unsigned distill_blocks(size_t rows, int per_block) {
 // launch would not fill the chip otherwise.  0: the rows do not lie one behind the other from a 16-byte boundary on, or
 // fewer than 8 fit.
 int tile_rows(const DistillArgs& a, bool gradient) {
-    const size_t b = e3_elem_bytes(a.dtype);
-    if (a.row_stride != a.classes || (reinterpret_cast<uintptr_t>(a.logits) & 15) != 0) return 0;
-    if (gradient && (a.g_row != a.classes || (reinterpret_cast<uintptr_t>(a.grad) & 15) != 0)) return 0;
+    const bool planes = planes_layout(a.row_stride, a.class_stride);
+    const size_t b = e3_elem_bytes(a.dtype), pitch = planes ? a.classes | 1 : a.classes;
+    if (!planes) {
+        if (a.row_stride != a.classes || (reinterpret_cast<uintptr_t>(a.logits) & 15) != 0) return 0;
+        if (gradient && (a.g_row != a.classes || (reinterpret_cast<uintptr_t>(a.grad) & 15) != 0)) return 0;
+    }
     size_t t = 256;
-    while (t >= 8 && (t * a.classes * b > TILE_BYTES || t * a.k * 12 > TILE_LABEL_BYTES)) t >>= 1;
+    while (t >= 8 && (t * pitch * b > TILE_BYTES || t * a.k * 12 > TILE_LABEL_BYTES)) t >>= 1;
     while (t > 8 && a.rows < t * 512) t >>= 1;
     return t >= 8 ? (int)t : 0;
 }
-template <typename T, int MODE>
-int distill_tile(const DistillArgs& a, int tile, unsigned& blocks, hipStream_t s) {
-    blocks = distill_blocks(a.rows, tile);
-    const size_t lds = tile_lds(tile, a.classes, a.k, sizeof(T));
-    if (tile == 256) distill_tile_kernel<T, MODE, 1><<<dim3(blocks), dim3(256), lds, s>>>(a);
-    else if (tile == 128) distill_tile_kernel<T, MODE, 2><<<dim3(blocks), dim3(256), lds, s>>>(a);
-    else if (tile == 64) distill_tile_kernel<T, MODE, 4><<<dim3(blocks), dim3(256), lds, s>>>(a);
-    else if (tile == 32) distill_tile_kernel<T, MODE, 8><<<dim3(blocks), dim3(256), lds, s>>>(a);
-    else if (tile == 16) distill_tile_kernel<T, MODE, 16><<<dim3(blocks), dim3(256), lds, s>>>(a);
-    else distill_tile_kernel<T, MODE, 32><<<dim3(blocks), dim3(256), lds, s>>>(a);
+template <bool PLANES, typename T, int MODE>
+int distill_tile_launch(const DistillArgs& a, int tile, unsigned blocks, hipStream_t s) {
+    const size_t lds = tile_lds(tile, PLANES ? a.classes | 1 : a.classes, a.k, sizeof(T));
+    if (tile == 256) distill_tile_kernel<PLANES, T, MODE, 1><<<dim3(blocks), dim3(256), lds, s>>>(a);
+    else if (tile == 128) distill_tile_kernel<PLANES, T, MODE, 2><<<dim3(blocks), dim3(256), lds, s>>>(a);
+    else if (tile == 64) distill_tile_kernel<PLANES, T, MODE, 4><<<dim3(blocks), dim3(256), lds, s>>>(a);
+    else if (tile == 32) distill_tile_kernel<PLANES, T, MODE, 8><<<dim3(blocks), dim3(256), lds, s>>>(a);
+    else if (tile == 16) distill_tile_kernel<PLANES, T, MODE, 16><<<dim3(blocks), dim3(256), lds, s>>>(a);
+    else distill_tile_kernel<PLANES, T, MODE, 32><<<dim3(blocks), dim3(256), lds, s>>>(a);
     LAUNCH_OK("distill_tile_kernel");
     return 0;
+}
+// whether n neighbouring pixels of every plane can be moved at once
+template <typename T>
+bool planes_wide(const void* p, size_t stride, size_t rows, size_t n) {
+    return rows % n == 0 && stride % n == 0 && (reinterpret_cast<uintptr_t>(p) & (n * sizeof(T) - 1)) == 0;
+}
+template <typename T, int MODE>
+int distill_tile(DistillArgs a, int tile, unsigned& blocks, hipStream_t s) {
+    blocks = distill_blocks(a.rows, tile);
+    if (!planes_layout(a.row_stride, a.class_stride)) return distill_tile_launch<false, T, MODE>(a, tile, blocks, s);
+    constexpr size_t V = Wide<T>::N;
+    a.planes_wide = planes_wide<T>(a.logits, a.class_stride, V, V) && (!(MODE & GRADIENT) || planes_wide<T>(a.grad, a.g_class, V, V));
+    return distill_tile_launch<true, T, MODE>(a, tile, blocks, s);
 }
 
 // Threads of a long row: a wave up to some thousand classes, a workgroup beyond that.
@@ -1082,31 +1015,23 @@ int distill_wide_bwd(const DistillArgs& a, hipStream_t s) {
     LAUNCH_OK("distill_bwd_wide_kernel");
     return 0;
 }
-// whether P neighbouring pixels of every plane can be moved at once
-template <typename T>
-bool planes_wide(const void* p, size_t stride, size_t rows, size_t n) {
-    return rows % n == 0 && stride % n == 0 && (reinterpret_cast<uintptr_t>(p) & (n * sizeof(T) - 1)) == 0;
-}
+// Planes go pixel by pixel (labels in registers, several pixels to a lane) where the list is short and there are enough pixels
+// to fill the chip that way; through tiles otherwise.  Value and gradient, by pixel / by tiles: 16384 x 200 fp32 84 / 24 us,
+// 65536 x 200 bf16 84 / 36 us, 262144 x 20 fp32 37 / 37 us, 262144 x 200 bf16 98 / 118 us, 2073600 x 64 fp32 359 / 419 us.
+constexpr size_t PIXELS = 262144;
+bool planes_by_pixel(const DistillArgs& a) { return a.k <= 8 && a.rows >= PIXELS; }
 
 template <typename T>
 int distill_t(const DistillArgs& a, bool backward, unsigned& blocks, hipStream_t s) {
-    if (planes_layout(a.row_stride, a.class_stride)) {
-        if (a.k <= 8) {
-            if (!backward) {
-                if (planes_wide<T>(a.logits, a.class_stride, a.rows, 2))
-                    return a.k <= 4 ? distill_wide_fwd<T, 2, 4>(a, blocks, s) : distill_wide_fwd<T, 2, 8>(a, blocks, s);
-                return a.k <= 4 ? distill_wide_fwd<T, 1, 4>(a, blocks, s) : distill_wide_fwd<T, 1, 8>(a, blocks, s);
-            }
-            if (planes_wide<T>(a.logits, a.class_stride, a.rows, 4) && planes_wide<T>(a.grad, a.g_class, a.rows, 4))
-                return a.k <= 4 ? distill_wide_bwd<T, 4, 4>(a, s) : distill_wide_bwd<T, 4, 8>(a, s);
-            return a.k <= 4 ? distill_wide_bwd<T, 1, 4>(a, s) : distill_wide_bwd<T, 1, 8>(a, s);
+    if (planes_layout(a.row_stride, a.class_stride) && planes_by_pixel(a)) {
+        if (!backward) {
+            if (planes_wide<T>(a.logits, a.class_stride, a.rows, 2))
+                return a.k <= 4 ? distill_wide_fwd<T, 2, 4>(a, blocks, s) : distill_wide_fwd<T, 2, 8>(a, blocks, s);
+            return a.k <= 4 ? distill_wide_fwd<T, 1, 4>(a, blocks, s) : distill_wide_fwd<T, 1, 8>(a, blocks, s);
         }
-        const size_t lds = (size_t)a.classes * 64 * sizeof(float);
-        blocks = distill_blocks(a.rows, 64);
-        if (backward) distill_bwd_planes_kernel<T><<<dim3(blocks), dim3(64), lds, s>>>(a);
-        else distill_fwd_planes_kernel<T><<<dim3(blocks), dim3(64), lds, s>>>(a);
-        LAUNCH_OK("distill_planes_kernel");
-        return 0;
+        if (planes_wide<T>(a.logits, a.class_stride, a.rows, 4) && planes_wide<T>(a.grad, a.g_class, a.rows, 4))
+            return a.k <= 4 ? distill_wide_bwd<T, 4, 4>(a, s) : distill_wide_bwd<T, 4, 8>(a, s);
+        return a.k <= 4 ? distill_wide_bwd<T, 1, 4>(a, s) : distill_wide_bwd<T, 1, 8>(a, s);
     }
     if (const int tile = tile_rows(a, backward))
         return backward ? distill_tile<T, GRADIENT>(a, tile, blocks, s) : distill_tile<T, VALUE>(a, tile, blocks, s);
@@ -1118,19 +1043,19 @@ int distill_any(const DistillArgs& a, bool backward, unsigned& blocks, hipStream
     return distill_t<bf16_t>(a, backward, blocks, s);
 }
 
-// Value and gradient in one pass over the scores.  blocks = 0: no such kernel for these (the caller runs both passes):
-// planes, rows too long for the registers of a workgroup, short rows that do not lie one behind the other.
+// Value and gradient in one pass over the scores.  blocks = 0: no such kernel for these (the caller runs both passes): planes
+// pixel by pixel, rows too long for the registers of a workgroup, short rows that do not lie one behind the other.
 template <typename T>
 int distill_both_t(DistillArgs a, uint32_t* counts, unsigned& blocks, hipStream_t s) {
     constexpr int V = Wide<T>::N;
     blocks = 0;
-    if (planes_layout(a.row_stride, a.class_stride)) return 0;
+    if (planes_layout(a.row_stride, a.class_stride) && planes_by_pixel(a)) return 0;
     const int tile = tile_rows(a, true);
     const size_t packs = a.classes / V;
     if (!tile && (a.classes * sizeof(T) <= 4096 || packs > 16384 || !rows_wide<T>(a, true))) return 0;
     blocks = distill_blocks(a.rows, tile ? tile : 1);
-    if (a.reduction == 1 && blocks > 1) {
-        const size_t need = (a.rows * a.k + 255) / 256;
+    if (a.reduction == 1 && blocks > 1 && a.rows * a.k > 4096) {      // (fewer are counted by every workgroup for itself)
+        const size_t need = (a.rows * (a.i_entry == 1 ? a.k : 1) + 255) / 256;
         a.counts = counts;
         a.ncounts = (uint32_t)(need < COUNT_BLOCKS ? need : COUNT_BLOCKS);
         distill_count_kernel<<<dim3(a.ncounts), dim3(256), 0, s>>>(a, counts);
@@ -1166,8 +1091,9 @@ DistillArgs distill_args(size_t rows, size_t classes, size_t k, const void* logi
 }
 }  // namespace
 
-bool e3_distill_layout_ok(size_t rows, size_t classes, size_t row_stride, size_t class_stride) {
-    return class_stride == 1 || rows == 1 ? class_stride == 1 : row_stride == 1 && classes <= (size_t)DISTILL_PLANES;
+bool e3_distill_layout_ok(size_t rows, size_t classes, size_t k, size_t row_stride, size_t class_stride) {
+    if (class_stride == 1 || rows == 1) return class_stride == 1;
+    return row_stride == 1 && classes <= (size_t)DISTILL_PLANES && k <= (size_t)DISTILL_PLANES;
 }
 size_t e3_distill_scratch_bytes(size_t rows) {
     (void)rows;

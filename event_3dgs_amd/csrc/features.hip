@@ -759,10 +759,12 @@ struct Tile {
     T single;
     __device__ __forceinline__ void load(const T* __restrict__ src, int elems) {
         const int packs = (int)(elems * sizeof(T) / 16), rest = packs * (16 / (int)sizeof(T));
+        if (packs > 0) {                     // (uniform; the loads are unconditional and in flight together)
 #pragma unroll
-        for (int u = 0; u < NORM_TILE_PACKS; ++u) {
-            const int i = u * 256 + threadIdx.x;
-            if (i < packs) in[u] = reinterpret_cast<const words_t*>(src)[i];
+            for (int u = 0; u < NORM_TILE_PACKS; ++u) {
+                const int i = u * 256 + threadIdx.x;
+                in[u] = reinterpret_cast<const words_t*>(src)[i < packs ? i : packs - 1];
+            }
         }
         if (rest + (int)threadIdx.x < elems) single = src[rest + threadIdx.x];
     }
