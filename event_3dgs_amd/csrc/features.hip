@@ -19,33 +19,38 @@ int launch_radix_sort_pairs(uint32_t* k0, uint32_t* k1, uint32_t* v0, uint32_t* 
 // ============================================================================================== embedding, forward
 // out[i, :] = round(scale * table[index[i], :]).  An index below 0 stands for "no row" (zeros); one past the table gives a
 // row of NaN -- an error that only the device sees, made visible without a wait.
-// One thread moves EMBED_PACKS packs of the flat output, a workgroup's packs are contiguous: every lane works whatever the
-// row length, the stores are whole lines, and the rows of a pack-block are found by one division each.
-constexpr int EMBED_PACKS = 4;
+// One thread moves several packs of the flat output (4 of 16 bytes, 8 of 4 or 8, 16 single elements: a workgroup waits for the
+// index, then for the row, and has to have enough behind that), a workgroup's packs are contiguous: every lane works whatever
+// the row length, the stores are whole lines, and the rows of a pack-block are found by one division each.
+template <typename T, int V>
+struct EmbedPacks {
+    static constexpr int N = V * (int)sizeof(T) == 16 ? 4 : V > 1 ? 8 : 16;
+};
 template <bool STREAM, typename T, int V, typename I>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(size_t n, long long rows, uint32_t ppr /* packs per row */,
                                                         const I* __restrict__ index, const T* __restrict__ table, size_t stride, float scale,
                                                         T* __restrict__ out) {
-    const size_t total = n * (size_t)ppr, base = (size_t)blockIdx.x * (256 * EMBED_PACKS);
+    constexpr int PACKS = EmbedPacks<T, V>::N;
+    const size_t total = n * (size_t)ppr, base = (size_t)blockIdx.x * (256 * PACKS);
     const size_t row0 = base / ppr;                                  // (uniform)
     const uint32_t rem0 = (uint32_t)(base - row0 * ppr);
-    I id[EMBED_PACKS];
-    uint32_t col[EMBED_PACKS];
-    Pack<T, V> p[EMBED_PACKS];
+    I id[PACKS];
+    uint32_t col[PACKS];
+    Pack<T, V> p[PACKS];
 #pragma unroll
-    for (int u = 0; u < EMBED_PACKS; ++u) {
+    for (int u = 0; u < PACKS; ++u) {
         const uint32_t x = rem0 + (uint32_t)u * 256 + threadIdx.x, q = x / ppr;
         col[u] = x - q * ppr;
         const size_t row = row0 + q;
         id[u] = index[row < n ? row : n - 1];                        // (unconditional loads, all in flight)
     }
 #pragma unroll
-    for (int u = 0; u < EMBED_PACKS; ++u) {
+    for (int u = 0; u < PACKS; ++u) {
         if (id[u] >= 0 && id[u] < rows)
             p[u] = *reinterpret_cast<const Pack<T, V>*>(table + (size_t)id[u] * stride + (size_t)col[u] * V);
     }
 #pragma unroll
-    for (int u = 0; u < EMBED_PACKS; ++u) {
+    for (int u = 0; u < PACKS; ++u) {
         const size_t at = base + (size_t)u * 256 + threadIdx.x;
         if (at >= total) continue;
         Pack<T, V> r;
@@ -56,23 +61,27 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(size_t n, long long rows
     }
 }
 
+template <bool STREAM, typename T, int V, typename I>
+static int embed_fwd_launch(size_t n, size_t rows, size_t dim, const void* index, const void* table, size_t stride, float scale,
+                            void* out, hipStream_t s) {
+    const size_t ppr = dim / V, each = 256 * EmbedPacks<T, V>::N, blocks = (n * ppr + each - 1) / each;
+    if (blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_forward: too many values");
+    embed_fwd_kernel<STREAM, T, V, I><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(
+        n, (long long)rows, (uint32_t)ppr, (const I*)index, (const T*)table, stride, scale, (T*)out);
+    LAUNCH_OK("embed_fwd_kernel");
+    return 0;
+}
 template <typename T, typename I>
 static int embed_fwd_t(size_t n, size_t rows, size_t dim, const void* index, const void* table, size_t stride, int dtype,
                        float scale, void* out, hipStream_t s) {
-    const bool wide = e3_rows_wide(table, stride, dim, dtype) && e3_rows_wide(out, dim, dim, dtype);
-    const size_t ppr = wide ? dim / Wide<T>::N : dim;
-    const size_t blocks = (n * ppr + 256 * EMBED_PACKS - 1) / (256 * EMBED_PACKS);
-    if (blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_forward: too many values");
-#define E3_FWD(S, V)                                                                                                          \
-    embed_fwd_kernel<S, T, V, I><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(n, (long long)rows, (uint32_t)ppr,            \
-                                                                            (const I*)index, (const T*)table, stride, scale, \
-                                                                            (T*)out)
-    if (!wide) E3_FWD(false, 1);
-    else if (n * dim * sizeof(T) > E3_STREAM_BYTES) E3_FWD(true, Wide<T>::N);
-    else E3_FWD(false, Wide<T>::N);
-#undef E3_FWD
-    LAUNCH_OK("embed_fwd_kernel");
-    return 0;
+    constexpr int N = Wide<T>::N;
+    const bool large = n * dim * sizeof(T) > E3_STREAM_BYTES;
+    auto fits = [&](size_t bytes) { return e3_rows_packs(table, stride, dim, dtype, bytes) && e3_rows_packs(out, dim, dim, dtype, bytes); };
+    if (fits(16) && large) return embed_fwd_launch<true, T, N, I>(n, rows, dim, index, table, stride, scale, out, s);
+    if (fits(16)) return embed_fwd_launch<false, T, N, I>(n, rows, dim, index, table, stride, scale, out, s);
+    if (fits(8)) return embed_fwd_launch<false, T, N / 2, I>(n, rows, dim, index, table, stride, scale, out, s);
+    if (N == 8 && fits(4)) return embed_fwd_launch<false, T, N == 8 ? 2 : 1, I>(n, rows, dim, index, table, stride, scale, out, s);
+    return embed_fwd_launch<false, T, 1, I>(n, rows, dim, index, table, stride, scale, out, s);
 }
 
 int e3_embedding_forward_impl(size_t n, size_t rows, size_t dim, const void* index, int index_bytes, const void* table,
@@ -90,7 +99,7 @@ int e3_embedding_forward_impl(size_t n, size_t rows, size_t dim, const void* ind
 // into chunks of equal length, a group of lanes sums the rows of one chunk (times a slice of the columns), and
 //   * a run inside a chunk is finished there,
 //   * a run that crosses chunks leaves one fp32 partial row per chunk, which embed_join_kernel adds up in order,
-//   * a table row without a position is cleared by embed_zero_kernel.
+//   * a table row without a position is cleared by further workgroups of the same launch (embed_zero).
 // So a row that half of all positions share costs no more than rows with one position each.
 constexpr uint32_t EMBED_NONE = 0xFFFFFFFFu;
 
@@ -135,6 +144,24 @@ __device__ __forceinline__ void embed_zero(uint32_t n, const uint32_t* __restric
         empty = at >= n || keys[at] != row;
     }
     unsigned long long todo = __ballot(empty);
+    const uint32_t count = (uint32_t)__popcll(todo), mine = rows - first < per ? (uint32_t)(rows - first) : per;
+    if (V == 1 && count == mine) {
+        // none of the wave's rows is named (most waves of a large table): one stretch of memory, in 16-byte packs (with packs of
+        // 4 or 8 bytes row by row is the quicker way: 44064 rows of 84 bf16 14 us, as one stretch 17)
+        constexpr int N = Wide<T>::N;
+        T* p = d_table + first * dim;
+        const size_t total = (size_t)mine * dim;
+        size_t head = ((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T);
+        if (head > total) head = total;
+        const size_t packs = (total - head) / N, tail = head + packs * N;
+        Pack<T, N> z;
+#pragma unroll
+        for (int j = 0; j < N; ++j) z.v[j] = (T)0.0f;
+        for (size_t i = lane; i < packs; i += 64) put<STREAM, T, N>(p + head + i * N, z);
+        if ((size_t)lane < head) p[lane] = (T)0.0f;
+        if (tail + lane < total) p[tail + lane] = (T)0.0f;
+        return;
+    }
     Pack<T, V> z;
 #pragma unroll
     for (int j = 0; j < V; ++j) z.v[j] = (T)0.0f;
@@ -146,59 +173,107 @@ __device__ __forceinline__ void embed_zero(uint32_t n, const uint32_t* __restric
     }
 }
 
-// Up to EMBED_TINY positions: every workgroup of the sums sorts them for itself (the rank of a position is the number of smaller
-// indices, and of equal ones before it, counted in LDS), which is quicker than a launch that does it for all.  Indices outside
-// the table are left out.  Returns their number; keys and positions are in LDS.
+// Up to EMBED_TINY positions go in one launch: a workgroup per run (times a slice of the columns), each of which sorts the
+// positions for itself (the rank of a position is the number of smaller indices, and of equal ones before it, counted in LDS:
+// quicker than a launch that does it for all), and further workgroups that clear the rows without a position.  The groups of
+// a workgroup share its run, their sums are added in order.  (132 positions, 9 rows of 1187 fp16: 9 us; one group of lanes to a
+// slice for all runs took 17.)
 constexpr uint32_t EMBED_TINY = 256;
 struct TinySort {
-    uint32_t raw[EMBED_TINY], key[EMBED_TINY], pos[EMBED_TINY], kept;
+    uint32_t raw[EMBED_TINY], key[EMBED_TINY], pos[EMBED_TINY], start[EMBED_TINY + 1], kept, runs;
 };
-__device__ __forceinline__ uint32_t embed_sort_tiny(TinySort& L, uint32_t n, uint32_t rows, const void* __restrict__ index,
-                                                    int index_bytes) {
+__device__ __forceinline__ void embed_sort_tiny(TinySort& L, uint32_t n, uint32_t rows, const void* __restrict__ index,
+                                                int index_bytes) {
     const uint32_t i = threadIdx.x;
     const unsigned long long id = i < n ? (unsigned long long)load_index_flat(index, i, index_bytes) : ~0ull;
     const uint32_t k = id < rows ? (uint32_t)id : EMBED_NONE;
     L.raw[i] = k;
-    if (i == 0) L.kept = 0;
+    if (i == 0) L.kept = L.runs = 0;
     __syncthreads();
     const unsigned long long ok = __ballot(k != EMBED_NONE);
     if ((i & 63) == 0) atomicAdd(&L.kept, (uint32_t)__popcll(ok));
-    uint32_t rank = 0;
+    uint32_t rank = 0, before = 0;                         // `before`: equal indices before this one
     for (uint32_t j = 0; j < n; j += 4) {
         const uint4 q = *reinterpret_cast<const uint4*>(L.raw + j);      // (behind the last one: EMBED_NONE, not smaller)
-        rank += (q.x < k || (q.x == k && j < i)) + (q.y < k || (q.y == k && j + 1 < i)) + (q.z < k || (q.z == k && j + 2 < i)) +
-                (q.w < k || (q.w == k && j + 3 < i));
+        rank += (q.x < k) + (q.y < k) + (q.z < k) + (q.w < k);
+        before += (q.x == k && j < i) + (q.y == k && j + 1 < i) + (q.z == k && j + 2 < i) + (q.w == k && j + 3 < i);
     }
     if (k != EMBED_NONE) {
-        L.key[rank] = k;
-        L.pos[rank] = i;
+        L.key[rank + before] = k;
+        L.pos[rank + before] = i;
     }
     __syncthreads();
-    return L.kept;
+    // the first position of each run, in order
+    const bool first = i < L.kept && (i == 0 || L.key[i] != L.key[i - 1]);
+    const unsigned long long firsts = __ballot(first);
+    if ((i & 63) == 0) L.raw[i >> 6] = (uint32_t)__popcll(firsts);
+    __syncthreads();
+    uint32_t at = (uint32_t)__popcll(firsts & ((1ull << (i & 63)) - 1ull));
+    for (uint32_t w = 0; w < i >> 6; ++w) at += L.raw[w];
+    if (first) L.start[at] = i;
+    if (i == EMBED_TINY - 1) {
+        L.runs = at + (first ? 1u : 0u);
+        L.start[L.runs] = L.kept;
+    }
+    __syncthreads();
+}
+template <typename T, int V, int G>
+__global__ __launch_bounds__(256) void embed_tiny_kernel(uint32_t n, uint32_t rows, const void* __restrict__ index, int index_bytes,
+                                                         uint32_t nslices, size_t dim, const T* __restrict__ d_out, size_t stride,
+                                                         float scale, T* __restrict__ d_table, uint32_t sum_blocks, uint32_t zero_rows) {
+    __shared__ __attribute__((aligned(16))) TinySort L;
+    __shared__ float sums[256 * V];
+    embed_sort_tiny(L, n, rows, index, index_bytes);
+    if (blockIdx.x >= sum_blocks) {
+        const size_t wave = (size_t)(blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6);
+        if ((size_t)rows * dim * sizeof(T) > E3_STREAM_BYTES) embed_zero<true, T, V>(L.kept, L.key, rows, zero_rows, dim, d_table, wave);
+        else embed_zero<false, T, V>(L.kept, L.key, rows, zero_rows, dim, d_table, wave);
+        return;
+    }
+    constexpr int GROUPS = 256 / G, UNROLL = 8;
+    const uint32_t run = blockIdx.x / nslices, slice = blockIdx.x - run * nslices;
+    if (run >= L.runs) return;                                          // (uniform)
+    const int g = threadIdx.x / G, lane = threadIdx.x % G;
+    const size_t col = ((size_t)slice * G + lane) * V;
+    const uint32_t j0 = L.start[run], m = L.start[run + 1] - j0;
+    const uint32_t lo = j0 + m * g / GROUPS, hi = j0 + m * (g + 1) / GROUPS;
+    float acc[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = 0.0f;
+    for (uint32_t b = lo; b < hi && col < dim; b += UNROLL) {
+        Pack<T, V> r[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+            r[u] = *reinterpret_cast<const Pack<T, V>*>(d_out + (size_t)L.pos[b + u < hi ? b + u : hi - 1] * stride + col);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            if (b + u >= hi) break;
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] += (float)r[u].v[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) sums[threadIdx.x * V + j] = acc[j];
+    __syncthreads();
+    if (g != 0 || col >= dim) return;
+    for (int k = 1; k < GROUPS; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] += sums[(k * G + lane) * V + j];
+    embed_store<T, V>(d_table, dim, L.key[j0], col, scale, acc);
 }
 
 constexpr int EMBED_UNROLL = 8;
-template <bool TINY, typename T, int V, int G>
-__global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restrict__ kept, const uint32_t* keys,
-                                                        const uint32_t* pos, uint32_t chunk, uint32_t nchunks,
+template <typename T, int V, int G>
+__global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restrict__ kept, const uint32_t* __restrict__ keys,
+                                                        const uint32_t* __restrict__ pos, uint32_t chunk, uint32_t nchunks,
                                                         uint32_t nslices, size_t dim, const T* __restrict__ d_out,
                                                         size_t stride, float scale, T* __restrict__ d_table,
                                                         float* __restrict__ part, uint32_t sum_blocks, uint32_t rows,
-                                                        uint32_t zero_rows, uint32_t tiny_n, const void* __restrict__ index,
-                                                        int index_bytes) {
-    __shared__ __attribute__((aligned(16))) char tiny_mem[TINY ? sizeof(TinySort) : 4];
-    uint32_t n;
-    if (TINY) {
-        TinySort& L = *reinterpret_cast<TinySort*>(tiny_mem);
-        n = embed_sort_tiny(L, tiny_n, rows, index, index_bytes);
-        keys = L.key;
-        pos = L.pos;
-    } else {
-        n = *kept;
-    }
+                                                        uint32_t zero_rows) {
+    const uint32_t n = *kept;
     if (blockIdx.x >= sum_blocks) {      // (in the same launch: the sums wait for their gathers, the stores do not)
         const size_t wave = (size_t)(blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6);
-        if (V > 1 && (size_t)rows * dim * sizeof(T) > E3_STREAM_BYTES) embed_zero<true, T, V>(n, keys, rows, zero_rows, dim, d_table, wave);
+        if ((size_t)rows * dim * sizeof(T) > E3_STREAM_BYTES) embed_zero<true, T, V>(n, keys, rows, zero_rows, dim, d_table, wave);
         else embed_zero<false, T, V>(n, keys, rows, zero_rows, dim, d_table, wave);
         return;
     }
@@ -253,10 +328,10 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restri
 // Adds up the partials of the runs that cross chunks: slot 1 of the chunk a run starts in, slot 0 of the following ones.
 // Workgroups of two kinds in one launch:
 //   short runs   a group of 16 lanes takes a chunk (times a slice of 16 V columns) and adds up to JOIN_SHORT partials in order
-//   long runs    a workgroup looks at JOIN_SHORT neighbouring chunks (times a slice of JOIN_COLS columns): only the last run
-//                that starts among them can be longer than JOIN_SHORT partials; 64 groups of 16 lanes take a 64th of them
-//                each, the 64 sums are added in order
-constexpr uint32_t JOIN_SHORT = 32, JOIN_COLS = 64;
+//   long runs    a workgroup looks at JOIN_SHORT neighbouring chunks (times a slice of the columns, 16 at a time): only the
+//                last run that starts among them can be longer than JOIN_SHORT partials; 64 groups of 16 lanes take a 64th
+//                of them each, the 64 sums are added eight by eight
+constexpr uint32_t JOIN_SHORT = 32;
 // Whether a run starts in chunk c and goes on behind it; its key.
 __device__ __forceinline__ bool embed_crossing(const uint32_t* __restrict__ keys, uint32_t n, uint32_t chunk, uint32_t c,
                                                uint32_t& key) {
@@ -272,7 +347,7 @@ __device__ __forceinline__ bool embed_in_run(const uint32_t* __restrict__ keys, 
 template <typename T, int V>
 __global__ __launch_bounds__(1024) void embed_join_kernel(const uint32_t* __restrict__ kept,
                                                           const uint32_t* __restrict__ keys, uint32_t chunk,
-                                                          uint32_t nchunks, uint32_t short_blocks, size_t dim,
+                                                          uint32_t nchunks, uint32_t short_blocks, uint32_t cols, size_t dim,
                                                           const float* __restrict__ part, float scale,
                                                           T* __restrict__ d_table) {
     __shared__ float sums[64][17];
@@ -308,7 +383,7 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(const uint32_t* __rest
         embed_store<T, V>(d_table, dim, key, col, scale, acc);
         return;
     }
-    const uint32_t nparts = (uint32_t)((dim + JOIN_COLS - 1) / JOIN_COLS), unit = blockIdx.x - short_blocks;
+    const uint32_t nparts = (uint32_t)((dim + cols - 1) / cols), unit = blockIdx.x - short_blocks;
     const uint32_t first = unit / nparts * JOIN_SHORT;
     if (threadIdx.x < 64) {
         const uint32_t c = first + threadIdx.x;
@@ -325,9 +400,19 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(const uint32_t* __rest
     __syncthreads();
     const uint32_t c = long_chunk;
     if (c == 0xFFFFFFFFu) return;                                              // (uniform)
-    const uint32_t m = (lower_bound_u32(keys, c * chunk + chunk, n, long_key + 1u) - 1u) / chunk - c + 1u;
+    // partials: chunks from c on that belong to the run, the last one found by 64 probes at a time
+    uint32_t in = c + JOIN_SHORT, out = nchunks;                               // `in` begins with the key, `out` does not
+    while (out - in > 1) {
+        const uint32_t step = (out - in - 1) / 64 + 1, at = in + 1 + (threadIdx.x & 63) * step;
+        const unsigned long long hit = __ballot(at < out && embed_in_run(keys, n, chunk, at, long_key));
+        const uint32_t k = (uint32_t)__popcll(hit);                            // (the run is contiguous: the first k probes)
+        const uint32_t low = k ? in + 1 + (k - 1) * step : in, high = in + 1 + k * step;
+        out = high < out && k < 64 ? high : out;
+        in = low;
+    }
+    const uint32_t m = in - c + 1u;
     const uint32_t lo = (uint32_t)((unsigned long long)m * g / 64), hi = (uint32_t)((unsigned long long)m * (g + 1) / 64);
-    const size_t col0 = (size_t)(unit % nparts) * JOIN_COLS, col1 = col0 + JOIN_COLS < dim ? col0 + JOIN_COLS : dim;
+    const size_t col0 = (size_t)(unit % nparts) * cols, col1 = col0 + cols < dim ? col0 + cols : dim;
     for (size_t col = col0 + lane; col < col1 + lane; col += 16) {             // (every lane takes part in the barriers)
         float s = 0.0f;
         if (col < col1) {
@@ -336,9 +421,17 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(const uint32_t* __rest
         }
         sums[g][lane] = s;
         __syncthreads();
+        if (g < 8) {
+            s = sums[8 * g][lane];
+#pragma unroll
+            for (int w = 1; w < 8; ++w) s += sums[8 * g + w][lane];
+        }
+        __syncthreads();
+        if (g < 8) sums[g][lane] = s;
+        __syncthreads();
         if (g == 0 && col < col1) {
-            s = sums[0][lane];
-            for (int w = 1; w < 64; ++w) s += sums[w][lane];
+#pragma unroll
+            for (int w = 1; w < 8; ++w) s += sums[w][lane];
             d_table[(size_t)long_key * dim + col] = (T)(scale * s);
         }
         __syncthreads();
@@ -454,7 +547,6 @@ struct EmbedScratch {
     static uint32_t chunk(size_t n, size_t dim) {
         // Rows of a chunk: 128 where there is plenty of work, fewer where the groups would otherwise not fill the chip (each
         // group moves `chunk` row slices of at most 1 KB).
-        if (n <= EMBED_TINY) return EMBED_TINY;                // (one chunk: nothing to join)
         uint32_t c = 128;
         while (c > 8 && (n / c) * ((dim + 511) / 512) < 4096) c >>= 1;
         return c;
@@ -478,20 +570,25 @@ template <typename T, int V, int G>
 int embed_sum_launch(const EmbedScratch& w, const uint32_t* keys, const uint32_t* pos, size_t n, size_t rows, size_t dim,
                      const void* d_out, size_t stride, float scale, void* d_table, const void* index, int index_bytes,
                      hipStream_t s) {
-    const uint32_t chunk = EmbedScratch::chunk(n, dim), nchunks = EmbedScratch::chunks(n, dim);
-    const size_t nslices = (dim + (size_t)G * V - 1) / ((size_t)G * V), units = nslices * nchunks;
-    const size_t blocks = (units + 256 / G - 1) / (256 / G);
+    const size_t nslices = (dim + (size_t)G * V - 1) / ((size_t)G * V);
     size_t per = 16384 / (dim * sizeof(T));                    // about 16 KB of table rows to a wave that clears them
     per = per < 1 ? 1 : (per > 64 ? 64 : per);
     const size_t zero_blocks = (rows + 4 * per - 1) / (4 * per);
+    if (n <= EMBED_TINY) {
+        const size_t most = n < rows ? n : rows, blocks = most * nslices;
+        if (blocks + zero_blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
+        embed_tiny_kernel<T, V, G><<<dim3((unsigned)(blocks + zero_blocks)), dim3(256), 0, s>>>(
+            (uint32_t)n, (uint32_t)rows, index, index_bytes, (uint32_t)nslices, dim, (const T*)d_out, stride, scale, (T*)d_table,
+            (uint32_t)blocks, (uint32_t)per);
+        LAUNCH_OK("embed_tiny_kernel");
+        return 0;
+    }
+    const uint32_t chunk = EmbedScratch::chunk(n, dim), nchunks = EmbedScratch::chunks(n, dim);
+    const size_t units = nslices * nchunks, blocks = (units + 256 / G - 1) / (256 / G);
     if (blocks + zero_blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
-#define E3_SUM_LAUNCH(TINY)                                                                                                   \
-    embed_sum_kernel<TINY, T, V, G><<<dim3((unsigned)(blocks + zero_blocks)), dim3(256), 0, s>>>(                             \
-        w.kept, keys, pos, chunk, nchunks, (uint32_t)nslices, dim, (const T*)d_out, stride, scale, (T*)d_table, w.part,       \
-        (uint32_t)blocks, (uint32_t)rows, (uint32_t)per, (uint32_t)n, index, index_bytes)
-    if (n <= EMBED_TINY) E3_SUM_LAUNCH(true);
-    else E3_SUM_LAUNCH(false);
-#undef E3_SUM_LAUNCH
+    embed_sum_kernel<T, V, G><<<dim3((unsigned)(blocks + zero_blocks)), dim3(256), 0, s>>>(
+        w.kept, keys, pos, chunk, nchunks, (uint32_t)nslices, dim, (const T*)d_out, stride, scale, (T*)d_table, w.part,
+        (uint32_t)blocks, (uint32_t)rows, (uint32_t)per);
     LAUNCH_OK("embed_sum_kernel");
     return 0;
 }
@@ -501,10 +598,13 @@ int embed_join_launch(const EmbedScratch& w, const uint32_t* keys, size_t n, siz
     const uint32_t chunk = EmbedScratch::chunk(n, dim), nchunks = EmbedScratch::chunks(n, dim);
     if (nchunks <= 1) return 0;
     const size_t shorts = ((size_t)nchunks * ((dim + 16 * V - 1) / (16 * V)) + 63) / 64;
-    const size_t longs = nchunks > JOIN_SHORT ? (size_t)((nchunks + JOIN_SHORT - 1) / JOIN_SHORT) * ((dim + JOIN_COLS - 1) / JOIN_COLS) : 0;
+    // (columns of a workgroup of the second kind: 16 as long as that is not far more workgroups than the chip holds, most of
+    // which find no long run: 5539 positions, 12 rows of 289 bf16 5.6 us, with 64 columns 14.4)
+    const size_t groups = nchunks > JOIN_SHORT ? (nchunks + JOIN_SHORT - 1) / JOIN_SHORT : 0;
+    const size_t cols = groups * ((dim + 15) / 16) <= 2048 ? 16 : 64, longs = groups * ((dim + cols - 1) / cols);
     if (shorts + longs > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
     embed_join_kernel<T, V><<<dim3((unsigned)(shorts + longs)), dim3(1024), 0, s>>>(w.kept, keys, chunk, nchunks, (uint32_t)shorts,
-                                                                                  dim, w.part, scale, (T*)d_table);
+                                                                                  (uint32_t)cols, dim, w.part, scale, (T*)d_table);
     LAUNCH_OK("embed_join_kernel");
     return 0;
 }
@@ -524,14 +624,13 @@ int embed_bwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_
     EmbedScratch w = EmbedScratch::from(scratch, n, dim);
     uint32_t *keys = w.key0, *pos = w.pos0;
     int rc = 0;
-    if (n <= EMBED_TINY) {                                      // (sorted by the workgroups of the sums)
-    } else if (n <= 16384) {
+    if (n > EMBED_TINY && n <= 16384) {
         int nbits = 1;
         while (rows >> nbits) ++nbits;                         // (the key `rows` itself occurs)
         if (index_bytes == 8) embed_sort_small((uint32_t)n, (uint32_t)rows, nbits, (const long long*)index, keys, pos, w.kept, s);
         else embed_sort_small((uint32_t)n, (uint32_t)rows, nbits, (const int*)index, keys, pos, w.kept, s);
         LAUNCH_OK("embed_sort_small_kernel");
-    } else {
+    } else if (n > EMBED_TINY) {
         embed_keys_kernel<<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s>>>(n, rows, index, index_bytes, w.key0);
         LAUNCH_OK("embed_keys_kernel");
         int nbits = 1;
@@ -540,23 +639,29 @@ int embed_bwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_
                                      nullptr, 0, nullptr, nullptr);
         if (rc) return rc;
     }
-    const bool wide = e3_rows_wide(d_out, stride, dim, dtype) && e3_rows_wide(d_table, dim, dim, dtype);
-    const size_t packs = wide ? dim / Wide<T>::N : dim;
-    constexpr int N = Wide<T>::N;
+    auto fits = [&](size_t bytes) { return e3_rows_packs(d_out, stride, dim, dtype, bytes) && e3_rows_packs(d_table, dim, dim, dtype, bytes); };
+    constexpr int N = Wide<T>::N, HALF = N / 2, QUARTER = N == 8 ? 2 : 1;
 #define E3_SUM(V, G) rc = embed_sum_launch<T, V, G>(w, keys, pos, n, rows, dim, d_out, stride, scale, d_table, index, index_bytes, s)
-    if (wide) {
+    if (fits(16)) {
+        const size_t packs = dim / N;
         if (packs <= 4) E3_SUM(N, 4);
         else if (packs <= 8) E3_SUM(N, 8);
         else if (packs <= 16) E3_SUM(N, 16);
         else if (packs <= 32) E3_SUM(N, 32);
         else E3_SUM(N, 64);
+    } else if (fits(8)) {
+        if (dim / HALF <= 16) E3_SUM(HALF, 16);
+        else E3_SUM(HALF, 64);
+    } else if (N == 8 && fits(4)) {
+        if (dim / QUARTER <= 16) E3_SUM(QUARTER, 16);
+        else E3_SUM(QUARTER, 64);
     } else {
-        if (packs <= 4) E3_SUM(1, 4);
-        else if (packs <= 16) E3_SUM(1, 16);
+        if (dim <= 4) E3_SUM(1, 4);
+        else if (dim <= 16) E3_SUM(1, 16);
         else E3_SUM(1, 64);
     }
 #undef E3_SUM
-    if (rc) return rc;
+    if (rc || n <= EMBED_TINY) return rc;
     // (partial rows start on 16-byte boundaries where dim is a multiple of 4)
     return dim % 4 == 0 && e3_rows_wide(d_table, dim, dim, dtype) ? embed_join_launch<T, 4>(w, keys, n, dim, scale, d_table, s)
                                                                  : embed_join_launch<T, 1>(w, keys, n, dim, scale, d_table, s);

@@ -60,10 +60,13 @@ __device__ __forceinline__ void put(T* p, const Pack<T, V>& r) {
 static inline size_t e3_elem_bytes(int dtype) { return dtype == E3_F32 ? 4 : 2; }
 static inline bool e3_dtype_ok(int dtype) { return dtype >= E3_F32 && dtype <= E3_BF16; }
 
-// Whether rows at `p`, `stride` elements apart and `dim` long, can be read as 16-byte packs.
+// Whether rows at `p`, `stride` elements apart and `dim` long, can be read as packs of `bytes` bytes (a power of two).
+static inline bool e3_rows_packs(const void* p, size_t stride, size_t dim, int dtype, size_t bytes) {
+    const size_t n = bytes / e3_elem_bytes(dtype);
+    return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0 && stride % n == 0 && dim % n == 0;
+}
 static inline bool e3_rows_wide(const void* p, size_t stride, size_t dim, int dtype) {
-    const size_t b = e3_elem_bytes(dtype), n = 16 / b;
-    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % n == 0 && dim % n == 0;
+    return e3_rows_packs(p, stride, dim, dtype, 16);
 }
 
 // One element of an array whose type is a launch argument (uniform branch): parameters and labels, which are read once per

@@ -72,6 +72,13 @@ def test_embedding(dtype, n, rows, dim, skew):
     check_embedding(tokens(n, rows, skew=skew, empty=0.1), rand(rows, dim).to(dtype), 1.75, rand(n, dim, seed=1).to(dtype))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [2, 6, 12, 20, 66, 132, 1186])
+@pytest.mark.parametrize("n, rows", [(130, 1), (256, 9), (255, 3001), (257, 2), (2900, 5)])
+def test_embedding_rows_of_four_and_eight_bytes(dtype, dim, n, rows):
+    check_embedding(tokens(n, rows, skew=2, empty=0.05), rand(rows, dim).to(dtype), 1.0, rand(n, dim, seed=1).to(dtype))
+
+
 @pytest.mark.parametrize("rows, dim", [(1, 48), (1, 1), (257, 256), (1, 2052)])
 def test_embedding_one_row_for_all(rows, dim):
     n = 30011
