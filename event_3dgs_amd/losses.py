@@ -317,9 +317,10 @@ def distill_loss(logits, teacher_logits, teacher_index, temperature=1.0, reducti
     (class_dim=0 of (classes, H, W), read as they lie up to 256 classes).  An entry counts when its index is >= 0 and its
     score above -inf; a row without one is unlabelled: it adds 0, its gradient is 0, the mean leaves it out (a mean over no
     row is 0).  A class may be listed twice (its weights add up); an index past the classes makes the row NaN.  Logits of
-    -inf or the type's lowest value switch a class off.
+    -inf or the type's lowest value switch a class off.  `temperature` lies between 1e-6 and 1e6, k is at most 1024.
 
-    Returns fp32: a scalar ('mean', 'sum') or one value per row ('none').  The gradient goes to `logits` only."""
+    Returns fp32: a scalar ('mean', 'sum') or one value per row ('none').  The gradient goes to `logits` only
+    (a teacher that requires a gradient is refused: detach it)."""
     from .features import _ext
     return _ext().distill(logits, teacher_logits, teacher_index, float(temperature), _reduction(reduction), int(class_dim))
 

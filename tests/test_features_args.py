@@ -82,3 +82,15 @@ def test_distill_gradient_layout(hip_lib):
     assert "layout" in text()
     assert hip_lib.e3dgs_distill_forward(*head, PTR, PTR, None, None, 0, 0, PTR, None) != 0
     assert "null pointer" in text()
+
+
+def test_workspaces_off_their_boundary(hip_lib):
+    off = C.c_void_p(4096 + 4)
+    assert hip_lib.e3dgs_layer_norm_backward(3, 4, PTR, 4, PTR, 4, 0, PTR, 0, PTR, PTR, PTR, PTR, PTR, off, None) != 0
+    assert "16-byte aligned" in text()
+    head = (5, 9, 2, PTR, 9, 1, 0, PTR, 2, 1, 0, PTR, 2, 1, 4, 1.0, 1)
+    for stats, scratch in ((off, PTR), (PTR, off)):
+        assert hip_lib.e3dgs_distill_forward(*head, stats, PTR, PTR, None, 0, 0, scratch, None) != 0
+        assert "8-byte aligned" in text()
+    assert hip_lib.e3dgs_distill_backward(*head, off, PTR, PTR, 9, 1, None) != 0
+    assert "8-byte aligned" in text()

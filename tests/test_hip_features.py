@@ -704,3 +704,48 @@ def test_large_results_are_streamed():
     mag = torch.zeros(500, 64, dtype=torch.float64, device=DEV).index_add_(0, index[:5000], rand(5000, 64).double().abs())
     close(g[:500], keep, half_step(keep, torch.float32) * 1.01 + (count + 2) * U * mag)
     assert g[500:].count_nonzero() == 0
+
+
+@pytest.mark.parametrize("classes, k", [(300, 3), (40, 257), (300, 1024)])
+def test_distill_planes_past_their_limits(classes, k):
+    """More than 256 classes or entries in planes: the scores are laid out as rows, the gradient comes back as planes."""
+    g = torch.Generator().manual_seed(classes + k)
+    index = torch.randint(-1, classes, (k, 5, 6), generator=g).to(DEV)
+    check_distill(rand(classes, 5, 6) * 2, rand(k, 5, 6), index, 1.0, 0)
+    leaf = rand(classes, 5, 6).requires_grad_(True)
+    (d,) = torch.autograd.grad(losses.distill_loss(leaf, rand(k, 5, 6), index, class_dim=0), leaf)
+    assert d.shape == leaf.shape
+
+
+def test_captured_and_replayed_at_size():
+    """As many positions as take the general sort, rows of an odd length, a mean that is counted in a launch of its own."""
+    n, rows, dim = 20000, 900, 33
+
+    def inputs(seed):
+        t, ids = label(n, dim, 5, seed)
+        return [tokens(n, rows, seed, 2.0, 0.05), rand(rows, dim, seed=seed), rand(dim, seed=seed), rand(dim, seed=seed + 1), t, ids]
+
+    def step(index, table, w, b, t, ids):
+        p = [x.detach().requires_grad_(True) for x in (table, w, b)]
+        z = features.layer_norm(features.embedding(index, p[0], 2.0), p[1], p[2])
+        value, d = losses.distill_loss_raw(z, t, ids, 2.0)
+        return [value, *torch.autograd.grad(z, p, d)]
+
+    sets = [inputs(k) for k in range(3)]
+    want = [step(*v) for v in sets]
+    held = [x.clone() for x in sets[0]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*held)
+    for k in (1, 2, 0, 2, 1):
+        for a, b in zip(held, sets[k]):
+            a.copy_(b)
+        graph.replay()
+        step(*sets[(k + 1) % 3])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[k])), k
