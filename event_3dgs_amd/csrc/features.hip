@@ -34,30 +34,40 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(size_t n, long long rows
     const size_t total = n * (size_t)ppr, base = (size_t)blockIdx.x * (256 * PACKS);
     const size_t row0 = base / ppr;                                  // (uniform)
     const uint32_t rem0 = (uint32_t)(base - row0 * ppr);
+    const uint32_t last = n - 1 - row0 < 0x7FFFFFFFu ? (uint32_t)(n - 1 - row0) : 0x7FFFFFFFu;
+    const uint32_t count = total - base < 256 * PACKS ? (uint32_t)(total - base) : 256 * PACKS;
+    index += row0;
+    out += base * V;
+    const uint32_t dq = 256 / ppr, dr = 256 - dq * ppr;              // one pack on to the next: one division for all
+    uint32_t q = (rem0 + threadIdx.x) / ppr, c = rem0 + threadIdx.x - q * ppr;
     I id[PACKS];
     uint32_t col[PACKS];
     Pack<T, V> p[PACKS];
 #pragma unroll
     for (int u = 0; u < PACKS; ++u) {
-        const uint32_t x = rem0 + (uint32_t)u * 256 + threadIdx.x, q = x / ppr;
-        col[u] = x - q * ppr;
-        const size_t row = row0 + q;
-        id[u] = index[row < n ? row : n - 1];                        // (unconditional loads, all in flight)
+        col[u] = c;
+        id[u] = index[q < last ? q : last];                          // (unconditional loads, all in flight)
+        q += dq;
+        c += dr;
+        if (c >= ppr) {
+            c -= ppr;
+            ++q;
+        }
     }
 #pragma unroll
     for (int u = 0; u < PACKS; ++u) {
         if (id[u] >= 0 && id[u] < rows)
-            p[u] = *reinterpret_cast<const Pack<T, V>*>(table + (size_t)id[u] * stride + (size_t)col[u] * V);
+            p[u] = *reinterpret_cast<const Pack<T, V>*>(table + (size_t)(uint32_t)id[u] * stride + (size_t)col[u] * V);
     }
 #pragma unroll
     for (int u = 0; u < PACKS; ++u) {
-        const size_t at = base + (size_t)u * 256 + threadIdx.x;
-        if (at >= total) continue;
+        const uint32_t at = (uint32_t)u * 256 + threadIdx.x;
+        if (at >= count) continue;
         Pack<T, V> r;
 #pragma unroll
         for (int j = 0; j < V; ++j)
             r.v[j] = id[u] < 0 ? (T)0.0f : (id[u] < rows ? (T)(scale * (float)p[u].v[j]) : (T)__builtin_nanf(""));
-        put<STREAM, T, V>(out + at * V, r);
+        put<STREAM, T, V>(out + (size_t)at * V, r);
     }
 }
 
@@ -130,20 +140,12 @@ __device__ __forceinline__ void embed_store(T* __restrict__ d_table, size_t dim,
     *reinterpret_cast<Pack<T, V>*>(d_table + (size_t)row * dim + col) = r;
 }
 
-// Clears the table rows without a position: a wave looks `per` rows up in the sorted keys (one lane each) and clears those
-// that are not there.
+// Clears table rows: a wave takes `per` rows from `first` on, each of its lanes knows whether one of them is to be cleared.
 template <bool STREAM, typename T, int V>
-__device__ __forceinline__ void embed_zero(uint32_t n, const uint32_t* __restrict__ keys, uint32_t rows, uint32_t per,
-                                           size_t dim, T* __restrict__ d_table, size_t wave) {
+__device__ __forceinline__ void embed_zero(bool empty, size_t first, uint32_t rows, uint32_t per, size_t dim, T* __restrict__ d_table) {
     const int lane = threadIdx.x & 63;
-    const size_t first = wave * per;
-    if (first >= rows) return;
-    bool empty = false;
-    if ((uint32_t)lane < per && first + lane < rows) {
-        const uint32_t row = (uint32_t)(first + lane), at = lower_bound_u32(keys, 0, n, row);
-        empty = at >= n || keys[at] != row;
-    }
     unsigned long long todo = __ballot(empty);
+    if (todo == 0ull) return;
     const uint32_t count = (uint32_t)__popcll(todo), mine = rows - first < per ? (uint32_t)(rows - first) : per;
     if (V == 1 && count == mine) {
         // none of the wave's rows is named (most waves of a large table): one stretch of memory, in 16-byte packs (with packs of
@@ -165,6 +167,21 @@ __device__ __forceinline__ void embed_zero(uint32_t n, const uint32_t* __restric
     Pack<T, V> z;
 #pragma unroll
     for (int j = 0; j < V; ++j) z.v[j] = (T)0.0f;
+    if (dim < 64 * V) {                                    // short rows: a lane walks over the packs of all of them
+        const uint32_t ppr = (uint32_t)(dim / V), dq = 64 / ppr, dr = 64 - dq * ppr;
+        uint32_t r = (uint32_t)lane / ppr, c = (uint32_t)lane - r * ppr;
+        T* p = d_table + first * dim;
+        for (size_t i = lane; r < mine; i += 64) {
+            if (todo >> r & 1ull) put<STREAM, T, V>(p + i * V, z);
+            r += dq;
+            c += dr;
+            if (c >= ppr) {
+                c -= ppr;
+                ++r;
+            }
+        }
+        return;
+    }
     while (todo) {
         const int r = __builtin_ctzll(todo);
         todo &= todo - 1;
@@ -173,70 +190,64 @@ __device__ __forceinline__ void embed_zero(uint32_t n, const uint32_t* __restric
     }
 }
 
-// Up to EMBED_TINY positions go in one launch: a workgroup per run (times a slice of the columns), each of which sorts the
-// positions for itself (the rank of a position is the number of smaller indices, and of equal ones before it, counted in LDS:
-// quicker than a launch that does it for all), and further workgroups that clear the rows without a position.  The groups of
-// a workgroup share its run, their sums are added in order.  (132 positions, 9 rows of 1187 fp16: 9 us; one group of lanes to a
-// slice for all runs took 17.)
+// Up to EMBED_TINY positions go in one launch and without a sort.  A workgroup stands for a position (times a slice of the
+// columns): it lists the positions with the same index, in order, and sums their rows when its own is the first of them.  The
+// groups of a workgroup share the list, their sums are added in order.  Further workgroups clear the rows that no position
+// names.  (191 positions, 1580 rows of 802 fp32: 5 us; with a sort in every workgroup 18.)
 constexpr uint32_t EMBED_TINY = 256;
-struct TinySort {
-    uint32_t raw[EMBED_TINY], key[EMBED_TINY], pos[EMBED_TINY], start[EMBED_TINY + 1], kept, runs;
-};
-__device__ __forceinline__ void embed_sort_tiny(TinySort& L, uint32_t n, uint32_t rows, const void* __restrict__ index,
-                                                int index_bytes) {
-    const uint32_t i = threadIdx.x;
-    const unsigned long long id = i < n ? (unsigned long long)load_index_flat(index, i, index_bytes) : ~0ull;
-    const uint32_t k = id < rows ? (uint32_t)id : EMBED_NONE;
-    L.raw[i] = k;
-    if (i == 0) L.kept = L.runs = 0;
-    __syncthreads();
-    const unsigned long long ok = __ballot(k != EMBED_NONE);
-    if ((i & 63) == 0) atomicAdd(&L.kept, (uint32_t)__popcll(ok));
-    uint32_t rank = 0, before = 0;                         // `before`: equal indices before this one
-    for (uint32_t j = 0; j < n; j += 4) {
-        const uint4 q = *reinterpret_cast<const uint4*>(L.raw + j);      // (behind the last one: EMBED_NONE, not smaller)
-        rank += (q.x < k) + (q.y < k) + (q.z < k) + (q.w < k);
-        before += (q.x == k && j < i) + (q.y == k && j + 1 < i) + (q.z == k && j + 2 < i) + (q.w == k && j + 3 < i);
-    }
-    if (k != EMBED_NONE) {
-        L.key[rank + before] = k;
-        L.pos[rank + before] = i;
-    }
-    __syncthreads();
-    // the first position of each run, in order
-    const bool first = i < L.kept && (i == 0 || L.key[i] != L.key[i - 1]);
-    const unsigned long long firsts = __ballot(first);
-    if ((i & 63) == 0) L.raw[i >> 6] = (uint32_t)__popcll(firsts);
-    __syncthreads();
-    uint32_t at = (uint32_t)__popcll(firsts & ((1ull << (i & 63)) - 1ull));
-    for (uint32_t w = 0; w < i >> 6; ++w) at += L.raw[w];
-    if (first) L.start[at] = i;
-    if (i == EMBED_TINY - 1) {
-        L.runs = at + (first ? 1u : 0u);
-        L.start[L.runs] = L.kept;
-    }
-    __syncthreads();
-}
 template <typename T, int V, int G>
 __global__ __launch_bounds__(256) void embed_tiny_kernel(uint32_t n, uint32_t rows, const void* __restrict__ index, int index_bytes,
                                                          uint32_t nslices, size_t dim, const T* __restrict__ d_out, size_t stride,
                                                          float scale, T* __restrict__ d_table, uint32_t sum_blocks, uint32_t zero_rows) {
-    __shared__ __attribute__((aligned(16))) TinySort L;
+    constexpr int PER = EMBED_TINY / 256, GROUPS = 256 / G, UNROLL = 8;
+    __shared__ uint32_t list[EMBED_TINY], found[4 * PER];
     __shared__ float sums[256 * V];
-    embed_sort_tiny(L, n, rows, index, index_bytes);
+    uint32_t key[PER];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+        const uint32_t i = u * 256 + threadIdx.x;
+        const unsigned long long id = (unsigned long long)load_index_flat(index, i < n ? i : n - 1, index_bytes);
+        key[u] = i < n && id < rows ? (uint32_t)id : EMBED_NONE;
+    }
     if (blockIdx.x >= sum_blocks) {
-        const size_t wave = (size_t)(blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6);
-        if ((size_t)rows * dim * sizeof(T) > E3_STREAM_BYTES) embed_zero<true, T, V>(L.kept, L.key, rows, zero_rows, dim, d_table, wave);
-        else embed_zero<false, T, V>(L.kept, L.key, rows, zero_rows, dim, d_table, wave);
+        const uint32_t row0 = (blockIdx.x - sum_blocks) * 4 * zero_rows;       // (4 * zero_rows <= 256 rows)
+        list[threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < PER; ++u)
+            if (key[u] - row0 < 4 * zero_rows) list[key[u] - row0] = 1;        // (several threads: the same value)
+        __syncthreads();
+        const uint32_t lane = threadIdx.x & 63, mine = (threadIdx.x >> 6) * zero_rows;
+        const bool empty = lane < zero_rows && (size_t)row0 + mine + lane < rows && list[mine + lane] == 0;
+        const size_t first = (size_t)row0 + mine;
+        if ((size_t)rows * dim * sizeof(T) > E3_STREAM_BYTES) embed_zero<true, T, V>(empty, first, rows, zero_rows, dim, d_table);
+        else embed_zero<false, T, V>(empty, first, rows, zero_rows, dim, d_table);
         return;
     }
-    constexpr int GROUPS = 256 / G, UNROLL = 8;
-    const uint32_t run = blockIdx.x / nslices, slice = blockIdx.x - run * nslices;
-    if (run >= L.runs) return;                                          // (uniform)
+    const uint32_t own = blockIdx.x / nslices, slice = blockIdx.x - own * nslices;
+    const unsigned long long id = (unsigned long long)load_index_flat(index, own, index_bytes);
+    if (id >= rows) return;                                                    // (uniform)
+    unsigned long long hit[PER];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+        hit[u] = __ballot(key[u] == (uint32_t)id);
+        if ((threadIdx.x & 63) == 0) found[u * 4 + (threadIdx.x >> 6)] = (uint32_t)__popcll(hit[u]);
+    }
+    __syncthreads();
+    uint32_t m = 0;
+#pragma unroll
+    for (int u = 0; u < PER; ++u)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            if (w == (int)(threadIdx.x >> 6) && key[u] == (uint32_t)id)
+                list[m + (uint32_t)__popcll(hit[u] & ((1ull << (threadIdx.x & 63)) - 1ull))] = u * 256 + threadIdx.x;
+            m += found[u * 4 + w];
+        }
+    __syncthreads();
+    if (list[0] != own) return;                                                // (uniform)
     const int g = threadIdx.x / G, lane = threadIdx.x % G;
     const size_t col = ((size_t)slice * G + lane) * V;
-    const uint32_t j0 = L.start[run], m = L.start[run + 1] - j0;
-    const uint32_t lo = j0 + m * g / GROUPS, hi = j0 + m * (g + 1) / GROUPS;
+    const uint32_t lo = m * g / GROUPS, hi = m * (g + 1) / GROUPS;
     float acc[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = 0.0f;
@@ -244,7 +255,7 @@ __global__ __launch_bounds__(256) void embed_tiny_kernel(uint32_t n, uint32_t ro
         Pack<T, V> r[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
-            r[u] = *reinterpret_cast<const Pack<T, V>*>(d_out + (size_t)L.pos[b + u < hi ? b + u : hi - 1] * stride + col);
+            r[u] = *reinterpret_cast<const Pack<T, V>*>(d_out + (size_t)list[b + u < hi ? b + u : hi - 1] * stride + col);
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             if (b + u >= hi) break;
@@ -252,14 +263,19 @@ __global__ __launch_bounds__(256) void embed_tiny_kernel(uint32_t n, uint32_t ro
             for (int j = 0; j < V; ++j) acc[j] += (float)r[u].v[j];
         }
     }
+    if (m > 1) {                                                               // (uniform)
 #pragma unroll
-    for (int j = 0; j < V; ++j) sums[threadIdx.x * V + j] = acc[j];
-    __syncthreads();
-    if (g != 0 || col >= dim) return;
-    for (int k = 1; k < GROUPS; ++k)
+        for (int j = 0; j < V; ++j) sums[threadIdx.x * V + j] = acc[j];
+        __syncthreads();
+    }
+    // (a list of one: the last group has it)
+    if (m == 1 ? g != GROUPS - 1 : g != 0) return;
+    if (col >= dim) return;
+    if (m > 1)
+        for (int k = 1; k < GROUPS; ++k)
 #pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] += sums[(k * G + lane) * V + j];
-    embed_store<T, V>(d_table, dim, L.key[j0], col, scale, acc);
+            for (int j = 0; j < V; ++j) acc[j] += sums[(k * G + lane) * V + j];
+    embed_store<T, V>(d_table, dim, (uint32_t)id, col, scale, acc);
 }
 
 // A group of G lanes sums one chunk of the sorted list, times a slice of G V columns, EMBED_UNROLL gathered rows in flight.
@@ -275,9 +291,14 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restri
                                                         uint32_t zero_rows) {
     const uint32_t n = *kept;
     if (blockIdx.x >= sum_blocks) {      // (in the same launch: the sums wait for their gathers, the stores do not)
-        const size_t wave = (size_t)(blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6);
-        if ((size_t)rows * dim * sizeof(T) > E3_STREAM_BYTES) embed_zero<true, T, V>(n, keys, rows, zero_rows, dim, d_table, wave);
-        else embed_zero<false, T, V>(n, keys, rows, zero_rows, dim, d_table, wave);
+        const size_t first = ((size_t)(blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6)) * zero_rows;
+        bool empty = false;                                 // (a lane looks one row up in the sorted keys)
+        if ((threadIdx.x & 63) < zero_rows && first + (threadIdx.x & 63) < rows) {
+            const uint32_t row = (uint32_t)first + (threadIdx.x & 63), at = lower_bound_u32(keys, 0, n, row);
+            empty = at >= n || keys[at] != row;
+        }
+        if ((size_t)rows * dim * sizeof(T) > E3_STREAM_BYTES) embed_zero<true, T, V>(empty, first, rows, zero_rows, dim, d_table);
+        else embed_zero<false, T, V>(empty, first, rows, zero_rows, dim, d_table);
         return;
     }
     const size_t unit = (size_t)blockIdx.x * (256 / G) + threadIdx.x / G;
@@ -543,6 +564,180 @@ __global__ __launch_bounds__(1024) void embed_sort_small_kernel(uint32_t n, uint
     if (threadIdx.x == 0) *kept = L.valid;
 }
 
+// More positions: passes of up to 8 bits over tiles of 1024 * ITEMS keys, two launches each.  The first counts the digits of
+// every tile (and makes the keys); in the second every tile adds up the counts before its own (at most SORT_TILES of them, a
+// kilobyte each: cheaper than a launch that scans them), ranks its keys, puts them in order in LDS and writes them out
+// digit by digit.  1M positions of 12 bits: 39 us (the general sort with its seven launches 43), 60905 of 16 bits: 21 us (36),
+// 372939 of 17 bits: 55 us (65).  Keys to a thread: 1 up to 128 tiles of one, 2 up to 128 tiles of two, and so on; 560085
+// positions took 12 us a scatter with 137 tiles of four, 14 with 69 tiles of eight, 372939 took 9 with 92 tiles and 10 with 183.
+constexpr uint32_t SORT_TILES = 256;
+__device__ __forceinline__ uint32_t sort_digit(uint32_t key, int shift, uint32_t mask) { return key >> shift & mask; }
+template <int ITEMS, bool FIRST, typename I>
+__global__ __launch_bounds__(1024) void embed_count_kernel(uint32_t n, uint32_t rows, int shift, uint32_t mask,
+                                                           const I* __restrict__ index, uint32_t* __restrict__ keys,
+                                                           uint32_t* __restrict__ counts, uint32_t* __restrict__ valid) {
+    __shared__ uint32_t cnt[4][256], ok_count;
+    for (int d = threadIdx.x; d < 4 * 256; d += 1024) cnt[d >> 8][d & 255] = 0;
+    if (threadIdx.x == 0) ok_count = 0;
+    __syncthreads();
+    const uint32_t tile0 = blockIdx.x * (1024 * ITEMS);
+    uint32_t k[ITEMS], ok = 0;
+    if (FIRST) {
+        I id[ITEMS];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t at = tile0 + i * 1024 + threadIdx.x;
+            id[i] = index[at < n ? at : n - 1];
+        }
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t at = tile0 + i * 1024 + threadIdx.x;
+            const bool in = id[i] >= 0 && (long long)id[i] < (long long)rows;
+            k[i] = in ? (uint32_t)id[i] : rows;
+            if (at < n) {
+                keys[at] = k[i];
+                ok += in ? 1u : 0u;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t at = tile0 + i * 1024 + threadIdx.x;
+            k[i] = keys[at < n ? at : n - 1];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+        if (tile0 + i * 1024 + threadIdx.x < n) atomicAdd(&cnt[threadIdx.x >> 6 & 3][sort_digit(k[i], shift, mask)], 1u);
+    if (FIRST) {
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) ok += __shfl_xor(ok, o, 64);
+        if ((threadIdx.x & 63) == 0) atomicAdd(&ok_count, ok);
+    }
+    __syncthreads();
+    if (threadIdx.x < 256) counts[blockIdx.x * 256 + threadIdx.x] =
+        (cnt[0][threadIdx.x] + cnt[1][threadIdx.x]) + (cnt[2][threadIdx.x] + cnt[3][threadIdx.x]);
+    if (FIRST && threadIdx.x == 0) valid[blockIdx.x] = ok_count;
+}
+// Exclusive prefix sum over 256 values, one per thread of the first four waves; every thread of the workgroup takes part.
+__device__ __forceinline__ uint32_t prefix_256(uint32_t v, uint32_t* wave_totals) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const uint32_t t = __shfl_up(inc, o, 64); if (lane >= o) inc += t; }
+    if (lane == 63 && wave < 4) wave_totals[wave] = inc;
+    __syncthreads();
+    uint32_t run = inc - v;
+    for (int w = 0; w < wave && w < 4; ++w) run += wave_totals[w];
+    return run;
+}
+template <int ITEMS>
+struct SortTile {
+    uint32_t key[1024 * ITEMS], pos[1024 * ITEMS];
+    uint32_t cnt[16][256], all[256], before[256], to[256], wl[4], wg[4];
+};
+template <int ITEMS, bool FIRST>
+__global__ __launch_bounds__(1024) void embed_scatter_kernel(uint32_t n, int shift, int bits, uint32_t tiles,
+                                                             const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
+                                                             const uint32_t* __restrict__ counts, const uint32_t* __restrict__ valid,
+                                                             uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out,
+                                                             uint32_t* __restrict__ kept) {
+    __shared__ SortTile<ITEMS> L;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t mask = (1u << bits) - 1u, tile0 = blockIdx.x * (1024 * ITEMS), base = tile0 + (uint32_t)wave * (64 * ITEMS) + lane;
+    const unsigned long long before = (1ull << lane) - 1ull;
+    uint32_t k[ITEMS], p[ITEMS], rank[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {                       // (behind the list: the largest digit, last of all)
+        const uint32_t at = base + i * 64;
+        k[i] = keys[at < n ? at : n - 1];
+        p[i] = FIRST ? at : pos[at < n ? at : n - 1];
+        if (at >= n) k[i] = 0xFFFFFFFFu;
+    }
+    for (int d = threadIdx.x; d < 16 * 256; d += 1024) L.cnt[d >> 8][d & 255] = 0;
+    if (threadIdx.x < 256) L.all[threadIdx.x] = L.before[threadIdx.x] = 0;
+    __syncthreads();
+    if (4u * lane <= mask) {   // counts of the digits in all tiles, and in those before this one: four digits to a lane
+        uint32_t all[4] = {0, 0, 0, 0}, less[4] = {0, 0, 0, 0};
+        for (uint32_t t0 = wave; t0 < tiles; t0 += 16 * 8) {
+            uint4 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {                   // (a batch of loads in flight; behind the last tile the first again)
+                const uint32_t t = t0 + 16 * u;
+                v[u] = reinterpret_cast<const uint4*>(counts + (t < tiles ? t : t0) * 256)[lane];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const uint32_t t = t0 + 16 * u;
+                if (t >= tiles) break;
+                const uint32_t x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    all[j] += x[j];
+                    less[j] += t < blockIdx.x ? x[j] : 0u;
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            atomicAdd(&L.all[4 * lane + j], all[j]);
+            atomicAdd(&L.before[4 * lane + j], less[j]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t d = sort_digit(k[i], shift, mask);
+        unsigned long long peers = ~0ull;                   // lanes with the same digit
+        for (int b = 0; b < bits; ++b) {
+            const unsigned long long bal = __ballot(d >> b & 1u);
+            peers &= d >> b & 1u ? bal : ~bal;
+        }
+        const uint32_t first = L.cnt[wave][d];
+        wave_sync();
+        if ((peers & before) == 0ull) L.cnt[wave][d] = first + (uint32_t)__popcll(peers);
+        wave_sync();
+        rank[i] = first + (uint32_t)__popcll(peers & before);
+    }
+    __syncthreads();
+    uint32_t c[16], local = 0, all = 0, less = 0;
+    if (threadIdx.x < 256) {
+#pragma unroll
+        for (int w = 0; w < 16; ++w) { c[w] = L.cnt[w][threadIdx.x]; local += c[w]; }
+        all = L.all[threadIdx.x];
+        less = L.before[threadIdx.x];
+    }
+    uint32_t run = prefix_256(local, L.wl);
+    const uint32_t start = prefix_256(all, L.wg) + less;
+    if (threadIdx.x < 256) {
+        L.to[threadIdx.x] = start - run;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) { L.cnt[w][threadIdx.x] = run; run += c[w]; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t at = L.cnt[wave][sort_digit(k[i], shift, mask)] + rank[i];
+        L.key[at] = k[i];
+        L.pos[at] = p[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t at = i * 1024 + threadIdx.x;
+        if (tile0 + at >= n) continue;
+        const uint32_t key = L.key[at], to = L.to[sort_digit(key, shift, mask)] + at;
+        keys_out[to] = key;
+        pos_out[to] = L.pos[at];
+    }
+    if (FIRST && blockIdx.x == 0 && wave == 15) {
+        uint32_t m = 0;
+        for (uint32_t t = lane; t < tiles; t += 64) m += valid[t];
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) m += __shfl_xor(m, o, 64);
+        if (lane == 0) *kept = m;
+    }
+}
+
 namespace {
 struct EmbedScratch {
     uint32_t *key0, *key1, *pos0, *pos1, *kept, *sort;
@@ -563,7 +758,8 @@ struct EmbedScratch {
         s.pos0 = carve<uint32_t>(p, m);
         s.pos1 = carve<uint32_t>(p, m);
         s.kept = carve<uint32_t>(p, 1);
-        s.sort = carve<uint32_t>(p, sort_scratch_words(m));
+        const size_t general = sort_scratch_words(m), tiles = SORT_TILES * 257;
+        s.sort = carve<uint32_t>(p, general > tiles ? general : tiles);
         s.part = carve<float>(p, m <= EMBED_TINY ? 1 : 2 * (size_t)chunks(m, dim) * dim);      // (few positions: no partials)
         return s;
     }
@@ -578,7 +774,7 @@ int embed_sum_launch(const EmbedScratch& w, const uint32_t* keys, const uint32_t
     per = per < 1 ? 1 : (per > 64 ? 64 : per);
     const size_t zero_blocks = (rows + 4 * per - 1) / (4 * per);
     if (n <= EMBED_TINY) {
-        const size_t most = n < rows ? n : rows, blocks = most * nslices;
+        const size_t blocks = n * nslices;
         if (blocks + zero_blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
         embed_tiny_kernel<T, V, G><<<dim3((unsigned)(blocks + zero_blocks)), dim3(256), 0, s>>>(
             (uint32_t)n, (uint32_t)rows, index, index_bytes, (uint32_t)nslices, dim, (const T*)d_out, stride, scale, (T*)d_table,
@@ -621,6 +817,33 @@ void embed_sort_small(uint32_t n, uint32_t rows, int nbits, const I* index, uint
     else embed_sort_small_kernel<16, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, nbits, index, keys, pos, kept);
 }
 
+// The tiles' sort; keys / pos: where the result lies.
+template <int ITEMS>
+int embed_sort_tiles(const EmbedScratch& w, uint32_t n, uint32_t rows, const void* index, int index_bytes, uint32_t** keys,
+                     uint32_t** pos, hipStream_t s) {
+    int nbits = 1;
+    while (rows >> nbits) ++nbits;                             // (the key `rows` itself occurs)
+    const int passes = (nbits + 7) / 8, bits = (nbits + passes - 1) / passes;
+    const uint32_t tiles = (n + 1024 * ITEMS - 1) / (1024 * ITEMS), mask = (1u << bits) - 1u;
+    uint32_t *counts = w.sort, *valid = w.sort + SORT_TILES * 256;
+    uint32_t *k0 = w.key0, *k1 = w.key1, *p0 = w.pos0, *p1 = w.pos1;
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * bits;
+        if (pass > 0) embed_count_kernel<ITEMS, false, int><<<dim3(tiles), dim3(1024), 0, s>>>(n, rows, shift, mask, nullptr, k0, counts, valid);
+        else if (index_bytes == 8) embed_count_kernel<ITEMS, true, long long><<<dim3(tiles), dim3(1024), 0, s>>>(n, rows, shift, mask, (const long long*)index, k0, counts, valid);
+        else embed_count_kernel<ITEMS, true, int><<<dim3(tiles), dim3(1024), 0, s>>>(n, rows, shift, mask, (const int*)index, k0, counts, valid);
+        LAUNCH_OK("embed_count_kernel");
+        if (pass > 0) embed_scatter_kernel<ITEMS, false><<<dim3(tiles), dim3(1024), 0, s>>>(n, shift, bits, tiles, k0, p0, counts, valid, k1, p1, w.kept);
+        else embed_scatter_kernel<ITEMS, true><<<dim3(tiles), dim3(1024), 0, s>>>(n, shift, bits, tiles, k0, nullptr, counts, valid, k1, p1, w.kept);
+        LAUNCH_OK("embed_scatter_kernel");
+        uint32_t* t = k0; k0 = k1; k1 = t;
+        t = p0; p0 = p1; p1 = t;
+    }
+    *keys = k0;
+    *pos = p0;
+    return 0;
+}
+
 template <typename T>
 int embed_bwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_bytes, const void* d_out, size_t stride,
                 int dtype, float scale, void* d_table, char* scratch, hipStream_t s) {
@@ -633,6 +856,11 @@ int embed_bwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_
         if (index_bytes == 8) embed_sort_small((uint32_t)n, (uint32_t)rows, nbits, (const long long*)index, keys, pos, w.kept, s);
         else embed_sort_small((uint32_t)n, (uint32_t)rows, nbits, (const int*)index, keys, pos, w.kept, s);
         LAUNCH_OK("embed_sort_small_kernel");
+    } else if (n > EMBED_TINY && n <= SORT_TILES * 8192) {
+#define E3_TILES(ITEMS) embed_sort_tiles<ITEMS>(w, (uint32_t)n, (uint32_t)rows, index, index_bytes, &keys, &pos, s)
+        rc = n <= 128 * 1024 ? E3_TILES(1) : n <= 128 * 2048 ? E3_TILES(2) : n <= 256 * 4096 ? E3_TILES(4) : E3_TILES(8);
+#undef E3_TILES
+        if (rc) return rc;
     } else if (n > EMBED_TINY) {
         embed_keys_kernel<<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s>>>(n, rows, index, index_bytes, w.key0);
         LAUNCH_OK("embed_keys_kernel");
@@ -654,13 +882,17 @@ int embed_bwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_
         else E3_SUM(N, 64);
     } else if (fits(8)) {
         if (dim / HALF <= 16) E3_SUM(HALF, 16);
+        else if (dim / HALF <= 32) E3_SUM(HALF, 32);
         else E3_SUM(HALF, 64);
     } else if (N == 8 && fits(4)) {
-        if (dim / QUARTER <= 16) E3_SUM(QUARTER, 16);
+        if (dim / QUARTER <= 4) E3_SUM(QUARTER, 4);
+        else if (dim / QUARTER <= 16) E3_SUM(QUARTER, 16);
+        else if (dim / QUARTER <= 32) E3_SUM(QUARTER, 32);
         else E3_SUM(QUARTER, 64);
     } else {
         if (dim <= 4) E3_SUM(1, 4);
         else if (dim <= 16) E3_SUM(1, 16);
+        else if (dim <= 32) E3_SUM(1, 32);
         else E3_SUM(1, 64);
     }
 #undef E3_SUM

@@ -662,7 +662,9 @@ def test_inputs_changed_in_between_are_noticed():
 
 @pytest.mark.parametrize("n, rows, dim", [(255, 40, 48), (256, 40, 48), (257, 40, 48), (256, 3, 1000), (1024, 9, 20), (1025, 9, 20),
                                           (4096, 300, 16), (4097, 300, 16), (8192, 20, 12), (8193, 20, 12), (16384, 4000, 8),
-                                          (16385, 4000, 8), (300000, 70000, 4)])
+                                          (16385, 4000, 8), (300000, 70000, 4), (524288, 255, 3), (524289, 256, 3),
+                                          (1048576, 65535, 2), (1048577, 65536, 2), (2097152, 300, 1), (2097153, 300, 1),
+                                          (20011, 17000000, 1)])
 def test_embedding_sort_sizes(n, rows, dim):
     """Position counts around which another sort takes over, int32 and int64 indices, masked ends."""
     index = tokens(n, rows, skew=2.0, empty=0.2)
