@@ -983,7 +983,7 @@ __device__ __forceinline__ void load_affine(const void* __restrict__ p, int dtyp
 // ... V neighbouring ones (col a multiple of V), in 16-byte loads where the array allows it
 template <int V>
 __device__ __forceinline__ void load_affine_pack(const void* __restrict__ p, int dtype, int col, int dim, float none, float v[V]) {
-    if (V == 1 || !p || (reinterpret_cast<uintptr_t>(p) & 15) != 0 || (V == 4 && dtype != E3_F32)) {
+    if (V < 4 || !p || (reinterpret_cast<uintptr_t>(p) & 15) != 0 || (V == 4 && dtype != E3_F32)) {
         load_affine<V>(p, dtype, col, 1, dim, none, v);
         return;
     }
@@ -1084,6 +1084,23 @@ struct NormSums {
         if (dtype == E3_F32) reinterpret_cast<float*>(out)[col] = v;
         else if (dtype == E3_F16) reinterpret_cast<f16_t*>(out)[col] = (f16_t)v;
         else reinterpret_cast<bf16_t*>(out)[col] = (bf16_t)v;
+    }
+    // V neighbouring columns from a multiple of V on, in a row of a multiple of V
+    template <int V>
+    __device__ __forceinline__ void put_pack(int dim, int which, int col, const float v[V]) const {
+        if (gridDim.x > 1) {
+            constexpr int N = V < 4 ? V : 4;
+#pragma unroll
+            for (int j = 0; j < V; j += N) {
+                Pack<float, N> p;
+#pragma unroll
+                for (int u = 0; u < N; ++u) p.v[u] = v[j + u];
+                *reinterpret_cast<Pack<float, N>*>(part + ((size_t)blockIdx.x * 2 + which) * dim + col + j) = p;
+            }
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) put(dim, which, col + j, v[j]);
     }
 };
 
@@ -1410,9 +1427,7 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_bwd_kernel(size_t ro
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
                 const int col = (i * G + lane) * V;
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (col < dim) sums.put(dim, which, col + j, a[i][j]);
+                if (col < dim) sums.template put_pack<V>(dim, which, col, a[i]);
             }
         }
     }
@@ -1511,9 +1526,14 @@ unsigned norm_blocks(size_t rows, int per_block, size_t most) {
 }
 // ... of the gradient: what one workgroup does in four rounds goes to one, which saves the launch that would join the sums (10
 // rows of 64 values with autograd around it: 66 us of host time with the second launch, 61 us without; a round takes about
-// 1.5 us, the launch 2.5 us on the GPU and 4 us on the host)
+// 1.5 us, the launch 2.5 us on the GPU and 4 us on the host).  Beyond 256 workgroups each takes four rounds before there are
+// more of them: their partial sums cost as much as their rows (1000 x 1446 bf16 with a workgroup per row 27 us, so 22; 500 x 4096
+// bf16 32 and 25 us).
 unsigned norm_bwd_blocks(size_t rows, int per_block, size_t most) {
-    return rows <= 4 * (size_t)per_block ? 1u : norm_blocks(rows, per_block, most);
+    const size_t need = (rows + per_block - 1) / per_block;
+    if (need <= 4) return 1u;
+    const size_t blocks = need <= 256 ? need : need / 4 < 256 ? 256 : need / 4;
+    return (unsigned)(blocks < most ? blocks : most);
 }
 constexpr size_t NORM_FWD_BLOCKS = 4096, NORM_BWD_BLOCKS = 1024, NORM_TILE_BLOCKS = 1024, NORM_LONG_PARTS = 64;
 
@@ -1531,11 +1551,12 @@ NormSums norm_sums(const NormArgs& a) { return {a.part, a.dweight, a.dbias, a.af
 
 template <typename T, int V, int G, int ITEMS>
 int norm_fwd_launch(const NormArgs& a) {
-    const dim3 blocks(norm_blocks(a.rows, NormRow<G>::PER_BLOCK, NORM_FWD_BLOCKS)), threads(NormRow<G>::THREADS);
+    const dim3 blocks(norm_blocks(a.rows, NormRow<G>::PER_BLOCK, G >= 256 ? NORM_FWD_BLOCKS / 2 : NORM_FWD_BLOCKS)), threads(NormRow<G>::THREADS);
 #define E3_NORM(S)                                                                                                            \
     norm_fwd_kernel<(S), T, V, G, ITEMS><<<blocks, threads, 0, a.s>>>(a.rows, (int)a.dim, (const T*)a.x, a.x_stride, a.weight, \
                                                                   a.bias, a.affine_dtype, a.eps, (T*)a.out, a.mean, a.rstd)
-    if (V > 1 && a.rows * a.dim * sizeof(T) > E3_STREAM_BYTES) E3_NORM(V > 1);
+    constexpr bool WIDE = V == Wide<T>::N;
+    if (WIDE && a.rows * a.dim * sizeof(T) > E3_STREAM_BYTES) E3_NORM(WIDE);
     else E3_NORM(false);
 #undef E3_NORM
     LAUNCH_OK("norm_fwd_kernel");
@@ -1543,16 +1564,18 @@ int norm_fwd_launch(const NormArgs& a) {
 }
 template <typename T, int V, int G, int ITEMS>
 int norm_bwd_launch(const NormArgs& a, uint32_t& nparts) {
-    nparts = norm_bwd_blocks(a.rows, NormRow<G>::PER_BLOCK, NORM_BWD_BLOCKS);
+    nparts = norm_bwd_blocks(a.rows, NormRow<G>::PER_BLOCK, G > 256 ? NORM_BWD_BLOCKS / 2 : NORM_BWD_BLOCKS);
     const dim3 blocks(nparts), threads(NormRow<G>::THREADS);
 #define E3_NORM(S)                                                                                                            \
     norm_bwd_kernel<(S), T, V, G, ITEMS><<<blocks, threads, 0, a.s>>>(a.rows, (int)a.dim, (const T*)a.dy, a.dy_stride,          \
                                                                   (const T*)a.x, a.x_stride, a.weight, a.affine_dtype,       \
                                                                   a.mean, a.rstd, (T*)a.dx, norm_sums(a))
-    if (V > 1 && a.rows * a.dim * sizeof(T) > E3_STREAM_BYTES) E3_NORM(V > 1);
+    constexpr bool WIDE = V == Wide<T>::N;
+    if (WIDE && a.rows * a.dim * sizeof(T) > E3_STREAM_BYTES) E3_NORM(WIDE);
     else E3_NORM(false);
 #undef E3_NORM
     LAUNCH_OK("norm_bwd_kernel");
+    if (nparts == 1) nparts = 0;
     return 0;
 }
 // Values of a row to a lane.  The gradient keeps five arrays of them in registers: 8 while 32 lanes are enough for the row.
@@ -1596,58 +1619,109 @@ int norm_bwd_tile(const NormArgs& a, int tile, uint32_t& nparts) {
     else E3_TILE_BWD(NORM_TILE_ITEMS);
 #undef E3_TILE_BWD
     LAUNCH_OK("norm_bwd_tile_kernel");
+    if (nparts == 1) nparts = 0;
     return 0;
 }
 template <typename T, int V>
-int norm_fwd_v(const NormArgs& a) {
-    const size_t packs = a.dim / V;
-    if (const int tile = norm_tile_rows(a, sizeof(T), false)) return norm_fwd_tile<T>(a, tile);
-    if (packs <= 8) return norm_fwd_launch<T, V, 8, 1>(a);
-    if (packs <= 16) return norm_fwd_launch<T, V, 16, 1>(a);
-    if (packs <= 32) return norm_fwd_launch<T, V, 32, 1>(a);
-    if (packs <= 64) return norm_fwd_launch<T, V, 64, 1>(a);
-    if (packs <= 128) return norm_fwd_launch<T, V, 64, 2>(a);
-    if (packs <= 256) return norm_fwd_launch<T, V, 64, 4>(a);
-    if (packs <= 512) return norm_fwd_launch<T, V, 256, 2>(a);
-    if (packs <= 1024) return norm_fwd_launch<T, V, 256, 4>(a);
+int norm_fwd_again(const NormArgs& a) {
     const unsigned blocks = (unsigned)(a.rows < 2048 ? a.rows : 2048);
     norm_fwd_long_kernel<T, V><<<dim3(blocks), dim3(1024), 0, a.s>>>(a.rows, a.dim, (const T*)a.x, a.x_stride, a.weight,
                                                                     a.bias, a.affine_dtype, a.eps, (T*)a.out, a.mean, a.rstd);
     LAUNCH_OK("norm_fwd_long_kernel");
     return 0;
 }
+// Rows of more than 256 packs (V values each, 16, 8 or 4 bytes or a single one): workgroups of 256 threads up to 1024 packs, of
+// 512 or 1024 threads up to 16384 values; longer rows, and single values past 1024, are read again for every step.  Held in
+// registers / read again: 2000 x 16384 bf16 50 / 85 us, 4096 x 4588 bf16 40 / 66 us, 300 x 16384 fp32 12 / 24 us, but
+// 2000 x 4097 bf16 33 / 29 us.
 template <typename T, int V>
-int norm_bwd_v(const NormArgs& a) {
+int norm_fwd_long(const NormArgs& a) {
     const size_t packs = a.dim / V;
+    constexpr int MORE = V < 8 ? 4 : 2, MOST = V < 4 ? 8 : MORE;
+    if (packs <= 256) return norm_fwd_launch<T, V, 64, 4>(a);
+    if (packs <= 512) return norm_fwd_launch<T, V, 256, 2>(a);
+    if (packs <= 1024) return norm_fwd_launch<T, V, 256, 4>(a);
+    if (V == 1) return norm_fwd_again<T, V>(a);
+    if (packs <= 2048) return norm_fwd_launch<T, V, 512, 4>(a);
+    if (packs <= 1024 * MORE) return norm_fwd_launch<T, V, 1024, MORE>(a);
+    if (packs <= 1024 * MOST) return norm_fwd_launch<T, V, 1024, MOST>(a);
+    return norm_fwd_again<T, V>(a);
+}
+template <typename T, int V>
+int norm_fwd_v(const NormArgs& a) {
+    const size_t packs = a.dim / V;
+    if (packs <= 8) return norm_fwd_launch<T, V, 8, 1>(a);
+    if (packs <= 16) return norm_fwd_launch<T, V, 16, 1>(a);
+    if (packs <= 32) return norm_fwd_launch<T, V, 32, 1>(a);
+    if (packs <= 64) return norm_fwd_launch<T, V, 64, 1>(a);
+    if (packs <= 128) return norm_fwd_launch<T, V, 64, 2>(a);
+    return norm_fwd_long<T, V>(a);
+}
+template <typename T>
+int norm_fwd_t(const NormArgs& a, int dtype) {
+    constexpr int N = Wide<T>::N;
+    auto fits = [&](size_t bytes) { return e3_rows_packs(a.x, a.x_stride, a.dim, dtype, bytes) && e3_rows_packs(a.out, a.dim, a.dim, dtype, bytes); };
+    if (const int tile = norm_tile_rows(a, sizeof(T), false)) return norm_fwd_tile<T>(a, tile);
+    if (fits(16)) return norm_fwd_v<T, N>(a);
+    if (a.dim > 512 && fits(8)) return norm_fwd_long<T, N / 2>(a);
+    if (a.dim > 512 && N == 8 && fits(4)) return norm_fwd_long<T, N == 8 ? 2 : 1>(a);
+    return norm_fwd_v<T, 1>(a);
+}
+// The gradient, which keeps five arrays of the row, up to 16384 values where there are rows enough to make up for the partial
+// sums of the workgroups: 2000 x 16384 bf16 83 us (read again: 123), 4096 x 4588 bf16 53 us (90), 113 x 4588 bf16 11 us (15);
+// with 16 values to a thread 300 x 16384 fp32 took 47 us (38).
+// nparts: how many partial sums there are for norm_join_kernel, 0: the results are written
+template <typename T, int V>
+int norm_bwd_long(const NormArgs& a, uint32_t& nparts) {
+    const size_t packs = a.dim / V;
+    constexpr int MORE = V < 8 ? 4 : 2, MOST = V < 4 ? 8 : MORE;
+    if (packs <= 256) return norm_bwd_launch<T, V, 256, 1>(a, nparts);
+    if (packs <= 512) return norm_bwd_launch<T, V, 256, 2>(a, nparts);
+    if (packs <= 1024) return norm_bwd_launch<T, V, 256, 4>(a, nparts);
+    if (packs <= 2048) return norm_bwd_launch<T, V, V == 8 ? 512 : 1024, V == 8 ? 4 : 2>(a, nparts);
+    const size_t most = a.rows >= 1024 || V == 1 ? 1024 * MOST : 8192 / V;
+    if (packs <= 1024 * MORE && packs <= most) return norm_bwd_launch<T, V, 1024, MORE>(a, nparts);
+    if (packs <= most) return norm_bwd_launch<T, V, 1024, MOST>(a, nparts);
+    if (a.dx) {
+        const unsigned blocks = (unsigned)(a.rows < 2048 ? a.rows : 2048);
+        norm_bwd_long_kernel<T, V><<<dim3(blocks), dim3(1024), 0, a.s>>>(a.rows, a.dim, (const T*)a.dy, a.dy_stride,
+                                                                        (const T*)a.x, a.x_stride, a.weight,
+                                                                        a.affine_dtype, a.mean, a.rstd, (T*)a.dx);
+        LAUNCH_OK("norm_bwd_long_kernel");
+    }
+    if (a.part) {
+        nparts = (uint32_t)(a.rows < NORM_LONG_PARTS ? a.rows : NORM_LONG_PARTS);
+        norm_cols_kernel<T><<<dim3(nparts, (unsigned)((a.dim + 255) / 256)), dim3(256), 0, a.s>>>(
+            a.rows, a.dim, (const T*)a.dy, a.dy_stride, (const T*)a.x, a.x_stride, a.mean, a.rstd, a.part);
+        LAUNCH_OK("norm_cols_kernel");
+    }
+    return 0;
+}
+template <typename T, int V>
+int norm_bwd_v(const NormArgs& a, uint32_t& nparts) {
+    const size_t packs = a.dim / V;
+    if (packs <= 8) return norm_bwd_launch<T, V, 8, 1>(a, nparts);
+    if (packs <= 16) return norm_bwd_launch<T, V, 16, 1>(a, nparts);
+    if (packs <= 32) return norm_bwd_launch<T, V, 32, 1>(a, nparts);
+    if (packs <= 64) return norm_bwd_launch<T, V, 64, 1>(a, nparts);
+    if (packs <= 128) return norm_bwd_launch<T, V, 64, 2>(a, nparts);
+    return norm_bwd_long<T, V>(a, nparts);
+}
+template <typename T>
+int norm_bwd_t(const NormArgs& a, int dtype) {
+    constexpr int N = Wide<T>::N;
     uint32_t nparts = 0;
     int rc = 0;
-    bool long_rows = false;
+    auto fits = [&](size_t bytes) {
+        return e3_rows_packs(a.x, a.x_stride, a.dim, dtype, bytes) && e3_rows_packs(a.dy, a.dy_stride, a.dim, dtype, bytes) &&
+               (!a.dx || e3_rows_packs(a.dx, a.dim, a.dim, dtype, bytes));
+    };
     if (const int tile = norm_tile_rows(a, sizeof(T), true)) rc = norm_bwd_tile<T>(a, tile, nparts);
-    else if (packs <= 8) rc = norm_bwd_launch<T, V, 8, 1>(a, nparts);
-    else if (packs <= 16) rc = norm_bwd_launch<T, V, 16, 1>(a, nparts);
-    else if (packs <= 32) rc = norm_bwd_launch<T, V, 32, 1>(a, nparts);
-    else if (packs <= 64) rc = norm_bwd_launch<T, V, 64, 1>(a, nparts);
-    else if (packs <= 128) rc = norm_bwd_launch<T, V, 64, 2>(a, nparts);
-    else if (packs <= 256) rc = norm_bwd_launch<T, V, 256, 1>(a, nparts);
-    else if (packs <= 512) rc = norm_bwd_launch<T, V, 256, 2>(a, nparts);
-    else if (packs <= 1024) rc = norm_bwd_launch<T, V, 256, 4>(a, nparts);
-    else {
-        long_rows = true;
-        if (a.dx) {
-            const unsigned blocks = (unsigned)(a.rows < 2048 ? a.rows : 2048);
-            norm_bwd_long_kernel<T, V><<<dim3(blocks), dim3(1024), 0, a.s>>>(a.rows, a.dim, (const T*)a.dy, a.dy_stride,
-                                                                            (const T*)a.x, a.x_stride, a.weight,
-                                                                            a.affine_dtype, a.mean, a.rstd, (T*)a.dx);
-            LAUNCH_OK("norm_bwd_long_kernel");
-        }
-        if (a.part) {
-            nparts = (uint32_t)(a.rows < NORM_LONG_PARTS ? a.rows : NORM_LONG_PARTS);
-            norm_cols_kernel<T><<<dim3(nparts, (unsigned)((a.dim + 255) / 256)), dim3(256), 0, a.s>>>(
-                a.rows, a.dim, (const T*)a.dy, a.dy_stride, (const T*)a.x, a.x_stride, a.mean, a.rstd, a.part);
-            LAUNCH_OK("norm_cols_kernel");
-        }
-    }
-    if (rc || !a.part || (nparts == 1 && !long_rows)) return rc;
+    else if (fits(16)) rc = norm_bwd_v<T, N>(a, nparts);
+    else if (a.dim > 512 && fits(8)) rc = norm_bwd_long<T, N / 2>(a, nparts);
+    else if (a.dim > 512 && N == 8 && fits(4)) rc = norm_bwd_long<T, N == 8 ? 2 : 1>(a, nparts);
+    else rc = norm_bwd_v<T, 1>(a, nparts);
+    if (rc || !a.part || nparts == 0) return rc;
     norm_join_kernel<<<dim3((unsigned)((2 * a.dim + 63) / 64)), dim3(1024), 0, a.s>>>(nparts, a.dim, a.part, a.affine_dtype,
                                                                                     a.dweight, a.dbias);
     LAUNCH_OK("norm_join_kernel");
@@ -1662,10 +1736,8 @@ int e3_layer_norm_forward_impl(size_t rows, size_t dim, const void* x, size_t x_
     NormArgs a{};
     a.rows = rows; a.dim = dim; a.x = x; a.x_stride = x_stride; a.weight = weight; a.bias = bias;
     a.affine_dtype = affine_dtype; a.eps = eps; a.out = out; a.mean = mean; a.rstd = rstd; a.s = s;
-    const bool wide = e3_rows_wide(x, x_stride, dim, dtype) && e3_rows_wide(out, dim, dim, dtype);
-    if (dtype == E3_F32) return wide ? norm_fwd_v<float, 4>(a) : norm_fwd_v<float, 1>(a);
-    if (dtype == E3_F16) return wide ? norm_fwd_v<f16_t, 8>(a) : norm_fwd_v<f16_t, 1>(a);
-    return wide ? norm_fwd_v<bf16_t, 8>(a) : norm_fwd_v<bf16_t, 1>(a);
+    if (dtype == E3_F32) return norm_fwd_t<float>(a, dtype);
+    return dtype == E3_F16 ? norm_fwd_t<f16_t>(a, dtype) : norm_fwd_t<bf16_t>(a, dtype);
 }
 
 size_t e3_layer_norm_scratch_bytes(size_t rows, size_t dim) {
@@ -1686,9 +1758,6 @@ int e3_layer_norm_backward_impl(size_t rows, size_t dim, const void* dy, size_t 
         LAUNCH_OK("norm_join_kernel");
         return 0;
     }
-    const bool wide = e3_rows_wide(x, x_stride, dim, dtype) && e3_rows_wide(dy, dy_stride, dim, dtype) &&
-                      (!dx || e3_rows_wide(dx, dim, dim, dtype));
-    if (dtype == E3_F32) return wide ? norm_bwd_v<float, 4>(a) : norm_bwd_v<float, 1>(a);
-    if (dtype == E3_F16) return wide ? norm_bwd_v<f16_t, 8>(a) : norm_bwd_v<f16_t, 1>(a);
-    return wide ? norm_bwd_v<bf16_t, 8>(a) : norm_bwd_v<bf16_t, 1>(a);
+    if (dtype == E3_F32) return norm_bwd_t<float>(a, dtype);
+    return dtype == E3_F16 ? norm_bwd_t<f16_t>(a, dtype) : norm_bwd_t<bf16_t>(a, dtype);
 }

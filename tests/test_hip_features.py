@@ -193,6 +193,16 @@ def test_layer_norm_long_rows(dtype, dim):
         check_layer_norm(rand(n, dim).to(dtype), rand(dim, seed=1).to(dtype), rand(dim, seed=2).to(dtype), rand(n, dim, seed=3).to(dtype))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [514, 516, 1020, 1026, 1446, 1537, 2050, 2052, 4090, 4097, 4100, 4588, 8190, 8193, 8196, 8200, 12290,
+                                 16382, 16384, 16386, 16388, 16392])
+def test_layer_norm_rows_of_four_and_eight_bytes(dtype, dim):
+    """Long rows on boundaries of 2, 4, 8 and 16 bytes, up to where another kernel takes over; one workgroup and several."""
+    for n in (3, 11):
+        check_layer_norm((rand(n, dim) + 0.5).to(dtype), (1 + 0.2 * rand(dim)).to(dtype), rand(dim, seed=3).to(dtype),
+                         rand(n, dim, seed=4).to(dtype))
+
+
 @pytest.mark.parametrize("n, dim", [(0, 8), (1, 48), (2, 4096), (20000, 48), (9000, 5), (5003, 59), (3000, 264)])
 def test_layer_norm_row_counts(n, dim):
     grads = check_layer_norm(rand(n, dim), rand(dim), rand(dim, seed=1), rand(n, dim, seed=2))
