@@ -1519,6 +1519,20 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(uint32_t nparts, size_t
 }
 
 namespace {
+// Workgroups of 256 CUs that are resident together.  Long rows are spread over no more than that, each the same number of
+// rows: more workgroups fetch the parameters again, and the last ones leave most of the chip idle (forward, 4096 x 8192 bf16
+// with 4096 workgroups 55 us, 1024 52 us, 768 = all resident 40 us).
+template <typename K>
+size_t resident_blocks(K kernel, int threads) {
+    int n = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, reinterpret_cast<const void*>(kernel), threads, 0) != hipSuccess || n < 1) n = 1;
+    (void)hipGetLastError();
+    return (size_t)n * 256;
+}
+unsigned even_blocks(size_t need, size_t most) {
+    const size_t rounds = (need + most - 1) / most;
+    return (unsigned)((need + rounds - 1) / rounds);
+}
 // workgroups of a launch over `rows` rows: enough to fill 256 CUs several times over, each with a few rows of its own
 unsigned norm_blocks(size_t rows, int per_block, size_t most) {
     const size_t need = (rows + per_block - 1) / per_block;
@@ -1533,7 +1547,9 @@ unsigned norm_bwd_blocks(size_t rows, int per_block, size_t most) {
     const size_t need = (rows + per_block - 1) / per_block;
     if (need <= 4) return 1u;
     const size_t blocks = need <= 256 ? need : need / 4 < 256 ? 256 : need / 4;
-    return (unsigned)(blocks < most ? blocks : most);
+    // (a workgroup per row: the same number of rounds for all; otherwise there are many rounds, and 1024 partial sums are
+    // joined faster than 962)
+    return per_block == 1 ? even_blocks(need, blocks < most ? blocks : most) : (unsigned)(blocks < most ? blocks : most);
 }
 constexpr size_t NORM_FWD_BLOCKS = 4096, NORM_BWD_BLOCKS = 1024, NORM_TILE_BLOCKS = 1024, NORM_LONG_PARTS = 64;
 
@@ -1551,7 +1567,9 @@ NormSums norm_sums(const NormArgs& a) { return {a.part, a.dweight, a.dbias, a.af
 
 template <typename T, int V, int G, int ITEMS>
 int norm_fwd_launch(const NormArgs& a) {
-    const dim3 blocks(norm_blocks(a.rows, NormRow<G>::PER_BLOCK, G >= 256 ? NORM_FWD_BLOCKS / 2 : NORM_FWD_BLOCKS)), threads(NormRow<G>::THREADS);
+    const dim3 threads(NormRow<G>::THREADS);
+    static const size_t most = resident_blocks(norm_fwd_kernel<false, T, V, G, ITEMS>, NormRow<G>::THREADS);
+    const dim3 blocks(G < 256 ? norm_blocks(a.rows, NormRow<G>::PER_BLOCK, NORM_FWD_BLOCKS) : even_blocks(a.rows, most));
 #define E3_NORM(S)                                                                                                            \
     norm_fwd_kernel<(S), T, V, G, ITEMS><<<blocks, threads, 0, a.s>>>(a.rows, (int)a.dim, (const T*)a.x, a.x_stride, a.weight, \
                                                                   a.bias, a.affine_dtype, a.eps, (T*)a.out, a.mean, a.rstd)
@@ -1564,7 +1582,8 @@ int norm_fwd_launch(const NormArgs& a) {
 }
 template <typename T, int V, int G, int ITEMS>
 int norm_bwd_launch(const NormArgs& a, uint32_t& nparts) {
-    nparts = norm_bwd_blocks(a.rows, NormRow<G>::PER_BLOCK, G > 256 ? NORM_BWD_BLOCKS / 2 : NORM_BWD_BLOCKS);
+    static const size_t most = resident_blocks(norm_bwd_kernel<false, T, V, G, ITEMS>, NormRow<G>::THREADS);
+    nparts = norm_bwd_blocks(a.rows, NormRow<G>::PER_BLOCK, G < 256 || most > NORM_BWD_BLOCKS ? NORM_BWD_BLOCKS : most);
     const dim3 blocks(nparts), threads(NormRow<G>::THREADS);
 #define E3_NORM(S)                                                                                                            \
     norm_bwd_kernel<(S), T, V, G, ITEMS><<<blocks, threads, 0, a.s>>>(a.rows, (int)a.dim, (const T*)a.dy, a.dy_stride,          \
