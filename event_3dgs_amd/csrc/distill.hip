@@ -315,24 +315,27 @@ __global__ __launch_bounds__(RowsLds<G>::THREADS) void distill_fwd_rows_kernel(c
             soft_add<1>(m, s, &v, c);
         }
         const Pack<T, V>* zp = reinterpret_cast<const Pack<T, V>*>(z + cut.head);
-        uint32_t i = lane;
-        for (; i + (SOFT_UNROLL - 1) * G < cut.packs; i += SOFT_UNROLL * G) {
+        for (uint32_t i = lane; i < cut.packs; i += SOFT_UNROLL * G) {      // (a batch of loads, unconditional)
             Pack<T, V> p[SOFT_UNROLL];
 #pragma unroll
-            for (int u = 0; u < SOFT_UNROLL; ++u) p[u] = zp[i + u * G];
-            float v[SOFT_UNROLL * V];
+            for (int u = 0; u < SOFT_UNROLL; ++u) p[u] = zp[i + u * G < cut.packs ? i + u * G : i];
+            if (i - lane + SOFT_UNROLL * G <= cut.packs) {                  // (the same for all lanes)
+                float v[SOFT_UNROLL * V];
 #pragma unroll
-            for (int u = 0; u < SOFT_UNROLL; ++u)
+                for (int u = 0; u < SOFT_UNROLL; ++u)
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[u * V + j] = (float)p[u].v[j];
-            soft_add<SOFT_UNROLL * V>(m, s, v, c);
-        }
-        for (; i < cut.packs; i += G) {
-            const Pack<T, V> p = zp[i];
-            float v[V];
+                    for (int j = 0; j < V; ++j) v[u * V + j] = (float)p[u].v[j];
+                soft_add<SOFT_UNROLL * V>(m, s, v, c);
+                continue;
+            }
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = (float)p.v[j];
-            soft_add<V>(m, s, v, c);
+            for (int u = 0; u < SOFT_UNROLL; ++u) {
+                if (i + u * G >= cut.packs) break;
+                float v[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] = (float)p[u].v[j];
+                soft_add<V>(m, s, v, c);
+            }
         }
         row_soft<G>(m, s, c, L);
         if (labeller) {
@@ -971,7 +974,6 @@ int distill_tile(DistillArgs a, int tile, unsigned& blocks, hipStream_t s) {
     return distill_tile_launch<true, T, MODE>(a, tile, blocks, s);
 }
 
-// Threads of a long row: a wave up to some thousand classes, a workgroup beyond that.
 template <typename T, int V, int G>
 int distill_rows_launch(const DistillArgs& a, bool backward, unsigned& blocks, hipStream_t s) {
     blocks = distill_blocks(a.rows, RowsLds<G>::ROWS);
@@ -982,10 +984,16 @@ int distill_rows_launch(const DistillArgs& a, bool backward, unsigned& blocks, h
     LAUNCH_OK("distill_rows_kernel");
     return 0;
 }
+// Lanes of a long row: a wave for as long as the rows fill the chip that way (every workgroup of a row waits for the slowest
+// wave and for the label: value of 25061 x 2653 fp16 95 us with 256 threads to a row, 54 with a wave; 10000 x 9000 bf16 53 and
+// 44 us, its gradient 61 and 64), 256 threads beyond, 1024 threads for the gradient of long rows and where there are fewer rows
+// than CUs (value of 4096 x 32000 bf16 118 us with 1024 threads, 54 with 256; of 100 x 128000 15 and 18 us; gradient of
+// 2000 x 128000 186 and 207 us).
 template <typename T, int V>
 int distill_rows(const DistillArgs& a, bool backward, unsigned& blocks, hipStream_t s) {
-    if (a.classes <= 2048) return distill_rows_launch<T, V, 64>(a, backward, blocks, s);
-    if (a.classes <= 16384) return distill_rows_launch<T, V, 256>(a, backward, blocks, s);
+    const size_t bytes = a.classes * sizeof(T);
+    if (a.classes <= 2048 || (a.rows >= 1024 && bytes <= (backward ? 16384 : 32768))) return distill_rows_launch<T, V, 64>(a, backward, blocks, s);
+    if (a.classes <= 16384 || (!backward && a.rows >= 256)) return distill_rows_launch<T, V, 256>(a, backward, blocks, s);
     return distill_rows_launch<T, V, 1024>(a, backward, blocks, s);
 }
 

@@ -462,6 +462,20 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(const uint32_t* __rest
     }
 }
 
+// The lanes of a wave that hold the same digit of `bits` bits (up to 8).
+__device__ __forceinline__ unsigned long long digit_peers(uint32_t d, int bits) {
+    uint32_t lo = ~0u, hi = ~0u;
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        if (b >= bits) break;
+        const int bit = (int)(d << (31 - b)) >> 31;          // 0 or -1
+        const unsigned long long bal = __ballot(bit < 0);
+        lo &= ~((uint32_t)bal ^ (uint32_t)bit);
+        hi &= ~((uint32_t)(bal >> 32) ^ (uint32_t)bit);
+    }
+    return (unsigned long long)hi << 32 | lo;
+}
+
 // Sorts up to 1024 * ITEMS positions by index in one workgroup (stable, 8 bits a pass): for few positions the launches of the
 // general sort would cost more than everything else.  A wave owns 64 * ITEMS consecutive keys and ranks 64 at a time with
 // ballots; the digits' counters of the 16 waves are joined by a prefix over waves and digits.  Indices outside the table get
@@ -475,7 +489,7 @@ struct SmallSort {
     uint32_t wtot[4], valid;
 };
 template <int ITEMS, typename I>
-__global__ __launch_bounds__(1024) void embed_sort_small_kernel(uint32_t n, uint32_t rows, int nbits,
+__global__ __launch_bounds__(1024) void embed_sort_small_kernel(uint32_t n, uint32_t rows, int passes, int bits,
                                                                 const I* __restrict__ index, uint32_t* __restrict__ keys,
                                                                 uint32_t* __restrict__ pos, uint32_t* __restrict__ kept) {
     __shared__ SmallSort<ITEMS> L;
@@ -500,21 +514,14 @@ __global__ __launch_bounds__(1024) void embed_sort_small_kernel(uint32_t n, uint
         mine += (uint32_t)__popcll(__ballot(ok));
     }
     if (lane == 0) atomicAdd(&L.valid, mine);
-    for (int shift = 0; shift < nbits; shift += 8) {
+    const uint32_t mask = (1u << bits) - 1u;
+    for (int pass = 0, shift = 0; pass < passes; ++pass, shift += bits) {
         for (int d = threadIdx.x; d < 16 * 256; d += 1024) L.cnt[d >> 8][d & 255] = 0;
         __syncthreads();
 #pragma unroll 1
         for (int i = 0; i < ITEMS; ++i) {
-            const uint32_t d = (L.key[base + i * 64] >> shift) & 255u;
-            uint32_t plo = ~0u, phi = ~0u;                   // lanes with the same digit
-#pragma unroll
-            for (int b = 0; b < 8; ++b) {
-                const int bit = (int)(d << (31 - b)) >> 31;  // 0 or -1
-                const unsigned long long bal = __ballot(bit < 0);
-                plo &= ~((uint32_t)bal ^ (uint32_t)bit);
-                phi &= ~((uint32_t)(bal >> 32) ^ (uint32_t)bit);
-            }
-            const unsigned long long peers = (unsigned long long)phi << 32 | plo;
+            const uint32_t d = L.key[base + i * 64] >> shift & mask;
+            const unsigned long long peers = digit_peers(d, bits);
             const uint32_t first = L.cnt[wave][d];
             wave_sync();
             if ((peers & before) == 0ull) L.cnt[wave][d] = first + (uint32_t)__popcll(peers);
@@ -542,7 +549,7 @@ __global__ __launch_bounds__(1024) void embed_sort_small_kernel(uint32_t n, uint
         for (int i = 0; i < ITEMS; ++i) {
             k[i] = L.key[base + i * 64];
             p[i] = L.pos[base + i * 64];
-            const uint32_t d = (k[i] >> shift) & 255u, q = d >> 6;
+            const uint32_t d = k[i] >> shift & mask, q = d >> 6;
             to[i] = L.cnt[wave][d] + L.rank[base + i * 64] + (q == 0 ? 0u : q == 1 ? t1 : q == 2 ? t2 : t3);
         }
         __syncthreads();
@@ -687,11 +694,7 @@ __global__ __launch_bounds__(1024) void embed_scatter_kernel(uint32_t n, int shi
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const uint32_t d = sort_digit(k[i], shift, mask);
-        unsigned long long peers = ~0ull;                   // lanes with the same digit
-        for (int b = 0; b < bits; ++b) {
-            const unsigned long long bal = __ballot(d >> b & 1u);
-            peers &= d >> b & 1u ? bal : ~bal;
-        }
+        const unsigned long long peers = digit_peers(d, bits);
         const uint32_t first = L.cnt[wave][d];
         wave_sync();
         if ((peers & before) == 0ull) L.cnt[wave][d] = first + (uint32_t)__popcll(peers);
@@ -808,22 +811,28 @@ int embed_join_launch(const EmbedScratch& w, const uint32_t* keys, size_t n, siz
     return 0;
 }
 
+// Passes and bits of a digit (up to 8, the same in every pass) for the keys 0 .. rows: the key `rows` itself occurs.
+void embed_digits(uint32_t rows, int& passes, int& bits) {
+    int nbits = 1;
+    while (rows >> nbits) ++nbits;
+    passes = (nbits + 7) / 8;
+    bits = (nbits + passes - 1) / passes;
+}
 template <typename I>
-void embed_sort_small(uint32_t n, uint32_t rows, int nbits, const I* index, uint32_t* keys, uint32_t* pos, uint32_t* kept,
+void embed_sort_small(uint32_t n, uint32_t rows, int passes, int bits, const I* index, uint32_t* keys, uint32_t* pos, uint32_t* kept,
                       hipStream_t s) {
-    if (n <= 1024) embed_sort_small_kernel<1, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, nbits, index, keys, pos, kept);
-    else if (n <= 4096) embed_sort_small_kernel<4, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, nbits, index, keys, pos, kept);
-    else if (n <= 8192) embed_sort_small_kernel<8, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, nbits, index, keys, pos, kept);
-    else embed_sort_small_kernel<16, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, nbits, index, keys, pos, kept);
+    if (n <= 1024) embed_sort_small_kernel<1, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, passes, bits, index, keys, pos, kept);
+    else if (n <= 4096) embed_sort_small_kernel<4, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, passes, bits, index, keys, pos, kept);
+    else if (n <= 8192) embed_sort_small_kernel<8, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, passes, bits, index, keys, pos, kept);
+    else embed_sort_small_kernel<16, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, passes, bits, index, keys, pos, kept);
 }
 
 // The tiles' sort; keys / pos: where the result lies.
 template <int ITEMS>
 int embed_sort_tiles(const EmbedScratch& w, uint32_t n, uint32_t rows, const void* index, int index_bytes, uint32_t** keys,
                      uint32_t** pos, hipStream_t s) {
-    int nbits = 1;
-    while (rows >> nbits) ++nbits;                             // (the key `rows` itself occurs)
-    const int passes = (nbits + 7) / 8, bits = (nbits + passes - 1) / passes;
+    int passes, bits;
+    embed_digits(rows, passes, bits);
     const uint32_t tiles = (n + 1024 * ITEMS - 1) / (1024 * ITEMS), mask = (1u << bits) - 1u;
     uint32_t *counts = w.sort, *valid = w.sort + SORT_TILES * 256;
     uint32_t *k0 = w.key0, *k1 = w.key1, *p0 = w.pos0, *p1 = w.pos1;
@@ -851,10 +860,10 @@ int embed_bwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_
     uint32_t *keys = w.key0, *pos = w.pos0;
     int rc = 0;
     if (n > EMBED_TINY && n <= 16384) {
-        int nbits = 1;
-        while (rows >> nbits) ++nbits;                         // (the key `rows` itself occurs)
-        if (index_bytes == 8) embed_sort_small((uint32_t)n, (uint32_t)rows, nbits, (const long long*)index, keys, pos, w.kept, s);
-        else embed_sort_small((uint32_t)n, (uint32_t)rows, nbits, (const int*)index, keys, pos, w.kept, s);
+        int passes, bits;
+        embed_digits((uint32_t)rows, passes, bits);
+        if (index_bytes == 8) embed_sort_small((uint32_t)n, (uint32_t)rows, passes, bits, (const long long*)index, keys, pos, w.kept, s);
+        else embed_sort_small((uint32_t)n, (uint32_t)rows, passes, bits, (const int*)index, keys, pos, w.kept, s);
         LAUNCH_OK("embed_sort_small_kernel");
     } else if (n > EMBED_TINY && n <= SORT_TILES * 8192) {
 #define E3_TILES(ITEMS) embed_sort_tiles<ITEMS>(w, (uint32_t)n, (uint32_t)rows, index, index_bytes, &keys, &pos, s)
@@ -1660,7 +1669,6 @@ int norm_fwd_long(const NormArgs& a) {
     if (packs <= 256) return norm_fwd_launch<T, V, 64, 4>(a);
     if (packs <= 512) return norm_fwd_launch<T, V, 256, 2>(a);
     if (packs <= 1024) return norm_fwd_launch<T, V, 256, 4>(a);
-    if (V == 1) return norm_fwd_again<T, V>(a);
     if (packs <= 2048) return norm_fwd_launch<T, V, 512, 4>(a);
     if (packs <= 1024 * MORE) return norm_fwd_launch<T, V, 1024, MORE>(a);
     if (packs <= 1024 * MOST) return norm_fwd_launch<T, V, 1024, MOST>(a);
