@@ -259,9 +259,9 @@ __device__ __forceinline__ Cut cut_row(const T* p, uint32_t n) {
 }
 
 // LDS of a workgroup of the row kernels: a label per row, the waves' (max, sum), the label's summary
-template <int G>
+template <int G, int WORKGROUP = (G > 256 ? G : 256)>
 struct RowsLds {
-    static constexpr int THREADS = G > 256 ? G : 256;
+    static constexpr int THREADS = WORKGROUP;
     static constexpr int ROWS = THREADS / G;
     int ids[ROWS][DISTILL_MAX_K];
     float ws[ROWS][DISTILL_MAX_K];
@@ -270,19 +270,19 @@ struct RowsLds {
 };
 // (max, sum) over the lanes of a row.  Workgroup rows: ONE barrier (the caller keeps another between two uses).
 template <int G>
-__device__ __forceinline__ void row_soft(float& m, float& s, float c, RowsLds<G>& L) {
+__device__ __forceinline__ void row_soft(float& m, float& s, float c, float* ms) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
         soft_merge(m, s, m2, s2, c);
     }
     if (G == 64) return;
-    if ((threadIdx.x & 63) == 0) { L.ms[2 * (threadIdx.x >> 6)] = m; L.ms[2 * (threadIdx.x >> 6) + 1] = s; }
+    if ((threadIdx.x & 63) == 0) { ms[2 * (threadIdx.x >> 6)] = m; ms[2 * (threadIdx.x >> 6) + 1] = s; }
     __syncthreads();
-    m = L.ms[0];
-    s = L.ms[1];
+    m = ms[0];
+    s = ms[1];
 #pragma unroll
-    for (int w = 1; w < G / 64; ++w) soft_merge(m, s, L.ms[2 * w], L.ms[2 * w + 1], c);
+    for (int w = 1; w < G / 64; ++w) soft_merge(m, s, ms[2 * w], ms[2 * w + 1], c);
 }
 template <int G>
 __device__ __forceinline__ void row_sync() {      // orders the row's stores before and behind this point
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(RowsLds<G>::THREADS) void distill_fwd_rows_kernel(c
                 soft_add<V>(m, s, v, c);
             }
         }
-        row_soft<G>(m, s, c, L);
+        row_soft<G>(m, s, c, L.ms);
         if (labeller) {
             const Label l = wave_label(a, row, c, L.ids[slot], L.ws[slot]);
             float d = label_value(a, row, l, L.ids[slot], L.ws[slot], threadIdx.x & 63, 64, m, s, rt,
@@ -418,7 +418,7 @@ __global__ __launch_bounds__(RowsLds<G>::THREADS) void distill_bwd_rows_kernel(c
 // statistics and the gradient, so the scores are read once and the gradient is written once.
 template <bool STREAM, typename T, int V, int G, int ITEMS>
 __global__ __launch_bounds__(G) void distill_both_rows_kernel(const DistillArgs a) {
-    __shared__ RowsLds<G> L;
+    __shared__ RowsLds<G, G> L;
     const int lane = threadIdx.x;
     const float rt = 1.0f / a.temperature, c = LOG2E * rt;
     const float f = a.temperature * row_weight<G>(a, reinterpret_cast<uint32_t*>(L.ms));
@@ -469,7 +469,7 @@ __global__ __launch_bounds__(G) void distill_both_rows_kernel(const DistillArgs 
             }
 #pragma unroll
         for (int u = 0; u < ITEMS; ++u) forget(p[u]);
-        row_soft<G>(m, s, c, L);
+        row_soft<G>(m, s, c, L.ms);
         if (threadIdx.x < 64) {
             float d = label_value(a, row, l, L.ids[0], L.ws[0], lane, 64, m, s, rt, [&](int id) { return (float)z[id]; });
             d = group_sum<64>(d) * (a.temperature * a.temperature);
@@ -1064,7 +1064,9 @@ int distill_both_t(DistillArgs a, uint32_t* counts, unsigned& blocks, hipStream_
     const size_t packs = a.classes / V;
     if (!tile && (a.classes * sizeof(T) <= 4096 || packs > 16384 || !rows_wide<T>(a, true))) return 0;
     blocks = distill_blocks(a.rows, tile ? tile : 1);
-    if (a.reduction == 1 && blocks > 1 && a.rows * a.k > 4096) {      // (fewer are counted by every workgroup for itself)
+    // a wave to a row of up to 16 KB where the rows fill the chip that way (50000 x 2500 bf16: with 256 threads 293 us)
+    const bool wave_rows = !tile && a.rows >= 1024 && packs <= 1024;
+    if (a.reduction == 1 && blocks > 1 && (wave_rows || a.rows * a.k > 4096)) {      // (fewer are counted by every workgroup for itself)
         const size_t need = (a.rows * (a.i_entry == 1 ? a.k : 1) + 255) / 256;
         a.counts = counts;
         a.ncounts = (uint32_t)(need < COUNT_BLOCKS ? need : COUNT_BLOCKS);
@@ -1075,7 +1077,9 @@ int distill_both_t(DistillArgs a, uint32_t* counts, unsigned& blocks, hipStream_
 #define E3_BOTH(G, ITEMS)                                                                                          \
     if (grad_streams<T>(a)) distill_both_rows_kernel<true, T, V, G, ITEMS><<<dim3(blocks), dim3(G), 0, s>>>(a);    \
     else distill_both_rows_kernel<false, T, V, G, ITEMS><<<dim3(blocks), dim3(G), 0, s>>>(a)
-    if (packs <= 1024) { E3_BOTH(256, 4); }
+    if (wave_rows && packs <= 512) { E3_BOTH(64, 8); }
+    else if (wave_rows) { E3_BOTH(64, 16); }
+    else if (packs <= 1024) { E3_BOTH(256, 4); }
     else if (packs <= 2048) { E3_BOTH(256, 8); }
     else if (packs <= 4096) { E3_BOTH(256, 16); }
     else if (packs <= 8192) { E3_BOTH(1024, 8); }

@@ -336,7 +336,9 @@ def check_distill(z, t, index, temp=1.0, class_dim=-1, reductions=("none", "mean
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n, classes, k, temp", [
     (1, 1, 1, 1.0), (3, 2, 1, 1.0), (70, 7, 7, 2.0), (33, 19, 3, 1.0), (17, 64, 5, 0.5), (40, 65, 64, 1.0), (9, 151, 8, 2.0),
-    (21, 1000, 20, 1.0), (600, 50, 2, 1.0), (5, 2048, 100, 4.0), (30, 40, 40, 1.0), (2, 9000, 1000, 1.0), (700, 5000, 9, 1.0), (6, 2049, 33, 1.0), (3, 16384, 7, 1.0), (2, 16391, 300, 2.0), (2, 50001, 64, 1.0)])
+    (21, 1000, 20, 1.0), (600, 50, 2, 1.0), (5, 2048, 100, 4.0), (30, 40, 40, 1.0), (2, 9000, 1000, 1.0), (700, 5000, 9, 1.0), (6, 2049, 33, 1.0), (3, 16384, 7, 1.0), (2, 16391, 300, 2.0), (2, 50001, 64, 1.0),
+                                                (1100, 2100, 3, 2.0), (1024, 3001, 70, 1.0), (1030, 4001, 2, 1.0), (1050, 8000, 5, 1.0), (1040, 9000, 3, 1.0),
+                                                (300, 20000, 3, 1.0)])
 def test_distill_rows(dtype, n, classes, k, temp):
     t, index = label(n, classes, k)
     check_distill((rand(n, classes) * 3).to(dtype), t.to(dtype), index.int(), temp)
@@ -428,6 +430,24 @@ def test_distill_unusable_rows(planes, classes):
     ref = torch.softmax(z[4], 0)
     ref[1:3] -= 0.5
     close(d[4], ref, 300 * U * (ref.abs() + 1), "a class that is switched off")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows, classes", [(1600, 2500), (1600, 4000), (1600, 5000), (1600, 30), (400, 2500), (300, 17000)])
+def test_distill_hard_rows_among_many(dtype, rows, classes):
+    """Rows without a label, of one listed class, of switched off classes and of NaN, as many as take another kernel."""
+    inf = math.inf
+    z = (rand(rows, classes) * 2).to(dtype)
+    t, index = label(rows, classes, 4, empty=0.3)
+    z[0::7, 1] = -inf
+    z[3::11, 2:classes // 2] = torch.finfo(dtype).min
+    z[(index < 0).all(1)] = float("nan")                         # not looked at
+    z.scatter_(1, index.clamp(min=0), torch.where((index < 0).all(1, keepdim=True), float("nan"), 1.5).to(dtype).expand(-1, 4).contiguous())
+    check_distill(z, t, index, 2.0)
+    index[5] = classes                                           # a broken row makes its own value and gradient NaN
+    value, d = losses.distill_loss_raw(z, t, index, 2.0, "none")
+    assert torch.isnan(value[5]) and torch.isnan(d[5]).all()
+    assert torch.isfinite(value[6:]).all() and torch.isfinite(d[6:]).all() and torch.isfinite(value[:5]).all()
 
 
 def test_distill_lowest_values():
