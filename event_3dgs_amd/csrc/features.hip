@@ -19,12 +19,11 @@ int launch_radix_sort_pairs(uint32_t* k0, uint32_t* k1, uint32_t* v0, uint32_t* 
 // ============================================================================================== embedding, forward
 // out[i, :] = round(scale * table[index[i], :]).  An index below 0 stands for "no row" (zeros); one past the table gives a
 // row of NaN -- an error that only the device sees, made visible without a wait.
-// One thread moves several packs of the flat output (4 of 16 bytes, 8 of 4 or 8, 16 single elements: a workgroup waits for the
-// index, then for the row, and has to have enough behind that), a workgroup's packs are contiguous: every lane works whatever
+// One thread moves several packs of the flat output (4 of 16 bytes, 8 of 4 or 8: a workgroup waits for the index, then for the row, and has to have enough behind that), a workgroup's packs are contiguous: every lane works whatever
 // the row length, the stores are whole lines, and the rows of a pack-block are found by one division each.
 template <typename T, int V>
 struct EmbedPacks {
-    static constexpr int N = V * (int)sizeof(T) == 16 ? 4 : V > 1 ? 8 : 16;
+    static constexpr int N = V * (int)sizeof(T) == 16 ? 4 : 8;
 };
 template <bool STREAM, typename T, int V, typename I>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(size_t n, long long rows, uint32_t ppr /* packs per row */,
@@ -71,6 +70,57 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(size_t n, long long rows
     }
 }
 
+// Rows that are no multiple of 4 bytes (8 for fp32), or do not lie on such a boundary: a workgroup gathers EMBED_FLAT values one
+// by one into LDS and stores them from there in packs.  The indices of its rows wait in LDS too: with an index, a value and a
+// store to each value the memory pipeline's issue rate was the bound (408482 x 115 fp16 51 us, EMBED_FLAT_ME).
+constexpr int EMBED_FLAT = 4096;
+template <bool STREAM, typename T, typename I>
+__global__ __launch_bounds__(256) void embed_fwd_odd_kernel(size_t n, long long rows, uint32_t dim, const I* __restrict__ index,
+                                                            const T* __restrict__ table, size_t stride, float scale, T* __restrict__ out) {
+    constexpr int EACH = EMBED_FLAT / 256, BATCH = 8, N = Wide<T>::N;
+    __shared__ words_t tile[EMBED_FLAT / N];
+    __shared__ int ids[EMBED_FLAT + 2];                              // -1: zeros, ID_PAST: NaN
+    constexpr int ID_PAST = 0x7FFFFFFF;
+    T* values = reinterpret_cast<T*>(tile);
+    const size_t total = n * (size_t)dim, base = (size_t)blockIdx.x * EMBED_FLAT;
+    const size_t row0 = base / dim;                                  // (uniform)
+    const uint32_t rem0 = (uint32_t)(base - row0 * dim);
+    const uint32_t count = total - base < EMBED_FLAT ? (uint32_t)(total - base) : EMBED_FLAT;
+    const uint32_t nids = (rem0 + count - 1) / dim + 1;
+    for (uint32_t i = threadIdx.x; i < nids; i += 256) {
+        const I id = index[row0 + i];
+        ids[i] = id < 0 ? -1 : id < rows ? (int)id : ID_PAST;
+    }
+    __syncthreads();
+    const uint32_t dq = 256 / dim, dr = 256 - dq * dim;
+    uint32_t q = (rem0 + threadIdx.x) / dim, c = rem0 + threadIdx.x - q * dim;
+#pragma unroll
+    for (int b = 0; b < EACH; b += BATCH) {
+        int id[BATCH];
+        uint32_t v[BATCH];                                           // (a register each: halves of one would wait for each other)
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+            id[u] = (uint32_t)(b + u) * 256 + threadIdx.x < count ? ids[q] : -1;
+            const bool in = id[u] >= 0 && id[u] != ID_PAST;
+            v[u] = reinterpret_cast<const Bits<T>*>(table)[in ? (size_t)(uint32_t)id[u] * stride + c : 0];      // (unconditional)
+            q += dq;
+            c += dr;
+            if (c >= dim) {
+                c -= dim;
+                ++q;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u)
+            values[(b + u) * 256 + threadIdx.x] = id[u] < 0 ? (T)0.0f : id[u] == ID_PAST ? (T)__builtin_nanf("") : (T)(scale * (float)bits_elem<T>(v[u]));
+    }
+    __syncthreads();
+    out += base;
+    const uint32_t packs = (reinterpret_cast<uintptr_t>(out) & 15) == 0 ? count / N : 0u;
+    for (uint32_t i = threadIdx.x; i < packs; i += 256) put<STREAM, T, N>(out + (size_t)i * N, reinterpret_cast<const Pack<T, N>*>(tile)[i]);
+    for (uint32_t i = packs * N + threadIdx.x; i < count; i += 256) out[i] = values[i];
+}
+
 template <bool STREAM, typename T, int V, typename I>
 static int embed_fwd_launch(size_t n, size_t rows, size_t dim, const void* index, const void* table, size_t stride, float scale,
                             void* out, hipStream_t s) {
@@ -86,12 +136,20 @@ static int embed_fwd_t(size_t n, size_t rows, size_t dim, const void* index, con
                        float scale, void* out, hipStream_t s) {
     constexpr int N = Wide<T>::N;
     const bool large = n * dim * sizeof(T) > E3_STREAM_BYTES;
+    if (rows == 0) table = index;                              // (no row is read; the odd kernel's loads need some address)
     auto fits = [&](size_t bytes) { return e3_rows_packs(table, stride, dim, dtype, bytes) && e3_rows_packs(out, dim, dim, dtype, bytes); };
     if (fits(16) && large) return embed_fwd_launch<true, T, N, I>(n, rows, dim, index, table, stride, scale, out, s);
     if (fits(16)) return embed_fwd_launch<false, T, N, I>(n, rows, dim, index, table, stride, scale, out, s);
     if (fits(8)) return embed_fwd_launch<false, T, N / 2, I>(n, rows, dim, index, table, stride, scale, out, s);
-    if (N == 8 && fits(4)) return embed_fwd_launch<false, T, N == 8 ? 2 : 1, I>(n, rows, dim, index, table, stride, scale, out, s);
-    return embed_fwd_launch<false, T, 1, I>(n, rows, dim, index, table, stride, scale, out, s);
+    if (N == 8 && fits(4)) return embed_fwd_launch<false, T, 2, I>(n, rows, dim, index, table, stride, scale, out, s);
+    const size_t blocks = (n * dim + EMBED_FLAT - 1) / EMBED_FLAT;
+    if (blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_forward: too many values");
+    if (large) embed_fwd_odd_kernel<true, T, I><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(
+        n, (long long)rows, (uint32_t)dim, (const I*)index, (const T*)table, stride, scale, (T*)out);
+    else embed_fwd_odd_kernel<false, T, I><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(
+        n, (long long)rows, (uint32_t)dim, (const I*)index, (const T*)table, stride, scale, (T*)out);
+    LAUNCH_OK("embed_fwd_odd_kernel");
+    return 0;
 }
 
 int e3_embedding_forward_impl(size_t n, size_t rows, size_t dim, const void* index, int index_bytes, const void* table,
@@ -252,15 +310,14 @@ __global__ __launch_bounds__(256) void embed_tiny_kernel(uint32_t n, uint32_t ro
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = 0.0f;
     for (uint32_t b = lo; b < hi && col < dim; b += UNROLL) {
-        Pack<T, V> r[UNROLL];
+        Held<T, V> r[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-            r[u] = *reinterpret_cast<const Pack<T, V>*>(d_out + (size_t)list[b + u < hi ? b + u : hi - 1] * stride + col);
+        for (int u = 0; u < UNROLL; ++u) r[u].load(d_out + (size_t)list[b + u < hi ? b + u : hi - 1] * stride + col);
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             if (b + u >= hi) break;
 #pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] += (float)r[u].v[j];
+            for (int j = 0; j < V; ++j) acc[j] += r[u].value(j);
         }
     }
     if (m > 1) {                                                               // (uniform)
@@ -313,12 +370,12 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restri
     bool from_before = j0 > 0 && keys[j0 - 1] == cur;       // the run in hand began in an earlier chunk
     for (uint32_t b = j0; b < j1; b += EMBED_UNROLL) {
         uint32_t k[EMBED_UNROLL];
-        Pack<T, V> r[EMBED_UNROLL];
+        Held<T, V> r[EMBED_UNROLL];
 #pragma unroll
         for (int u = 0; u < EMBED_UNROLL; ++u) {            // (entries behind the chunk read its last one and are not added)
             const uint32_t at = b + u < j1 ? b + u : j1 - 1;
             k[u] = keys[at];
-            r[u] = *reinterpret_cast<const Pack<T, V>*>(d_out + (size_t)pos[at] * stride + col);
+            r[u].load(d_out + (size_t)pos[at] * stride + col);
         }
 #pragma unroll
         for (int u = 0; u < EMBED_UNROLL; ++u) {
@@ -336,7 +393,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restri
                 for (int j = 0; j < V; ++j) acc[j] = 0.0f;
             }
 #pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] += (float)r[u].v[j];
+            for (int j = 0; j < V; ++j) acc[j] += r[u].value(j);
         }
     }
     const bool goes_on = j1 < n && keys[j1] == cur;
@@ -1034,19 +1091,21 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_fwd_kernel(size_t ro
         const size_t row = base + threadIdx.x / G;
         const bool live = row < rows;
         float v[ITEMS][V], s = 0.0f;
+        const T* xr = x + (live ? row : rows - 1) * stride;
+        Held<T, V> xh[ITEMS];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {                   // (unconditional loads, all in flight)
+            const int col = (i * G + lane) * V;
+            xh[i].load(xr + (col < dim ? col : 0));
+        }
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            const int col = (i * G + lane) * V;
-            if (live && col < dim) {
-                const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(x + row * stride + col);
+            const bool in = (i * G + lane) * V < dim;
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[i][j] = (float)p.v[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
+            for (int j = 0; j < V; ++j) {
+                v[i][j] = in ? xh[i].value(j) : 0.0f;
+                s += v[i][j];
             }
-#pragma unroll
-            for (int j = 0; j < V; ++j) s += v[i][j];
         }
         const float mean = R::sum(s, lds) * inv;
         float q = 0.0f;
@@ -1377,19 +1436,43 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_bwd_kernel(size_t ro
     for (size_t base = (size_t)blockIdx.x * R::PER_BLOCK; base < rows; base += step) {
         const size_t row = base + threadIdx.x / G;
         const bool live = row < rows;
+        const size_t at = live ? row : rows - 1;
         const float mean = live ? mean_in[row] : 0.0f, rstd = live ? rstd_in[row] : 0.0f;
         float h[ITEMS][V], g[ITEMS][V], s1 = 0.0f, s2 = 0.0f;
+        // All loads first, unconditional, where a thread has four packs or more (4096 x 8192 bf16 44 us, pack by pack 52); with
+        // two of them the other waves hide the latency (8192 x 4096 bf16 42 us, 45 so), and 16 values in 1024 threads leave no
+        // registers for it.
+        if constexpr (ITEMS >= 4 && !(G == 1024 && ITEMS * V == 16)) {
+            Held<T, V> xh[ITEMS], dh[ITEMS];
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int col = (i * G + lane) * V;
-            if (live && col < dim) {
-                const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(x + row * stride + col);
-                const Pack<T, V> d = *reinterpret_cast<const Pack<T, V>*>(dy + row * dy_stride + col);
+            for (int i = 0; i < ITEMS; ++i) {
+                const int col = (i * G + lane) * V < dim ? (i * G + lane) * V : 0;
+                xh[i].load(x + at * stride + col);
+                dh[i].load(dy + at * dy_stride + col);
+            }
 #pragma unroll
-                for (int j = 0; j < V; ++j) { h[i][j] = (float)p.v[j]; g[i][j] = (float)d.v[j]; }
-            } else {
+            for (int i = 0; i < ITEMS; ++i) {
+                const bool in = live && (i * G + lane) * V < dim;
 #pragma unroll
-                for (int j = 0; j < V; ++j) { h[i][j] = mean; g[i][j] = 0.0f; }
+                for (int j = 0; j < V; ++j) {
+                    h[i][j] = in ? xh[i].value(j) : mean;
+                    g[i][j] = in ? dh[i].value(j) : 0.0f;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int col = (i * G + lane) * V;
+                if (live && col < dim) {
+                    Held<T, V> p, d;
+                    p.load(x + row * stride + col);
+                    d.load(dy + row * dy_stride + col);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) { h[i][j] = p.value(j); g[i][j] = d.value(j); }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) { h[i][j] = mean; g[i][j] = 0.0f; }
+                }
             }
         }
 #pragma unroll

@@ -60,6 +60,28 @@ __device__ __forceinline__ void put(T* p, const Pack<T, V>& r) {
 static inline size_t e3_elem_bytes(int dtype) { return dtype == E3_F32 ? 4 : 2; }
 static inline bool e3_dtype_ok(int dtype) { return dtype >= E3_F32 && dtype <= E3_BF16; }
 
+// The bits of one element, and a pack on its way from memory.  A single 16-bit value is loaded into a register of its own: loads
+// that fill the halves of one register wait for each other.
+template <typename T>
+using Bits = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+template <typename T>
+__device__ __forceinline__ T bits_elem(uint32_t v) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, v);
+    else return __builtin_bit_cast(T, (uint16_t)v);
+}
+template <typename T, int V>
+struct Held {
+    Pack<T, V> p;
+    __device__ __forceinline__ void load(const T* src) { p = *reinterpret_cast<const Pack<T, V>*>(src); }
+    __device__ __forceinline__ float value(int j) const { return (float)p.v[j]; }
+};
+template <typename T>
+struct Held<T, 1> {
+    uint32_t bits;
+    __device__ __forceinline__ void load(const T* src) { bits = *reinterpret_cast<const Bits<T>*>(src); }
+    __device__ __forceinline__ float value(int) const { return (float)bits_elem<T>(bits); }
+};
+
 // Whether rows at `p`, `stride` elements apart and `dim` long, can be read as packs of `bytes` bytes (a power of two).
 static inline bool e3_rows_packs(const void* p, size_t stride, size_t dim, int dtype, size_t bytes) {
     const size_t n = bytes / e3_elem_bytes(dtype);

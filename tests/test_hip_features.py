@@ -105,9 +105,11 @@ def test_embedding_nothing_to_look_up():
     for index in (torch.empty(0, dtype=torch.int64, device=DEV), torch.full((70,), -1, device=DEV)):
         check_embedding(index, rand(5, 12), 1.0, rand(index.numel(), 12))
     check_embedding(torch.empty(0, 3, dtype=torch.int32, device=DEV), rand(4, 3).half(), 1.0, rand(0, 3, 3).half())
-    none = torch.empty(0, 8, device=DEV)
-    assert (features.embedding(torch.full((2,), -5, device=DEV), none) == 0).all()
-    assert torch.isnan(features.embedding(torch.zeros(2, dtype=torch.int64, device=DEV), none)).all()
+    for dim in (8, 7, 2, 1):
+        for dtype in TYPES:
+            none = torch.empty(0, dim, device=DEV, dtype=dtype)
+            assert (features.embedding(torch.full((2,), -5, device=DEV), none) == 0).all()
+            assert torch.isnan(features.embedding(torch.zeros(2, dtype=torch.int64, device=DEV), none)).all()
 
 
 def test_embedding_index_past_the_table():
