@@ -71,8 +71,8 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(size_t n, long long rows
 }
 
 // Rows that are no multiple of 4 bytes (8 for fp32), or do not lie on such a boundary: a workgroup gathers EMBED_FLAT values one
-// by one into LDS and stores them from there in packs.  The indices of its rows wait in LDS too: with an index, a value and a
-// store to each value the memory pipeline's issue rate was the bound (408482 x 115 fp16 51 us, EMBED_FLAT_ME).
+// by one into LDS and stores them from there in packs; the indices of its rows wait in LDS too.  Bound by the issue of the
+// single loads (408482 x 115 fp16 41 us; with an index and a store to every value 51 us; 21053 x 567 fp32 15 and 20 us).
 constexpr int EMBED_FLAT = 4096;
 template <bool STREAM, typename T, typename I>
 __global__ __launch_bounds__(256) void embed_fwd_odd_kernel(size_t n, long long rows, uint32_t dim, const I* __restrict__ index,
