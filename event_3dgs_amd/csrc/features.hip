@@ -1617,9 +1617,9 @@ namespace {
 template <typename K>
 size_t resident_blocks(K kernel, int threads) {
     int n = 0;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, reinterpret_cast<const void*>(kernel), threads, 0) != hipSuccess || n < 1) n = 1;
-    (void)hipGetLastError();
-    return (size_t)n * 256;
+    const hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, reinterpret_cast<const void*>(kernel), threads, 0);
+    if (e != hipSuccess) (void)hipGetLastError();          // (its own error alone is taken back)
+    return e == hipSuccess && n > 0 ? (size_t)n * 256 : 256;
 }
 unsigned even_blocks(size_t need, size_t most) {
     const size_t rounds = (need + most - 1) / most;
