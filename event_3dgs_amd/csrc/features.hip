@@ -1244,10 +1244,12 @@ __global__ __launch_bounds__(256) void norm_fwd_tile_kernel(size_t rows, int dim
         if (first + step < rows) next.load(x + (first + step) * dim, tile_count(rows, first + step, tile) * dim);
         const bool live = r < n;
         float v[NORM_TILE_ITEMS], s = 0.0f, q = 0.0f;
+        Held<T, 1> zh[NORM_TILE_ITEMS];
+#pragma unroll
+        for (int i = 0; i < NORM_TILE_ITEMS; ++i) zh[i].load(z + (i * LANES + lane < dim ? i * LANES + lane : 0));
 #pragma unroll
         for (int i = 0; i < NORM_TILE_ITEMS; ++i) {
-            const int c = i * LANES + lane;
-            v[i] = live && c < dim ? (float)z[c] : 0.0f;
+            v[i] = live && i * LANES + lane < dim ? zh[i].value(0) : 0.0f;
             s += v[i];
         }
         const float mean = lanes_sum(s, LANES) * inv;
@@ -1313,12 +1315,30 @@ __global__ __launch_bounds__(256) void norm_bwd_tile_kernel(size_t rows, int dim
         __syncthreads();
         if (first + step < rows) load(first + step, tile_count(rows, first + step, tile));
         float h[ITEMS], g[ITEMS], s1 = 0.0f, s2 = 0.0f;
+        // (16 values: all LDS reads first, 100000 x 300 bf16 87 us, value by value 99; with 8 values that would cost a workgroup of the
+        // CU its registers, 748061 x 65 fp16 152 us value by value, 235 so)
+        if constexpr (ITEMS > 8) {
+            Held<T, 1> zh[ITEMS], gh[ITEMS];
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int c = i * LANES + lane;
-            const bool in = live && c < dim;
-            h[i] = in ? (float)z[c] : mean;
-            g[i] = in ? (float)gr[c] : 0.0f;
+            for (int i = 0; i < ITEMS; ++i) {
+                const int c = i * LANES + lane < dim ? i * LANES + lane : 0;
+                zh[i].load(z + c);
+                gh[i].load(gr + c);
+            }
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const bool in = live && i * LANES + lane < dim;
+                h[i] = in ? zh[i].value(0) : mean;
+                g[i] = in ? gh[i].value(0) : 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int c = i * LANES + lane;
+                const bool in = live && c < dim;
+                h[i] = in ? (float)z[c] : mean;
+                g[i] = in ? (float)gr[c] : 0.0f;
+            }
         }
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
@@ -1721,7 +1741,8 @@ int norm_fwd_tile(const NormArgs& a, int tile) {
 template <typename T>
 int norm_bwd_tile(const NormArgs& a, int tile, uint32_t& nparts) {
     const size_t lds = 2 * ((tile * a.dim * sizeof(T) + 15) / 16 * 16);
-    nparts = norm_bwd_blocks(a.rows, tile, NORM_TILE_BLOCKS);
+    // (16 values to a lane: two workgroups fit a CU, and no more are launched: 30112 x 483 fp32 37 us, with 1024 workgroups 44)
+    nparts = norm_bwd_blocks(a.rows, tile, norm_tile_items(a.dim, true) > 8 ? NORM_TILE_BLOCKS / 2 : NORM_TILE_BLOCKS);
 #define E3_TILE_BWD(ITEMS)                                                                                                    \
     norm_bwd_tile_kernel<T, ITEMS><<<dim3(nparts), dim3(256), lds, a.s>>>(a.rows, (int)a.dim, tile, (const T*)a.dy,           \
                                                                         (const T*)a.x, a.weight, a.affine_dtype, a.mean,     \
