@@ -631,8 +631,8 @@ __global__ __launch_bounds__(1024) void embed_sort_small_kernel(uint32_t n, uint
 // More positions: passes of up to 8 bits over tiles of 1024 * ITEMS keys, two launches each.  The first counts the digits of
 // every tile (and makes the keys); in the second every tile adds up the counts before its own (at most SORT_TILES of them, a
 // kilobyte each: cheaper than a launch that scans them), ranks its keys, puts them in order in LDS and writes them out
-// digit by digit.  1M positions of 12 bits: 39 us (the general sort with its seven launches 43), 60905 of 16 bits: 21 us (36),
-// 372939 of 17 bits: 55 us (65).  Keys to a thread: 1 up to 128 tiles of one, 2 up to 128 tiles of two, and so on; 560085
+// digit by digit.  1M positions of 12 bits: 37 us (the general sort with its seven launches 43), 60905 of 16 bits: 21 us (36),
+// 372939 of 17 bits: 40 us (65).  Keys to a thread: 1 up to 128 tiles, then 2 up to 128 tiles, then 4, then 8; 560085
 // positions took 12 us a scatter with 137 tiles of four, 14 with 69 tiles of eight, 372939 took 9 with 92 tiles and 10 with 183.
 constexpr uint32_t SORT_TILES = 256;
 __device__ __forceinline__ uint32_t sort_digit(uint32_t key, int shift, uint32_t mask) { return key >> shift & mask; }
@@ -1633,7 +1633,7 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(uint32_t nparts, size_t
 namespace {
 // Workgroups of 256 CUs that are resident together.  Long rows are spread over no more than that, each the same number of
 // rows: more workgroups fetch the parameters again, and the last ones leave most of the chip idle (forward, 4096 x 8192 bf16
-// with 4096 workgroups 55 us, 1024 52 us, 768 = all resident 40 us).
+// with 4096 workgroups 55 us, 1024 52 us, 768 = all resident 40 us; 30 us with a row's loads all in flight).
 template <typename K>
 size_t resident_blocks(K kernel, int threads) {
     int n = 0;
@@ -1763,9 +1763,8 @@ int norm_fwd_again(const NormArgs& a) {
     return 0;
 }
 // Rows of more than 256 packs (V values each, 16, 8 or 4 bytes or a single one): workgroups of 256 threads up to 1024 packs, of
-// 512 or 1024 threads up to 16384 values; longer rows, and single values past 1024, are read again for every step.  Held in
-// registers / read again: 2000 x 16384 bf16 50 / 85 us, 4096 x 4588 bf16 40 / 66 us, 300 x 16384 fp32 12 / 24 us, but
-// 2000 x 4097 bf16 33 / 29 us.
+// 512 or 1024 threads up to 16384 values (8192 single ones); longer rows are read again for every step.  Held in registers / read
+// again: 2000 x 16384 bf16 31 / 85 us, 4096 x 4588 bf16 29 / 66 us, 300 x 16384 fp32 11 / 24 us, 2000 x 4097 bf16 23 / 29 us.
 template <typename T, int V>
 int norm_fwd_long(const NormArgs& a) {
     const size_t packs = a.dim / V;
@@ -1799,7 +1798,7 @@ int norm_fwd_t(const NormArgs& a, int dtype) {
     return norm_fwd_v<T, 1>(a);
 }
 // The gradient, which keeps five arrays of the row, up to 16384 values where there are rows enough to make up for the partial
-// sums of the workgroups: 2000 x 16384 bf16 83 us (read again: 123), 4096 x 4588 bf16 53 us (90), 113 x 4588 bf16 11 us (15);
+// sums of the workgroups: 2000 x 16384 bf16 57 us (read again: 123), 4096 x 4588 bf16 50 us (90), 113 x 4588 bf16 11 us (15);
 // with 16 values to a thread 300 x 16384 fp32 took 47 us (38).
 // nparts: how many partial sums there are for norm_join_kernel, 0: the results are written
 template <typename T, int V>
