@@ -337,7 +337,7 @@ __global__ __launch_bounds__(256) void embed_tiny_kernel(uint32_t n, uint32_t ro
 
 // A group of G lanes sums one chunk of the sorted list, times a slice of G V columns, EMBED_UNROLL gathered rows in flight.
 // Bound by the gather: 1M rows of 48 fp32 values into 4096 table rows 48 us (4.0 TB/s of gradient read), 8192 rows of 4096
-// bf16 values into 32000 62 us, of which 262 MB are the cleared rows of the table (5.3 TB/s in all).
+// bf16 values into a cleared table of 32000 rows 33 us.
 constexpr int EMBED_UNROLL = 8;
 template <typename T, int V, int G>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t* __restrict__ kept, const uint32_t* __restrict__ keys,
@@ -545,11 +545,34 @@ struct SmallSort {
     uint32_t cnt[16][256];
     uint32_t wtot[4], valid;
 };
+// The other workgroups of the launch clear the table's gradient meanwhile, all of it (the sums then write the rows that have
+// positions): gradient of 1328 positions, 23345 rows of 1571 fp32 36 us, 50 where the sums' launch clears the rows without one;
+// lookup and gradient of 8192 positions, 32000 rows of 4096 bf16 106 and 113 us.
 template <int ITEMS, typename I>
 __global__ __launch_bounds__(1024) void embed_sort_small_kernel(uint32_t n, uint32_t rows, int passes, int bits,
                                                                 const I* __restrict__ index, uint32_t* __restrict__ keys,
-                                                                uint32_t* __restrict__ pos, uint32_t* __restrict__ kept) {
+                                                                uint32_t* __restrict__ pos, uint32_t* __restrict__ kept,
+                                                                uint16_t* __restrict__ table, size_t halves) {
     __shared__ SmallSort<ITEMS> L;
+    if (blockIdx.x > 0) {
+        size_t head = ((16 - (reinterpret_cast<uintptr_t>(table) & 15)) & 15) / 2;
+        if (head > halves) head = halves;
+        const size_t packs = (halves - head) / 8, tail = head + packs * 8, first = (size_t)(blockIdx.x - 1) * 4096 + threadIdx.x;
+        Pack<f16_t, 8> z;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z.v[j] = (f16_t)0.0f;
+        f16_t* body = reinterpret_cast<f16_t*>(table + head);
+        for (size_t i = first; i < packs; i += (size_t)(gridDim.x - 1) * 4096) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i + u * 1024 < packs) put<false, f16_t, 8>(body + (i + u * 1024) * 8, z);
+        }
+        if (blockIdx.x == 1) {
+            if (threadIdx.x < head) table[threadIdx.x] = 0;
+            if (tail + threadIdx.x < halves) table[tail + threadIdx.x] = 0;
+        }
+        return;
+    }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t base = (uint32_t)wave * (64 * ITEMS) + lane;
     const unsigned long long before = (1ull << lane) - 1ull;
@@ -798,6 +821,7 @@ __global__ __launch_bounds__(1024) void embed_scatter_kernel(uint32_t n, int shi
     }
 }
 
+constexpr size_t EMBED_SMALL = 16384;            // positions that one workgroup sorts
 namespace {
 struct EmbedScratch {
     uint32_t *key0, *key1, *pos0, *pos1, *kept, *sort;
@@ -844,8 +868,9 @@ int embed_sum_launch(const EmbedScratch& w, const uint32_t* keys, const uint32_t
     }
     const uint32_t chunk = EmbedScratch::chunk(n, dim), nchunks = EmbedScratch::chunks(n, dim);
     const size_t units = nslices * nchunks, blocks = (units + 256 / G - 1) / (256 / G);
-    if (blocks + zero_blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
-    embed_sum_kernel<T, V, G><<<dim3((unsigned)(blocks + zero_blocks)), dim3(256), 0, s>>>(
+    const size_t clears = n <= EMBED_SMALL ? 0 : zero_blocks;  // (the launch of the small sort has cleared the table)
+    if (blocks + clears > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
+    embed_sum_kernel<T, V, G><<<dim3((unsigned)(blocks + clears)), dim3(256), 0, s>>>(
         w.kept, keys, pos, chunk, nchunks, (uint32_t)nslices, dim, (const T*)d_out, stride, scale, (T*)d_table, w.part,
         (uint32_t)blocks, (uint32_t)rows, (uint32_t)per);
     LAUNCH_OK("embed_sum_kernel");
@@ -876,14 +901,20 @@ void embed_digits(uint32_t rows, int& passes, int& bits) {
     bits = (nbits + passes - 1) / passes;
 }
 template <typename I>
-void embed_sort_small(uint32_t n, uint32_t rows, int passes, int bits, const I* index, uint32_t* keys, uint32_t* pos, uint32_t* kept,
-                      hipStream_t s) {
-    if (n <= 1024) embed_sort_small_kernel<1, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, passes, bits, index, keys, pos, kept);
-    else if (n <= 4096) embed_sort_small_kernel<4, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, passes, bits, index, keys, pos, kept);
-    else if (n <= 8192) embed_sort_small_kernel<8, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, passes, bits, index, keys, pos, kept);
-    else embed_sort_small_kernel<16, I><<<dim3(1), dim3(1024), 0, s>>>(n, rows, passes, bits, index, keys, pos, kept);
+void embed_sort_small(uint32_t n, uint32_t rows, const I* index, uint32_t* keys, uint32_t* pos, uint32_t* kept, void* table,
+                      size_t bytes, hipStream_t s) {
+    int passes, bits;
+    embed_digits(rows, passes, bits);
+    const size_t need = (bytes + 65535) / 65536;               // 64 KB to a workgroup, at most one to each of the other CUs
+    const dim3 blocks(1 + (unsigned)(need < 255 ? need : 255)), threads(1024);
+#define E3_SMALL(ITEMS) \
+    embed_sort_small_kernel<ITEMS, I><<<blocks, threads, 0, s>>>(n, rows, passes, bits, index, keys, pos, kept, (uint16_t*)table, bytes / 2)
+    if (n <= 1024) E3_SMALL(1);
+    else if (n <= 4096) E3_SMALL(4);
+    else if (n <= 8192) E3_SMALL(8);
+    else E3_SMALL(16);
+#undef E3_SMALL
 }
-
 // The tiles' sort; keys / pos: where the result lies.
 template <int ITEMS>
 int embed_sort_tiles(const EmbedScratch& w, uint32_t n, uint32_t rows, const void* index, int index_bytes, uint32_t** keys,
@@ -916,11 +947,10 @@ int embed_bwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_
     EmbedScratch w = EmbedScratch::from(scratch, n, dim);
     uint32_t *keys = w.key0, *pos = w.pos0;
     int rc = 0;
-    if (n > EMBED_TINY && n <= 16384) {
-        int passes, bits;
-        embed_digits((uint32_t)rows, passes, bits);
-        if (index_bytes == 8) embed_sort_small((uint32_t)n, (uint32_t)rows, passes, bits, (const long long*)index, keys, pos, w.kept, s);
-        else embed_sort_small((uint32_t)n, (uint32_t)rows, passes, bits, (const int*)index, keys, pos, w.kept, s);
+    if (n > EMBED_TINY && n <= EMBED_SMALL) {
+        const size_t bytes = rows * dim * sizeof(T);
+        if (index_bytes == 8) embed_sort_small((uint32_t)n, (uint32_t)rows, (const long long*)index, keys, pos, w.kept, d_table, bytes, s);
+        else embed_sort_small((uint32_t)n, (uint32_t)rows, (const int*)index, keys, pos, w.kept, d_table, bytes, s);
         LAUNCH_OK("embed_sort_small_kernel");
     } else if (n > EMBED_TINY && n <= SORT_TILES * 8192) {
 #define E3_TILES(ITEMS) embed_sort_tiles<ITEMS>(w, (uint32_t)n, (uint32_t)rows, index, index_bytes, &keys, &pos, s)
