@@ -167,7 +167,8 @@ int e3_embedding_forward_impl(size_t n, size_t rows, size_t dim, const void* ind
 // into chunks of equal length, a group of lanes sums the rows of one chunk (times a slice of the columns), and
 //   * a run inside a chunk is finished there,
 //   * a run that crosses chunks leaves one fp32 partial row per chunk, which embed_join_kernel adds up in order,
-//   * a table row without a position is cleared by further workgroups of the same launch (embed_zero).
+//   * a table row without a position is cleared by further workgroups of the same launch (embed_zero), or with all others beside
+//     the sort where one workgroup sorts.
 // So a row that half of all positions share costs no more than rows with one position each.
 constexpr uint32_t EMBED_NONE = 0xFFFFFFFFu;
 
