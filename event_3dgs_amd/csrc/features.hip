@@ -1115,7 +1115,7 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_fwd_kernel(size_t ro
         load_affine_pack<V>(weight, affine_dtype, col, dim, 1.0f, w[i]);
         load_affine_pack<V>(bias, affine_dtype, col, dim, 0.0f, b[i]);
     }
-    const float inv = 1.0f / (float)dim;
+    const float len = (float)dim;                          // (divided by: its reciprocal would be rounded once more)
     const size_t step = (size_t)gridDim.x * R::PER_BLOCK;
     // (every lane of a wave, and every wave of a workgroup that shares a row, runs the same number of rounds)
     for (size_t base = (size_t)blockIdx.x * R::PER_BLOCK; base < rows; base += step) {
@@ -1138,7 +1138,7 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_fwd_kernel(size_t ro
                 s += v[i][j];
             }
         }
-        const float mean = R::sum(s, lds) * inv;
+        const float mean = R::sum(s, lds) / len;
         float q = 0.0f;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
@@ -1149,7 +1149,7 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_fwd_kernel(size_t ro
                 if (col < dim) q = FMA(v[i][j], v[i][j], q);
             }
         }
-        const float rstd = 1.0f / __builtin_sqrtf(FMA(R::sum(q, lds), inv, eps));
+        const float rstd = 1.0f / __builtin_sqrtf(R::sum(q, lds) / len + eps);
         if (!live) continue;
         if (lane == 0) {
             if (mean_out) mean_out[row] = mean;
@@ -1263,7 +1263,7 @@ __global__ __launch_bounds__(256) void norm_fwd_tile_kernel(size_t rows, int dim
     float w[NORM_TILE_ITEMS], b[NORM_TILE_ITEMS];
     load_affine<NORM_TILE_ITEMS>(weight, affine_dtype, lane, LANES, dim, 1.0f, w);
     load_affine<NORM_TILE_ITEMS>(bias, affine_dtype, lane, LANES, dim, 0.0f, b);
-    const float inv = 1.0f / (float)dim;
+    const float len = (float)dim;                          // (divided by: its reciprocal would be rounded once more)
     const size_t step = (size_t)gridDim.x * tile;
     size_t first = (size_t)blockIdx.x * tile;
     int n = tile_count(rows, first, tile);
@@ -1283,13 +1283,13 @@ __global__ __launch_bounds__(256) void norm_fwd_tile_kernel(size_t rows, int dim
             v[i] = live && i * LANES + lane < dim ? zh[i].value(0) : 0.0f;
             s += v[i];
         }
-        const float mean = lanes_sum(s, LANES) * inv;
+        const float mean = lanes_sum(s, LANES) / len;
 #pragma unroll
         for (int i = 0; i < NORM_TILE_ITEMS; ++i) {
             v[i] -= mean;
             if (i * LANES + lane < dim) q = FMA(v[i], v[i], q);
         }
-        const float rstd = 1.0f / __builtin_sqrtf(FMA(lanes_sum(q, LANES), inv, eps));
+        const float rstd = 1.0f / __builtin_sqrtf(lanes_sum(q, LANES) / len + eps);
         if (live) {
 #pragma unroll
             for (int i = 0; i < NORM_TILE_ITEMS; ++i) {
@@ -1323,7 +1323,7 @@ __global__ __launch_bounds__(256) void norm_bwd_tile_kernel(size_t rows, int dim
     load_affine<ITEMS>(weight, affine_dtype, lane, LANES, dim, 1.0f, w);
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) dw[i] = db[i] = 0.0f;
-    const float inv = 1.0f / (float)dim;
+    const float len = (float)dim;                          // (divided by: its reciprocal would be rounded once more)
     const size_t step = (size_t)gridDim.x * tile;
     size_t first = (size_t)blockIdx.x * tile;
     int n = tile_count(rows, first, tile);
@@ -1380,8 +1380,8 @@ __global__ __launch_bounds__(256) void norm_bwd_tile_kernel(size_t rows, int dim
             s1 += g[i];
             s2 = FMA(g[i], h[i], s2);
         }
-        s1 = lanes_sum(s1, LANES) * inv;
-        s2 = lanes_sum(s2, LANES) * inv;
+        s1 = lanes_sum(s1, LANES) / len;
+        s2 = lanes_sum(s2, LANES) / len;
         if (dx) {
             if (live) {
 #pragma unroll
@@ -1426,7 +1426,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(size_t rows, size_t
                                                              float* __restrict__ mean_out, float* __restrict__ rstd_out) {
     using R = NormRow<1024>;
     __shared__ float lds[16];
-    const float inv = 1.0f / (float)dim;
+    const float len = (float)dim;                          // (divided by: its reciprocal would be rounded once more)
     for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T* xr = x + row * stride;
         float s = 0.0f;
@@ -1435,14 +1435,14 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(size_t rows, size_t
 #pragma unroll
             for (int j = 0; j < V; ++j) s += (float)p.v[j];
         }
-        const float mean = R::sum(s, lds) * inv;
+        const float mean = R::sum(s, lds) / len;
         float q = 0.0f;
         for (size_t col = (size_t)threadIdx.x * V; col < dim; col += 1024 * V) {
             const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(xr + col);
 #pragma unroll
             for (int j = 0; j < V; ++j) { const float d = (float)p.v[j] - mean; q = FMA(d, d, q); }
         }
-        const float rstd = 1.0f / __builtin_sqrtf(FMA(R::sum(q, lds), inv, eps));
+        const float rstd = 1.0f / __builtin_sqrtf(R::sum(q, lds) / len + eps);
         if (threadIdx.x == 0) {
             if (mean_out) mean_out[row] = mean;
             if (rstd_out) rstd_out[row] = rstd;
@@ -1482,7 +1482,7 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_bwd_kernel(size_t ro
 #pragma unroll
         for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.0f;
     }
-    const float inv = 1.0f / (float)dim;
+    const float len = (float)dim;                          // (divided by: its reciprocal would be rounded once more)
     const size_t step = (size_t)gridDim.x * R::PER_BLOCK;
     for (size_t base = (size_t)blockIdx.x * R::PER_BLOCK; base < rows; base += step) {
         const size_t row = base + threadIdx.x / G;
@@ -1537,8 +1537,8 @@ __global__ __launch_bounds__(NormRow<G>::THREADS) void norm_bwd_kernel(size_t ro
                 s1 += g[i][j];
                 s2 = FMA(g[i][j], h[i][j], s2);
             }
-        s1 = R::sum(s1, lds) * inv;
-        s2 = R::sum(s2, lds) * inv;
+        s1 = R::sum(s1, lds) / len;
+        s2 = R::sum(s2, lds) / len;
         if (!live || !dx) continue;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
@@ -1585,7 +1585,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_long_kernel(size_t rows, size_t
                                                              const float* __restrict__ rstd_in, T* __restrict__ dx) {
     using R = NormRow<1024>;
     __shared__ float lds[16];
-    const float inv = 1.0f / (float)dim;
+    const float len = (float)dim;                          // (divided by: its reciprocal would be rounded once more)
     for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T *xr = x + row * stride, *dr = dy + row * dy_stride;
         const float mean = mean_in[row], rstd = rstd_in[row];
@@ -1599,8 +1599,8 @@ __global__ __launch_bounds__(1024) void norm_bwd_long_kernel(size_t rows, size_t
                 s2 = FMA(g, ((float)p.v[j] - mean) * rstd, s2);
             }
         }
-        s1 = R::sum(s1, lds) * inv;
-        s2 = R::sum(s2, lds) * inv;
+        s1 = R::sum(s1, lds) / len;
+        s2 = R::sum(s2, lds) / len;
         for (size_t col = (size_t)threadIdx.x * V; col < dim; col += 1024 * V) {
             const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(xr + col), d = *reinterpret_cast<const Pack<T, V>*>(dr + col);
             Pack<T, V> r;
