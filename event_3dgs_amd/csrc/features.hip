@@ -15,6 +15,8 @@ int launch_radix_sort_pairs(uint32_t* k0, uint32_t* k1, uint32_t* v0, uint32_t* 
         hipError_t _e = hipGetLastError();                    \
         if (_e != hipSuccess) return e3_fail(_e, name);       \
     } while (0)
+// whether one launch takes that many workgroups: the threads past 2^32 would be cut off without an error
+static inline bool grid_fits(size_t blocks, size_t threads) { return blocks < ((size_t)1 << 32) / threads; }
 
 // ============================================================================================== embedding, forward
 // out[i, :] = round(scale * table[index[i], :]).  An index below 0 stands for "no row" (zeros); one past the table gives a
@@ -125,7 +127,6 @@ template <bool STREAM, typename T, int V, typename I>
 static int embed_fwd_launch(size_t n, size_t rows, size_t dim, const void* index, const void* table, size_t stride, float scale,
                             void* out, hipStream_t s) {
     const size_t ppr = dim / V, each = 256 * EmbedPacks<T, V>::N, blocks = (n * ppr + each - 1) / each;
-    if (blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_forward: too many values");
     embed_fwd_kernel<STREAM, T, V, I><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(
         n, (long long)rows, (uint32_t)ppr, (const I*)index, (const T*)table, stride, scale, (T*)out);
     LAUNCH_OK("embed_fwd_kernel");
@@ -143,7 +144,6 @@ static int embed_fwd_t(size_t n, size_t rows, size_t dim, const void* index, con
     if (fits(8)) return embed_fwd_launch<false, T, N / 2, I>(n, rows, dim, index, table, stride, scale, out, s);
     if (N == 8 && fits(4)) return embed_fwd_launch<false, T, 2, I>(n, rows, dim, index, table, stride, scale, out, s);
     const size_t blocks = (n * dim + EMBED_FLAT - 1) / EMBED_FLAT;
-    if (blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_forward: too many values");
     if (large) embed_fwd_odd_kernel<true, T, I><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(
         n, (long long)rows, (uint32_t)dim, (const I*)index, (const T*)table, stride, scale, (T*)out);
     else embed_fwd_odd_kernel<false, T, I><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(
@@ -154,11 +154,20 @@ static int embed_fwd_t(size_t n, size_t rows, size_t dim, const void* index, con
 
 int e3_embedding_forward_impl(size_t n, size_t rows, size_t dim, const void* index, int index_bytes, const void* table,
                               size_t stride, int dtype, float scale, void* out, hipStream_t s) {
-    if (n == 0) return 0;
-#define E3_FWD(T) (index_bytes == 8 ? embed_fwd_t<T, long long>(n, rows, dim, index, table, stride, dtype, scale, out, s) \
-                                    : embed_fwd_t<T, int>(n, rows, dim, index, table, stride, dtype, scale, out, s))
-    return dtype == E3_F32 ? E3_FWD(float) : dtype == E3_F16 ? E3_FWD(f16_t) : E3_FWD(bf16_t);
+    // A launch ends before 2^32 threads (those past it are cut off without an error), so large results take several: 2^35 values
+    // are at most 2^23 workgroups of 4096 values or more.  A slice is a multiple of 8 rows: `out` keeps its boundary.
+    const size_t each = ((size_t)1 << 35) / dim / 8 * 8;
+    for (size_t at = 0; at < n; at += each) {
+        const size_t m = n - at < each ? n - at : each;
+        const void* idx = reinterpret_cast<const char*>(index) + at * index_bytes;
+        void* to = reinterpret_cast<char*>(out) + at * dim * e3_elem_bytes(dtype);
+#define E3_FWD(T) (index_bytes == 8 ? embed_fwd_t<T, long long>(m, rows, dim, idx, table, stride, dtype, scale, to, s) \
+                                    : embed_fwd_t<T, int>(m, rows, dim, idx, table, stride, dtype, scale, to, s))
+        const int rc = dtype == E3_F32 ? E3_FWD(float) : dtype == E3_F16 ? E3_FWD(f16_t) : E3_FWD(bf16_t);
 #undef E3_FWD
+        if (rc) return rc;
+    }
+    return 0;
 }
 
 // ============================================================================================== embedding, gradient
@@ -860,7 +869,7 @@ int embed_sum_launch(const EmbedScratch& w, const uint32_t* keys, const uint32_t
     const size_t zero_blocks = (rows + 4 * per - 1) / (4 * per);
     if (n <= EMBED_TINY) {
         const size_t blocks = n * nslices;
-        if (blocks + zero_blocks > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
+        if (!grid_fits(blocks + zero_blocks, 256)) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
         embed_tiny_kernel<T, V, G><<<dim3((unsigned)(blocks + zero_blocks)), dim3(256), 0, s>>>(
             (uint32_t)n, (uint32_t)rows, index, index_bytes, (uint32_t)nslices, dim, (const T*)d_out, stride, scale, (T*)d_table,
             (uint32_t)blocks, (uint32_t)per);
@@ -870,7 +879,7 @@ int embed_sum_launch(const EmbedScratch& w, const uint32_t* keys, const uint32_t
     const uint32_t chunk = EmbedScratch::chunk(n, dim), nchunks = EmbedScratch::chunks(n, dim);
     const size_t units = nslices * nchunks, blocks = (units + 256 / G - 1) / (256 / G);
     const size_t clears = n <= EMBED_SMALL ? 0 : zero_blocks;  // (the launch of the small sort has cleared the table)
-    if (blocks + clears > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
+    if (!grid_fits(blocks + clears, 256)) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
     embed_sum_kernel<T, V, G><<<dim3((unsigned)(blocks + clears)), dim3(256), 0, s>>>(
         w.kept, keys, pos, chunk, nchunks, (uint32_t)nslices, dim, (const T*)d_out, stride, scale, (T*)d_table, w.part,
         (uint32_t)blocks, (uint32_t)rows, (uint32_t)per);
@@ -887,7 +896,7 @@ int embed_join_launch(const EmbedScratch& w, const uint32_t* keys, size_t n, siz
     // which find no long run: 5539 positions, 12 rows of 289 bf16 5.6 us, with 64 columns 14.4)
     const size_t groups = nchunks > JOIN_SHORT ? (nchunks + JOIN_SHORT - 1) / JOIN_SHORT : 0;
     const size_t cols = groups * ((dim + 15) / 16) <= 2048 ? 16 : 64, longs = groups * ((dim + cols - 1) / cols);
-    if (shorts + longs > 0x7FFFFFFFull) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
+    if (!grid_fits(shorts + longs, 1024)) return e3_fail(hipErrorInvalidValue, "e3dgs_embedding_backward: too many values");
     embed_join_kernel<T, V><<<dim3((unsigned)(shorts + longs)), dim3(1024), 0, s>>>(w.kept, keys, chunk, nchunks, (uint32_t)shorts,
                                                                                   (uint32_t)cols, dim, w.part, scale, (T*)d_table);
     LAUNCH_OK("embed_join_kernel");

@@ -94,3 +94,10 @@ def test_workspaces_off_their_boundary(hip_lib):
         assert "8-byte aligned" in text()
     assert hip_lib.e3dgs_distill_backward(*head, off, PTR, PTR, 9, 1, None) != 0
     assert "8-byte aligned" in text()
+
+
+def test_embedding_past_one_launch(hip_lib):
+    """A table whose gradient would take more than 2^32 threads to clear (and 2^52 bytes)."""
+    rows, dim = (1 << 31) - 2, 1 << 20
+    assert hip_lib.e3dgs_embedding_backward(4, rows, dim, PTR, 4, PTR, dim, 1, 1.0, PTR, PTR, None) != 0
+    assert "too many values" in text()
