@@ -45,6 +45,11 @@ void same_device(const Tensor& t, const Tensor& with, const char* name) {
 void once(const char* who) {
     TORCH_CHECK(!at::GradMode::is_enabled(), who, " is differentiable once only (create_graph is not supported)");
 }
+// ... and so would a forward-mode derivative, which needs no requires_grad
+void no_tangent(const char* who, std::initializer_list<Tensor> inputs) {
+    for (const Tensor& t : inputs)
+        TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), who, " has no forward-mode derivative (its inputs must not be dual tensors)");
+}
 char* bytes(const Tensor& t) { return reinterpret_cast<char*>(t.data_ptr()); }
 Tensor scratch_of(size_t n, const Tensor& like) { return torch::empty({(int64_t)n}, like.options().dtype(torch::kByte)); }
 
@@ -102,6 +107,7 @@ struct EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
         once("embedding");
         const auto saved = ctx->get_saved_variables();
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
+        no_tangent("embedding", {grads[0]});
         const Guard guard(grads[0].device());
         const int64_t rows = ctx->saved_data["rows"].toInt();
         const Tensor index = saved[0].contiguous();
@@ -126,6 +132,7 @@ Tensor embedding(const Tensor& index, const Tensor& table, double scale) {
     TORCH_CHECK(std::isfinite((float)scale), "scale must be finite (in float32)");
     dtype_of(table, "table");
     index_bytes_of(index);
+    no_tangent("embedding", {table});
     if (!(at::GradMode::is_enabled() && table.requires_grad())) return embedding_forward(index, table, scale);
     return EmbeddingFunction::apply(index, table, scale);
 }
@@ -163,6 +170,7 @@ struct LayerNormFunction : public torch::autograd::Function<LayerNormFunction> {
         once("layer_norm");
         const auto saved = ctx->get_saved_variables();
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+        no_tangent("layer_norm", {grads[0]});
         const Tensor &x = saved[0], &weight = saved[1], &st = saved[2];
         const Guard guard(x.device());
         const Rows r = rows_of(x), g = rows_of(grads[0]);
@@ -202,6 +210,7 @@ Tensor layer_norm(const Tensor& x, const c10::optional<Tensor>& weight_, const c
         grad = grad || p.first->requires_grad();
     }
     TORCH_CHECK(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(), "weight and bias must have one type");
+    no_tangent("layer_norm", {x, weight, bias});
     if (!(at::GradMode::is_enabled() && grad)) return std::get<0>(layer_norm_forward(x, weight, bias, eps, false));
     return LayerNormFunction::apply(x, weight_, bias_, eps);
 }
@@ -296,6 +305,7 @@ struct DistillFunction : public torch::autograd::Function<DistillFunction> {
         once("distill_loss");
         const auto saved = ctx->get_saved_variables();
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        no_tangent("distill_loss", {grads[0]});
         const Guard guard(saved[0].device());
         const Scores s = scores_of(saved[0], saved[1], saved[2], ctx->saved_data["class_dim"].toInt());
         const Tensor g = grads[0].to(torch::kFloat32).contiguous();
@@ -328,6 +338,7 @@ int64_t distill_check(const Tensor& logits, const Tensor& teacher, const Tensor&
 
 Tensor distill(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature, int64_t reduction, int64_t class_dim) {
     class_dim = distill_check(logits, teacher, index, temperature, class_dim);
+    no_tangent("distill_loss", {logits, teacher});
     if (at::GradMode::is_enabled() && logits.requires_grad())
         return DistillFunction::apply(logits, teacher, index, temperature, reduction, class_dim);
     const Guard guard(logits.device());

@@ -6,9 +6,9 @@ of a decoder, and trained through the rasteriser (renderer.render(override_color
 (losses.distill_loss).  They take a batch of any size, a single row included.
 
 float32, float16 and bfloat16; sums and statistics are fp32, every result is rounded once.  No CPU path.  The order of
-every sum is fixed by sizes, strides and alignment: the same call gives the same bits.  Work is enqueued on the current stream of the tensors' device
-(whichever device is current) and may be captured into a graph; the gradients are differentiable once (a call under
-create_graph raises).
+every sum is fixed by sizes, strides and alignment: the same call gives the same bits.  Work is enqueued on the current stream
+of the tensors' device (whichever device is current) and may be captured into a graph; the gradients are differentiable once
+(a call under create_graph raises), and forward-mode derivatives are refused.
 """
 from . import _lib
 

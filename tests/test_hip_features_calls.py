@@ -1,8 +1,9 @@
 """Calls of embedding, layer_norm and distill_loss beside the ordinary ones."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
-from event_3dgs_amd import features
+from event_3dgs_amd import features, losses
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -10,6 +11,35 @@ DEV = "cuda"
 
 def rand(*shape, seed=0):
     return torch.randn(shape, generator=torch.Generator().manual_seed(seed + sum(shape))).to(DEV)
+
+
+def test_forward_mode_is_refused():
+    """A result without a tangent would be read as a derivative of zero."""
+    x, w, d = rand(4, 6), rand(6), rand(4, 6, seed=1)
+    t, ids = rand(4, 2), torch.zeros(4, 2, dtype=torch.int64, device=DEV)
+    for grad in (False, True):
+        with fwd.dual_level():
+            dual = fwd.make_dual(x.clone().requires_grad_(grad), d)
+            dual_w = fwd.make_dual(w.clone().requires_grad_(grad), d[0])
+            dual_t = fwd.make_dual(t.clone(), d[:, :2])
+            calls = [lambda: features.embedding(ids, dual), lambda: features.layer_norm(dual), lambda: features.layer_norm(x, dual_w),
+                     lambda: features.layer_norm(x, None, dual_w), lambda: losses.distill_loss(dual, t, ids),
+                     lambda: losses.distill_loss(x, dual_t, ids)]
+            for k, call in enumerate(calls):
+                for mode in (torch.enable_grad(), torch.no_grad()):
+                    with mode, pytest.raises(RuntimeError, match="forward-mode"):
+                        call()
+                        pytest.fail("call %d was not refused" % k)
+            # without autograd: value and gradient of the primal
+            value, grad_x = losses.distill_loss_raw(dual, t, ids)
+            assert fwd.unpack_dual(value).tangent is None and fwd.unpack_dual(grad_x).tangent is None
+            features.layer_norm(x, w)                            # (no tangent among the inputs)
+    leaf = x.clone().requires_grad_(True)
+    for call in (lambda: features.embedding(ids, leaf), lambda: features.layer_norm(leaf), lambda: losses.distill_loss(leaf, t, ids)):
+        with fwd.dual_level():                                   # ... or of the gradient that comes back
+            y = call()
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))
 
 
 @pytest.mark.parametrize("dim", [66, 65])
