@@ -160,9 +160,7 @@ struct LayerNormFunction : public torch::autograd::Function<LayerNormFunction> {
         const Tensor weight = weight_ ? *weight_ : Tensor(), bias = bias_ ? *bias_ : Tensor();
         auto r = layer_norm_forward(x, weight, bias, eps, true);
         ctx->save_for_backward({x, weight, std::get<1>(r)});
-        ctx->saved_data["x_grad"] = x.requires_grad();
-        ctx->saved_data["weight_grad"] = weight.defined() && weight.requires_grad();
-        ctx->saved_data["bias_grad"] = bias.defined() && bias.requires_grad();
+        ctx->saved_data["bias"] = bias.defined();
         ctx->saved_data["affine"] = (int64_t)(weight.defined() ? weight.scalar_type() : bias.defined() ? bias.scalar_type() : x.scalar_type());
         return std::get<0>(r);
     }
@@ -177,9 +175,11 @@ struct LayerNormFunction : public torch::autograd::Function<LayerNormFunction> {
         const int64_t dim = x.size(-1), rows = x.numel() / dim;
         const Tensor w = weight.defined() ? weight.contiguous() : weight;
         const auto affine = x.options().dtype((c10::ScalarType)ctx->saved_data["affine"].toInt());
-        Tensor dx = ctx->saved_data["x_grad"].toBool() ? torch::empty(x.sizes(), x.options()) : Tensor();
-        Tensor dw = ctx->saved_data["weight_grad"].toBool() ? torch::empty({dim}, affine) : Tensor();
-        Tensor db = ctx->saved_data["bias_grad"].toBool() ? torch::empty({dim}, affine) : Tensor();
+        // (what this call of the backward pass asks for; the inputs are numbered without those that are None)
+        const size_t bias_input = weight.defined() ? 2 : 1;
+        Tensor dx = ctx->needs_input_grad(0) ? torch::empty(x.sizes(), x.options()) : Tensor();
+        Tensor dw = weight.defined() && ctx->needs_input_grad(1) ? torch::empty({dim}, affine) : Tensor();
+        Tensor db = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(bias_input) ? torch::empty({dim}, affine) : Tensor();
         Tensor scratch;
         if (dw.defined() || db.defined()) scratch = scratch_of(e3dgs_layer_norm_backward_scratch_bytes((size_t)rows, (size_t)dim), x);
         const auto kind = affine.dtype().toScalarType();

@@ -42,6 +42,32 @@ def test_forward_mode_is_refused():
                 torch.autograd.grad(y, leaf, fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))
 
 
+def peak_of(call):
+    torch.cuda.synchronize()
+    base = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = call()
+    torch.cuda.synchronize()
+    return out, torch.cuda.max_memory_allocated() - base
+
+
+def test_layer_norm_forms_the_gradients_asked_for():
+    x, w, b = (rand(*s).requires_grad_(True) for s in ((20000, 256), (256,), (256,)))
+    d = rand(20000, 256, seed=1)
+    # dx, and the partial sums of the parameters' gradients (at most 1024 pairs of rows).  The allocator keeps up to 1 MiB behind
+    # an allocation with it (it cuts a block only where more is left): the 20480000 bytes of dx are 20971520 in its steps of 2 MiB.
+    size, sums = 20000 * 256 * 4 + 2 ** 20, 1024 * 2 * 256 * 4 + 2 ** 20
+    full = torch.autograd.grad(features.layer_norm(x, w, b), (x, w, b), d)
+    y = features.layer_norm(x, w, b)
+    for wanted in ((0,), (1,), (2,), (0, 2), (1, 2)):
+        got, peak = peak_of(lambda: torch.autograd.grad(y, [(x, w, b)[k] for k in wanted], d, retain_graph=True))
+        assert all(torch.equal(g, full[k]) for g, k in zip(got, wanted))
+        assert peak <= (size if 0 in wanted else 0) + (sums if wanted != (0,) else 0) + 65536, wanted
+    y = features.layer_norm(x, None, b)                          # (the bias in the weight's place among the gradients)
+    (got,), peak = peak_of(lambda: torch.autograd.grad(y, b, d))
+    assert torch.equal(got, full[2]) and peak <= sums + 65536
+
+
 @pytest.mark.parametrize("dim", [66, 65])
 def test_embedding_past_one_launch(dim):
     """More workgroups than one launch takes (2^32 threads): 2^36 values and some more, in packs of 4 bytes and one by one."""
