@@ -1703,7 +1703,9 @@ unsigned norm_bwd_blocks(size_t rows, int per_block, size_t most) {
     // joined faster than 962)
     return per_block == 1 ? even_blocks(need, blocks < most ? blocks : most) : (unsigned)(blocks < most ? blocks : most);
 }
-constexpr size_t NORM_FWD_BLOCKS = 4096, NORM_BWD_BLOCKS = 1024, NORM_TILE_BLOCKS = 1024, NORM_LONG_PARTS = 64;
+// (a row of more than NORM_HELD values is never held in registers, whatever its type and boundary: its column sums come from
+// norm_cols_kernel, in NORM_LONG_PARTS partial rows)
+constexpr size_t NORM_FWD_BLOCKS = 4096, NORM_BWD_BLOCKS = 1024, NORM_TILE_BLOCKS = 1024, NORM_LONG_PARTS = 64, NORM_HELD = 16384;
 
 struct NormArgs {
     size_t rows, dim, x_stride, dy_stride;
@@ -1845,6 +1847,7 @@ template <typename T, int V>
 int norm_bwd_long(const NormArgs& a, uint32_t& nparts) {
     const size_t packs = a.dim / V;
     constexpr int MORE = V < 8 ? 4 : 2, MOST = V < 4 ? 8 : MORE;
+    static_assert(1024 * MOST * V <= NORM_HELD, "e3_layer_norm_scratch_bytes");
     if (packs <= 256) return norm_bwd_launch<T, V, 256, 1>(a, nparts);
     if (packs <= 512) return norm_bwd_launch<T, V, 256, 2>(a, nparts);
     if (packs <= 1024) return norm_bwd_launch<T, V, 256, 4>(a, nparts);
@@ -1911,7 +1914,8 @@ int e3_layer_norm_forward_impl(size_t rows, size_t dim, const void* x, size_t x_
 }
 
 size_t e3_layer_norm_scratch_bytes(size_t rows, size_t dim) {
-    return (rows < NORM_BWD_BLOCKS ? (rows ? rows : 1) : NORM_BWD_BLOCKS) * 2 * dim * sizeof(float) + 256;
+    const size_t most = dim > NORM_HELD ? NORM_LONG_PARTS : NORM_BWD_BLOCKS;
+    return (rows < most ? (rows ? rows : 1) : most) * 2 * dim * sizeof(float) + 256;
 }
 
 int e3_layer_norm_backward_impl(size_t rows, size_t dim, const void* dy, size_t dy_stride, const void* x, size_t x_stride,

@@ -101,3 +101,10 @@ def test_embedding_past_one_launch(hip_lib):
     rows, dim = (1 << 31) - 2, 1 << 20
     assert hip_lib.e3dgs_embedding_backward(4, rows, dim, PTR, 4, PTR, dim, 1, 1.0, PTR, PTR, None) != 0
     assert "too many values" in text()
+
+
+@pytest.mark.parametrize("rows, dim, parts", [(1024, 1 << 20, 64), (4096, 40000, 64), (4096, 16385, 64), (7, 40000, 7), (4096, 16384, 1024),
+                                              (4096, 48, 1024), (30, 48, 30), (0, 48, 1)])
+def test_layer_norm_scratch(hip_lib, rows, dim, parts):
+    """Partial sums of both parameters: long rows leave 64 of them, others one to a workgroup."""
+    assert hip_lib.e3dgs_layer_norm_backward_scratch_bytes(rows, dim) == parts * 2 * dim * 4 + 256
