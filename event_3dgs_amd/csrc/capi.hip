@@ -920,7 +920,7 @@ static int distill_args(const char* who, size_t rows, size_t classes, size_t k, 
                         int index_bytes, float temperature, int reduction) {
     if (classes < 1 || classes >= 0x7FFFFFFFull || k < 1 || k > E3DGS_DISTILL_MAX_K || rows >= 0x7FFFFFFFull)
         return feature_args_fail(who, rows, classes, dtype, "bad sizes");
-    if (!(temperature > 0.0f) || temperature > 1e30f || reduction < 0 || reduction > 2)
+    if (!(temperature > 1e-6f && temperature < 1e6f) || reduction < 0 || reduction > 2)
         return feature_args_fail(who, rows, classes, dtype, "bad temperature or reduction");
     if (dtype < E3DGS_F32 || dtype > E3DGS_BF16 || teacher_dtype < E3DGS_F32 || teacher_dtype > E3DGS_BF16 ||
         (index_bytes != 4 && index_bytes != 8))

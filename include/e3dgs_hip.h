@@ -775,7 +775,7 @@ int e3dgs_layer_norm_backward(size_t rows, size_t dim, const void* grad_out, siz
  * (the weights add up).  An index at or past `classes` makes the row and its gradient NaN.
  * Strides in elements: logits (row_stride, class_stride) with class_stride 1, or row_stride 1 and at most
  * E3DGS_DISTILL_MAX_PLANES classes and entries (planes, as an image lies); teacher and index (row, entry) as they are.
- * reduction: 0 none, 1 mean over the labelled rows, 2 sum.
+ * temperature: between 1e-6 and 1e6.  reduction: 0 none, 1 mean over the labelled rows, 2 sum.
  *   stats     2 floats per row and one more, for the backward call; 8-B aligned
  *   row_loss  one float per row (may be NULL)
  *   loss      one float: the value (sum or mean; for `none` the sum)

@@ -108,3 +108,13 @@ def test_embedding_past_one_launch(hip_lib):
 def test_layer_norm_scratch(hip_lib, rows, dim, parts):
     """Partial sums of both parameters: long rows leave 64 of them, others one to a workgroup."""
     assert hip_lib.e3dgs_layer_norm_backward_scratch_bytes(rows, dim) == parts * 2 * dim * 4 + 256
+
+
+@pytest.mark.parametrize("temperature", [1e-39, 1e-6, 1e6, 1e25, -1.0])
+def test_distill_temperature(hip_lib, temperature):
+    """Temperatures whose reciprocal or square is no fp32 number, and the rest of what distill_loss refuses too."""
+    head = (5, 9, 2, PTR, 9, 1, 0, PTR, 2, 1, 0, PTR, 2, 1, 4, temperature, 1)
+    assert hip_lib.e3dgs_distill_forward(*head, PTR, PTR, PTR, None, 0, 0, PTR, None) != 0
+    assert "temperature" in text()
+    assert hip_lib.e3dgs_distill_backward(*head, PTR, PTR, PTR, 9, 1, None) != 0
+    assert "temperature" in text()
