@@ -35,6 +35,9 @@ def lib():
     L.e3dgs_abi_version.restype = C.c_int
     if L.e3dgs_abi_version() != ABI_VERSION:
         raise HipLibraryError("libe3dgs_hip.so ABI version mismatch; rebuild")
+    missing = [name for name in EXPORTED_SYMBOLS if not hasattr(L, name)]
+    if missing:                                         # (entry points were added under this version)
+        raise HipLibraryError("libe3dgs_hip.so is older than this package: it lacks %s; rebuild" % ", ".join(missing))
     L.e3dgs_last_error.restype = C.c_char_p
     L.e3dgs_rasterize_forward.restype = C.c_int
     L.e3dgs_rasterize_forward.argtypes = (

@@ -118,3 +118,13 @@ def test_distill_temperature(hip_lib, temperature):
     assert "temperature" in text()
     assert hip_lib.e3dgs_distill_backward(*head, PTR, PTR, PTR, 9, 1, None) != 0
     assert "temperature" in text()
+
+
+def test_library_without_the_entry_points(hip_lib, monkeypatch):
+    """A library of the same version from before they were added is refused by name."""
+    import types
+    old = types.SimpleNamespace(**{name: (lambda: _lib.ABI_VERSION) for name in _lib.EXPORTED_SYMBOLS if "distill" not in name})
+    monkeypatch.setattr(_lib, "_lib", None)
+    monkeypatch.setattr(_lib.C, "CDLL", lambda path: old)
+    with pytest.raises(_lib.HipLibraryError, match="e3dgs_distill_forward.*rebuild"):
+        _lib.lib()
