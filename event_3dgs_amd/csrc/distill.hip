@@ -983,8 +983,9 @@ template <typename T, int V, int G>
 int distill_rows_launch(const DistillArgs& a, bool backward, unsigned& blocks, hipStream_t s) {
     blocks = distill_blocks(a.rows, RowsLds<G>::ROWS);
     const dim3 threads(RowsLds<G>::THREADS);
-    if (!backward) distill_fwd_rows_kernel<T, V, G><<<dim3(blocks), threads, 0, s>>>(a);
-    else if (V > 1 && a.rows * a.classes * sizeof(T) > E3_STREAM_BYTES) distill_bwd_rows_kernel<(V > 1), T, V, G><<<dim3(blocks), threads, 0, s>>>(a);
+    if (!backward) {
+        if constexpr (V > 1) distill_fwd_rows_kernel<T, V, G><<<dim3(blocks), threads, 0, s>>>(a);      // (rows_wide)
+    } else if (V > 1 && a.rows * a.classes * sizeof(T) > E3_STREAM_BYTES) distill_bwd_rows_kernel<(V > 1), T, V, G><<<dim3(blocks), threads, 0, s>>>(a);
     else distill_bwd_rows_kernel<false, T, V, G><<<dim3(blocks), threads, 0, s>>>(a);
     LAUNCH_OK("distill_rows_kernel");
     return 0;

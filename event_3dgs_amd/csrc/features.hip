@@ -1,8 +1,8 @@
 // features.hip -- rows of learned features: lookup in a shared table with the gradient by sorted index, layer norm.
 //
 // Both are bound by memory: a value is touched by a handful of operations, so the kernels are laid out for 16-byte packs,
-// few passes over the data and enough bytes in flight.  All sums run in fp32 and in an order that depends on the sizes
-// alone (no floating-point atomics): results are the same bit for bit from call to call.
+// few passes over the data and enough bytes in flight.  All sums run in fp32 and in an order that depends on sizes, strides
+// and alignment alone (no floating-point atomics): results are the same bit for bit from call to call.
 #include "rows.h"
 
 int e3_fail(hipError_t e, const char* what);
@@ -21,8 +21,9 @@ static inline bool grid_fits(size_t blocks, size_t threads) { return blocks < ((
 // ============================================================================================== embedding, forward
 // out[i, :] = round(scale * table[index[i], :]).  An index below 0 stands for "no row" (zeros); one past the table gives a
 // row of NaN -- an error that only the device sees, made visible without a wait.
-// One thread moves several packs of the flat output (4 of 16 bytes, 8 of 4 or 8: a workgroup waits for the index, then for the row, and has to have enough behind that), a workgroup's packs are contiguous: every lane works whatever
-// the row length, the stores are whole lines, and the rows of a pack-block are found by one division each.
+// One thread moves several packs of the flat output (4 of 16 bytes, 8 of 4 or 8: a workgroup waits for the index, then for the
+// row, and has to have enough behind that), a workgroup's packs are contiguous: every lane works whatever the row length, the
+// stores are whole lines, and the rows of a pack-block are found by one division each.
 template <typename T, int V>
 struct EmbedPacks {
     static constexpr int N = V * (int)sizeof(T) == 16 ? 4 : 8;
@@ -1008,12 +1009,8 @@ int embed_bwd_t(size_t n, size_t rows, size_t dim, const void* index, int index_
                                                                  : embed_join_launch<T, 1>(w, keys, n, dim, scale, d_table, s);
 }
 
-template <typename T, int V>
-__global__ __launch_bounds__(256) void fill_zero_kernel(size_t packs, Pack<T, V>* __restrict__ out) {
-    Pack<T, V> z;
-#pragma unroll
-    for (int j = 0; j < V; ++j) z.v[j] = (T)0.0f;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < packs; i += (size_t)gridDim.x * 256) out[i] = z;
+__global__ __launch_bounds__(256) void fill_zero_kernel(size_t halves, uint16_t* __restrict__ out) {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < halves; i += (size_t)gridDim.x * 256) out[i] = 0;
 }
 }  // namespace
 
@@ -1029,8 +1026,7 @@ int e3_embedding_backward_impl(size_t n, size_t rows, size_t dim, const void* in
         // no positions: clear the table's gradient with a kernel (a captured memset is not repeatable on every replay)
         const size_t bytes = rows * dim * e3_elem_bytes(dtype);
         const size_t blocks = (bytes / 2 + 255) / 256;
-        fill_zero_kernel<f16_t, 1><<<dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s>>>(
-            bytes / 2, (Pack<f16_t, 1>*)d_table);
+        fill_zero_kernel<<<dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s>>>(bytes / 2, (uint16_t*)d_table);
         LAUNCH_OK("fill_zero_kernel");
         return 0;
     }
@@ -1043,7 +1039,8 @@ int e3_embedding_backward_impl(size_t n, size_t rows, size_t dim, const void* in
 // y = (x - mean) * rstd * weight + bias per row, mean and rstd = 1 / sqrt(var + eps) in fp32.  A row stays in the registers
 // of its lanes between the statistics and the output (one pass over memory); the variance is the mean square of
 // x - mean, not a difference of sums, so a row far from zero keeps its digits.
-// Lanes per row: a group of 8 .. 64 lanes of one wave, or a workgroup of 256 threads for long rows (NormRow).
+// Lanes per row: a group of 8 .. 64 lanes of one wave, or a workgroup of 256, 512 or 1024 threads for long rows
+// (NormRow).
 template <int G>
 struct NormRow {      // sums over the lanes of a row
     static constexpr int THREADS = G > 256 ? G : 256;
@@ -1755,7 +1752,7 @@ int norm_bwd_launch(const NormArgs& a, uint32_t& nparts) {
 int norm_tile_items(size_t dim, bool backward) { return backward && dim <= 256 ? 8 : NORM_TILE_ITEMS; }
 
 // Rows of a tile, or 0 where the tile kernels do not apply: rows that do not lie one behind the other from a 16-byte boundary
-// on, rows past 64 lanes of NORM_TILE_ITEMS values, and those that a group of lanes reads in packs as well (5 packs or
+// on, rows past 32 lanes of NORM_TILE_ITEMS values, and those that a group of lanes reads in packs as well (5 packs or
 // more).  256 / the lanes of a row, with more lanes to it when the launch would not fill the chip otherwise; at least 8 rows,
 // so that every tile begins on a 16-byte boundary.
 int norm_tile_rows(const NormArgs& a, size_t bytes, bool backward) {
@@ -1811,12 +1808,18 @@ template <typename T, int V>
 int norm_fwd_long(const NormArgs& a) {
     const size_t packs = a.dim / V;
     constexpr int MORE = V < 8 ? 4 : 2, MOST = V < 4 ? 8 : MORE;
-    if (packs <= 256) return norm_fwd_launch<T, V, 64, 4>(a);
+    if constexpr (V != 2) {                                // (packs of two values: only rows of more than 512 values)
+        if (packs <= 256) return norm_fwd_launch<T, V, 64, 4>(a);
+    }
     if (packs <= 512) return norm_fwd_launch<T, V, 256, 2>(a);
     if (packs <= 1024) return norm_fwd_launch<T, V, 256, 4>(a);
     if (packs <= 2048) return norm_fwd_launch<T, V, 512, 4>(a);
-    if (packs <= 1024 * MORE) return norm_fwd_launch<T, V, 1024, MORE>(a);
-    if (packs <= 1024 * MOST) return norm_fwd_launch<T, V, 1024, MOST>(a);
+    if constexpr (MORE > 2) {
+        if (packs <= 1024 * MORE) return norm_fwd_launch<T, V, 1024, MORE>(a);
+    }
+    if constexpr (MOST > MORE) {
+        if (packs <= 1024 * MOST) return norm_fwd_launch<T, V, 1024, MOST>(a);
+    }
     return norm_fwd_again<T, V>(a);
 }
 template <typename T, int V>
@@ -1848,13 +1851,19 @@ int norm_bwd_long(const NormArgs& a, uint32_t& nparts) {
     const size_t packs = a.dim / V;
     constexpr int MORE = V < 8 ? 4 : 2, MOST = V < 4 ? 8 : MORE;
     static_assert(1024 * MOST * V <= NORM_HELD, "e3_layer_norm_scratch_bytes");
-    if (packs <= 256) return norm_bwd_launch<T, V, 256, 1>(a, nparts);
+    if constexpr (V != 2) {
+        if (packs <= 256) return norm_bwd_launch<T, V, 256, 1>(a, nparts);
+    }
     if (packs <= 512) return norm_bwd_launch<T, V, 256, 2>(a, nparts);
     if (packs <= 1024) return norm_bwd_launch<T, V, 256, 4>(a, nparts);
     if (packs <= 2048) return norm_bwd_launch<T, V, V == 8 ? 512 : 1024, V == 8 ? 4 : 2>(a, nparts);
-    const size_t most = a.rows >= 1024 || V == 1 ? 1024 * MOST : 8192 / V;
-    if (packs <= 1024 * MORE && packs <= most) return norm_bwd_launch<T, V, 1024, MORE>(a, nparts);
-    if (packs <= most) return norm_bwd_launch<T, V, 1024, MOST>(a, nparts);
+    [[maybe_unused]] const size_t most = a.rows >= 1024 || V == 1 ? 1024 * MOST : 8192 / V;
+    if constexpr (MORE > 2) {
+        if (packs <= 1024 * MORE && packs <= most) return norm_bwd_launch<T, V, 1024, MORE>(a, nparts);
+    }
+    if constexpr (MOST > MORE) {
+        if (packs <= most) return norm_bwd_launch<T, V, 1024, MOST>(a, nparts);
+    }
     if (a.dx) {
         const unsigned blocks = (unsigned)(a.rows < 2048 ? a.rows : 2048);
         norm_bwd_long_kernel<T, V><<<dim3(blocks), dim3(1024), 0, a.s>>>(a.rows, a.dim, (const T*)a.dy, a.dy_stride,

@@ -58,7 +58,6 @@ __device__ __forceinline__ void put(T* p, const Pack<T, V>& r) {
 }
 
 static inline size_t e3_elem_bytes(int dtype) { return dtype == E3_F32 ? 4 : 2; }
-static inline bool e3_dtype_ok(int dtype) { return dtype >= E3_F32 && dtype <= E3_BF16; }
 
 // The bits of one element, and a pack on its way from memory.  A single 16-bit value is loaded into a register of its own: loads
 // that fill the halves of one register wait for each other.
