@@ -314,10 +314,11 @@ def distill_loss(logits, teacher_logits, teacher_index, temperature=1.0, reducti
 
     teacher_logits / teacher_index have the shape of `logits` with k entries along `class_dim`: the scores the teacher gave
     its best classes, and which classes those are.  `logits` may be rows of classes (class_dim=-1) or planes of an image
-    (class_dim=0 of (classes, H, W), read as they lie up to 256 classes).  An entry counts when its index is >= 0 and its
-    score above -inf; a row without one is unlabelled: it adds 0, its gradient is 0, the mean leaves it out (a mean over no
-    row is 0).  A class may be listed twice (its weights add up); an index past the classes makes the row NaN.  Logits of
-    -inf or the type's lowest value switch a class off.  `temperature` lies between 1e-6 and 1e6, k is at most 1024.
+    (class_dim=0 of (classes, H, W), read as they lie up to 256 classes; a batch of images is copied into rows first).  An
+    entry counts when its index is >= 0 and its score above -inf; a row without one is unlabelled: it adds 0, its gradient is
+    0, the mean leaves it out (a mean over no row is 0).  A class may be listed twice (the value is the sum over the entries,
+    their weights add up in the gradient); an index past the classes makes the row NaN.  Logits of -inf or the type's lowest
+    value switch a class off.  `temperature` lies between 1e-6 and 1e6, k is at most 1024.
 
     Returns fp32: a scalar ('mean', 'sum') or one value per row ('none').  The gradient goes to `logits` only
     (a teacher that requires a gradient is refused: detach it)."""
