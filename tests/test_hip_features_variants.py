@@ -171,7 +171,10 @@ def test_embedding_gradient_of_whole_numbers(dtype, n, dim):
         table = torch.zeros(rows, dim, dtype=dtype, device=DEV, requires_grad=True)
         (got,) = torch.autograd.grad(features.embedding(index, table, 0.5), table, d)
         there = index >= 0
-        want = torch.zeros(rows, dim, dtype=torch.float64, device=DEV).index_add_(0, index[there], flat[there]) * 0.5
+        if rows <= 2:
+            want = torch.stack([flat[index == r].sum(0) for r in range(rows)]) * 0.5
+        else:
+            want = torch.zeros(rows, dim, dtype=torch.float64, device=DEV).index_add_(0, index[there], flat[there]) * 0.5
         assert torch.equal(got, want.to(dtype)), rows
 
 
